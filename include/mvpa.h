@@ -45,6 +45,7 @@ extern "C" {
 #define MVPA_F32 0  /* fp32 I/O, fp32 arithmetic on CUDA cores                      */
 #define MVPA_BF16 1 /* bf16 I/O, tcgen05 tensor cores with fp32 accumulation in TMEM */
 #define MVPA_F16 2  /* fp16 I/O (the reference op takes it too), fp32 arithmetic on CUDA cores */
+#define MVPA_E8M0 3 /* scales of 8-bit operands only: a power of two, one byte, 2^(byte - 127), 255 is NaN */
 
 /* Problem description.  Mirrors the constexpr arguments of the reference launch
  * (`attentions/attn.py:1103-1120`: Z, H_Q, H_KV, N_CTX, TIME_CTX, CHANNEL_CTX,
@@ -275,6 +276,49 @@ int mvpa_channel_mean(const void* h, void* out, int32_t B, int32_t T, int32_t C,
 int mvpa_contrastive_logits(const void* pred, const void* enc, const int32_t* negatives,
                             float* logits, int32_t B, int32_t T, int32_t C, int32_t E, int32_t K,
                             float temperature, int32_t dtype, void* cuda_stream);
+
+/* ---- the block in 8 bits ----------------------------------------------------------------------
+ * A row in 8 bits is a pair: q in e4m3, and one scale for each block of 128 neighbours (the row's last
+ * block as long as the row leaves it); a weight has one scale for each block of 128 x 128.  The pair
+ * stands for q * scale.  These entry points write
+ *
+ *   scale = the smallest 2^e, e >= -126, with max|y| <= 448 * 2^e   (MVPA_E8M0),   q = e4m3(y / scale)
+ *
+ * rounded once, to nearest, ties to even; a block that holds an infinity or a NaN has the scale NaN and
+ * every q NaN.  q: base and rows (ld_q) on 16-byte boundaries, nothing past a row's width is written;
+ * scales: bytes, (rows, ceil(width / 128)) with leading dimension ld_s.  Inputs MVPA_F32 / MVPA_BF16,
+ * any width and alignment (16-byte aligned rows are read faster).  Zero rows are no work and no error.
+ * These have no counterpart in the reference, whose block is bf16 throughout. */
+
+/* x (rows, width), leading dimension ld_x.  block_rows: 1, or 128 for a weight, whose scales are then
+ * (ceil(rows / 128), ceil(width / 128)). */
+int mvpa_quantize_fp8(const void* x, int64_t ld_x, void* q, int64_t ld_q, void* scales, int64_t ld_s,
+                      int64_t rows, int32_t width, int32_t block_rows, int32_t dtype, void* cuda_stream);
+
+/* mvpa_rmsnorm with y as a pair: rmsnorm(h) * weight goes from fp32 to e4m3 in one rounding.  x, add,
+ * weight, sum_out as there (sum_out may be x); width <= 4096 (bf16) / 2048 (fp32). */
+int mvpa_rmsnorm_fp8(const void* x, const void* add, const void* weight, void* sum_out, void* q,
+                     int64_t ld_q, void* scales, int64_t ld_s, int64_t rows, int32_t width, float eps,
+                     int32_t dtype, void* cuda_stream);
+
+/* silu(gate) * up as a pair, from fp32 in one rounding (mvpa_silu_mul rounds silu to the element type
+ * in between). */
+int mvpa_silu_mul_fp8(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* scales,
+                      int64_t ld_s, int64_t rows, int32_t width, int32_t dtype, void* cuda_stream);
+
+/*
+ * out = A B^T:  out[m, n] = sum_kb a_scales[m, kb] b_scales[n / 128, kb] sum_{k in kb} a[m, k] b[n, k].
+ * a (M, K) and b (N, K) in e4m3, bases and rows (ld_a, ld_b) on 16-byte boundaries; scales MVPA_E8M0 or
+ * MVPA_F32 (both the same), any strides in elements; out (M, N) MVPA_BF16 or MVPA_F32, leading dimension
+ * ld_out.  A block's products are summed in fp32, scaled by the fp32 product of the two scales and summed
+ * over the blocks in fp32, in an order that depends on the sizes alone; K = 0 gives zeros.  `status` (may be
+ * NULL): 64 ints, zeroed by the caller, of which the first is non-zero afterwards if one of the kernel's
+ * bounded waits ran out (the results are then NaN); mvpa_workspace_status(status, 256, stream) reads it.
+ */
+int mvpa_matmul_fp8(const void* a, int64_t ld_a, const void* a_scales, int64_t a_stride_m, int64_t a_stride_k,
+                    const void* b, int64_t ld_b, const void* b_scales, int64_t b_stride_n, int64_t b_stride_k,
+                    int32_t scale_dtype, void* out, int64_t ld_out, int64_t M, int32_t N, int32_t K,
+                    int32_t out_dtype, int32_t* status, void* cuda_stream);
 
 /* Text of the last error raised on this host thread ("" if none).
  * Stands where the reference raises RuntimeError / assert

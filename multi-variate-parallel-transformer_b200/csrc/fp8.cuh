@@ -1,0 +1,96 @@
+// What the 8-bit kernels share: blocks of 128 values in e4m3 with one scale.
+//
+//   scale = the smallest 2^e, e >= -126, with max|y| <= 448 * 2^e,   q = e4m3(y / scale)
+//
+// A power of two: y / scale is exact, so the only rounding is the step to e4m3 (to nearest, ties to even), and a value that is
+// representable comes back as it was; against a scale of max|y| / 448 a block gives away less than one binade at the bottom
+// of e4m3's range, where a value is 2^-15 of the block's largest.  The scale is held as its exponent's byte (e8m0, bias 127).
+// A block that holds an infinity or a NaN has the scale NaN (255) and every q NaN: it does not pass unnoticed.
+#pragma once
+#include "block_rows.cuh"
+
+namespace mvpa {
+namespace fp8 {
+
+constexpr int kBlock = 128;
+
+// The byte of the scale from the largest magnitude's bits (the bits of non-negative floats order like the floats do, with
+// infinity and then NaN above).  448 = 1.75 * 2^8: above 1.75 in the mantissa (0x600000) the next power is needed.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top_bits) {
+  if (top_bits >= 0x7f800000u) return 255u;
+  const int b = (int)((top_bits + 0x1fffffu) >> 23) - 8;
+  return (uint32_t)(b < 1 ? 1 : b);
+}
+// 1 / scale, exact; NaN for the byte 255.
+__device__ __forceinline__ float inverse_scale(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float((254u - byte) << 23);
+}
+// The scale itself (bytes from elsewhere may be 0: 2^-127).
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+
+__device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
+
+// The largest of the values of eight neighbouring lanes: a block of 128 is eight lanes with sixteen values each.
+__device__ __forceinline__ uint32_t max8(uint32_t v) {
+  v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  v = max(v, __shfl_xor_sync(0xffffffffu, v, 2));
+  return max(v, __shfl_xor_sync(0xffffffffu, v, 4));
+}
+
+constexpr int kLane = 16;  // values a lane holds of a block: 16 bytes of e4m3, one store
+
+// Sixteen values of a row from column `col`, zeros past `width`.  VEC: base and rows on 16-byte boundaries.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T* __restrict__ row, int col, int width, float (&y)[kLane]) {
+  constexpr int N = Vec<T>::N;
+  if (VEC && col + kLane <= width) {
+    uint4 raw[kLane / N];
+#pragma unroll
+    for (int i = 0; i < kLane / N; ++i) raw[i] = *reinterpret_cast<const uint4*>(row + col + i * N);
+#pragma unroll
+    for (int i = 0; i < kLane / N; ++i) {
+      float f[N];
+      Vec<T>::unpack(raw[i], f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[i * N + e] = f[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) y[e] = col + e < width ? to_f32<T>(row[col + e]) : 0.f;
+  }
+}
+
+// Sixteen values in e4m3 to a row whose start is on a 16-byte boundary; nothing past `width` is written.
+__device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int width, const float (&y)[kLane], float inverse) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = e4m3x4(y[4 * i] * inverse, y[4 * i + 1] * inverse, y[4 * i + 2] * inverse, y[4 * i + 3] * inverse);
+  if (col + kLane <= width) {
+    *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kLane; ++e)
+      if (col + e < width) row[col + e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+  }
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t top_of(const float (&y)[N]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) top = max(top, magnitude(y[e]));
+  return top;
+}
+
+}  // namespace fp8
+}  // namespace mvpa

@@ -143,7 +143,14 @@ __device__ __forceinline__ bool mbar_wait_a(uint32_t bar, uint32_t parity, int* 
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
-// 3-D tiled load (x = innermost).  x must keep the 16-byte rule: x * sizeof(elem) % 16 == 0.
+// 2-D and 3-D tiled loads (x = innermost).  x must keep the 16-byte rule: x * sizeof(elem) % 16 == 0.
+__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x,
                                             int y, int z) {
   asm volatile(
@@ -328,6 +335,25 @@ __device__ __forceinline__ void mma_ss_w(uint32_t el, uint32_t d_tmem, DescHalve
       "r"(accumulate), "r"(el)
       : "memory");
 }
+// Four consecutive K-steps of 32 bytes, D[tmem] = A[smem] * B[smem] for 8-bit operands, K-major in 128-byte rows; the first
+// step overwrites D.
+__device__ __forceinline__ void mma_f8_ss_x4_w(uint32_t el, uint32_t d_tmem, DescHalves a, DescHalves b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p0, p1, pe;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+      "setp.ne.b32 p0, 0, 0;\n\t"
+      "setp.eq.b32 p1, 0, 0;\n\t"
+      "setp.ne.b32 pe, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t mov.b64 db, {%3, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p0;\n\t"
+      "add.u32 la, %1, 2;\n\t add.u32 lb, %3, 2;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p1;\n\t"
+      "add.u32 la, %1, 4;\n\t add.u32 lb, %3, 4;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p1;\n\t"
+      "add.u32 la, %1, 6;\n\t add.u32 lb, %3, 6;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p1;\n\t}" ::"r"(d_tmem),
+      "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el)
+      : "memory");
+}
 __device__ __forceinline__ void mma_ts_w(uint32_t el, uint32_t d_tmem, uint32_t a_tmem, DescHalves b,
                                          uint32_t b_off_bytes, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -370,7 +396,12 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int b_mn_ma
          ((uint32_t)(M >> 4) << 24);
 }
 
-// Same with both operand majors selectable (bit 15: A is MN-major, bit 16: B is MN-major).
+// Instruction descriptor for kind::f8f6f4 with e4m3 A/B (format 0), K-major, and fp32 accumulation.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// make_idesc_bf16 with both operand majors selectable (bit 15: A is MN-major, bit 16: B is MN-major).
 __host__ __device__ constexpr uint32_t make_idesc_bf16_ab(int M, int N, int a_mn_major, int b_mn_major) {
   return make_idesc_bf16(M, N, b_mn_major) | ((uint32_t)a_mn_major << 15);
 }

@@ -51,8 +51,8 @@ struct TensorMapSlot {
 };
 constexpr int kTensorMapSlots = 64;
 
-inline int encode_bf16_sw128_uncached(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                                      const uint64_t* strides_bytes, const uint32_t* box);
+inline int encode_sw128(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims,
+                        const uint64_t* strides_bytes, const uint32_t* box);
 
 // bf16 tensor of `rank` dims (dims[0] innermost, contiguous), byte strides for dims 1..rank-1,
 // box of `box` elements, 128-byte swizzle, zero fill outside the tensor.
@@ -74,7 +74,7 @@ inline int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const
     *map = slot.map;
     return MVPA_OK;
   }
-  const int rc = encode_bf16_sw128_uncached(map, base, rank, dims, strides_bytes, box);
+  const int rc = encode_sw128(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides_bytes, box);
   if (rc == MVPA_OK) {
     slot.key = key;
     slot.map = *map;
@@ -83,8 +83,9 @@ inline int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const
   return rc;
 }
 
-inline int encode_bf16_sw128_uncached(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                                      const uint64_t* strides_bytes, const uint32_t* box) {
+// The same for any element type, encoded anew.
+inline int encode_sw128(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims,
+                        const uint64_t* strides_bytes, const uint32_t* box) {
   // The driver call needs a current context, and a thread's first runtime call is what binds one: make that call here,
   // whatever the caller has done on this thread so far (autograd runs backwards on threads of its own).
   int device = 0;
@@ -104,7 +105,7 @@ inline int encode_bf16_sw128_uncached(CUtensorMap* map, const void* base, int ra
     estr[i] = 1;
     if (i > 0) gstr[i - 1] = strides_bytes[i - 1];
   }
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr,
+  CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr,
                   bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {

@@ -1,8 +1,9 @@
 """Torch-tensor front ends of the C-ABI kernels that surround the attention in an MVPFormer block,
 its encoder and its heads (``include/mvpa.h``: mvpa_rmsnorm, mvpa_silu_mul, mvpa_wave_encode,
-mvpa_channel_mean, mvpa_contrastive_logits, and the backwards mvpa_rmsnorm_bwd, mvpa_silu_mul_bwd).
+mvpa_channel_mean, mvpa_contrastive_logits, the backwards mvpa_rmsnorm_bwd, mvpa_silu_mul_bwd, and the
+block in 8 bits: mvpa_quantize_fp8, mvpa_rmsnorm_fp8, mvpa_silu_mul_fp8, mvpa_matmul_fp8).
 `rmsnorm_train` and `swiglu` are differentiable and take any tensor (torch expressions serve what the
-kernels do not); the others are forward only, CUDA tensors, bf16 or fp32.
+kernels do not); the others are forward only, CUDA tensors, bf16 or fp32 (and their pairs in 8 bits).
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import torch
 
 import mvpa_host as _host
 import mvpa_native as _nat
+from attentions import attn as _attn
 
 
 def _code(t: torch.Tensor) -> int:
@@ -259,4 +261,143 @@ def contrastive_logits(pred, enc, negatives, temperature):
         st = _nat.lib().mvpa_contrastive_logits(pred.data_ptr(), enc.data_ptr(), negatives.data_ptr(), out.data_ptr(), B, T,
                                                 C, E, K, float(temperature), _code(pred), _stream(pred))
     _nat.check(st, "mvpa_contrastive_logits")
+    return out
+
+
+# ---- the block in 8 bits ----
+# A row in 8 bits is a pair (q, scales): q (rows, width) float8_e4m3fn whose rows start on 16-byte boundaries, scales
+# (rows, ceil(width / 128)) float8_e8m0fnu, one power of two for each block of 128 neighbours; a weight has one for each block
+# of 128 x 128.  The pair stands for q * scale.  scale is the smallest 2^e, e >= -126, with max|y| <= 448 * 2^e over the block,
+# q = y / scale rounded once, to nearest, ties to even.  A block that holds an infinity or a NaN is NaN throughout.
+
+FP8_BLOCK = 128
+_FP8_SCALES = {torch.float8_e8m0fnu: _nat.MVPA_E8M0, torch.float32: _nat.MVPA_F32}
+
+
+def _fp8_inputs(what, *ts):
+    """Ordinary CUDA tensors on one device that no gradient has to flow through."""
+    t0 = ts[0]
+    for t in ts:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: tensors must be on a CUDA device (no CPU path)")
+        if t.device != t0.device:
+            raise RuntimeError(f"{what}: tensors are on {t0.device} and {t.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _fp8_rows(what, t, name):
+    """Leading dimension of a matrix with unit inner stride (that of one row, or of an empty matrix, is never used)."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise RuntimeError(f"{what}: {name} must be a matrix with unit inner stride, got shape {tuple(t.shape)}, strides {t.stride()}")
+    if t.shape[0] < 2 or t.numel() == 0:
+        return (t.shape[1] + 15) // 16 * 16
+    if t.stride(0) < t.shape[1]:
+        raise RuntimeError(f"{what}: the rows of {name} overlap (strides {t.stride()})")
+    return t.stride(0)
+
+
+def _fp8_pair(what, out, rows, width, block_rows, device):
+    """(q, scales) to write into: the caller's, or new ones."""
+    shape, blocks = (rows, width), (-(-rows // block_rows), -(-width // FP8_BLOCK))
+    if out is None:
+        ld = (width + 15) // 16 * 16
+        q = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)
+        return (q if ld == width else q[:, :width]), torch.empty(blocks, dtype=torch.float8_e8m0fnu, device=device)
+    q, scales = out
+    if (q.shape != shape or q.dtype != torch.float8_e4m3fn or scales.shape != blocks or scales.dtype != torch.float8_e8m0fnu
+            or q.device != device or scales.device != device):
+        raise RuntimeError(f"{what}: out must be q {shape} float8_e4m3fn and scales {blocks} float8_e8m0fnu on {device}, got "
+                           f"{tuple(q.shape)} {q.dtype} {q.device} and {tuple(scales.shape)} {scales.dtype} {scales.device}")
+    return q, scales
+
+
+def quantize_fp8(x, block_rows=1, out=None):
+    """x (rows, width), bf16 or fp32, in 8 bits: (q, scales).  `block_rows=1` gives every row its own scales (activations),
+    `block_rows=128` every block of 128 x 128 one (weights).  `out=(q, scales)` writes into the caller's tensors, which may be
+    column blocks of wider ones."""
+    _fp8_inputs("quantize_fp8", x)
+    if block_rows not in (1, FP8_BLOCK):
+        raise RuntimeError(f"quantize_fp8: block_rows is 1 or {FP8_BLOCK}, got {block_rows}")
+    ld = _fp8_rows("quantize_fp8", x, "x")
+    rows, width = x.shape
+    q, scales = _fp8_pair("quantize_fp8", out, rows, width, block_rows, x.device)
+    ld_q, ld_s = _fp8_rows("quantize_fp8", q, "q"), _fp8_rows("quantize_fp8", scales, "scales")
+    with _nat.on_device(x.device):
+        st = _nat.lib().mvpa_quantize_fp8(x.data_ptr(), ld, q.data_ptr(), ld_q, scales.data_ptr(), ld_s, rows, width, block_rows,
+                                          _code(x), _stream(x))
+    _nat.check(st, "mvpa_quantize_fp8")
+    return q, scales
+
+
+def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None):
+    """`rmsnorm` with the result in 8 bits: (q, scales) of rmsnorm(h) * weight, h = x (+ add), for x (..., E) with all leading
+    dimensions as rows.  h is rounded to x's type, as in `rmsnorm`, and written to `sum_out` (which may be `x`); the normalised
+    row goes from fp32 to e4m3 in one rounding.  E up to 4096 in bf16, 2048 in fp32."""
+    extra = [t for t in (add, sum_out) if t is not None]
+    _fp8_inputs("rmsnorm_fp8", x, weight, *extra)
+    E = x.shape[-1]
+    if not all(t.is_contiguous() and t.dtype == x.dtype for t in (x, weight, *extra)):
+        raise RuntimeError("rmsnorm_fp8: x, weight, add and sum_out must be contiguous and of one type")
+    if weight.shape != (E,) or any(t.numel() != x.numel() or t.shape[-1:] != (E,) for t in extra):
+        raise RuntimeError(f"rmsnorm_fp8: shapes do not go together: x {tuple(x.shape)}, weight {tuple(weight.shape)}, "
+                           + ", ".join(str(tuple(t.shape)) for t in extra))
+    rows = x.numel() // E if E else 0
+    q, scales = _fp8_pair("rmsnorm_fp8", out, rows, E, 1, x.device)
+    ld_q, ld_s = _fp8_rows("rmsnorm_fp8", q, "q"), _fp8_rows("rmsnorm_fp8", scales, "scales")
+    with _nat.on_device(x.device):
+        st = _nat.lib().mvpa_rmsnorm_fp8(x.data_ptr(), add.data_ptr() if add is not None else None, weight.data_ptr(),
+                                         sum_out.data_ptr() if sum_out is not None else None, q.data_ptr(), ld_q,
+                                         scales.data_ptr(), ld_s, rows, E, float(eps), _code(x), _stream(x))
+    _nat.check(st, "mvpa_rmsnorm_fp8")
+    return q, scales
+
+
+def silu_mul_fp8(gate, up, out=None):
+    """silu(gate) * up in 8 bits: (q, scales).  gate, up (rows, width) with unit inner stride (column blocks of a wider buffer
+    are fine).  From fp32 to e4m3 in one rounding; `silu_mul` rounds silu(gate) to the type in between, as eager PyTorch does."""
+    _fp8_inputs("silu_mul_fp8", gate, up)
+    ld = _fp8_rows("silu_mul_fp8", gate, "gate")
+    if up.shape != gate.shape or up.dtype != gate.dtype or _fp8_rows("silu_mul_fp8", up, "up") != ld:
+        raise RuntimeError(f"silu_mul_fp8: gate and up must have one shape, type and row stride, got {tuple(gate.shape)} {gate.dtype} "
+                           f"{gate.stride()} and {tuple(up.shape)} {up.dtype} {up.stride()}")
+    rows, width = gate.shape
+    q, scales = _fp8_pair("silu_mul_fp8", out, rows, width, 1, gate.device)
+    ld_q, ld_s = _fp8_rows("silu_mul_fp8", q, "q"), _fp8_rows("silu_mul_fp8", scales, "scales")
+    with _nat.on_device(gate.device):
+        st = _nat.lib().mvpa_silu_mul_fp8(gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ld_q, scales.data_ptr(), ld_s, rows,
+                                          width, _code(gate), _stream(gate))
+    _nat.check(st, "mvpa_silu_mul_fp8")
+    return q, scales
+
+
+def matmul_fp8(a, a_scales, b, b_scales, out=None, dtype=torch.bfloat16):
+    """a @ b.T for pairs in 8 bits: a (M, K) with scales (M, ceil(K / 128)), b (N, K), a weight, with scales
+    (ceil(N / 128), ceil(K / 128)); the result (M, N) in `dtype` (bfloat16 or float32), or in `out`, which may be a column
+    block of a wider buffer.  The scales are both float8_e8m0fnu, as the functions above write them, or both float32, with any
+    strides.  Products and sums are in fp32, rounded once."""
+    what = "matmul_fp8"
+    _fp8_inputs(what, a, a_scales, b, b_scales)
+    ld_a, ld_b = _fp8_rows(what, a, "a"), _fp8_rows(what, b, "b")
+    (M, K), N = a.shape, b.shape[0]
+    kb = -(-K // FP8_BLOCK)
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn or a_scales.dtype != b_scales.dtype or a_scales.dtype not in _FP8_SCALES:
+        raise RuntimeError(f"matmul_fp8: operands are float8_e4m3fn with scales both float8_e8m0fnu or both float32, got {a.dtype}, "
+                           f"{a_scales.dtype}, {b.dtype}, {b_scales.dtype}")
+    if b.shape[1] != K or a_scales.shape != (M, kb) or b_scales.shape != (-(-N // FP8_BLOCK), kb):
+        raise RuntimeError(f"matmul_fp8: shapes do not go together: a {tuple(a.shape)} with scales {tuple(a_scales.shape)}, "
+                           f"b {tuple(b.shape)} with scales {tuple(b_scales.shape)}")
+    if out is None:
+        out = torch.empty((M, N), dtype=dtype, device=a.device)
+    elif out.shape != (M, N) or out.device != a.device:
+        raise RuntimeError(f"matmul_fp8: out must be {(M, N)} on {a.device}, got {tuple(out.shape)} on {out.device}")
+    ld_out = _fp8_rows(what, out, "out")
+    status = torch.zeros(64, dtype=torch.int32, device=a.device) if _attn._CHECK_STATUS else None
+    with _nat.on_device(a.device):
+        st = _nat.lib().mvpa_matmul_fp8(a.data_ptr(), ld_a, a_scales.data_ptr(), *a_scales.stride(), b.data_ptr(), ld_b,
+                                        b_scales.data_ptr(), *b_scales.stride(), _FP8_SCALES[a_scales.dtype], out.data_ptr(), ld_out,
+                                        M, N, K, _code(out), None if status is None else status.data_ptr(), _stream(a))
+        _nat.check(st, "mvpa_matmul_fp8")
+        if status is not None:  # debugging aid: synchronises the stream
+            _nat.check(_nat.lib().mvpa_workspace_status(status.data_ptr(), 256, _stream(a)), "mvpa_matmul_fp8 kernel")
     return out
