@@ -48,9 +48,9 @@ struct BwdArgs {
 
 // A launch whose CTAs may come up while the kernel before it in the stream runs out: the kernel starts with griddep_wait()
 // (tc_ptx.cuh), before it touches memory that an earlier kernel may have written.  Saves part of the gap between two
-// dependent kernels.  `cluster_z`: CTAs of a cluster along the grid's z.
+// dependent kernels.  `cluster`: CTAs of a cluster.
 template <typename... P>
-inline cudaError_t launch_dependent(unsigned cluster_z, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, P... args) {
+inline cudaError_t launch_dependent(dim3 cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, P... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -60,11 +60,17 @@ inline cudaError_t launch_dependent(unsigned cluster_z, void (*kernel)(P...), di
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = cluster_z;
+  attr[1].val.clusterDim.x = cluster.x;
+  attr[1].val.clusterDim.y = cluster.y;
+  attr[1].val.clusterDim.z = cluster.z;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster_z > 1 ? 2 : 1;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+// The same with clusters along the grid's z.
+template <typename... P>
+inline cudaError_t launch_dependent(unsigned cluster_z, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, P... args) {
+  return launch_dependent(dim3(1, 1, cluster_z), kernel, grid, block, smem, s, args...);
 }
 
 void set_error(const char* fmt, ...);

@@ -22,30 +22,42 @@ struct MatmulArgs {
   int* status;
 };
 
+// The two scales of a block as they lie in memory: loaded two blocks ahead, and not touched before they are wanted, since the
+// first use is what waits for the load.
 template <typename S>
-__device__ __forceinline__ float load_scale(const void* p, int64_t i) {
-  if constexpr (sizeof(S) == 1) return scale_value(static_cast<const uint8_t*>(p)[i]);
-  else return static_cast<const float*>(p)[i];
-}
+struct Scales {
+  S a, b;
+  __device__ __forceinline__ float product() const {
+    if constexpr (sizeof(S) == 1) return scale_value(a) * scale_value(b);
+    else return a * b;
+  }
+};
 
 template <typename Out>
 __device__ __forceinline__ void store_out(void* out, int64_t i, float v) {
   static_cast<Out*>(out)[i] = from_f32<Out>(v);
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // The float at `p`'s place in the shared memory of the cluster's CTA `rank`.
 __device__ __forceinline__ float peer_load(const float* p, uint32_t rank) {
-  uint32_t at;
   float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_map(ptx::smem_u32(p), rank)) : "memory");
   return v;
 }
 
 enum : int { kGiveUpEmpty = 71, kGiveUpFull = 72, kGiveUpTmemEmpty = 73, kGiveUpTmemFull = 74, kGiveUpDrain = 75 };
+
+// The kernel's shared memory is granted once per device (and thread) and not at every call.
+template <auto kernel>
+cudaError_t grant_smem(size_t bytes) {
+  static thread_local uint64_t granted = 0;  // a bit per device
+  int device = 0;
+  const cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || (device < 64 && (granted >> device & 1))) return e;
+  const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (set == cudaSuccess && device < 64) granted |= (uint64_t)1 << device;
+  return set;
+}
 
 // ---- few rows: 128 weight rows x NT tokens a CTA ----------------------------------------------------------------------------
 // The weights are the product's M side, so that one token fills 1/16 of a tile and not 1/128; the tile is transposed in TMEM
@@ -99,9 +111,10 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
   ptx::tc_fence_after();
   const uint32_t tmem = s_tmem;
   volatile int* dead = &s_dead;
-  const auto wait = [&](uint64_t& bar, int parity, int code) {
+  const auto wait = [&](uint64_t& bar, uint32_t parity, int code) {
+    if (ptx::mbar_test_wait(&bar, parity)) return true;
     if (*dead) return false;
-    if (ptx::mbar_wait(&bar, (uint32_t)parity, g.status, code)) return true;
+    if (ptx::mbar_wait(&bar, parity, g.status, code)) return true;
     *dead = 1;
     return false;
   };
@@ -147,16 +160,19 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
     const uint32_t at = tmem + ((uint32_t)quad << 21);
     const bool mine = t < NT && m0 + t < g.M;
     const int64_t ia = (m0 + t) * g.sa_m, ib = (int64_t)blockIdx.x * g.sb_n;
-    const auto scale_of = [&](int i) {
-      return mine && i < nkb ? load_scale<S>(g.sa, ia + (kb0 + i) * g.sa_k) * load_scale<S>(g.sb, ib + (kb0 + i) * g.sb_k) : 0.f;
+    const S *pa = static_cast<const S*>(g.sa) + ia, *pb = static_cast<const S*>(g.sb) + ib;
+    const auto scales_of = [&](int i) {
+      Scales<S> v = {};
+      if (mine && i < nkb) v = {pa[(kb0 + i) * g.sa_k], pb[(kb0 + i) * g.sb_k]};
+      return v;
     };
-    if (t < NT) s_scale[0][t] = scale_of(0);
-    float next = scale_of(1);
+    if (t < NT) s_scale[0][t] = scales_of(0).product();
+    Scales<S> next = scales_of(1);
     asm volatile("bar.sync 1, 128;" ::: "memory");
     for (int i = 0; i < nkb; ++i) {
       const int buf = i & 1;
-      const float after = scale_of(i + 2);
-      if (t < NT) s_scale[buf ^ 1][t] = next;
+      const Scales<S> after = scales_of(i + 2);
+      if (t < NT) s_scale[buf ^ 1][t] = next.product();
       next = after;
       wait(s_tfull[buf], (i >> 1) & 1, kGiveUpTmemFull);
       ptx::tc_fence_after();
@@ -203,7 +219,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
       for (int j = 0; j < NT; ++j) part[j * 128 + row] = acc[j] + poison;
     }
     __syncwarp();
-    cluster_sync();
+    ptx::cluster_sync();
     if (inside) {
       for (int j = blockIdx.z; j < NT && m0 + j < g.M; j += splits) {
         float v = 0.f;
@@ -212,7 +228,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
       }
     }
     __syncwarp();
-    cluster_sync();  // nobody's memory goes while it is read
+    ptx::cluster_sync();  // nobody's memory goes while it is read
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -233,9 +249,255 @@ int run_few(const CUtensorMap& map_w, const CUtensorMap& map_x, MatmulArgs g, cu
   while (splits < 8 && tiles_n * tiles_m * splits * 2 <= device_sm_count() && g.KB >= 4 * splits) splits *= 2;
   g.per = (g.KB + splits - 1) / splits;
   splits = (g.KB + g.per - 1) / g.per;
-  const auto kernel = matmul_few_kernel<NT, Out, S>;
-  MVPA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
+  constexpr auto kernel = matmul_few_kernel<NT, Out, S>;
+  MVPA_CUDA_CHECK(grant_smem<kernel>(C::kSmem));
   MVPA_CUDA_CHECK(launch_dependent(splits, kernel, dim3(tiles_n, (unsigned)tiles_m, splits), 192, C::kSmem, s, map_w, map_x, g));
+  count_launch();
+  MVPA_CUDA_CHECK(cudaGetLastError());
+  return MVPA_OK;
+}
+
+// ---- many rows: 256 tokens x 256 weight rows a pair of CTAs ------------------------------------------------------------------
+// One product over both CTAs' operands (cta_group::2): each CTA loads 128 tokens and 128 weight rows a block and holds its 128
+// tokens x 256 sums, so a loaded byte meets twice the operands that it would in one CTA's tile.  The pairs are resident and take
+// their tiles one after the other; TMEM holds the products of two blocks, and eight warps a CTA bring them home: a thread has one
+// token's 128 columns in registers.
+struct ManyRows {
+  static constexpr int kStageBytes = 2 * 128 * 128;
+  static constexpr int kStages = 6;
+  static constexpr size_t kSmem = 1024 + kStages * kStageBytes;
+};
+// Four warps that load and issue, eight that add up.  Registers: 384 x 168 at launch, of which the four keep 56 a thread and the
+// eight take 216 (128 x 56 + 256 x 216 = 62464 of 64512).
+constexpr int kManyThreads = 384;
+
+// Eight 32-bit words to a 32-byte boundary: a whole sector.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+struct Tile {
+  int m0, n0;
+};
+// Tiles in bands of eight along M: the pairs at work together share few panels of both operands.
+__device__ __forceinline__ Tile tile_at(uint32_t t, uint32_t tiles_n, uint32_t tiles_m) {
+  constexpr uint32_t kBand = 8;
+  const uint32_t band = t / (kBand * tiles_n), rest = t - band * kBand * tiles_n;
+  const uint32_t high = min(kBand, tiles_m - band * kBand), n = rest / high;
+  return {(int)((band * kBand + rest - n * high) * 256), (int)(n * 256)};
+}
+
+// A place in a ring of N, and the parity of the pass over it.
+template <uint32_t N>
+struct Ring {
+  uint32_t at = 0, parity = 0;
+  __device__ __forceinline__ void step() {
+    if (++at == N) {
+      at = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+template <typename Out, typename S>
+__global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                      const __grid_constant__ CUtensorMap map_x, const MatmulArgs g) {
+  using C = ManyRows;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_dead;
+  const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_rank();
+  const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t tiles_n = (uint32_t)(g.N + 255) / 256, tiles_m = (uint32_t)((g.M + 255) / 256), tiles = tiles_n * tiles_m;
+  if (warp == 0) {
+    ptx::prefetch_tensormap(&map_w);
+    ptx::prefetch_tensormap(&map_x);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < C::kStages; ++i) {
+        ptx::mbar_init(&s_full[i], 1);
+        ptx::mbar_init(&s_empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(&s_tfull[i], 1);
+        ptx::mbar_init(&s_tempty[i], 16);
+      }
+      ptx::mbar_fence_init();
+      s_dead = 0;
+    }
+    __syncwarp();
+    ptx::tmem_alloc_pair(&s_tmem, 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* dead = &s_dead;
+  const auto wait = [&](uint64_t& bar, uint32_t parity, int code) {
+    if (ptx::mbar_test_wait(&bar, parity)) return true;
+    if (*dead) return false;
+    if (ptx::mbar_wait(&bar, parity, g.status, code)) return true;
+    *dead = 1;
+    return false;
+  };
+  ptx::griddep_wait();
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      if (lane == 0) {
+        Ring<C::kStages> st;
+        uint32_t loads = 0;
+        bool on = true;
+        for (uint32_t t = pair; t < tiles && on; t += pairs) {
+          const Tile at = tile_at(t, tiles_n, tiles_m);
+          const int m = at.m0 + (int)rank * 128, n = at.n0 + (int)rank * 128;
+          for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
+            if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
+              on = false;
+              break;
+            }
+            const uint32_t full = ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0), x = stages + st.at * C::kStageBytes;
+            if (rank == 0) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * C::kStageBytes);  // (the other CTA's loads count here too)
+            ptx::tma_load_2d_pair(x, &map_x, full, kb * 128, m);
+            ptx::tma_load_2d_pair(x + 128 * 128, &map_w, full, kb * 128, n);
+          }
+        }
+        if (rank == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one below)
+          const uint32_t n = min(loads, (uint32_t)C::kStages);
+          for (uint32_t k = loads - n; k != loads; ++k)
+            if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      const uint32_t el = ptx::elect_one();
+      constexpr uint32_t idesc = ptx::make_idesc_e4m3(256, 256);
+      Ring<C::kStages> st;
+      Ring<2> buf;
+      uint32_t last = 0, last_parity = 0;
+      const uint32_t mine = pair < tiles ? ((tiles - pair + pairs - 1) / pairs) * (uint32_t)g.KB : 0;
+      uint32_t i = 0;
+      for (; i < mine; ++i, st.step(), buf.step()) {
+        const uint32_t x = stages + st.at * C::kStageBytes;
+        const ptx::DescHalves a = ptx::make_desc_halves_sw128(x, 16, 1024), b = ptx::make_desc_halves_sw128(x + 128 * 128, 16, 1024);
+        if (!wait(s_full[st.at], st.parity, kGiveUpFull)) break;
+        if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
+        ptx::tc_fence_after();
+        ptx::mma_f8_ss_x4_pair_w(el, tmem + buf.at * 256, a, b, idesc);
+        ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_tfull[buf.at]));
+        ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_empty[st.at]));
+        last = st.at;
+        last_parity = st.parity;
+      }
+      if (i > 0) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int row = (int)rank * 128 + (warp & 3) * 32 + lane, half = (warp - 4) >> 2;
+    const uint32_t at_tmem = tmem + ((uint32_t)(warp & 3) << 21) + half * 128;
+    const uint32_t tempty[2] = {ptx::cluster_map(ptx::smem_u32(&s_tempty[0]), 0), ptx::cluster_map(ptx::smem_u32(&s_tempty[1]), 0)};
+    constexpr int kWords = 32 / sizeof(Out);  // columns a 32-byte store takes
+    const bool aligned = ((reinterpret_cast<uintptr_t>(g.out) | (uintptr_t)(g.ld_out * (int64_t)sizeof(Out))) & 31) == 0;
+    Ring<2> buf;
+    for (uint32_t t = pair; t < tiles; t += pairs) {
+      const Tile at = tile_at(t, tiles_n, tiles_m);
+      const int64_t m = at.m0 + row;
+      const int n0 = at.n0 + half * 128;
+      const bool mine = m < g.M && n0 < g.N;
+      const S* pa = static_cast<const S*>(g.sa) + m * g.sa_m;
+      const S* pb = static_cast<const S*>(g.sb) + (int64_t)(n0 / 128) * g.sb_n;
+      const auto scales_of = [&](int kb) {
+        Scales<S> v = {};
+        if (mine && kb < g.KB) v = {pa[kb * g.sa_k], pb[kb * g.sb_k]};
+        return v;
+      };
+      float2 acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.f, 0.f);
+      Scales<S> now = scales_of(0), next = scales_of(1);
+#pragma unroll 1
+      for (int kb = 0; kb < g.KB; ++kb, buf.step()) {
+        const Scales<S> after = scales_of(kb + 2);
+        wait(s_tfull[buf.at], buf.parity, kGiveUpTmemFull);
+        __syncwarp();
+        ptx::tc_fence_after();
+        const uint32_t from = at_tmem + buf.at * 256;
+        uint32_t r0[32], r1[32];
+        float2 s2;
+        const auto add = [&](int c, const uint32_t (&r)[32]) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[c * 16 + j] = ptx::ffma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[c * 16 + j]);
+        };
+        ptx::tmem_ld32(from, r0);
+        ptx::tmem_ld32(from + 32, r1);
+        s2.x = s2.y = now.product();
+        ptx::tmem_ld_wait();
+        add(0, r0);
+        ptx::tmem_ld32(from + 64, r0);
+        add(1, r1);
+        ptx::tmem_ld32(from + 96, r1);
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(tempty[buf.at]);
+        add(2, r0);
+        add(3, r1);
+        now = next;
+        next = after;
+      }
+      if (*dead) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j].x = acc[j].y = __uint_as_float(0x7fffffffu);
+      }
+      if (!mine) continue;
+      Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n0;
+      const int width = min(g.N - n0, 128);
+#pragma unroll
+      for (int c = 0; c < 128; c += kWords) {
+        if (aligned && c + kWords <= width) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (sizeof(Out) == 2) w[j] = ptx::pack_bf16(acc[c / 2 + j].x, acc[c / 2 + j].y);
+            else w[j] = __float_as_uint(j & 1 ? acc[c / 2 + j / 2].y : acc[c / 2 + j / 2].x);
+          }
+          store32(out + c, w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kWords; ++j)
+            if (c + j < width) out[c + j] = from_f32<Out>(j & 1 ? acc[(c + j) / 2].y : acc[(c + j) / 2].x);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();  // neither CTA's memory goes while the other's products or barriers use it
+  ptx::tc_fence_after();
+  if (warp == 1) ptx::tmem_dealloc_pair(tmem, 512);
+}
+
+template <typename Out, typename S>
+int run_many(const CUtensorMap& map_w, const CUtensorMap& map_x, const MatmulArgs& g, cudaStream_t s) {
+  const int64_t tiles = (int64_t)((g.N + 255) / 256) * ((g.M + 255) / 256);
+  const int64_t pairs = device_sm_count() / 2;
+  if (tiles * g.KB > 0x7fffffff) {
+    set_error("mvpa_matmul_fp8: more than 2^31 blocks of 256 x 256 x 128");
+    return MVPA_ERR_UNSUPPORTED;
+  }
+  constexpr auto kernel = matmul_many_kernel<Out, S>;
+  MVPA_CUDA_CHECK(grant_smem<kernel>(ManyRows::kSmem));
+  MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kManyThreads, ManyRows::kSmem, s, map_w,
+                                   map_x, g));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
@@ -249,6 +511,12 @@ int encode_bytes(CUtensorMap* map, const void* base, int64_t rows, int64_t width
 
 template <typename Out, typename S>
 int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
+  if (g.M > 256) {
+    CUtensorMap map_w, map_x;
+    int rc = encode_bytes(&map_w, b, g.N, K, ld_b, 128);
+    if (rc == MVPA_OK) rc = encode_bytes(&map_x, a, g.M, K, ld_a, 128);
+    return rc == MVPA_OK ? run_many<Out, S>(map_w, map_x, g, s) : rc;
+  }
   const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   CUtensorMap map_w, map_x;
   int rc = encode_bytes(&map_w, b, g.N, K, ld_b, 128);

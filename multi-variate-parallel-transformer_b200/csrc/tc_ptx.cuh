@@ -354,6 +354,69 @@ __device__ __forceinline__ void mma_f8_ss_x4_w(uint32_t el, uint32_t d_tmem, Des
       "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el)
       : "memory");
 }
+// ---- pairs: one product over two CTAs of a cluster (cta_group::2), issued by the CTA of rank 0 ----
+// M = 256: each CTA stages its 128 rows of A and its half of B's rows, and holds its 128 rows of D in its own TMEM.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_map(uint32_t smem_addr, uint32_t rank) {  // the same place in another CTA
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// (`bar` from cluster_map.  Release at the scope of the CTA, as in mbar_arrive: what the arrival orders is TMEM, by
+// tc_fence_before.  At the scope of the cluster it is a fence that waits for every load and store of the thread: the 8-bit
+// product, which arrives once a block, ran at 984 instead of over 2000 TFLOP/s.)
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t ncols) {  // one full warp of each CTA
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// A load into this CTA's shared memory that counts at a barrier of either CTA of the pair (`bar` from cluster_map).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_pair_w(uint32_t el, uint32_t bar) {  // the barrier of this place in both CTAs
+  asm volatile(
+      "{\n\t.reg .pred pe;\n\t.reg .b16 both;\n\tsetp.ne.b32 pe, %1, 0;\n\tmov.b16 both, 3;\n\t"
+      "@pe tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar),
+      "r"(el)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f8_ss_x4_pair_w(uint32_t el, uint32_t d_tmem, DescHalves a, DescHalves b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p0, p1, pe;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+      "setp.ne.b32 p0, 0, 0;\n\t"
+      "setp.eq.b32 p1, 0, 0;\n\t"
+      "setp.ne.b32 pe, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t mov.b64 db, {%3, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p0;\n\t"
+      "add.u32 la, %1, 2;\n\t add.u32 lb, %3, 2;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p1;\n\t"
+      "add.u32 la, %1, 4;\n\t add.u32 lb, %3, 4;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p1;\n\t"
+      "add.u32 la, %1, 6;\n\t add.u32 lb, %3, 6;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p1;\n\t}" ::"r"(d_tmem),
+      "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el)
+      : "memory");
+}
 __device__ __forceinline__ void mma_ts_w(uint32_t el, uint32_t d_tmem, uint32_t a_tmem, DescHalves b,
                                          uint32_t b_off_bytes, uint32_t idesc, uint32_t accumulate) {
   asm volatile(

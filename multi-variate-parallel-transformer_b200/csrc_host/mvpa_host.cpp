@@ -43,6 +43,10 @@ struct Api {
   decltype(&mvpa_workspace_status) fwd_status;
   decltype(&mvpa_bwd_status) bwd_status;
   decltype(&mvpa_last_error_string) last_error;
+  decltype(&mvpa_quantize_fp8) quantize_fp8;
+  decltype(&mvpa_rmsnorm_fp8) rmsnorm_fp8;
+  decltype(&mvpa_silu_mul_fp8) silu_mul_fp8;
+  decltype(&mvpa_matmul_fp8) matmul_fp8;
 } api;
 
 PyObject* device_mode = nullptr;  // torch.utils._device.DeviceContext
@@ -528,6 +532,141 @@ PyObject* branches(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the block in 8 bits (`mvpa_ops.quantize_fp8` and its neighbours): ordinary calls; anything else is answered None, and the Python
+// ---- path serves or refuses it ----
+
+constexpr int64_t kFp8Block = 128;
+int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+// Tensors on one device that nothing watches and no gradient has to flow through.
+bool fp8_inputs(std::initializer_list<const Tensor*> ts) {
+  const Tensor& t0 = **ts.begin();
+  const bool grad = c10::GradMode::is_enabled();
+  for (const Tensor* t : ts)
+    if (t->defined() && (!ordinary(*t) || t->device() != t0.device() || (grad && t->requires_grad()))) return false;
+  return !function_modes() && !watched();
+}
+// A matrix with at least one element, unit inner stride and rows that do not overlap; -> its leading dimension, or 0.
+int64_t matrix_ld(const Tensor& t) {
+  if (t.dim() != 2 || t.numel() == 0 || (t.stride(1) != 1 && t.size(1) > 1)) return 0;
+  if (t.size(0) < 2) return (t.size(1) + 15) / 16 * 16;
+  return t.stride(0) < t.size(1) ? 0 : t.stride(0);
+}
+bool bf16_or_fp32(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
+
+struct Pair {
+  Tensor q, scales;
+  int64_t ld;
+  Pair(int64_t rows, int64_t width, int64_t tall, const Tensor& like) {
+    ld = (width + 15) / 16 * 16;
+    const auto options = like.options().requires_grad(false);
+    q = at::empty({rows, ld}, options.dtype(at::kFloat8_e4m3fn));
+    if (ld != width) q = q.narrow(1, 0, width);
+    scales = at::empty({(rows + tall - 1) / tall, blocks_of(width)}, options.dtype(at::kFloat8_e8m0fnu));
+  }
+};
+
+bool take(PyObject* a, Tensor& t) {  // (None leaves the tensor undefined)
+  if (a == Py_None) return true;
+  if (!THPVariable_CheckExact(a)) return false;
+  t = THPVariable_Unpack(a);
+  return true;
+}
+
+// quantize_fp8(x, block_rows) -> (q, scales) or None
+PyObject* quantize_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 2)) return nullptr;
+  Tensor x;
+  if (a[0] == Py_None || !take(a[0], x) || !PyLong_CheckExact(a[1])) Py_RETURN_NONE;
+  const int64_t tall = PyLong_AsLongLong(a[1]);
+  if (PyErr_Occurred()) return nullptr;
+  if ((tall != 1 && tall != kFp8Block) || !fp8_inputs({&x}) || !bf16_or_fp32(x)) Py_RETURN_NONE;
+  const int64_t ld = matrix_ld(x);
+  if (ld == 0 || x.size(1) > INT32_MAX) Py_RETURN_NONE;
+  std::optional<Body> body(std::in_place, x);
+  Pair out(x.size(0), x.size(1), tall, x);
+  check(api.quantize_fp8(x.const_data_ptr(), ld, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.scales.size(1), x.size(0),
+                         (int32_t)x.size(1), (int32_t)tall, dtype_code(x), stream_of(x)), "mvpa_quantize_fp8");
+  body.reset();  // (the interpreter is wanted again)
+  return wrap({std::move(out.q), std::move(out.scales)});
+  END_HANDLE_TH_ERRORS
+}
+
+// rmsnorm_fp8(x, weight, eps, add or None, sum_out or None) -> (q, scales) or None
+PyObject* rmsnorm_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 5)) return nullptr;
+  Tensor x, w, add, sum;
+  if (a[0] == Py_None || a[1] == Py_None || !take(a[0], x) || !take(a[1], w) || !PyFloat_Check(a[2]) || !take(a[3], add) || !take(a[4], sum))
+    Py_RETURN_NONE;
+  if (!fp8_inputs({&x, &w, &add, &sum}) || !bf16_or_fp32(x) || x.dim() < 1 || x.numel() == 0) Py_RETURN_NONE;
+  const int64_t E = x.size(-1);
+  for (const Tensor* t : {&x, &w, &add, &sum})
+    if (t->defined() && (!t->is_contiguous() || t->scalar_type() != x.scalar_type())) Py_RETURN_NONE;
+  for (const Tensor* t : {&add, &sum})
+    if (t->defined() && (t->numel() != x.numel() || t->dim() < 1 || t->size(-1) != E)) Py_RETURN_NONE;
+  if (w.dim() != 1 || w.size(0) != E || E > 4096) Py_RETURN_NONE;
+  std::optional<Body> body(std::in_place, x);
+  Pair out(x.numel() / E, E, 1, x);
+  check(api.rmsnorm_fp8(x.const_data_ptr(), add.defined() ? add.const_data_ptr() : nullptr, w.const_data_ptr(),
+                        sum.defined() ? sum.data_ptr() : nullptr, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.scales.size(1),
+                        x.numel() / E, (int32_t)E, (float)PyFloat_AS_DOUBLE(a[2]), dtype_code(x), stream_of(x)), "mvpa_rmsnorm_fp8");
+  body.reset();  // (the interpreter is wanted again)
+  return wrap({std::move(out.q), std::move(out.scales)});
+  END_HANDLE_TH_ERRORS
+}
+
+// silu_mul_fp8(gate, up) -> (q, scales) or None
+PyObject* silu_mul_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 2)) return nullptr;
+  Tensor g, u;
+  if (a[0] == Py_None || a[1] == Py_None || !take(a[0], g) || !take(a[1], u) || !fp8_inputs({&g, &u}) || !bf16_or_fp32(g)) Py_RETURN_NONE;
+  const int64_t ld = matrix_ld(g);
+  if (ld == 0 || matrix_ld(u) != ld || u.sizes() != g.sizes() || u.scalar_type() != g.scalar_type() || g.size(1) > INT32_MAX) Py_RETURN_NONE;
+  std::optional<Body> body(std::in_place, g);
+  Pair out(g.size(0), g.size(1), 1, g);
+  check(api.silu_mul_fp8(g.const_data_ptr(), u.const_data_ptr(), ld, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.scales.size(1),
+                         g.size(0), (int32_t)g.size(1), dtype_code(g), stream_of(g)), "mvpa_silu_mul_fp8");
+  body.reset();  // (the interpreter is wanted again)
+  return wrap({std::move(out.q), std::move(out.scales)});
+  END_HANDLE_TH_ERRORS
+}
+
+// matmul_fp8(a, a_scales, b, b_scales, out or None, out is fp32, status) -> out or None
+PyObject* matmul_fp8(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 7)) return nullptr;
+  const bool status = p[6] == Py_True;
+  Tensor a, sa, b, sb, out;
+  if (p[0] == Py_None || p[1] == Py_None || p[2] == Py_None || p[3] == Py_None || !take(p[0], a) || !take(p[1], sa) || !take(p[2], b) ||
+      !take(p[3], sb) || !take(p[4], out) || !fp8_inputs({&a, &sa, &b, &sb, &out}))
+    Py_RETURN_NONE;
+  const int64_t ld_a = matrix_ld(a), ld_b = matrix_ld(b);
+  const bool exponents = sa.scalar_type() == at::kFloat8_e8m0fnu;
+  if (ld_a == 0 || ld_b == 0 || a.scalar_type() != at::kFloat8_e4m3fn || b.scalar_type() != at::kFloat8_e4m3fn ||
+      sa.scalar_type() != sb.scalar_type() || (!exponents && sa.scalar_type() != at::kFloat))
+    Py_RETURN_NONE;
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0), KB = blocks_of(K);
+  if (b.size(1) != K || sa.sizes() != at::IntArrayRef({M, KB}) || sb.sizes() != at::IntArrayRef({blocks_of(N), KB}) || N > INT32_MAX ||
+      K > INT32_MAX || (out.defined() && (out.sizes() != at::IntArrayRef({M, N}) || !bf16_or_fp32(out) || matrix_ld(out) == 0)))
+    Py_RETURN_NONE;
+  {
+    const Body body(a);
+    if (!out.defined())
+      out = at::empty({M, N}, a.options().dtype(p[5] == Py_True ? at::kFloat : at::kBFloat16).requires_grad(false));
+    const Tensor word = status ? at::zeros({64}, a.options().dtype(at::kInt).requires_grad(false)) : Tensor();
+    int32_t* w = status ? word.data_ptr<int32_t>() : nullptr;
+    check(api.matmul_fp8(a.const_data_ptr(), ld_a, sa.const_data_ptr(), sa.stride(0), sa.stride(1), b.const_data_ptr(), ld_b,
+                         sb.const_data_ptr(), sb.stride(0), sb.stride(1), exponents ? MVPA_E8M0 : MVPA_F32, out.data_ptr(), matrix_ld(out),
+                         M, (int32_t)N, (int32_t)K, dtype_code(out), w, stream_of(a)), "mvpa_matmul_fp8");
+    if (status) check(api.fwd_status(w, 256, stream_of(a)), "mvpa_matmul_fp8 kernel");  // synchronises the stream
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // init(path of libmvpa_b200.so, which is already loaded; the class of the mode that a default device is)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 2)) return nullptr;
@@ -549,13 +688,16 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(api.silu_mul, "mvpa_silu_mul"); get(api.silu_mul_bwd, "mvpa_silu_mul_bwd");
   get(api.fwd_status, "mvpa_workspace_status"); get(api.bwd_status, "mvpa_bwd_status");
   get(api.last_error, "mvpa_last_error_string");
+  get(api.quantize_fp8, "mvpa_quantize_fp8"); get(api.rmsnorm_fp8, "mvpa_rmsnorm_fp8");
+  get(api.silu_mul_fp8, "mvpa_silu_mul_fp8"); get(api.matmul_fp8, "mvpa_matmul_fp8");
   if (missing) { PyErr_Format(PyExc_ImportError, "%s has no %s", p, missing); return nullptr; }
   Py_RETURN_NONE;
 }
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init), FAST(attend), FAST(forward), FAST(backward), FAST(plain), FAST(block_forward),
-                         FAST(block_backward), FAST(branches), {nullptr, nullptr, 0, nullptr}};
+                         FAST(block_backward), FAST(branches), FAST(quantize_fp8), FAST(rmsnorm_fp8), FAST(silu_mul_fp8),
+                         FAST(matmul_fp8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "mvpa_host_b200", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

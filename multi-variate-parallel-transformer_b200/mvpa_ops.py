@@ -316,6 +316,10 @@ def quantize_fp8(x, block_rows=1, out=None):
     """x (rows, width), bf16 or fp32, in 8 bits: (q, scales).  `block_rows=1` gives every row its own scales (activations),
     `block_rows=128` every block of 128 x 128 one (weights).  `out=(q, scales)` writes into the caller's tensors, which may be
     column blocks of wider ones."""
+    if out is None and _host.usable(x):
+        pair = _host.module().quantize_fp8(x, block_rows)
+        if pair is not None:
+            return pair
     _fp8_inputs("quantize_fp8", x)
     if block_rows not in (1, FP8_BLOCK):
         raise RuntimeError(f"quantize_fp8: block_rows is 1 or {FP8_BLOCK}, got {block_rows}")
@@ -334,6 +338,10 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None):
     """`rmsnorm` with the result in 8 bits: (q, scales) of rmsnorm(h) * weight, h = x (+ add), for x (..., E) with all leading
     dimensions as rows.  h is rounded to x's type, as in `rmsnorm`, and written to `sum_out` (which may be `x`); the normalised
     row goes from fp32 to e4m3 in one rounding.  E up to 4096 in bf16, 2048 in fp32."""
+    if out is None and _host.usable(x):
+        pair = _host.module().rmsnorm_fp8(x, weight, eps, add, sum_out)
+        if pair is not None:
+            return pair
     extra = [t for t in (add, sum_out) if t is not None]
     _fp8_inputs("rmsnorm_fp8", x, weight, *extra)
     E = x.shape[-1]
@@ -356,6 +364,10 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None):
 def silu_mul_fp8(gate, up, out=None):
     """silu(gate) * up in 8 bits: (q, scales).  gate, up (rows, width) with unit inner stride (column blocks of a wider buffer
     are fine).  From fp32 to e4m3 in one rounding; `silu_mul` rounds silu(gate) to the type in between, as eager PyTorch does."""
+    if out is None and _host.usable(gate):
+        pair = _host.module().silu_mul_fp8(gate, up)
+        if pair is not None:
+            return pair
     _fp8_inputs("silu_mul_fp8", gate, up)
     ld = _fp8_rows("silu_mul_fp8", gate, "gate")
     if up.shape != gate.shape or up.dtype != gate.dtype or _fp8_rows("silu_mul_fp8", up, "up") != ld:
@@ -376,6 +388,10 @@ def matmul_fp8(a, a_scales, b, b_scales, out=None, dtype=torch.bfloat16):
     (ceil(N / 128), ceil(K / 128)); the result (M, N) in `dtype` (bfloat16 or float32), or in `out`, which may be a column
     block of a wider buffer.  The scales are both float8_e8m0fnu, as the functions above write them, or both float32, with any
     strides.  Products and sums are in fp32, rounded once."""
+    if (out is not None or dtype is torch.bfloat16 or dtype is torch.float32) and _host.usable(a):
+        done = _host.module().matmul_fp8(a, a_scales, b, b_scales, out, dtype is torch.float32, _attn._CHECK_STATUS)
+        if done is not None:
+            return done if out is None else out
     what = "matmul_fp8"
     _fp8_inputs(what, a, a_scales, b, b_scales)
     ld_a, ld_b = _fp8_rows(what, a, "a"), _fp8_rows(what, b, "b")
