@@ -48,26 +48,92 @@ __device__ __forceinline__ uint32_t max8(uint32_t v) {
 
 constexpr int kLane = 16;  // values a lane holds of a block: 16 bytes of e4m3, one store
 
-// Sixteen values of a row from column `col`, zeros past `width`.  VEC: base and rows on 16-byte boundaries.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* __restrict__ row, int col, int width, float (&y)[kLane]) {
-  constexpr int N = Vec<T>::N;
-  if (VEC && col + kLane <= width) {
-    uint4 raw[kLane / N];
+// A lane's sixteen values of its block where rows start on 16-byte boundaries: as they lie in memory.
+template <typename T>
+struct Raw {
+  static constexpr int kWords = kLane / Vec<T>::N;
+  uint4 w[kWords];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int col, int width) {
+    if (col + kLane <= width) {
 #pragma unroll
-    for (int i = 0; i < kLane / N; ++i) raw[i] = *reinterpret_cast<const uint4*>(row + col + i * N);
+      for (int i = 0; i < kWords; ++i) w[i] = *reinterpret_cast<const uint4*>(row + col + i * Vec<T>::N);
+    } else {
+      float y[kLane];
 #pragma unroll
-    for (int i = 0; i < kLane / N; ++i) {
-      float f[N];
-      Vec<T>::unpack(raw[i], f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) y[i * N + e] = f[e];
+      for (int e = 0; e < kLane; ++e) y[e] = col + e < width ? to_f32<T>(row[col + e]) : 0.f;
+      pack(y);
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kLane; ++e) y[e] = col + e < width ? to_f32<T>(row[col + e]) : 0.f;
   }
-}
+  __device__ __forceinline__ void pack(const float (&y)[kLane]) {  // (values of T)
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      float f[Vec<T>::N];
+#pragma unroll
+      for (int e = 0; e < Vec<T>::N; ++e) f[e] = y[i * Vec<T>::N + e];
+      w[i] = Vec<T>::pack(f);
+    }
+  }
+  __device__ __forceinline__ void get(float (&y)[kLane]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      float f[Vec<T>::N];
+      Vec<T>::unpack(w[i], f);
+#pragma unroll
+      for (int e = 0; e < Vec<T>::N; ++e) y[i * Vec<T>::N + e] = f[e];
+    }
+  }
+  __device__ __forceinline__ void store(T* __restrict__ row, int col, int width) const {
+    if (col + kLane <= width) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4*>(row + col + i * Vec<T>::N) = w[i];
+    } else {
+      float y[kLane];
+      get(y);
+#pragma unroll
+      for (int e = 0; e < kLane; ++e)
+        if (col + e < width) row[col + e] = from_f32<T>(y[e]);
+    }
+  }
+};
+
+// Rows at any alignment: the eight lanes of a block read it eight neighbours at a time - whole sectors, where sixteen single
+// loads a lane would touch each sector again and again (2500 x 1027 in fp32 with the residual: 34 us so, 13 in this way) - and
+// pass it on through shared memory.  A warp's four blocks lie kTurn floats apart and the values of a lane 17: no two lanes of a
+// warp meet in a bank.
+constexpr int kTurn = kBlock + kBlock / kLane;
+struct Turn {
+  float* s;  // of this lane's block; 4 * kTurn floats a warp
+  int l;
+  __device__ __forceinline__ Turn(float* warp_s, int lane) : s(warp_s + (lane >> 3) * kTurn), l(lane & 7) {}
+  // (every lane of the warp takes part; `any`: this lane's block exists)
+  template <typename T>
+  __device__ __forceinline__ void load(const T* __restrict__ row, int block_col, int width, bool any, float (&y)[kLane]) const {
+    T v[kLane];
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      const int c = block_col + j * 8 + l;
+      v[j] = any && c < width ? row[c] : from_f32<T>(0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) s[j * 8 + l + (j >> 1)] = to_f32<T>(v[j]);
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) y[e] = s[l * (kLane + 1) + e];
+    __syncwarp();
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* __restrict__ row, int block_col, int width, bool any, const float (&y)[kLane]) const {
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) s[l * (kLane + 1) + e] = y[e];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      const int c = block_col + j * 8 + l;
+      if (any && c < width) row[c] = from_f32<T>(s[j * 8 + l + (j >> 1)]);
+    }
+    __syncwarp();
+  }
+};
 
 // Sixteen values in e4m3 to a row whose start is on a 16-byte boundary; nothing past `width` is written.
 __device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int width, const float (&y)[kLane], float inverse) {
@@ -84,11 +150,10 @@ __device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int 
   }
 }
 
-template <int N>
-__device__ __forceinline__ uint32_t top_of(const float (&y)[N]) {
+__device__ __forceinline__ uint32_t top_of(const float (&y)[kLane]) {
   uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < N; ++e) top = max(top, magnitude(y[e]));
+  for (int e = 0; e < kLane; ++e) top = max(top, magnitude(y[e]));
   return top;
 }
 

@@ -42,15 +42,46 @@ __device__ __forceinline__ void write_unit(const Unit& t, const float (&y)[kLane
   if ((threadIdx.x & 7) == 0) scales[t.row * ld_s + t.block] = (uint8_t)byte;
 }
 
+// A lane's values of one block.
+template <typename T, bool VEC>
+__device__ __forceinline__ void read_unit(const T* __restrict__ x, int64_t ld, const Unit& t, int width, float (&y)[kLane]) {
+  if constexpr (VEC) {
+    Raw<T> raw = {};
+    if (t.any && t.col < width) raw.load(x + t.row * ld, t.col, width);
+    raw.get(y);
+  } else {
+    __shared__ float s_turn[kThreads / 32][4 * kTurn];
+    Turn(s_turn[threadIdx.x / 32], threadIdx.x & 31).load(x + t.row * ld, t.block * kBlock, width, t.any, y);
+  }
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, int64_t ld_x, uint8_t* __restrict__ q,
                                                                  int64_t ld_q, uint8_t* __restrict__ scales, int64_t ld_s,
                                                                  int64_t rows, int width) {
   ptx::griddep_wait();
   const Unit t = unit_of(rows, width);
-  float y[kLane] = {};
-  if (t.any) load16<T, VEC>(x + t.row * ld_x, t.col, width, y);
+  float y[kLane];
+  read_unit<T, VEC>(x, ld_x, t, width, y);
   write_unit(t, y, q, ld_q, scales, ld_s, width);
+}
+
+__device__ __forceinline__ float reciprocal(float d) {  // of 1 <= d <= 2: an estimate and one step of Newton's
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return fmaf(r, fmaf(-d, r, 1.f), r);
+}
+
+// silu(g) = g / (1 + e^-g), from e = e^-|g| <= 1 so that nothing overflows: 1 / (1 + e) of g, or e / (1 + e) where g < 0.
+// e = 2^(-|g| log2 e): the product in two parts, since 2^x turns an error of x into a relative one (log2 e = kHi + kLo), and
+// 2^(hi + lo) = 2^hi (1 + lo ln 2) as |lo| < 2^-16.  (Past 200 e is zero in fp32; the bound keeps the products finite.)
+__device__ __forceinline__ float silu(float g) {
+  constexpr float kHi = 1.44269504f, kLo = 1.92596299e-8f, kLn2 = 0.693147181f;
+  const float a = fminf(fabsf(g), 200.f), hi = -a * kHi, lo = fmaf(-a, kLo, fmaf(-a, kHi, -hi));
+  float p;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(hi));
+  const float e = fmaf(p, lo * kLn2, p);
+  return g * ((g < 0.f ? e : 1.f) * reciprocal(1.f + e));
 }
 
 // silu(gate) * up, in fp32 from the inputs to the step to e4m3.
@@ -60,13 +91,11 @@ __global__ void __launch_bounds__(kThreads) silu_mul_fp8_kernel(const T* __restr
                                                                 int64_t ld_s, int64_t rows, int width) {
   ptx::griddep_wait();
   const Unit t = unit_of(rows, width);
-  float y[kLane] = {}, u[kLane] = {};
-  if (t.any) {
-    load16<T, VEC>(gate + t.row * ld_in, t.col, width, y);
-    load16<T, VEC>(up + t.row * ld_in, t.col, width, u);
-  }
+  float y[kLane], u[kLane];
+  read_unit<T, VEC>(gate, ld_in, t, width, y);
+  read_unit<T, VEC>(up, ld_in, t, width, u);
 #pragma unroll
-  for (int e = 0; e < kLane; ++e) y[e] = y[e] / (1.f + expf(-y[e])) * u[e];
+  for (int e = 0; e < kLane; ++e) y[e] = silu(y[e]) * u[e];
   write_unit(t, y, q, ld_q, scales, ld_s, width);
 }
 
@@ -79,14 +108,17 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const T* __re
   constexpr int kTimes = kBlock / (kThreads / 8);
   __shared__ uint32_t s_top[kThreads / 32];
   ptx::griddep_wait();
-  const int col = blockIdx.x * kBlock + (threadIdx.x & 7) * kLane;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock + threadIdx.x / 8;
-  float y[kTimes][kLane] = {};
+  Unit t[kTimes];
+  float y[kTimes][kLane];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
-    const int64_t row = row0 + i * (kThreads / 8);
-    if (row < rows) load16<T, VEC>(x + row * ld_x, col, width, y[i]);
+    t[i].row = row0 + i * (kThreads / 8);
+    t[i].block = blockIdx.x;
+    t[i].col = blockIdx.x * kBlock + (threadIdx.x & 7) * kLane;
+    t[i].any = t[i].row < rows;
+    read_unit<T, VEC>(x, ld_x, t[i], width, y[i]);
   }
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) top = max(top, top_of(y[i]));
@@ -97,77 +129,95 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const T* __re
   for (int i = 0; i < kThreads / 32; ++i) top = max(top, s_top[i]);
   const uint32_t byte = scale_byte(top);
 #pragma unroll
-  for (int i = 0; i < kTimes; ++i) {
-    const int64_t row = row0 + i * (kThreads / 8);
-    if (row < rows && col < width) store16(q + row * ld_q, col, width, y[i], inverse_scale(byte));
-  }
+  for (int i = 0; i < kTimes; ++i)
+    if (t[i].any && t[i].col < width) store16(q + t[i].row * ld_q, t[i].col, width, y[i], inverse_scale(byte));
   if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * ld_s + blockIdx.x] = (uint8_t)byte;
 }
 
 // y = rmsnorm(h) * w with h = x (+ a, in T as in rmsnorm_kernel); h written out, y to e4m3 without a rounding in between.  One
-// warp per row, NV times sixteen values a lane, which stay in registers in T.
+// warp per row, NV times sixteen values a lane, which stay in registers in T between the sum of squares and the scaling; all
+// loads of a row are on their way before the first is used.
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(kWarpsPerCta * 32) rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ a,
                                                                         const T* __restrict__ w, T* __restrict__ h_out,
                                                                         uint8_t* __restrict__ q, int64_t ld_q,
                                                                         uint8_t* __restrict__ scales, int64_t ld_s, int64_t rows,
                                                                         int E, float eps) {
-  constexpr int N = Vec<T>::N, P = kLane / N;
+  __shared__ float s_turn[VEC ? 1 : kWarpsPerCta][VEC ? 1 : 4 * kTurn];
   ptx::griddep_wait();
   const int64_t row = (int64_t)blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const int64_t at = row * E;
-  uint4 raw[NV][P];
+  const Turn turn(s_turn[VEC ? 0 : threadIdx.x >> 5], lane);
+  const auto col_of = [&](int i) { return (i * 32 + lane) * kLane; };
+  const auto block_of = [&](int i) { return (i * 4 + (lane >> 3)) * kBlock; };
+  Raw<T> raw[NV] = {};
   float ss = 0.f;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (col_of(i) < E) raw[i].load(x + at, col_of(i), E);
+    if (a != nullptr) {
+      Raw<T> more[NV] = {};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (col_of(i) < E) more[i].load(a + at, col_of(i), E);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float v[kLane], b[kLane];
+        raw[i].get(v);
+        more[i].get(b);
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) v[e] += b[e];
+        raw[i].pack(v);  // (rounds to T)
+        if (h_out != nullptr && col_of(i) < E) raw[i].store(h_out + at, col_of(i), E);
+      }
+    } else if (h_out != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (col_of(i) < E) raw[i].store(h_out + at, col_of(i), E);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i * 32 * kLane >= E) break;  // (the same for the whole warp)
+      const bool any = block_of(i) < E;
+      float v[kLane], b[kLane];
+      turn.load(x + at, block_of(i), E, any, v);
+      if (a != nullptr) {
+        turn.load(a + at, block_of(i), E, any, b);
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) v[e] += b[e];
+      }
+      raw[i].pack(v);
+      raw[i].get(v);
+      if (h_out != nullptr) turn.store(h_out + at, block_of(i), E, any, v);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int col = (i * 32 + lane) * kLane;
-    float v[kLane] = {};
-    if (col < E) load16<T, VEC>(x + at, col, E, v);
-    if (a != nullptr && col < E) {
-      float b[kLane];
-      load16<T, VEC>(a + at, col, E, b);
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) v[e] = Vec<T>::round(v[e] + b[e]);
-    }
+    float v[kLane];
+    raw[i].get(v);
 #pragma unroll
     for (int e = 0; e < kLane; ++e) ss = fmaf(v[e], v[e], ss);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      float f[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = v[p * N + e];
-      raw[i][p] = Vec<T>::pack(f);
-    }
-    if (h_out != nullptr && col < E) {
-      if (VEC && col + kLane <= E) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(h_out + at + col + p * N) = raw[i][p];
-      } else {
-#pragma unroll
-        for (int e = 0; e < kLane; ++e)
-          if (col + e < E) h_out[at + col + e] = from_f32<T>(v[e]);
-      }
-    }
   }
   const float rstd = rsqrtf(warp_sum(ss) / (float)E + eps);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int col = (i * 32 + lane) * kLane;
-    if (i * 32 * kLane >= E) break;  // (the same for the whole warp)
-    float y[kLane], g[kLane] = {};
-    if (col < E) load16<T, VEC>(w, col, E, g);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      float f[N];
-      Vec<T>::unpack(raw[i][p], f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) y[p * N + e] = f[e] * rstd * g[p * N + e];
+    if (i * 32 * kLane >= E) break;
+    const int col = col_of(i);
+    float y[kLane], g[kLane];
+    if constexpr (VEC) {
+      Raw<T> gain = {};
+      if (col < E) gain.load(w, col, E);
+      gain.get(g);
+    } else {
+      turn.load(w, block_of(i), E, block_of(i) < E, g);
     }
+    raw[i].get(y);
 #pragma unroll
-    for (int e = 0; e < kLane; ++e)
-      if (col + e >= E) y[e] = 0.f;  // (past the end 0 * rstd would be NaN where rstd is)
+    for (int e = 0; e < kLane; ++e) y[e] = col + e < E ? y[e] * rstd * g[e] : 0.f;  // (past the end 0 * rstd would be NaN where rstd is)
     const uint32_t byte = scale_byte(max8(top_of(y)));
     if (col < E) {
       store16(q + row * ld_q, col, E, y, inverse_scale(byte));
