@@ -30,14 +30,12 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
 }
 
-__device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
-
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
+__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) { return __byte_perm(e4m3x2(a.x, a.y), e4m3x2(b.x, b.y), 0x5410); }
 
 // The largest of the values of eight neighbouring lanes: a block of 128 is eight lanes with sixteen values each.
 __device__ __forceinline__ uint32_t max8(uint32_t v) {
@@ -137,10 +135,11 @@ struct Turn {
 
 // Sixteen values in e4m3 to a row whose start is on a 16-byte boundary; nothing past `width` is written.
 __device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int width, const float (&y)[kLane], float inverse) {
+  const float2 by = make_float2(inverse, inverse);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    w[i] = e4m3x4(y[4 * i] * inverse, y[4 * i + 1] * inverse, y[4 * i + 2] * inverse, y[4 * i + 3] * inverse);
+    w[i] = e4m3x4(ptx::fmul2(make_float2(y[4 * i], y[4 * i + 1]), by), ptx::fmul2(make_float2(y[4 * i + 2], y[4 * i + 3]), by));
   if (col + kLane <= width) {
     *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
@@ -150,11 +149,12 @@ __device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int 
   }
 }
 
+// The largest magnitude's bits; a NaN stays one.
 __device__ __forceinline__ uint32_t top_of(const float (&y)[kLane]) {
-  uint32_t top = 0;
+  float top = fabsf(y[0]);
 #pragma unroll
-  for (int e = 0; e < kLane; ++e) top = max(top, magnitude(y[e]));
-  return top;
+  for (int e = 1; e < kLane; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(y[e])));
+  return __float_as_uint(top);
 }
 
 }  // namespace fp8
