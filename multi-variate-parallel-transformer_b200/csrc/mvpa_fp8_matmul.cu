@@ -19,6 +19,7 @@ struct MatmulArgs {
   void* out;
   int64_t ld_out, M;
   int N, KB, per;  // blocks along K, blocks per split
+  int out_tma;     // out's rows are on 16-byte boundaries
   int* status;
 };
 
@@ -264,19 +265,40 @@ int run_few(const CUtensorMap& map_w, const CUtensorMap& map_x, MatmulArgs g, cu
 // token's 128 columns in registers.
 struct ManyRows {
   static constexpr int kStageBytes = 2 * 128 * 128;
-  static constexpr int kStages = 6;
-  static constexpr size_t kSmem = 1024 + kStages * kStageBytes;
+  static constexpr int kStages = 5;
+  static constexpr int kOutBytes = 8 * 2 * 32 * 128;  // a warp's tokens x 128 bytes of columns, twice
+  static constexpr size_t kSmem = 1024 + kStages * kStageBytes + kOutBytes;
 };
 // Four warps that load and issue, eight that add up.  Registers: 384 x 168 at launch, of which the four keep 56 a thread and the
 // eight take 216 (128 x 56 + 256 x 216 = 62464 of 64512).
 constexpr int kManyThreads = 384;
 
-// Eight 32-bit words to a 32-byte boundary: a whole sector.
-__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
-               "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
+// Results on their way out: a warp puts 32 tokens x 128 bytes of columns into shared memory (in the 128-byte swizzle: a token's
+// 16-byte pieces go to eight different places) and leaves them to the TMA, which writes whole lines, skips what lies past the
+// matrix, and lets the warp go on.  Stored from registers a tile of 256 x 256 held its warps for 4200 cycles of 20000.
+struct OutRing {
+  uint32_t smem;
+  uint32_t which = 0;
+  // Where the next 128 bytes of columns go; the store before the last has been read.
+  __device__ __forceinline__ uint32_t next(int lane) {
+    if (lane == 0) ptx::tma_store_wait_read<1>();
+    __syncwarp();
+    which ^= 1;
+    return smem + which * 4096;
+  }
+  __device__ __forceinline__ static void put(uint32_t at, int lane, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((piece ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+  }
+  __device__ __forceinline__ static void send(uint32_t at, int lane, const CUtensorMap* map, int x, int y) {
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      ptx::tma_store_2d(map, at, x, y);
+      ptx::tma_store_commit();
+    }
+  }
+};
 
 struct Tile {
   int m0, n0;
@@ -303,7 +325,8 @@ struct Ring {
 
 template <typename Out, typename S>
 __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __grid_constant__ CUtensorMap map_w,
-                                                                      const __grid_constant__ CUtensorMap map_x, const MatmulArgs g) {
+                                                                      const __grid_constant__ CUtensorMap map_x,
+                                                                      const __grid_constant__ CUtensorMap map_o, const MatmulArgs g) {
   using C = ManyRows;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2];
@@ -403,8 +426,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     const int row = (int)rank * 128 + (warp & 3) * 32 + lane, half = (warp - 4) >> 2;
     const uint32_t at_tmem = tmem + ((uint32_t)(warp & 3) << 21) + half * 128;
     const uint32_t tempty[2] = {ptx::cluster_map(ptx::smem_u32(&s_tempty[0]), 0), ptx::cluster_map(ptx::smem_u32(&s_tempty[1]), 0)};
-    constexpr int kWords = 32 / sizeof(Out);  // columns a 32-byte store takes
-    const bool aligned = ((reinterpret_cast<uintptr_t>(g.out) | (uintptr_t)(g.ld_out * (int64_t)sizeof(Out))) & 31) == 0;
+    OutRing ring = {stages + C::kStages * C::kStageBytes + (warp - 4) * 8192};
     Ring<2> buf;
     for (uint32_t t = pair; t < tiles; t += pairs) {
       const Tile at = tile_at(t, tiles_n, tiles_m);
@@ -457,26 +479,33 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j].x = acc[j].y = __uint_as_float(0x7fffffffu);
       }
-      if (!mine) continue;
-      Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n0;
-      const int width = min(g.N - n0, 128);
+      if (g.out_tma) {
+        constexpr int kCols = 128 / sizeof(Out);
+        const int y = at.m0 + row - lane;
 #pragma unroll
-      for (int c = 0; c < 128; c += kWords) {
-        if (aligned && c + kWords <= width) {
-          uint32_t w[8];
+        for (int c = 0; c < 128; c += kCols) {
+          if (y >= g.M || n0 + c >= g.N) break;  // (the same for the whole warp: a store does not begin past the matrix)
+          const uint32_t to = ring.next(lane);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if constexpr (sizeof(Out) == 2) w[j] = ptx::pack_bf16(acc[c / 2 + j].x, acc[c / 2 + j].y);
-            else w[j] = __float_as_uint(j & 1 ? acc[c / 2 + j / 2].y : acc[c / 2 + j / 2].x);
+          for (int k = 0; k < 8; ++k) {
+            const float2* v = acc + c / 2 + k * (16 / sizeof(Out) / 2);
+            if constexpr (sizeof(Out) == 2)
+              OutRing::put(to, lane, k, ptx::pack_bf16(v[0].x, v[0].y), ptx::pack_bf16(v[1].x, v[1].y), ptx::pack_bf16(v[2].x, v[2].y),
+                           ptx::pack_bf16(v[3].x, v[3].y));
+            else
+              OutRing::put(to, lane, k, __float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
           }
-          store32(out + c, w);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kWords; ++j)
-            if (c + j < width) out[c + j] = from_f32<Out>(j & 1 ? acc[(c + j) / 2].y : acc[(c + j) / 2].x);
+          OutRing::send(to, lane, &map_o, n0 + c, y);
         }
+      } else if (mine) {
+        Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n0;
+        const int width = min(g.N - n0, 128);
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c < width) out[c] = from_f32<Out>(c & 1 ? acc[c / 2].y : acc[c / 2].x);
       }
     }
+    if (lane == 0) ptx::tma_store_wait_all();
   }
   __syncwarp();
   ptx::tc_fence_before();
@@ -487,17 +516,26 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 }
 
 template <typename Out, typename S>
-int run_many(const CUtensorMap& map_w, const CUtensorMap& map_x, const MatmulArgs& g, cudaStream_t s) {
+int run_many(const CUtensorMap& map_w, const CUtensorMap& map_x, MatmulArgs g, cudaStream_t s) {
   const int64_t tiles = (int64_t)((g.N + 255) / 256) * ((g.M + 255) / 256);
   const int64_t pairs = device_sm_count() / 2;
   if (tiles * g.KB > 0x7fffffff) {
     set_error("mvpa_matmul_fp8: more than 2^31 blocks of 256 x 256 x 128");
     return MVPA_ERR_UNSUPPORTED;
   }
+  CUtensorMap map_o = {};
+  g.out_tma = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ld_out * (int64_t)sizeof(Out) % 16 == 0;
+  if (g.out_tma) {
+    const uint64_t dims[2] = {(uint64_t)g.N, (uint64_t)g.M}, strides[1] = {(uint64_t)g.ld_out * sizeof(Out)};
+    const uint32_t box[2] = {128 / sizeof(Out), 32};
+    const int rc = encode_sw128(&map_o, sizeof(Out) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.out, 2, dims,
+                                strides, box);
+    if (rc != MVPA_OK) return rc;
+  }
   constexpr auto kernel = matmul_many_kernel<Out, S>;
   MVPA_CUDA_CHECK(grant_smem<kernel>(ManyRows::kSmem));
   MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kManyThreads, ManyRows::kSmem, s, map_w,
-                                   map_x, g));
+                                   map_x, map_o, g));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
@@ -567,7 +605,7 @@ extern "C" int mvpa_matmul_fp8(const void* a, int64_t ld_a, const void* a_scales
     set_error("mvpa_matmul_fp8: the scales are NULL or not aligned to their elements");
     return MVPA_ERR_ALIGNMENT;
   }
-  MatmulArgs g = {a_scales, b_scales, a_stride_m, a_stride_k, b_stride_n, b_stride_k, out, ld_out, M, N, (int)(((int64_t)K + 127) / 128), 0, status};
+  MatmulArgs g = {a_scales, b_scales, a_stride_m, a_stride_k, b_stride_n, b_stride_k, out, ld_out, M, N, (int)(((int64_t)K + 127) / 128), 0, 0, status};
   if (out_dtype == MVPA_BF16)
     return scale_dtype == MVPA_E8M0 ? run_matmul<__nv_bfloat16, uint8_t>(a, ld_a, b, ld_b, K, g, s)
                                     : run_matmul<__nv_bfloat16, float>(a, ld_a, b, ld_b, K, g, s);
