@@ -304,11 +304,12 @@ struct Tile {
   int m0, n0;
 };
 // Tiles in bands of eight along M: the pairs at work together share few panels of both operands.
+template <int kTileN>
 __device__ __forceinline__ Tile tile_at(uint32_t t, uint32_t tiles_n, uint32_t tiles_m) {
   constexpr uint32_t kBand = 8;
   const uint32_t band = t / (kBand * tiles_n), rest = t - band * kBand * tiles_n;
   const uint32_t high = min(kBand, tiles_m - band * kBand), n = rest / high;
-  return {(int)((band * kBand + rest - n * high) * 256), (int)(n * 256)};
+  return {(int)((band * kBand + rest - n * high) * 256), (int)(n * kTileN)};
 }
 
 // A place in a ring of N, and the parity of the pass over it.
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
         uint32_t loads = 0;
         bool on = true;
         for (uint32_t t = pair; t < tiles && on; t += pairs) {
-          const Tile at = tile_at(t, tiles_n, tiles_m);
+          const Tile at = tile_at<256>(t, tiles_n, tiles_m);
           const int m = at.m0 + (int)rank * 128, n = at.n0 + (int)rank * 128;
           for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
             if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     OutRing ring = {stages + C::kStages * C::kStageBytes + (warp - 4) * 8192};
     Ring<2> buf;
     for (uint32_t t = pair; t < tiles; t += pairs) {
-      const Tile at = tile_at(t, tiles_n, tiles_m);
+      const Tile at = tile_at<256>(t, tiles_n, tiles_m);
       const int64_t m = at.m0 + row;
       const int n0 = at.n0 + half * 128;
       const bool mine = m < g.M && n0 < g.N;
@@ -515,30 +516,251 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
   if (warp == 1) ptx::tmem_dealloc_pair(tmem, 512);
 }
 
-template <typename Out, typename S>
-int run_many(const CUtensorMap& map_w, const CUtensorMap& map_x, MatmulArgs g, cudaStream_t s) {
-  const int64_t tiles = (int64_t)((g.N + 255) / 256) * ((g.M + 255) / 256);
-  const int64_t pairs = device_sm_count() / 2;
-  if (tiles * g.KB > 0x7fffffff) {
-    set_error("mvpa_matmul_fp8: more than 2^31 blocks of 256 x 256 x 128");
-    return MVPA_ERR_UNSUPPORTED;
+// ---- many rows, scales that are powers of two: the tensor cores apply them -----------------------------------------------------
+// The scales go to TMEM beside the products (kind::mxf8f6f4, which wants one for each 32 along K: a block's serves four times), so
+// a tile's sum stays in TMEM over the whole of K and comes home once.  In matmul_many_kernel a block's product has to be fetched
+// before the block after the next can start - 512 cycles of products, then some 1400 to hear of them, fetch them in both CTAs and
+// say so - which leaves the tensor cores idle half of the time.  Tiles of 256 tokens x 192 weight rows: two of them and the scales
+// of five blocks fill TMEM, so that a tile leaves while the next one is summed.
+//
+// Warps: 0 loads, 1 issues, 2 and 3 lay the scales out in shared memory (tokens, weights), 4 to 7 take the sums home.
+struct ScaledRows {
+  static constexpr int kTileN = 192, kHalfN = kTileN / 2;
+  static constexpr int kStages = 5;
+  static constexpr int kOperandBytes = 128 * 128 + kHalfN * 128;
+  static constexpr int kScaleBytes = 512 + 1024;  // 128 tokens; two groups of 128 weight rows
+  static constexpr int kOutBytes = 4 * 2 * 32 * 128;
+  static constexpr uint32_t kTmemScales = 2 * kTileN, kTmemScaleCols = 16;
+  static constexpr size_t kSmem = 1024 + kStages * (kOperandBytes + kScaleBytes) + kOutBytes;
+  static_assert(kTmemScales + kStages * kTmemScaleCols <= 512 && kOperandBytes % 1024 == 0, "");
+};
+constexpr int kScaledThreads = 256;
+
+template <typename Out>
+__global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                          const __grid_constant__ CUtensorMap map_x,
+                                                                          const __grid_constant__ CUtensorMap map_o, const MatmulArgs g) {
+  using C = ScaledRows;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_dead;
+  const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t outs = stages + C::kStages * C::kOperandBytes, scales = outs + C::kOutBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_rank();
+  const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t tiles_n = (uint32_t)(g.N + C::kTileN - 1) / C::kTileN, tiles_m = (uint32_t)((g.M + 255) / 256), tiles = tiles_n * tiles_m;
+  if (warp == 0) {
+    ptx::prefetch_tensormap(&map_w);
+    ptx::prefetch_tensormap(&map_x);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < C::kStages; ++i) {
+        ptx::mbar_init(&s_full[i], 5);  // the loads of both CTAs, two warps' scales in each
+        ptx::mbar_init(&s_empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(&s_tfull[i], 1);
+        ptx::mbar_init(&s_tempty[i], 8);
+      }
+      ptx::mbar_fence_init();
+      s_dead = 0;
+    }
+    __syncwarp();
+    ptx::tmem_alloc_pair(&s_tmem, 512);
+    ptx::tmem_relinquish_pair();
   }
-  CUtensorMap map_o = {};
-  g.out_tma = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ld_out * (int64_t)sizeof(Out) % 16 == 0;
-  if (g.out_tma) {
-    const uint64_t dims[2] = {(uint64_t)g.N, (uint64_t)g.M}, strides[1] = {(uint64_t)g.ld_out * sizeof(Out)};
-    const uint32_t box[2] = {128 / sizeof(Out), 32};
-    const int rc = encode_sw128(&map_o, sizeof(Out) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.out, 2, dims,
-                                strides, box);
-    if (rc != MVPA_OK) return rc;
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* dead = &s_dead;
+  const auto wait = [&](uint64_t& bar, uint32_t parity, int code) {
+    if (ptx::mbar_test_wait(&bar, parity)) return true;
+    if (*dead) return false;
+    if (ptx::mbar_wait(&bar, parity, g.status, code)) return true;
+    *dead = 1;
+    return false;
+  };
+  ptx::griddep_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring<C::kStages> st;
+      uint32_t loads = 0;
+      bool on = true;
+      for (uint32_t t = pair; t < tiles && on; t += pairs) {
+        const Tile at = tile_at<C::kTileN>(t, tiles_n, tiles_m);
+        const int m = at.m0 + (int)rank * 128, n = at.n0 + (int)rank * C::kHalfN;
+        for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
+          if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
+            on = false;
+            break;
+          }
+          const uint32_t full = ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0), x = stages + st.at * C::kOperandBytes;
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * C::kOperandBytes);  // (the other CTA's loads count here too)
+          ptx::tma_load_2d_pair(x, &map_x, full, kb * 128, m);
+          ptx::tma_load_2d_pair(x + 128 * 128, &map_w, full, kb * 128, n);
+        }
+      }
+      if (rank == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one below)
+        const uint32_t n = min(loads, (uint32_t)C::kStages);
+        for (uint32_t k = loads - n; k != loads; ++k)
+          if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t el = ptx::elect_one();
+      constexpr uint32_t idesc = ptx::make_idesc_e4m3_scaled(256, C::kTileN);
+      Ring<C::kStages> st;
+      Ring<2> buf;
+      uint32_t last = 0, last_parity = 0;
+      bool on = true, any = false;
+      for (uint32_t t = pair; t < tiles && on; t += pairs, buf.step()) {
+        if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
+        ptx::tc_fence_after();
+        for (int kb = 0; kb < g.KB; ++kb, st.step()) {
+          const uint32_t x = stages + st.at * C::kOperandBytes, s = scales + st.at * C::kScaleBytes;
+          const uint32_t sa = tmem + C::kTmemScales + st.at * C::kTmemScaleCols, sb = sa + 4;
+          const ptx::DescHalves a = ptx::make_desc_halves_sw128(x, 16, 1024), b = ptx::make_desc_halves_sw128(x + 128 * 128, 16, 1024);
+          if (!wait(s_full[st.at], st.parity, kGiveUpFull)) {
+            on = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          ptx::tmem_copy_scales_pair_w(el, sa, s);
+          ptx::tmem_copy_scales_pair_w(el, sb, s + 512);
+          ptx::tmem_copy_scales_pair_w(el, sb + 4, s + 1024);
+          ptx::mma_mxf8_ss_x4_pair_w(el, tmem + buf.at * C::kTileN, a, b, idesc, sa, sb, kb > 0);
+          ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_empty[st.at]));
+          last = st.at;
+          last_parity = st.parity;
+          any = true;
+        }
+        if (on) ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_tfull[buf.at]));
+      }
+      if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
+    }
+  } else if (warp < 4) {
+    // Word j of a lane: the scale of row 32 j + lane (four times the byte).  Warp 2: this CTA's 128 tokens; warp 3: the tile's 192
+    // weight rows, whose groups of 32 lie in one block of 128 each (192 and 128 are multiples of 32 and 64).  The bytes of four
+    // blocks are loaded ahead of their use.
+    constexpr int kAhead = 4, kWords = 6;
+    const bool tokens = warp == 2;
+    const int words = tokens ? 4 : kWords;
+    const uint8_t* base = static_cast<const uint8_t*>(tokens ? g.sa : g.sb);
+    const int64_t step_k = tokens ? g.sa_k : g.sb_k;
+    Ring<C::kStages> st;
+    for (uint32_t t = pair; t < tiles; t += pairs) {
+      const Tile at = tile_at<C::kTileN>(t, tiles_n, tiles_m);
+      const uint8_t* row[kWords];
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+        if (tokens) {
+          const int64_t m = at.m0 + (int)rank * 128 + 32 * j + lane;
+          row[j] = j < 4 && m < g.M ? base + m * g.sa_m : nullptr;
+        } else {
+          const int n = at.n0 + 32 * j;
+          row[j] = n < g.N ? base + (int64_t)(n / 128) * g.sb_n : nullptr;
+        }
+      }
+      uint32_t bytes[kAhead][kWords];
+      const auto load = [&](int kb0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int j = 0; j < kWords; ++j)
+            bytes[i][j] = j < words && row[j] != nullptr && kb0 + i < g.KB ? row[j][(kb0 + i) * step_k] : 127u;
+      };
+      load(0);
+      for (int kb0 = 0; kb0 < g.KB; kb0 += kAhead) {
+        uint32_t now[kAhead][kWords];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) now[i][j] = bytes[i][j] * 0x01010101u;
+        load(kb0 + kAhead);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (kb0 + i < g.KB) {
+            wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty);
+            __syncwarp();
+            const uint32_t to = scales + st.at * C::kScaleBytes + (tokens ? 0 : 512) + lane * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(now[i][0]), "r"(now[i][1]), "r"(now[i][2]), "r"(now[i][3])
+                         : "memory");
+            if (!tokens)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512), "r"(now[i][4]), "r"(now[i][5]), "r"(0), "r"(0)
+                           : "memory");
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0));
+            st.step();
+          }
+        }
+      }
+    }
+  } else {
+    const int quad = warp - 4;
+    const uint32_t at_tmem = tmem + ((uint32_t)quad << 21);
+    OutRing ring = {outs + quad * 8192};
+    Ring<2> buf;
+    for (uint32_t t = pair; t < tiles; t += pairs, buf.step()) {
+      const Tile at = tile_at<C::kTileN>(t, tiles_n, tiles_m);
+      wait(s_tfull[buf.at], buf.parity, kGiveUpTmemFull);
+      __syncwarp();
+      ptx::tc_fence_after();
+      const uint32_t from = at_tmem + buf.at * C::kTileN;
+      const int y = at.m0 + (int)rank * 128 + quad * 32;
+      constexpr int kCols = 128 / sizeof(Out);
+#pragma unroll 1
+      for (int c = 0; c < C::kTileN; c += kCols) {
+        uint32_t r[kCols];
+        if constexpr (kCols == 64) ptx::tmem_ld64(from + c, r);
+        else ptx::tmem_ld32(from + c, r);
+        ptx::tmem_ld_wait();
+        if (c + kCols == C::kTileN) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_tempty[buf.at]), 0));
+        }
+        if (*dead) {
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) r[j] = 0x7fffffffu;
+        }
+        if (y >= g.M || at.n0 + c >= g.N) continue;  // (the same for the whole warp: a store does not begin past the matrix)
+        if (g.out_tma) {
+          const uint32_t to = ring.next(lane);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t* v = r + k * (kCols / 8);
+            if constexpr (sizeof(Out) == 2) {
+              const auto two = [&](int i) { return ptx::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])); };
+              OutRing::put(to, lane, k, two(0), two(1), two(2), two(3));
+            } else {
+              OutRing::put(to, lane, k, v[0], v[1], v[2], v[3]);
+            }
+          }
+          OutRing::send(to, lane, &map_o, at.n0 + c, y);
+        } else if (y + lane < g.M) {
+          Out* out = static_cast<Out*>(g.out) + (int64_t)(y + lane) * g.ld_out + at.n0 + c;
+          const int width = min(g.N - at.n0 - c, kCols);
+#pragma unroll
+          for (int j = 0; j < kCols; ++j)
+            if (j < width) out[j] = from_f32<Out>(__uint_as_float(r[j]));
+        }
+      }
+    }
+    if (lane == 0) ptx::tma_store_wait_all();
   }
-  constexpr auto kernel = matmul_many_kernel<Out, S>;
-  MVPA_CUDA_CHECK(grant_smem<kernel>(ManyRows::kSmem));
-  MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kManyThreads, ManyRows::kSmem, s, map_w,
-                                   map_x, map_o, g));
-  count_launch();
-  MVPA_CUDA_CHECK(cudaGetLastError());
-  return MVPA_OK;
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();  // neither CTA's memory goes while the other's products or barriers use it
+  ptx::tc_fence_after();
+  if (warp == 1) ptx::tmem_dealloc_pair(tmem, 512);
 }
 
 int encode_bytes(CUtensorMap* map, const void* base, int64_t rows, int64_t width, int64_t ld, int box_rows) {
@@ -548,13 +770,43 @@ int encode_bytes(CUtensorMap* map, const void* base, int64_t rows, int64_t width
 }
 
 template <typename Out, typename S>
-int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
-  if (g.M > 256) {
-    CUtensorMap map_w, map_x;
-    int rc = encode_bytes(&map_w, b, g.N, K, ld_b, 128);
-    if (rc == MVPA_OK) rc = encode_bytes(&map_x, a, g.M, K, ld_a, 128);
-    return rc == MVPA_OK ? run_many<Out, S>(map_w, map_x, g, s) : rc;
+int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, MatmulArgs g, cudaStream_t s) {
+  constexpr bool kScaled = sizeof(S) == 1;
+  constexpr int kTileN = kScaled ? ScaledRows::kTileN : 256;
+  const int64_t tiles = (int64_t)((g.N + kTileN - 1) / kTileN) * ((g.M + 255) / 256);
+  const int64_t pairs = device_sm_count() / 2;
+  if (tiles * g.KB > 0x7fffffff) {
+    set_error("mvpa_matmul_fp8: more than 2^31 blocks of 256 x %d x 128", kTileN);
+    return MVPA_ERR_UNSUPPORTED;
   }
+  CUtensorMap map_w, map_x, map_o = {};
+  int rc = encode_bytes(&map_w, b, g.N, K, ld_b, kTileN / 2);
+  if (rc == MVPA_OK) rc = encode_bytes(&map_x, a, g.M, K, ld_a, 128);
+  g.out_tma = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ld_out * (int64_t)sizeof(Out) % 16 == 0;
+  if (rc == MVPA_OK && g.out_tma) {
+    const uint64_t dims[2] = {(uint64_t)g.N, (uint64_t)g.M}, strides[1] = {(uint64_t)g.ld_out * sizeof(Out)};
+    const uint32_t box[2] = {128 / sizeof(Out), 32};
+    rc = encode_sw128(&map_o, sizeof(Out) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.out, 2, dims, strides, box);
+  }
+  if (rc != MVPA_OK) return rc;
+  const dim3 grid(2 * (unsigned)(tiles < pairs ? tiles : pairs));
+  if constexpr (kScaled) {
+    constexpr auto kernel = matmul_scaled_kernel<Out>;
+    MVPA_CUDA_CHECK(grant_smem<kernel>(ScaledRows::kSmem));
+    MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, grid, kScaledThreads, ScaledRows::kSmem, s, map_w, map_x, map_o, g));
+  } else {
+    constexpr auto kernel = matmul_many_kernel<Out, S>;
+    MVPA_CUDA_CHECK(grant_smem<kernel>(ManyRows::kSmem));
+    MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, grid, kManyThreads, ManyRows::kSmem, s, map_w, map_x, map_o, g));
+  }
+  count_launch();
+  MVPA_CUDA_CHECK(cudaGetLastError());
+  return MVPA_OK;
+}
+
+template <typename Out, typename S>
+int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
+  if (g.M > 256) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
   const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   CUtensorMap map_w, map_x;
   int rc = encode_bytes(&map_w, b, g.N, K, ld_b, 128);

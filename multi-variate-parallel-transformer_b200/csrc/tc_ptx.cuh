@@ -236,6 +236,23 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
+      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, "
+      "%54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -378,9 +395,10 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t smem_addr, uint32_t ran
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// (`bar` from cluster_map.  Release at the scope of the CTA, as in mbar_arrive: what the arrival orders is TMEM, by
-// tc_fence_before.  At the scope of the cluster it is a fence that waits for every load and store of the thread: the 8-bit
-// product, which arrives once a block, ran at 984 instead of over 2000 TFLOP/s.)
+// (`bar` from cluster_map.  Release at the scope of the CTA, as in mbar_arrive: what such an arrival orders is TMEM, by
+// tc_fence_before, or shared memory that the tensor cores of this very CTA read next, by fence_proxy_async_smem.  At the scope of
+// the cluster it is a fence that waits for every load and store of the thread: the 8-bit product, whose warps arrive once a block
+// with the next blocks' scales still on their way, took 1.6 times as long.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -424,6 +442,37 @@ __device__ __forceinline__ void mma_f8_ss_x4_pair_w(uint32_t el, uint32_t d_tmem
       "add.u32 la, %1, 6;\n\t add.u32 lb, %3, 6;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
       "@pe tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p1;\n\t}" ::"r"(d_tmem),
       "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el)
+      : "memory");
+}
+// ---- the same with a scale (e8m0) for each row's 32 neighbours along K, read from TMEM (kind::mxf8f6f4) ----
+// A matrix of up to 128 rows has its scales in four columns of TMEM: row r in lane r % 32 of column r / 32, one byte of the
+// word (here all four alike: a scale stands for 128 along K, four products), in each quarter of the lanes.  Shared memory holds
+// them as 32 lines of four words; the copy below spreads them over the quarters, in both CTAs from their own shared memory.
+__device__ __forceinline__ void tmem_copy_scales_pair_w(uint32_t el, uint32_t d_tmem, uint32_t smem_addr) {
+  const uint32_t lo = ((smem_addr >> 4) & 0x3FFF) | (1u << 16), hi = (128u >> 4) | (1u << 14);  // 8 lines 128 bytes apart, no swizzle
+  asm volatile(
+      "{\n\t.reg .pred pe;\n\t.reg .b64 d;\n\tsetp.ne.b32 pe, %3, 0;\n\tmov.b64 d, {%1, %2};\n\t"
+      "@pe tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}" ::"r"(d_tmem),
+      "r"(lo), "r"(hi), "r"(el)
+      : "memory");
+}
+// Four consecutive K-steps; the first one overwrites D if `accumulate` is 0.
+__device__ __forceinline__ void mma_mxf8_ss_x4_pair_w(uint32_t el, uint32_t d_tmem, DescHalves a, DescHalves b, uint32_t idesc,
+                                                      uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p0, p1, pe;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+      "setp.ne.b32 p0, %9, 0;\n\t"
+      "setp.eq.b32 p1, 0, 0;\n\t"
+      "setp.ne.b32 pe, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t mov.b64 db, {%3, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p0;\n\t"
+      "add.u32 la, %1, 2;\n\t add.u32 lb, %3, 2;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p1;\n\t"
+      "add.u32 la, %1, 4;\n\t add.u32 lb, %3, 4;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p1;\n\t"
+      "add.u32 la, %1, 6;\n\t add.u32 lb, %3, 6;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p1;\n\t}" ::"r"(d_tmem),
+      "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el), "r"(scale_a), "r"(scale_b), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts_w(uint32_t el, uint32_t d_tmem, uint32_t a_tmem, DescHalves b,
@@ -471,6 +520,12 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int b_mn_ma
 // Instruction descriptor for kind::f8f6f4 with e4m3 A/B (format 0), K-major, and fp32 accumulation.
 __host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// Instruction descriptor for kind::mxf8f6f4: e4m3 A/B, K-major, e8m0 scales (bit 23) in byte 0 of their words, M >> 7 in
+// [27,29); accumulation is always fp32.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3_scaled(int M, int N) {
+  return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27);
 }
 
 // make_idesc_bf16 with both operand majors selectable (bit 15: A is MN-major, bit 16: B is MN-major).
