@@ -324,6 +324,38 @@ struct Ring {
   }
 };
 
+// One operand's tiles on their way in: a warp of each CTA loads its CTA's `rows` rows a block; the loads of both count at the barrier
+// of the CTA of rank 0, which the tokens' warp there tells how many bytes to expect.  (One lane that issued both operands' loads
+// from a branch of its own needed some 450 cycles a block, more than the products of it.)
+template <int kStages, int kTileN, int kBytes, typename Wait>
+__device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t to, bool tokens, int rows, uint64_t* full, uint64_t* empty,
+                                             uint32_t pair, uint32_t pairs, uint32_t tiles_n, uint32_t tiles_m, const MatmulArgs& g,
+                                             const Wait& wait) {
+  const uint32_t el = ptx::elect_one(), rank = ptx::cluster_rank(), tiles = tiles_n * tiles_m;
+  const uint32_t there = ptx::cluster_map(ptx::smem_u32(full), 0);
+  Ring<kStages> st;
+  uint32_t loads = 0;
+  bool on = true;
+  for (uint32_t t = pair; t < tiles && on; t += pairs) {
+    const Tile at = tile_at<kTileN>(t, tiles_n, tiles_m);
+    const int y = (tokens ? at.m0 : at.n0) + (int)rank * rows;
+    for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
+      if (!wait(empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
+        on = false;
+        break;
+      }
+      if (tokens && rank == 0 && el) ptx::mbar_arrive_expect_tx(&full[st.at], 2 * kBytes);
+      __syncwarp();
+      ptx::tma_load_2d_pair_w(el, to + st.at * kBytes, map, there + 8 * st.at, kb * 128, y);
+    }
+  }
+  if (tokens && rank == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one at the end)
+    const uint32_t n = min(loads, (uint32_t)kStages);
+    for (uint32_t k = loads - n; k != loads; ++k)
+      if (!ptx::mbar_wait(&full[k % kStages], (k / kStages) & 1, g.status, kGiveUpDrain)) break;
+  }
+}
+
 template <typename Out, typename S>
 __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                       const __grid_constant__ CUtensorMap map_x,
@@ -375,31 +407,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
-      if (lane == 0) {
-        Ring<C::kStages> st;
-        uint32_t loads = 0;
-        bool on = true;
-        for (uint32_t t = pair; t < tiles && on; t += pairs) {
-          const Tile at = tile_at<256>(t, tiles_n, tiles_m);
-          const int m = at.m0 + (int)rank * 128, n = at.n0 + (int)rank * 128;
-          for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
-            if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
-              on = false;
-              break;
-            }
-            const uint32_t full = ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0), x = stages + st.at * C::kStageBytes;
-            if (rank == 0) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * C::kStageBytes);  // (the other CTA's loads count here too)
-            ptx::tma_load_2d_pair(x, &map_x, full, kb * 128, m);
-            ptx::tma_load_2d_pair(x + 128 * 128, &map_w, full, kb * 128, n);
-          }
-        }
-        if (rank == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one below)
-          const uint32_t n = min(loads, (uint32_t)C::kStages);
-          for (uint32_t k = loads - n; k != loads; ++k)
-            if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
-        }
-      }
+    if (warp == 0 || warp == 2) {  // tokens, weights
+      load_operand<C::kStages, 256, C::kStageBytes>(warp == 0 ? &map_x : &map_w, stages + (warp == 0 ? 0 : 128 * 128), warp == 0, 128, s_full,
+                                                    s_empty, pair, pairs, tiles_n, tiles_m, g, wait);
     } else if (warp == 1 && rank == 0) {
       const uint32_t el = ptx::elect_one();
       constexpr uint32_t idesc = ptx::make_idesc_e4m3(256, 256);
@@ -523,7 +533,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 // say so - which leaves the tensor cores idle half of the time.  Tiles of 256 tokens x 192 weight rows: two of them and the scales
 // of five blocks fill TMEM, so that a tile leaves while the next one is summed.
 //
-// Warps: 0 loads, 1 issues, 2 and 3 lay the scales out in shared memory (tokens, weights), 4 to 7 take the sums home.
+// Warps: 0 loads, 1 issues, 4 to 7 take the sums home, 8 to 11 lay the scales out in shared memory, every fourth block each, with
+// the next one's bytes loaded ahead (two warps for all blocks, tokens and weights, were what the tensor cores waited for: 520 us
+// for 16384 x 15360 x 2048).
 struct ScaledRows {
   static constexpr int kTileN = 192, kHalfN = kTileN / 2;
   static constexpr int kStages = 5;
@@ -534,7 +546,7 @@ struct ScaledRows {
   static constexpr size_t kSmem = 1024 + kStages * (kOperandBytes + kScaleBytes) + kOutBytes;
   static_assert(kTmemScales + kStages * kTmemScaleCols <= 512 && kOperandBytes % 1024 == 0, "");
 };
-constexpr int kScaledThreads = 256;
+constexpr int kScaledThreads = 384, kScaleWarps = 4;
 
 template <typename Out>
 __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
   } else if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
-        ptx::mbar_init(&s_full[i], 5);  // the loads of both CTAs, two warps' scales in each
+        ptx::mbar_init(&s_full[i], 3);  // the loads of both CTAs, and the scales in each
         ptx::mbar_init(&s_empty[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
@@ -586,31 +598,9 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
   };
   ptx::griddep_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
-      Ring<C::kStages> st;
-      uint32_t loads = 0;
-      bool on = true;
-      for (uint32_t t = pair; t < tiles && on; t += pairs) {
-        const Tile at = tile_at<C::kTileN>(t, tiles_n, tiles_m);
-        const int m = at.m0 + (int)rank * 128, n = at.n0 + (int)rank * C::kHalfN;
-        for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
-          if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
-            on = false;
-            break;
-          }
-          const uint32_t full = ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0), x = stages + st.at * C::kOperandBytes;
-          if (rank == 0) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * C::kOperandBytes);  // (the other CTA's loads count here too)
-          ptx::tma_load_2d_pair(x, &map_x, full, kb * 128, m);
-          ptx::tma_load_2d_pair(x + 128 * 128, &map_w, full, kb * 128, n);
-        }
-      }
-      if (rank == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one below)
-        const uint32_t n = min(loads, (uint32_t)C::kStages);
-        for (uint32_t k = loads - n; k != loads; ++k)
-          if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
-      }
-    }
+  if (warp == 0 || warp == 2) {  // tokens, weights
+    load_operand<C::kStages, C::kTileN, C::kOperandBytes>(warp == 0 ? &map_x : &map_w, stages + (warp == 0 ? 0 : 128 * 128), warp == 0,
+                                                          warp == 0 ? 128 : C::kHalfN, s_full, s_empty, pair, pairs, tiles_n, tiles_m, g, wait);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t el = ptx::elect_one();
@@ -644,65 +634,63 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       }
       if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
     }
-  } else if (warp < 4) {
-    // Word j of a lane: the scale of row 32 j + lane (four times the byte).  Warp 2: this CTA's 128 tokens; warp 3: the tile's 192
-    // weight rows, whose groups of 32 lie in one block of 128 each (192 and 128 are multiples of 32 and 64).  The bytes of four
-    // blocks are loaded ahead of their use.
-    constexpr int kAhead = 4, kWords = 6;
-    const bool tokens = warp == 2;
-    const int words = tokens ? 4 : kWords;
-    const uint8_t* base = static_cast<const uint8_t*>(tokens ? g.sa : g.sb);
-    const int64_t step_k = tokens ? g.sa_k : g.sb_k;
+  } else if (warp >= 8) {
+    // Word j of lane l: the scale of row 32 j + l, the byte four times.  Four words for this CTA's 128 tokens; six for the tile's 192
+    // weight rows, whose groups of 32 lie in one block of 128 each (lane j loads the byte of group j).
+    const uint8_t *sa = static_cast<const uint8_t*>(g.sa), *sb = static_cast<const uint8_t*>(g.sb);
+    uint32_t t = pair;
+    int kb = warp - 8;
+    const uint8_t *row[4], *group;
+    const auto settle = [&]() {  // (t, kb) names a block again; where its scales lie
+      while (kb >= g.KB) {
+        kb -= g.KB;
+        t += pairs;
+      }
+      const Tile at = tile_at<C::kTileN>(t < tiles ? t : pair, tiles_n, tiles_m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t m = at.m0 + (int)rank * 128 + 32 * j + lane;
+        row[j] = t < tiles && m < g.M ? sa + m * g.sa_m : nullptr;
+      }
+      const int n = at.n0 + 32 * lane;
+      group = t < tiles && lane < 6 && n < g.N ? sb + (int64_t)(n / 128) * g.sb_n : nullptr;
+    };
+    uint32_t token[4], weight;
+    const auto load = [&]() {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) token[j] = row[j] != nullptr ? row[j][kb * g.sa_k] : 127u;
+      weight = group != nullptr ? group[kb * g.sb_k] : 127u;
+    };
     Ring<C::kStages> st;
-    for (uint32_t t = pair; t < tiles; t += pairs) {
-      const Tile at = tile_at<C::kTileN>(t, tiles_n, tiles_m);
-      const uint8_t* row[kWords];
+    st.at = warp - 8;
+    static_assert(kScaleWarps < C::kStages, "");
+    settle();
+    load();
+    while (t < tiles) {
+      uint32_t w[4], v[6];
 #pragma unroll
-      for (int j = 0; j < kWords; ++j) {
-        if (tokens) {
-          const int64_t m = at.m0 + (int)rank * 128 + 32 * j + lane;
-          row[j] = j < 4 && m < g.M ? base + m * g.sa_m : nullptr;
-        } else {
-          const int n = at.n0 + 32 * j;
-          row[j] = n < g.N ? base + (int64_t)(n / 128) * g.sb_n : nullptr;
-        }
-      }
-      uint32_t bytes[kAhead][kWords];
-      const auto load = [&](int kb0) {
+      for (int j = 0; j < 4; ++j) w[j] = token[j] * 0x01010101u;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-          for (int j = 0; j < kWords; ++j)
-            bytes[i][j] = j < words && row[j] != nullptr && kb0 + i < g.KB ? row[j][(kb0 + i) * step_k] : 127u;
+      for (int j = 0; j < 6; ++j) v[j] = __shfl_sync(0xffffffffu, weight, j) * 0x01010101u;
+      kb += kScaleWarps;
+      if (kb >= g.KB) settle();
+      load();
+      wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty);
+      __syncwarp();
+      const uint32_t to = scales + st.at * C::kScaleBytes + lane * 16;
+      const auto put = [](uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
       };
-      load(0);
-      for (int kb0 = 0; kb0 < g.KB; kb0 += kAhead) {
-        uint32_t now[kAhead][kWords];
+      put(to, w[0], w[1], w[2], w[3]);
+      put(to + 512, v[0], v[1], v[2], v[3]);
+      put(to + 1024, v[4], v[5], 0, 0);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0));
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-          for (int j = 0; j < kWords; ++j) now[i][j] = bytes[i][j] * 0x01010101u;
-        load(kb0 + kAhead);
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (kb0 + i < g.KB) {
-            wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty);
-            __syncwarp();
-            const uint32_t to = scales + st.at * C::kScaleBytes + (tokens ? 0 : 512) + lane * 16;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(now[i][0]), "r"(now[i][1]), "r"(now[i][2]), "r"(now[i][3])
-                         : "memory");
-            if (!tokens)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512), "r"(now[i][4]), "r"(now[i][5]), "r"(0), "r"(0)
-                           : "memory");
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0));
-            st.step();
-          }
-        }
-      }
+      for (int k = 0; k < kScaleWarps; ++k) st.step();
     }
-  } else {
+  } else if (warp >= 4) {
     const int quad = warp - 4;
     const uint32_t at_tmem = tmem + ((uint32_t)quad << 21);
     OutRing ring = {outs + quad * 8192};

@@ -412,12 +412,14 @@ __device__ __forceinline__ void tmem_relinquish_pair() {
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// A load into this CTA's shared memory that counts at a barrier of either CTA of the pair (`bar` from cluster_map).
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
+// A load into this CTA's shared memory that counts at a barrier of either CTA of the pair (`bar` from cluster_map), issued by the
+// elected lane of a convergent warp.
+__device__ __forceinline__ void tma_load_2d_pair_w(uint32_t el, uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(
+      "{\n\t.reg .pred pe;\n\tsetp.ne.b32 pe, %5, 0;\n\t"
+      "@pe cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(
           smem_dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y)
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(el)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit_pair_w(uint32_t el, uint32_t bar) {  // the barrier of this place in both CTAs
