@@ -533,20 +533,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 // say so - which leaves the tensor cores idle half of the time.  Tiles of 256 tokens x 192 weight rows: two of them and the scales
 // of five blocks fill TMEM, so that a tile leaves while the next one is summed.
 //
-// Warps: 0 loads, 1 issues, 4 to 7 take the sums home, 8 to 11 lay the scales out in shared memory, every fourth block each, with
-// the next one's bytes loaded ahead (two warps for all blocks, tokens and weights, were what the tensor cores waited for: 520 us
-// for 16384 x 15360 x 2048).
+// A word of TMEM has room for four scales, and a product names the byte that it wants: they are laid out and copied for four
+// blocks at once.  (For each block, four bytes alike, the three copies took the tensor cores' time as well, 100 cycles for 384 of
+// products: 470 us for 16384 x 15360 x 2048.)
+//
+// Warps: 0 and 2 load tokens and weights, 1 issues, 3 lays the scales out in shared memory, 4 to 7 take the sums home.
 struct ScaledRows {
   static constexpr int kTileN = 192, kHalfN = kTileN / 2;
-  static constexpr int kStages = 5;
+  static constexpr int kStages = 6;
+  static constexpr int kGroup = 4, kGroups = 3;   // blocks that share a word of scales; such groups on their way
   static constexpr int kOperandBytes = 128 * 128 + kHalfN * 128;
   static constexpr int kScaleBytes = 512 + 1024;  // 128 tokens; two groups of 128 weight rows
   static constexpr int kOutBytes = 4 * 2 * 32 * 128;
   static constexpr uint32_t kTmemScales = 2 * kTileN, kTmemScaleCols = 16;
-  static constexpr size_t kSmem = 1024 + kStages * (kOperandBytes + kScaleBytes) + kOutBytes;
-  static_assert(kTmemScales + kStages * kTmemScaleCols <= 512 && kOperandBytes % 1024 == 0, "");
+  static constexpr size_t kSmem = 1024 + kStages * kOperandBytes + kGroups * kScaleBytes + kOutBytes;
+  static_assert(kTmemScales + kGroups * kTmemScaleCols <= 512 && kOperandBytes % 1024 == 0, "");
 };
-constexpr int kScaledThreads = 384, kScaleWarps = 4;
+constexpr int kScaledThreads = 256;
 
 template <typename Out>
 __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -554,7 +557,8 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
                                                                           const __grid_constant__ CUtensorMap map_o, const MatmulArgs g) {
   using C = ScaledRows;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2];
+  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2], s_sfull[C::kGroups],
+      s_sempty[C::kGroups];
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;
   const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
@@ -569,8 +573,12 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
   } else if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
-        ptx::mbar_init(&s_full[i], 3);  // the loads of both CTAs, and the scales in each
+        ptx::mbar_init(&s_full[i], 1);
         ptx::mbar_init(&s_empty[i], 1);
+      }
+      for (int i = 0; i < C::kGroups; ++i) {
+        ptx::mbar_init(&s_sfull[i], 2);  // the scales in both CTAs
+        ptx::mbar_init(&s_sempty[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
         ptx::mbar_init(&s_tfull[i], 1);
@@ -603,49 +611,66 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
                                                           warp == 0 ? 128 : C::kHalfN, s_full, s_empty, pair, pairs, tiles_n, tiles_m, g, wait);
   } else if (warp == 1) {
     if (rank == 0) {
+      // (The loop has to be shorter than a block's 384 cycles of products: four blocks unrolled, their barriers by address, and each
+      // block's barrier looked at while the products of the one before are issued.)
       const uint32_t el = ptx::elect_one();
       constexpr uint32_t idesc = ptx::make_idesc_e4m3_scaled(256, C::kTileN);
+      const uint32_t full = ptx::smem_u32(s_full), empty = ptx::smem_u32(s_empty);
+      const ptx::DescHalves first = ptx::make_desc_halves_sw128(stages, 16, 1024);
       Ring<C::kStages> st;
+      Ring<C::kGroups> group;
       Ring<2> buf;
       uint32_t last = 0, last_parity = 0;
       bool on = true, any = false;
       for (uint32_t t = pair; t < tiles && on; t += pairs, buf.step()) {
         if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
-        ptx::tc_fence_after();
-        for (int kb = 0; kb < g.KB; ++kb, st.step()) {
-          const uint32_t x = stages + st.at * C::kOperandBytes, s = scales + st.at * C::kScaleBytes;
-          const uint32_t sa = tmem + C::kTmemScales + st.at * C::kTmemScaleCols, sb = sa + 4;
-          const ptx::DescHalves a = ptx::make_desc_halves_sw128(x, 16, 1024), b = ptx::make_desc_halves_sw128(x + 128 * 128, 16, 1024);
-          if (!wait(s_full[st.at], st.parity, kGiveUpFull)) {
+        const uint32_t d = tmem + buf.at * C::kTileN;
+        bool there = false;
+        for (int kb0 = 0; kb0 < g.KB && on; kb0 += C::kGroup, group.step()) {
+          if (!wait(s_sfull[group.at], group.parity, kGiveUpFull)) {
             on = false;
             break;
           }
           ptx::tc_fence_after();
+          const uint32_t sa = tmem + C::kTmemScales + group.at * C::kTmemScaleCols, sb = sa + 4, s = scales + group.at * C::kScaleBytes;
           ptx::tmem_copy_scales_pair_w(el, sa, s);
           ptx::tmem_copy_scales_pair_w(el, sb, s + 512);
           ptx::tmem_copy_scales_pair_w(el, sb + 4, s + 1024);
-          ptx::mma_mxf8_ss_x4_pair_w(el, tmem + buf.at * C::kTileN, a, b, idesc, sa, sb, kb > 0);
-          ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_empty[st.at]));
-          last = st.at;
-          last_parity = st.parity;
-          any = true;
+#pragma unroll
+          for (uint32_t byte = 0; byte < C::kGroup; ++byte) {
+            if (kb0 + (int)byte >= g.KB) break;
+            if (!there && !wait(s_full[st.at], st.parity, kGiveUpFull)) {
+              on = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            const ptx::DescHalves a = {first.lo + st.at * (C::kOperandBytes >> 4), first.hi}, b = {a.lo + (128 * 128 >> 4), first.hi};
+            ptx::mma_mxf8_ss_x4_pair_w(el, d, a, b, idesc | (byte << 4) | (byte << 29), sa, sb, kb0 > 0 || byte > 0);
+            ptx::mma_commit_pair_w(el, empty + 8 * st.at);
+            last = st.at;
+            last_parity = st.parity;
+            any = true;
+            st.step();
+            there = ptx::mbar_test_wait_a(full + 8 * st.at, st.parity);
+          }
+          ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_sempty[group.at]));
         }
         if (on) ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_tfull[buf.at]));
       }
       if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
     }
-  } else if (warp >= 8) {
-    // Word j of lane l: the scale of row 32 j + l, the byte four times.  Four words for this CTA's 128 tokens; six for the tile's 192
-    // weight rows, whose groups of 32 lie in one block of 128 each (lane j loads the byte of group j).
+  } else if (warp == 3) {
+    // Word j of lane l: the scales of row 32 j + l over a group of blocks, a byte each.  Four words for this CTA's 128 tokens; six for
+    // the tile's 192 weight rows, whose groups of 32 lie in one block of 128 each (lane j loads the word of rows 32 j).
     const uint8_t *sa = static_cast<const uint8_t*>(g.sa), *sb = static_cast<const uint8_t*>(g.sb);
+    const auto words = [](const void* p, int64_t rows, int64_t k) {  // four blocks' scales are an aligned word
+      return k == 1 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)rows) & 3) == 0;
+    };
+    const bool word_a = words(sa, g.sa_m, g.sa_k), word_b = words(sb, g.sb_n, g.sb_k);
     uint32_t t = pair;
-    int kb = warp - 8;
-    const uint8_t *row[4], *group;
-    const auto settle = [&]() {  // (t, kb) names a block again; where its scales lie
-      while (kb >= g.KB) {
-        kb -= g.KB;
-        t += pairs;
-      }
+    int kb = 0;
+    const uint8_t *row[4], *weights;
+    const auto settle = [&]() {  // where the scales of tile t lie
       const Tile at = tile_at<C::kTileN>(t < tiles ? t : pair, tiles_n, tiles_m);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -653,31 +678,44 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
         row[j] = t < tiles && m < g.M ? sa + m * g.sa_m : nullptr;
       }
       const int n = at.n0 + 32 * lane;
-      group = t < tiles && lane < 6 && n < g.N ? sb + (int64_t)(n / 128) * g.sb_n : nullptr;
+      weights = t < tiles && lane < 6 && n < g.N ? sb + (int64_t)(n / 128) * g.sb_n : nullptr;
     };
-    uint32_t token[4], weight;
+    const auto fetch = [&](const uint8_t* p, int64_t k, bool word, uint32_t (&v)[C::kGroup]) {  // (v[0] alone where it is a word)
+      if (word && kb + C::kGroup <= g.KB) {
+        v[0] = p != nullptr ? *reinterpret_cast<const uint32_t*>(p + kb) : 0u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < C::kGroup; ++i) v[i] = p != nullptr && kb + i < g.KB ? p[(kb + i) * k] : 0u;
+      }
+    };
+    const auto joined = [&](const uint32_t (&v)[C::kGroup], bool word) { return word ? v[0] : v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24; };
+    uint32_t token[4][C::kGroup], weight[C::kGroup];
     const auto load = [&]() {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) token[j] = row[j] != nullptr ? row[j][kb * g.sa_k] : 127u;
-      weight = group != nullptr ? group[kb * g.sb_k] : 127u;
+      for (int j = 0; j < 4; ++j) fetch(row[j], g.sa_k, word_a, token[j]);
+      fetch(weights, g.sb_k, word_b, weight);
     };
-    Ring<C::kStages> st;
-    st.at = warp - 8;
-    static_assert(kScaleWarps < C::kStages, "");
+    Ring<C::kGroups> group;
     settle();
     load();
-    while (t < tiles) {
+    for (; t < tiles; group.step()) {
+      const bool whole = kb + C::kGroup <= g.KB;
       uint32_t w[4], v[6];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = token[j] * 0x01010101u;
+      for (int j = 0; j < 4; ++j) w[j] = joined(token[j], word_a && whole);
+      const uint32_t mine = joined(weight, word_b && whole);
 #pragma unroll
-      for (int j = 0; j < 6; ++j) v[j] = __shfl_sync(0xffffffffu, weight, j) * 0x01010101u;
-      kb += kScaleWarps;
-      if (kb >= g.KB) settle();
-      load();
-      wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty);
+      for (int j = 0; j < 6; ++j) v[j] = __shfl_sync(0xffffffffu, mine, j);
+      kb += C::kGroup;
+      if (kb >= g.KB) {
+        kb = 0;
+        t += pairs;
+        settle();
+      }
+      load();  // (the next group's, used a group later)
+      wait(s_sempty[group.at], group.parity ^ 1, kGiveUpEmpty);
       __syncwarp();
-      const uint32_t to = scales + st.at * C::kScaleBytes + lane * 16;
+      const uint32_t to = scales + group.at * C::kScaleBytes + lane * 16;
       const auto put = [](uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
       };
@@ -686,9 +724,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       put(to + 1024, v[4], v[5], 0, 0);
       ptx::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_full[st.at]), 0));
-#pragma unroll
-      for (int k = 0; k < kScaleWarps; ++k) st.step();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_sfull[group.at]), 0));
     }
   } else if (warp >= 4) {
     const int quad = warp - 4;

@@ -447,9 +447,9 @@ __device__ __forceinline__ void mma_f8_ss_x4_pair_w(uint32_t el, uint32_t d_tmem
       : "memory");
 }
 // ---- the same with a scale (e8m0) for each row's 32 neighbours along K, read from TMEM (kind::mxf8f6f4) ----
-// A matrix of up to 128 rows has its scales in four columns of TMEM: row r in lane r % 32 of column r / 32, one byte of the
-// word (here all four alike: a scale stands for 128 along K, four products), in each quarter of the lanes.  Shared memory holds
-// them as 32 lines of four words; the copy below spreads them over the quarters, in both CTAs from their own shared memory.
+// A matrix of up to 128 rows has its scales in four columns of TMEM: row r in lane r % 32 of column r / 32, in the byte of the
+// word that the instruction descriptor names (A's in bits [29,31), B's in [4,6)), in each quarter of the lanes.  Shared memory
+// holds them as 32 lines of four words; the copy below spreads them over the quarters, in both CTAs from their own shared memory.
 __device__ __forceinline__ void tmem_copy_scales_pair_w(uint32_t el, uint32_t d_tmem, uint32_t smem_addr) {
   const uint32_t lo = ((smem_addr >> 4) & 0x3FFF) | (1u << 16), hi = (128u >> 4) | (1u << 14);  // 8 lines 128 bytes apart, no swizzle
   asm volatile(
@@ -524,8 +524,7 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// Instruction descriptor for kind::mxf8f6f4: e4m3 A/B, K-major, e8m0 scales (bit 23) in byte 0 of their words, M >> 7 in
-// [27,29); accumulation is always fp32.
+// Instruction descriptor for kind::mxf8f6f4: e4m3 A/B, K-major, e8m0 scales (bit 23), M >> 7 in [27,29); accumulation is always fp32.
 __host__ __device__ constexpr uint32_t make_idesc_e4m3_scaled(int M, int N) {
   return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27);
 }
