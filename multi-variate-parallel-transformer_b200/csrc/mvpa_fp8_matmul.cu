@@ -830,8 +830,8 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
 
 template <typename Out, typename S>
 int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
-  if (g.M > 256) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
-  const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
+  if (g.M > 64) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
+  const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : 64;
   CUtensorMap map_w, map_x;
   int rc = encode_bytes(&map_w, b, g.N, K, ld_b, 128);
   if (rc == MVPA_OK) rc = encode_bytes(&map_x, a, g.M, K, ld_a, nt);
@@ -839,8 +839,7 @@ int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, 
   switch (nt) {
     case 16: return run_few<16, Out, S>(map_w, map_x, g, s);
     case 32: return run_few<32, Out, S>(map_w, map_x, g, s);
-    case 64: return run_few<64, Out, S>(map_w, map_x, g, s);
-    default: return run_few<128, Out, S>(map_w, map_x, g, s);
+    default: return run_few<64, Out, S>(map_w, map_x, g, s);
   }
 }
 

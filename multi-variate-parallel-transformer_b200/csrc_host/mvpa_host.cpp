@@ -554,15 +554,26 @@ int64_t matrix_ld(const Tensor& t) {
 }
 bool bf16_or_fp32(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 
+// What an operator writes: the caller's pair, or a new one.
 struct Pair {
   Tensor q, scales;
-  int64_t ld;
-  Pair(int64_t rows, int64_t width, int64_t tall, const Tensor& like) {
+  int64_t ld = 0, ld_s = 0;
+  // Whether the caller's tensors (undefined: none) are a pair of these sizes.
+  bool fits(int64_t rows, int64_t width, int64_t tall) {
+    if (!q.defined() || !scales.defined()) return q.defined() == scales.defined();
+    ld = matrix_ld(q);
+    ld_s = matrix_ld(scales);
+    return q.scalar_type() == at::kFloat8_e4m3fn && scales.scalar_type() == at::kFloat8_e8m0fnu && ld != 0 && ld_s != 0 &&
+           q.sizes() == at::IntArrayRef({rows, width}) && scales.sizes() == at::IntArrayRef({(rows + tall - 1) / tall, blocks_of(width)});
+  }
+  void make(int64_t rows, int64_t width, int64_t tall, const Tensor& like) {
+    if (q.defined()) return;
     ld = (width + 15) / 16 * 16;
+    ld_s = blocks_of(width);
     const auto options = like.options().requires_grad(false);
     q = at::empty({rows, ld}, options.dtype(at::kFloat8_e4m3fn));
     if (ld != width) q = q.narrow(1, 0, width);
-    scales = at::empty({(rows + tall - 1) / tall, blocks_of(width)}, options.dtype(at::kFloat8_e8m0fnu));
+    scales = at::empty({(rows + tall - 1) / tall, ld_s}, options.dtype(at::kFloat8_e8m0fnu));
   }
 };
 
@@ -573,61 +584,68 @@ bool take(PyObject* a, Tensor& t) {  // (None leaves the tensor undefined)
   return true;
 }
 
-// quantize_fp8(x, block_rows) -> (q, scales) or None
+// quantize_fp8(x, block_rows, q or None, scales or None) -> (q, scales) or None
 PyObject* quantize_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 2)) return nullptr;
+  if (!arguments(n, 4)) return nullptr;
   Tensor x;
-  if (a[0] == Py_None || !take(a[0], x) || !PyLong_CheckExact(a[1])) Py_RETURN_NONE;
+  Pair out;
+  if (a[0] == Py_None || !take(a[0], x) || !PyLong_CheckExact(a[1]) || !take(a[2], out.q) || !take(a[3], out.scales)) Py_RETURN_NONE;
   const int64_t tall = PyLong_AsLongLong(a[1]);
   if (PyErr_Occurred()) return nullptr;
-  if ((tall != 1 && tall != kFp8Block) || !fp8_inputs({&x}) || !bf16_or_fp32(x)) Py_RETURN_NONE;
+  if ((tall != 1 && tall != kFp8Block) || !fp8_inputs({&x, &out.q, &out.scales}) || !bf16_or_fp32(x)) Py_RETURN_NONE;
   const int64_t ld = matrix_ld(x);
-  if (ld == 0 || x.size(1) > INT32_MAX) Py_RETURN_NONE;
+  if (ld == 0 || x.size(1) > INT32_MAX || !out.fits(x.size(0), x.size(1), tall)) Py_RETURN_NONE;
   std::optional<Body> body(std::in_place, x);
-  Pair out(x.size(0), x.size(1), tall, x);
-  check(api.quantize_fp8(x.const_data_ptr(), ld, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.scales.size(1), x.size(0),
+  out.make(x.size(0), x.size(1), tall, x);
+  check(api.quantize_fp8(x.const_data_ptr(), ld, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.ld_s, x.size(0),
                          (int32_t)x.size(1), (int32_t)tall, dtype_code(x), stream_of(x)), "mvpa_quantize_fp8");
   body.reset();  // (the interpreter is wanted again)
   return wrap({std::move(out.q), std::move(out.scales)});
   END_HANDLE_TH_ERRORS
 }
 
-// rmsnorm_fp8(x, weight, eps, add or None, sum_out or None) -> (q, scales) or None
+// rmsnorm_fp8(x, weight, eps, add or None, sum_out or None, q or None, scales or None) -> (q, scales) or None
 PyObject* rmsnorm_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 5)) return nullptr;
+  if (!arguments(n, 7)) return nullptr;
   Tensor x, w, add, sum;
-  if (a[0] == Py_None || a[1] == Py_None || !take(a[0], x) || !take(a[1], w) || !PyFloat_Check(a[2]) || !take(a[3], add) || !take(a[4], sum))
+  Pair out;
+  if (a[0] == Py_None || a[1] == Py_None || !take(a[0], x) || !take(a[1], w) || !PyFloat_Check(a[2]) || !take(a[3], add) || !take(a[4], sum) ||
+      !take(a[5], out.q) || !take(a[6], out.scales))
     Py_RETURN_NONE;
-  if (!fp8_inputs({&x, &w, &add, &sum}) || !bf16_or_fp32(x) || x.dim() < 1 || x.numel() == 0) Py_RETURN_NONE;
+  if (!fp8_inputs({&x, &w, &add, &sum, &out.q, &out.scales}) || !bf16_or_fp32(x) || x.dim() < 1 || x.numel() == 0) Py_RETURN_NONE;
   const int64_t E = x.size(-1);
   for (const Tensor* t : {&x, &w, &add, &sum})
     if (t->defined() && (!t->is_contiguous() || t->scalar_type() != x.scalar_type())) Py_RETURN_NONE;
   for (const Tensor* t : {&add, &sum})
     if (t->defined() && (t->numel() != x.numel() || t->dim() < 1 || t->size(-1) != E)) Py_RETURN_NONE;
-  if (w.dim() != 1 || w.size(0) != E || E > 4096) Py_RETURN_NONE;
+  if (w.dim() != 1 || w.size(0) != E || E > 4096 || !out.fits(x.numel() / E, E, 1)) Py_RETURN_NONE;
   std::optional<Body> body(std::in_place, x);
-  Pair out(x.numel() / E, E, 1, x);
+  out.make(x.numel() / E, E, 1, x);
   check(api.rmsnorm_fp8(x.const_data_ptr(), add.defined() ? add.const_data_ptr() : nullptr, w.const_data_ptr(),
-                        sum.defined() ? sum.data_ptr() : nullptr, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.scales.size(1),
+                        sum.defined() ? sum.data_ptr() : nullptr, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.ld_s,
                         x.numel() / E, (int32_t)E, (float)PyFloat_AS_DOUBLE(a[2]), dtype_code(x), stream_of(x)), "mvpa_rmsnorm_fp8");
   body.reset();  // (the interpreter is wanted again)
   return wrap({std::move(out.q), std::move(out.scales)});
   END_HANDLE_TH_ERRORS
 }
 
-// silu_mul_fp8(gate, up) -> (q, scales) or None
+// silu_mul_fp8(gate, up, q or None, scales or None) -> (q, scales) or None
 PyObject* silu_mul_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 2)) return nullptr;
+  if (!arguments(n, 4)) return nullptr;
   Tensor g, u;
-  if (a[0] == Py_None || a[1] == Py_None || !take(a[0], g) || !take(a[1], u) || !fp8_inputs({&g, &u}) || !bf16_or_fp32(g)) Py_RETURN_NONE;
+  Pair out;
+  if (a[0] == Py_None || a[1] == Py_None || !take(a[0], g) || !take(a[1], u) || !take(a[2], out.q) || !take(a[3], out.scales) ||
+      !fp8_inputs({&g, &u, &out.q, &out.scales}) || !bf16_or_fp32(g))
+    Py_RETURN_NONE;
   const int64_t ld = matrix_ld(g);
-  if (ld == 0 || matrix_ld(u) != ld || u.sizes() != g.sizes() || u.scalar_type() != g.scalar_type() || g.size(1) > INT32_MAX) Py_RETURN_NONE;
+  if (ld == 0 || matrix_ld(u) != ld || u.sizes() != g.sizes() || u.scalar_type() != g.scalar_type() || g.size(1) > INT32_MAX || !out.fits(g.size(0), g.size(1), 1))
+    Py_RETURN_NONE;
   std::optional<Body> body(std::in_place, g);
-  Pair out(g.size(0), g.size(1), 1, g);
-  check(api.silu_mul_fp8(g.const_data_ptr(), u.const_data_ptr(), ld, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.scales.size(1),
+  out.make(g.size(0), g.size(1), 1, g);
+  check(api.silu_mul_fp8(g.const_data_ptr(), u.const_data_ptr(), ld, out.q.data_ptr(), out.ld, out.scales.data_ptr(), out.ld_s,
                          g.size(0), (int32_t)g.size(1), dtype_code(g), stream_of(g)), "mvpa_silu_mul_fp8");
   body.reset();  // (the interpreter is wanted again)
   return wrap({std::move(out.q), std::move(out.scales)});

@@ -17,6 +17,9 @@ h = x + MLP(ln_1 x) + Attn(ln_1 x)) built for B200:
   * the relative keys of all layers (`position_net`, `channel_net` of the embeddings, which do not depend
     on the input) come from one GEMM each per forward.
 
+`MVPFormerModel.enable_fp8()` runs both projections of every block in 8 bits (e4m3, a scale for each block of 128): the norm
+and the gate write their results in 8 bits, and `mvpa_ops.matmul_fp8` takes the place of the two GEMMs.
+
 With gradients enabled the blocks run the reference's op order through differentiable operations: torch's
 projections, `mvpa_ops.rmsnorm_train` (one kernel forward and two backward instead of about ten elementwise
 launches), `mvpa_ops.swiglu` where the gate is large, and `attentions.flashmvpa`; as one autograd function where the
@@ -125,6 +128,7 @@ class MVPFormerBlock(torch.nn.Module):
         self.ln_2 = RMSNorm(config.hidden_size, eps=config.layer_norm_epsilon)   # unused, as in the reference
         self.mlp = LlamaMLP(config)
         self._fused = None
+        self._fused_fp8 = None
 
     def forward(self, hidden_states, positional_embedding, channel_embedding, layer_past=None, attention_mask=None,
                 head_mask=None, encoder_hidden_states=None, encoder_attention_mask=None, use_cache=False,
@@ -144,16 +148,53 @@ class MVPFormerBlock(torch.nn.Module):
         return (hidden_states,) + (outputs if use_cache else outputs[1:])
 
     # ---- fused inference path -------------------------------------------------------------------
-    def fused_weights(self):
-        """[q | k v | gate up] (rows) and [c_proj | down_proj] (columns), concatenated once per weight version."""
+    def _projections(self):
         ws = (self.attn.q_attn.weight, self.attn.c_attn.weight, self.mlp.gate_proj.weight, self.mlp.up_proj.weight,
               self.attn.c_proj.weight, self.mlp.down_proj.weight)
-        tag = tuple((w._version, w.data_ptr(), w.dtype) for w in ws)
+        return ws, tuple((w._version, w.data_ptr(), w.dtype, w.device) for w in ws)
+
+    @staticmethod
+    def _concatenated(ws):
+        return (torch.cat([w.detach() for w in ws[:4]], dim=0).contiguous(),
+                torch.cat([ws[4].detach(), ws[5].detach()], dim=1).contiguous())
+
+    def fused_weights(self):
+        """[q | k v | gate up] (rows) and [c_proj | down_proj] (columns), concatenated once per weight version."""
+        ws, tag = self._projections()
         if self._fused is None or self._fused[0] != tag:
-            w_in = torch.cat([w.detach() for w in ws[:4]], dim=0).contiguous()
-            w_out = torch.cat([ws[4].detach(), ws[5].detach()], dim=1).contiguous()
-            self._fused = (tag, w_in, w_out)
+            self._fused = (tag, *self._concatenated(ws))
         return self._fused[1], self._fused[2]
+
+    def fused_weights_fp8(self):
+        """The same two matrices in 8 bits, ((q, scales), (q, scales)), quantised once per weight version."""
+        ws, tag = self._projections()
+        if self._fused_fp8 is None or self._fused_fp8[0] != tag:
+            self._fused_fp8 = (tag, *(mvpa_ops.quantize_fp8(w, block_rows=mvpa_ops.FP8_BLOCK) for w in self._concatenated(ws)))
+        return self._fused_fp8[1], self._fused_fp8[2]
+
+    @torch.no_grad()
+    def fused_branches_fp8(self, pair, r_time, r_chan, B, T, C, dtype):
+        """`fused_branches` on the block's normalised input in 8 bits (`mvpa_ops.rmsnorm_fp8`), with both projections in 8
+        bits; what lies between them, the attention among it, is in `dtype`.  The attention's output and the gate go side by
+        side into the matrix that the second projection reads; hidden_size is a multiple of 128, so no block holds both."""
+        a = self.attn
+        E, H, Hkv, D = a.embed_dim, a.num_heads, a.num_kv_heads, a.head_dim
+        I = self.mlp.gate_proj.out_features
+        N, KV, rows = T * C, Hkv * D, B * T * C
+        w_in, w_out = self.fused_weights_fp8()
+        big = mvpa_ops.matmul_fp8(*pair, *w_in, dtype=dtype)             # (rows, E + 2 KV + 2 I)
+        head = lambda c, heads: big[:, c:c + heads * D].view(B, N, heads, D).permute(0, 2, 1, 3)
+        att = torch.empty((rows, E), dtype=dtype, device=big.device)
+        u, vt, z = (b.view(Hkv, D).to(dtype) for b in a.attn_bias.detach().split(KV))
+        flash_mvpa_into(att.view(B, N, H, D).permute(0, 2, 1, 3), head(0, H), u, vt, z, head(E, Hkv), r_time.to(dtype),
+                        r_chan.to(dtype), head(E + KV, Hkv), 1.0 / (D ** 0.5), 10)
+        blocks = E // mvpa_ops.FP8_BLOCK
+        q = torch.empty((rows, (E + I + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=big.device)[:, :E + I]
+        scales = torch.empty((rows, -(-(E + I) // mvpa_ops.FP8_BLOCK)), dtype=torch.float8_e8m0fnu, device=big.device)
+        mvpa_ops.quantize_fp8(att, out=(q[:, :E], scales[:, :blocks]))
+        g0 = E + 2 * KV
+        mvpa_ops.silu_mul_fp8(big[:, g0:g0 + I], big[:, g0 + I:], out=(q[:, E:], scales[:, blocks:]))
+        return mvpa_ops.matmul_fp8(q, scales, *w_out, dtype=dtype)
 
     @torch.no_grad()
     def fused_branches(self, x, r_time, r_chan, B, T, C):
@@ -233,6 +274,7 @@ class MVPFormerModel(torch.nn.Module):
         self.gradient_checkpointing = gradient_checkpointing
         self._rel = None
         self._use_graph, self._graphs = False, {}
+        self._fp8 = False
         std = config.initializer_range                                     # `_init_weights` (`:179-188`)
         for m in self.modules():
             if isinstance(m, (torch.nn.Linear, torch.nn.Embedding)):
@@ -289,6 +331,8 @@ class MVPFormerModel(torch.nn.Module):
         transport, frozen weights): the whole forward is captured in a CUDA graph on first use and replayed -
         its step counters live on the device, so every replay orders itself against the other ranks' replays;
         the result is the graph's own buffer, overwritten by the next call."""
+        if self._fp8:
+            raise NotImplementedError("forward_time_sharded does not run in 8 bits: call enable_fp8(False) first")
         if graph and transport == "p2p":
             key = ("sharded", tuple(embeds_local.shape), embeds_local.dtype, embeds_local.device.index, T, C, id(group))
             entry = self._graphs.get(key)
@@ -349,6 +393,19 @@ class MVPFormerModel(torch.nn.Module):
         self._graphs = {}
         return self
 
+    def enable_fp8(self, flag: bool = True):
+        """Inference with the blocks' projections in 8 bits: e4m3 weights with a scale for each block of 128 x 128, e4m3
+        activations with one for each 128 neighbours of a row (`mvpa_ops.quantize_fp8`); norms, attention, gate and the
+        residual stream as without.  Each of the two products takes in its operands with a relative rounding of up to 2^-4
+        (their mean squares: some 2.6 % each).  Weights are quantised on first use, and again after they change.  Concerns the
+        fused forward alone (no gradients, eval mode) and not `forward_time_sharded`; hidden_size has to be a multiple of 128.
+        Autocast has no effect on these products.  Captured graphs are dropped."""
+        if flag and self.embed_dim % mvpa_ops.FP8_BLOCK:
+            raise ValueError(f"enable_fp8: hidden_size must be a multiple of {mvpa_ops.FP8_BLOCK}, got {self.embed_dim}")
+        self._fp8 = bool(flag)
+        self._graphs = {}
+        return self
+
     def reset_cuda_graphs(self):
         self._graphs = {}
 
@@ -397,7 +454,12 @@ class MVPFormerModel(torch.nn.Module):
         branches = None
         for i, block in enumerate(self.h):
             w = block.ln_1.weight.detach().to(h.dtype)
-            x = mvpa_ops.rmsnorm(h, w, block.ln_1.eps, add=branches, sum_out=h if branches is not None else None)
+            sum_out = h if branches is not None else None
+            if self._fp8:
+                pair = mvpa_ops.rmsnorm_fp8(h, w, block.ln_1.eps, add=branches, sum_out=sum_out)
+                branches = block.fused_branches_fp8(pair, r_time[i], r_chan[i], B, T, C, h.dtype)
+                continue
+            x = mvpa_ops.rmsnorm(h, w, block.ln_1.eps, add=branches, sum_out=sum_out)
             branches = block.fused_branches(x, r_time[i], r_chan[i], B, T, C)
         return mvpa_ops.rmsnorm(h, self.ln_f.weight.detach().to(h.dtype), self.ln_f.eps, add=branches, sum_out=h)
 

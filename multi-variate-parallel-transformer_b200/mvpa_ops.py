@@ -316,8 +316,8 @@ def quantize_fp8(x, block_rows=1, out=None):
     """x (rows, width), bf16 or fp32, in 8 bits: (q, scales).  `block_rows=1` gives every row its own scales (activations),
     `block_rows=128` every block of 128 x 128 one (weights).  `out=(q, scales)` writes into the caller's tensors, which may be
     column blocks of wider ones."""
-    if out is None and _host.usable(x):
-        pair = _host.module().quantize_fp8(x, block_rows)
+    if _host.usable(x):
+        pair = _host.module().quantize_fp8(x, block_rows, *(out or (None, None)))
         if pair is not None:
             return pair
     _fp8_inputs("quantize_fp8", x)
@@ -338,8 +338,8 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None):
     """`rmsnorm` with the result in 8 bits: (q, scales) of rmsnorm(h) * weight, h = x (+ add), for x (..., E) with all leading
     dimensions as rows.  h is rounded to x's type, as in `rmsnorm`, and written to `sum_out` (which may be `x`); the normalised
     row goes from fp32 to e4m3 in one rounding.  E up to 4096 in bf16, 2048 in fp32."""
-    if out is None and _host.usable(x):
-        pair = _host.module().rmsnorm_fp8(x, weight, eps, add, sum_out)
+    if _host.usable(x):
+        pair = _host.module().rmsnorm_fp8(x, weight, eps, add, sum_out, *(out or (None, None)))
         if pair is not None:
             return pair
     extra = [t for t in (add, sum_out) if t is not None]
@@ -364,8 +364,8 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None):
 def silu_mul_fp8(gate, up, out=None):
     """silu(gate) * up in 8 bits: (q, scales).  gate, up (rows, width) with unit inner stride (column blocks of a wider buffer
     are fine).  From fp32 to e4m3 in one rounding; `silu_mul` rounds silu(gate) to the type in between, as eager PyTorch does."""
-    if out is None and _host.usable(gate):
-        pair = _host.module().silu_mul_fp8(gate, up)
+    if _host.usable(gate):
+        pair = _host.module().silu_mul_fp8(gate, up, *(out or (None, None)))
         if pair is not None:
             return pair
     _fp8_inputs("silu_mul_fp8", gate, up)
