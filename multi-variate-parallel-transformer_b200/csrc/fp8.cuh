@@ -46,7 +46,7 @@ __device__ __forceinline__ uint32_t max8(uint32_t v) {
 
 constexpr int kLane = 16;  // values a lane holds of a block: 16 bytes of e4m3, one store
 
-// A lane's sixteen values of its block where rows start on 16-byte boundaries: as they lie in memory.
+// A lane's sixteen values of its block, as they lie in memory.
 template <typename T>
 struct Raw {
   static constexpr int kWords = kLane / Vec<T>::N;
@@ -61,6 +61,46 @@ struct Raw {
       for (int e = 0; e < kLane; ++e) y[e] = col + e < width ? to_f32<T>(row[col + e]) : 0.f;
       pack(y);
     }
+  }
+  // Rows at any alignment: the 16-byte pieces that hold the values (and none that holds no value of the row, so that nothing is
+  // read from beyond a piece of memory that the row lies in), moved into place by words and then by halves.  Sixteen single loads
+  // a lane touch each sector again and again: 2500 x 1027 in fp32 with the residual took 34 us so.
+  __device__ __forceinline__ void load_any(const T* __restrict__ row, int col, int width) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row + col), end = p + min(width - col, kLane) * sizeof(T);
+    const uint4* from = reinterpret_cast<const uint4*>(p & ~(uintptr_t)15);
+    constexpr int W = 4 * kWords;
+    uint32_t v[W + 4];
+#pragma unroll
+    for (int i = 0; i <= kWords; ++i) {
+      uint4 r = make_uint4(0, 0, 0, 0);
+      if (reinterpret_cast<uintptr_t>(from + i) < end) r = from[i];
+      v[4 * i] = r.x; v[4 * i + 1] = r.y; v[4 * i + 2] = r.z; v[4 * i + 3] = r.w;
+    }
+    const uint32_t shift = (uint32_t)p & 15;
+    if (shift & 8) {
+#pragma unroll
+      for (int j = 0; j < W + 2; ++j) v[j] = v[j + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+      for (int j = 0; j < W + 1; ++j) v[j] = v[j + 1];
+    }
+    if constexpr (sizeof(T) == 2) {
+      if (shift & 2) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = __funnelshift_r(v[j], v[j + 1], 16);
+      }
+    }
+    if (col + kLane > width) {  // what follows the row
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int left = width - col - j * (4 / (int)sizeof(T));  // values of the row from this word on
+        if (left <= 0) v[j] = 0;
+        else if (sizeof(T) == 2 && left == 1) v[j] &= 0xffffu;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   }
   __device__ __forceinline__ void pack(const float (&y)[kLane]) {  // (values of T)
 #pragma unroll
@@ -94,44 +134,24 @@ struct Raw {
   }
 };
 
-// Rows at any alignment: the eight lanes of a block read it eight neighbours at a time - whole sectors, where sixteen single
-// loads a lane would touch each sector again and again (2500 x 1027 in fp32 with the residual: 34 us so, 13 in this way) - and
-// pass it on through shared memory.  A warp's four blocks lie kTurn floats apart and the values of a lane 17: no two lanes of a
-// warp meet in a bank.
+// The same to rows at any alignment, by way of shared memory: the eight lanes of a block write it eight neighbours at a time.  A
+// warp's four blocks lie kTurn floats apart and the values of a lane 17: no two lanes of a warp meet in a bank.
 constexpr int kTurn = kBlock + kBlock / kLane;
-struct Turn {
-  float* s;  // of this lane's block; 4 * kTurn floats a warp
-  int l;
-  __device__ __forceinline__ Turn(float* warp_s, int lane) : s(warp_s + (lane >> 3) * kTurn), l(lane & 7) {}
-  // (every lane of the warp takes part; `any`: this lane's block exists)
-  template <typename T>
-  __device__ __forceinline__ void load(const T* __restrict__ row, int block_col, int width, bool any, float (&y)[kLane]) const {
-    T v[kLane];
+template <typename T>  // (every lane of the warp takes part; `any`: this lane's block exists)
+__device__ __forceinline__ void store_any(float* warp_s, int lane, T* __restrict__ row, int block_col, int width, bool any,
+                                          const float (&y)[kLane]) {
+  float* s = warp_s + (lane >> 3) * kTurn;
+  const int l = lane & 7;
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      const int c = block_col + j * 8 + l;
-      v[j] = any && c < width ? row[c] : from_f32<T>(0.f);
-    }
+  for (int e = 0; e < kLane; ++e) s[l * (kLane + 1) + e] = y[e];
+  __syncwarp();
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) s[j * 8 + l + (j >> 1)] = to_f32<T>(v[j]);
-    __syncwarp();
-#pragma unroll
-    for (int e = 0; e < kLane; ++e) y[e] = s[l * (kLane + 1) + e];
-    __syncwarp();
+  for (int j = 0; j < kLane; ++j) {
+    const int c = block_col + j * 8 + l;
+    if (any && c < width) row[c] = from_f32<T>(s[j * 8 + l + (j >> 1)]);
   }
-  template <typename T>
-  __device__ __forceinline__ void store(T* __restrict__ row, int block_col, int width, bool any, const float (&y)[kLane]) const {
-#pragma unroll
-    for (int e = 0; e < kLane; ++e) s[l * (kLane + 1) + e] = y[e];
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      const int c = block_col + j * 8 + l;
-      if (any && c < width) row[c] = from_f32<T>(s[j * 8 + l + (j >> 1)]);
-    }
-    __syncwarp();
-  }
-};
+  __syncwarp();
+}
 
 // Sixteen values in e4m3 to a row whose start is on a 16-byte boundary; nothing past `width` is written.
 __device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int width, const float (&y)[kLane], float inverse) {
@@ -153,7 +173,9 @@ __device__ __forceinline__ void store16(uint8_t* __restrict__ row, int col, int 
 __device__ __forceinline__ uint32_t top_of(const float (&y)[kLane]) {
   float top = fabsf(y[0]);
 #pragma unroll
-  for (int e = 1; e < kLane; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(y[e])));
+  for (int e = 1; e + 1 < kLane; e += 2)
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(fabsf(y[e])), "f"(fabsf(y[e + 1])));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(y[kLane - 1])));
   return __float_as_uint(top);
 }
 

@@ -5,6 +5,8 @@
 // The inner sums are tcgen05 products (kind::f8f6f4, fp32 accumulators in TMEM); a block's product leaves TMEM once, is scaled
 // and added up in fp32 registers, while the tensor cores work on the next block in the other half of TMEM.  Any fp32 scales
 // therefore serve, not only powers of two, and no sum is longer than 128 products before it is scaled.
+#include <type_traits>
+
 #include "fp8.cuh"
 #include "tc_tma_host.cuh"
 
@@ -68,7 +70,8 @@ template <int NT>
 struct FewRows {
   static constexpr int kStageBytes = 128 * 128 + NT * 128;
   static constexpr int kStages = 6;
-  static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
+  static constexpr int kBuffers = 4;  // products on their way home
+  static constexpr int kTmemCols = kBuffers * NT;
   static constexpr size_t kSmem = 1024 + kStages * kStageBytes;
   static_assert(kStages * kStageBytes >= NT * 128 * 4, "the sums of a split wait in the stages' memory");
 };
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
                                                          const MatmulArgs g) {
   using C = FewRows<NT>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2];
+  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[C::kBuffers], s_tempty[C::kBuffers];
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;  // a wait ran out: nothing waits any more, and the results are NaN
   __shared__ __align__(16) float s_scale[2][NT];
@@ -96,7 +99,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
         ptx::mbar_init(&s_full[i], 1);
         ptx::mbar_init(&s_empty[i], 1);
       }
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < C::kBuffers; ++i) {
         ptx::mbar_init(&s_tfull[i], 1);
         ptx::mbar_init(&s_tempty[i], 4);
       }
@@ -119,6 +122,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
     *dead = 1;
     return false;
   };
+  ptx::griddep_launch();
   ptx::griddep_wait();
 
   float acc[NT];
@@ -145,8 +149,8 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
     const uint32_t base = ptx::smem_u32(stages);
     int i = 0;
     for (; i < nkb; ++i) {
-      const int st = i % C::kStages, buf = i & 1;
-      if (!wait(s_tempty[buf], ((i >> 1) & 1) ^ 1, kGiveUpTmemEmpty)) break;
+      const int st = i % C::kStages, buf = i % C::kBuffers;
+      if (!wait(s_tempty[buf], ((i / C::kBuffers) & 1) ^ 1, kGiveUpTmemEmpty)) break;
       if (!wait(s_full[st], (i / C::kStages) & 1, kGiveUpFull)) break;
       ptx::tc_fence_after();
       const uint32_t w = base + st * C::kStageBytes;
@@ -171,11 +175,11 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
     Scales<S> next = scales_of(1);
     asm volatile("bar.sync 1, 128;" ::: "memory");
     for (int i = 0; i < nkb; ++i) {
-      const int buf = i & 1;
+      const int buf = i % C::kBuffers, turn = i & 1;
       const Scales<S> after = scales_of(i + 2);
-      if (t < NT) s_scale[buf ^ 1][t] = next.product();
+      if (t < NT) s_scale[turn ^ 1][t] = next.product();
       next = after;
-      wait(s_tfull[buf], (i >> 1) & 1, kGiveUpTmemFull);
+      wait(s_tfull[buf], (i / C::kBuffers) & 1, kGiveUpTmemFull);
       ptx::tc_fence_after();
       constexpr int P = NT < 32 ? 16 : 32;
 #pragma unroll
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int j = 0; j < P; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(&s_scale[buf][c + j]);
+          const float4 s = *reinterpret_cast<const float4*>(&s_scale[turn][c + j]);
           acc[c + j] = fmaf(__uint_as_float(r[j]), s.x, acc[c + j]);
           acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]), s.y, acc[c + j + 1]);
           acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]), s.z, acc[c + j + 2]);
@@ -289,6 +293,32 @@ struct OutRing {
   __device__ __forceinline__ static void put(uint32_t at, int lane, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((piece ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
+  }
+  // The same without the TMA, for rows that do not start on 16-byte boundaries: lanes along the columns, a row at a time.
+  template <typename Out>
+  __device__ __forceinline__ static void write(uint32_t at, int lane, Out* out, int64_t ld, int rows, int cols) {
+    constexpr int kCols = 128 / sizeof(Out);
+    using Word = typename std::conditional<sizeof(Out) == 2, uint16_t, uint32_t>::type;
+    constexpr int kEach = kCols / 32, kRows = 8;
+    __syncwarp();
+    for (int r0 = 0; r0 < rows; r0 += kRows) {
+      Word v[kRows][kEach];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int c = 0; c < kEach; ++c) {
+          const int byte = (lane + 32 * c) * (int)sizeof(Out);
+          const uint32_t from = at + (r0 + r) * 128 + (((byte >> 4) ^ r) << 4) + (byte & 15);
+          if constexpr (sizeof(Out) == 2) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[r][c]) : "r"(from));
+          else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[r][c]) : "r"(from));
+        }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int c = 0; c < kEach; ++c)
+          if (r0 + r < rows && lane + 32 * c < cols) reinterpret_cast<Word*>(out)[(r0 + r) * ld + lane + 32 * c] = v[r][c];
+    }
+    __syncwarp();
   }
   __device__ __forceinline__ static void send(uint32_t at, int lane, const CUtensorMap* map, int x, int y) {
     ptx::fence_proxy_async_smem();
@@ -403,6 +433,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     *dead = 1;
     return false;
   };
+  ptx::griddep_launch();
   ptx::griddep_wait();
 
   if (warp < 4) {
@@ -490,30 +521,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j].x = acc[j].y = __uint_as_float(0x7fffffffu);
       }
-      if (g.out_tma) {
-        constexpr int kCols = 128 / sizeof(Out);
-        const int y = at.m0 + row - lane;
+      constexpr int kCols = 128 / sizeof(Out);
+      const int y = at.m0 + row - lane;
 #pragma unroll
-        for (int c = 0; c < 128; c += kCols) {
-          if (y >= g.M || n0 + c >= g.N) break;  // (the same for the whole warp: a store does not begin past the matrix)
-          const uint32_t to = ring.next(lane);
+      for (int c = 0; c < 128; c += kCols) {
+        if (y >= g.M || n0 + c >= g.N) break;  // (the same for the whole warp: a store does not begin past the matrix)
+        const uint32_t to = ring.next(lane);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float2* v = acc + c / 2 + k * (16 / sizeof(Out) / 2);
-            if constexpr (sizeof(Out) == 2)
-              OutRing::put(to, lane, k, ptx::pack_bf16(v[0].x, v[0].y), ptx::pack_bf16(v[1].x, v[1].y), ptx::pack_bf16(v[2].x, v[2].y),
-                           ptx::pack_bf16(v[3].x, v[3].y));
-            else
-              OutRing::put(to, lane, k, __float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
-          }
-          OutRing::send(to, lane, &map_o, n0 + c, y);
+        for (int k = 0; k < 8; ++k) {
+          const float2* v = acc + c / 2 + k * (16 / sizeof(Out) / 2);
+          if constexpr (sizeof(Out) == 2)
+            OutRing::put(to, lane, k, ptx::pack_bf16(v[0].x, v[0].y), ptx::pack_bf16(v[1].x, v[1].y), ptx::pack_bf16(v[2].x, v[2].y),
+                         ptx::pack_bf16(v[3].x, v[3].y));
+          else
+            OutRing::put(to, lane, k, __float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
         }
-      } else if (mine) {
-        Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n0;
-        const int width = min(g.N - n0, 128);
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c < width) out[c] = from_f32<Out>(c & 1 ? acc[c / 2].y : acc[c / 2].x);
+        if (g.out_tma) OutRing::send(to, lane, &map_o, n0 + c, y);
+        else OutRing::write(to, lane, static_cast<Out*>(g.out) + y * g.ld_out + n0 + c, g.ld_out, (int)min(g.M - y, (int64_t)32), g.N - n0 - c);
       }
     }
     if (lane == 0) ptx::tma_store_wait_all();
@@ -604,6 +628,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
     *dead = 1;
     return false;
   };
+  ptx::griddep_launch();
   ptx::griddep_wait();
 
   if (warp == 0 || warp == 2) {  // tokens, weights
@@ -755,26 +780,20 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
           for (int j = 0; j < kCols; ++j) r[j] = 0x7fffffffu;
         }
         if (y >= g.M || at.n0 + c >= g.N) continue;  // (the same for the whole warp: a store does not begin past the matrix)
-        if (g.out_tma) {
-          const uint32_t to = ring.next(lane);
+        const uint32_t to = ring.next(lane);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t* v = r + k * (kCols / 8);
-            if constexpr (sizeof(Out) == 2) {
-              const auto two = [&](int i) { return ptx::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])); };
-              OutRing::put(to, lane, k, two(0), two(1), two(2), two(3));
-            } else {
-              OutRing::put(to, lane, k, v[0], v[1], v[2], v[3]);
-            }
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t* v = r + k * (kCols / 8);
+          if constexpr (sizeof(Out) == 2) {
+            const auto two = [&](int i) { return ptx::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])); };
+            OutRing::put(to, lane, k, two(0), two(1), two(2), two(3));
+          } else {
+            OutRing::put(to, lane, k, v[0], v[1], v[2], v[3]);
           }
-          OutRing::send(to, lane, &map_o, at.n0 + c, y);
-        } else if (y + lane < g.M) {
-          Out* out = static_cast<Out*>(g.out) + (int64_t)(y + lane) * g.ld_out + at.n0 + c;
-          const int width = min(g.N - at.n0 - c, kCols);
-#pragma unroll
-          for (int j = 0; j < kCols; ++j)
-            if (j < width) out[j] = from_f32<Out>(__uint_as_float(r[j]));
         }
+        const int n = at.n0 + c;
+        if (g.out_tma) OutRing::send(to, lane, &map_o, n, y);
+        else OutRing::write(to, lane, static_cast<Out*>(g.out) + y * g.ld_out + n, g.ld_out, (int)min(g.M - y, (int64_t)32), g.N - n);
       }
     }
     if (lane == 0) ptx::tma_store_wait_all();
@@ -830,17 +849,13 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
 
 template <typename Out, typename S>
 int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
-  if (g.M > 64) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
-  const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : 64;
+  if (g.M > 32) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
+  const int nt = g.M <= 16 ? 16 : 32;
   CUtensorMap map_w, map_x;
   int rc = encode_bytes(&map_w, b, g.N, K, ld_b, 128);
   if (rc == MVPA_OK) rc = encode_bytes(&map_x, a, g.M, K, ld_a, nt);
   if (rc != MVPA_OK) return rc;
-  switch (nt) {
-    case 16: return run_few<16, Out, S>(map_w, map_x, g, s);
-    case 32: return run_few<32, Out, S>(map_w, map_x, g, s);
-    default: return run_few<64, Out, S>(map_w, map_x, g, s);
-  }
+  return nt == 16 ? run_few<16, Out, S>(map_w, map_x, g, s) : run_few<32, Out, S>(map_w, map_x, g, s);
 }
 
 }  // namespace

@@ -11,26 +11,40 @@ using namespace fp8;
 
 constexpr int kThreads = 256;
 
-// Row blocks are numbered along the rows; eight lanes take one.
+// Row blocks are numbered along the rows; eight lanes take one.  The row is the number by the blocks of a row: for numbers below
+// 2^31 a product with a multiplier that the host forms (n / d = (umulhi(n, m) + n) >> s with s = ceil log2 d and
+// m = floor(2^32 (2^s - d) / d) + 1), for more a division.
+struct Units {
+  int64_t rows;
+  int width, blocks;
+  uint32_t mul, shift;
+  bool small;
+  Units(int64_t r, int w) : rows(r), width(w), blocks((w + kBlock - 1) / kBlock), shift(0) {
+    while ((1u << shift) < (uint32_t)blocks) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - blocks)) / blocks + 1);
+    small = (r * blocks + kThreads / 8) < ((int64_t)1 << 31);
+  }
+  unsigned grid() const { return (unsigned)((rows * blocks + kThreads / 8 - 1) / (kThreads / 8)); }
+};
 struct Unit {
   int64_t row;
   int col;  // of this lane
   int block;
   bool any;
 };
-__device__ __forceinline__ Unit unit_of(int64_t rows, int width) {
-  const int blocks = (width + kBlock - 1) / kBlock;
+__device__ __forceinline__ Unit unit_of(const Units& g) {
   const int64_t u = (int64_t)blockIdx.x * (kThreads / 8) + threadIdx.x / 8;
   Unit t;
-  if (rows * blocks <= 0x7fffffff) {  // (a 32-bit division where that serves)
-    t.row = (uint32_t)u / (uint32_t)blocks;
-    t.block = (int)((uint32_t)u - (uint32_t)t.row * (uint32_t)blocks);
+  if (g.small) {
+    const uint32_t row = (__umulhi((uint32_t)u, g.mul) + (uint32_t)u) >> g.shift;
+    t.row = row;
+    t.block = (int)((uint32_t)u - row * (uint32_t)g.blocks);
   } else {
-    t.row = u / blocks;
-    t.block = (int)(u - t.row * blocks);
+    t.row = u / g.blocks;
+    t.block = (int)(u - t.row * g.blocks);
   }
   t.col = t.block * kBlock + (threadIdx.x & 7) * kLane;
-  t.any = t.row < rows;
+  t.any = t.row < g.rows;
   return t;
 }
 
@@ -45,25 +59,24 @@ __device__ __forceinline__ void write_unit(const Unit& t, const float (&y)[kLane
 // A lane's values of one block.
 template <typename T, bool VEC>
 __device__ __forceinline__ void read_unit(const T* __restrict__ x, int64_t ld, const Unit& t, int width, float (&y)[kLane]) {
-  if constexpr (VEC) {
-    Raw<T> raw = {};
-    if (t.any && t.col < width) raw.load(x + t.row * ld, t.col, width);
-    raw.get(y);
-  } else {
-    __shared__ float s_turn[kThreads / 32][4 * kTurn];
-    Turn(s_turn[threadIdx.x / 32], threadIdx.x & 31).load(x + t.row * ld, t.block * kBlock, width, t.any, y);
+  Raw<T> raw = {};
+  if (t.any && t.col < width) {
+    if constexpr (VEC) raw.load(x + t.row * ld, t.col, width);
+    else raw.load_any(x + t.row * ld, t.col, width);
   }
+  raw.get(y);
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, int64_t ld_x, uint8_t* __restrict__ q,
                                                                  int64_t ld_q, uint8_t* __restrict__ scales, int64_t ld_s,
-                                                                 int64_t rows, int width) {
+                                                                 const Units g) {
+  ptx::griddep_launch();
   ptx::griddep_wait();
-  const Unit t = unit_of(rows, width);
+  const Unit t = unit_of(g);
   float y[kLane];
-  read_unit<T, VEC>(x, ld_x, t, width, y);
-  write_unit(t, y, q, ld_q, scales, ld_s, width);
+  read_unit<T, VEC>(x, ld_x, t, g.width, y);
+  write_unit(t, y, q, ld_q, scales, ld_s, g.width);
 }
 
 // silu(g) u = g / (1 + e^-g) u of two numbers, from e = e^-|g| <= 1 so that nothing overflows: 1 / (1 + e), or e / (1 + e) where
@@ -93,19 +106,20 @@ __device__ __forceinline__ float2 silu_mul(float2 g, float2 u) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) silu_mul_fp8_kernel(const T* __restrict__ gate, const T* __restrict__ up, int64_t ld_in,
                                                                 uint8_t* __restrict__ q, int64_t ld_q, uint8_t* __restrict__ scales,
-                                                                int64_t ld_s, int64_t rows, int width) {
+                                                                int64_t ld_s, const Units g) {
+  ptx::griddep_launch();
   ptx::griddep_wait();
-  const Unit t = unit_of(rows, width);
+  const Unit t = unit_of(g);
   float y[kLane], u[kLane];
-  read_unit<T, VEC>(gate, ld_in, t, width, y);
-  read_unit<T, VEC>(up, ld_in, t, width, u);
+  read_unit<T, VEC>(gate, ld_in, t, g.width, y);
+  read_unit<T, VEC>(up, ld_in, t, g.width, u);
 #pragma unroll
   for (int e = 0; e < kLane; e += 2) {
     const float2 v = silu_mul(make_float2(y[e], y[e + 1]), make_float2(u[e], u[e + 1]));
     y[e] = v.x;
     y[e + 1] = v.y;
   }
-  write_unit(t, y, q, ld_q, scales, ld_s, width);
+  write_unit(t, y, q, ld_q, scales, ld_s, g.width);
 }
 
 // One CTA per block of 128 x 128: eight lanes a row, 32 rows at a time, four times; the values wait in registers for the
@@ -116,6 +130,7 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const T* __re
                                                                    int64_t rows, int width) {
   constexpr int kTimes = kBlock / (kThreads / 8);
   __shared__ uint32_t s_top[kThreads / 32];
+  ptx::griddep_launch();
   ptx::griddep_wait();
   const int64_t row0 = (int64_t)blockIdx.y * kBlock + threadIdx.x / 8;
   Unit t[kTimes];
@@ -143,35 +158,49 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const T* __re
   if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * ld_s + blockIdx.x] = (uint8_t)byte;
 }
 
-// y = rmsnorm(h) * w with h = x (+ a, in T as in rmsnorm_kernel); h written out, y to e4m3 without a rounding in between.  One
-// warp per row, NV times sixteen values a lane, which stay in registers in T between the sum of squares and the scaling; all
-// loads of a row are on their way before the first is used.
+// y = rmsnorm(h) * w with h = x (+ a, in T as in rmsnorm_kernel); h written out, y to e4m3 without a rounding in between.  A warp
+// has a row, NV times sixteen values a lane, which stay in registers in T between the sum of squares and the scaling.  AHEAD, for
+// aligned rows of up to 1024 values in fp32: resident warps that load their next row while they work on this one, the weight in
+// registers (20000 x 1000 with the residual: 46.5 us for 58.6 with a row a warp).  In bf16, twice the arithmetic a byte, that takes
+// registers from too many warps (65536 x 768: 86 us for 65): there and for longer rows each warp has one row.
+constexpr int kNormWarps = 4;
+
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(kWarpsPerCta * 32) rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ a,
-                                                                        const T* __restrict__ w, T* __restrict__ h_out,
-                                                                        uint8_t* __restrict__ q, int64_t ld_q,
-                                                                        uint8_t* __restrict__ scales, int64_t ld_s, int64_t rows,
-                                                                        int E, float eps) {
-  __shared__ float s_turn[VEC ? 1 : kWarpsPerCta][VEC ? 1 : 4 * kTurn];
+constexpr bool kNormAhead = VEC && sizeof(T) == 4 && NV <= 2;
+template <typename T, int NV, bool VEC>
+constexpr int kNormCtas = kNormAhead<T, NV, VEC> ? (NV == 1 ? 5 : 3) : NV * sizeof(T) <= 2 ? 10 : NV * sizeof(T) <= 4 ? 8 : NV * sizeof(T) <= 8 ? 5 : 2;
+
+template <typename T, int NV, bool VEC>
+__global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ a,
+                                                                                        const T* __restrict__ w, T* __restrict__ h_out,
+                                                                                        uint8_t* __restrict__ q, int64_t ld_q,
+                                                                                        uint8_t* __restrict__ scales, int64_t ld_s,
+                                                                                        int64_t rows, int E, float eps) {
+  constexpr bool AHEAD = kNormAhead<T, NV, VEC>;
+  __shared__ float s_turn[VEC ? 1 : kNormWarps][VEC ? 1 : 4 * kTurn];
+  ptx::griddep_launch();
   ptx::griddep_wait();
-  const int64_t row = (int64_t)blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const int64_t at = row * E;
-  const Turn turn(s_turn[VEC ? 0 : threadIdx.x >> 5], lane);
+  const int64_t step = (int64_t)gridDim.x * kNormWarps;
   const auto col_of = [&](int i) { return (i * 32 + lane) * kLane; };
-  const auto block_of = [&](int i) { return (i * 4 + (lane >> 3)) * kBlock; };
-  Raw<T> raw[NV] = {};
-  float ss = 0.f;
-  if constexpr (VEC) {
+  const auto load = [&](Raw<T>(&r)[NV], const T* p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (col_of(i) < E) raw[i].load(x + at, col_of(i), E);
+      if (col_of(i) < E) {
+        if constexpr (VEC) r[i].load(p, col_of(i), E);
+        else r[i].load_any(p, col_of(i), E);
+      }
+  };
+  int64_t row = (int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
+  Raw<T> raw[NV] = {}, more[NV] = {}, gain[AHEAD ? NV : 1] = {};
+  if (row < rows) {
+    load(raw, x + row * E);
+    if (a != nullptr) load(more, a + row * E);
+    if constexpr (AHEAD) load(gain, w);
+  }
+  for (; row < rows; row += step) {
+    const int64_t at = row * E;
     if (a != nullptr) {
-      Raw<T> more[NV] = {};
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (col_of(i) < E) more[i].load(a + at, col_of(i), E);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float v[kLane], b[kLane];
@@ -180,58 +209,62 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) rmsnorm_fp8_kernel(const T*
 #pragma unroll
         for (int e = 0; e < kLane; ++e) v[e] += b[e];
         raw[i].pack(v);  // (rounds to T)
-        if (h_out != nullptr && col_of(i) < E) raw[i].store(h_out + at, col_of(i), E);
       }
-    } else if (h_out != nullptr) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (col_of(i) < E) raw[i].store(h_out + at, col_of(i), E);
     }
-  } else {
+    float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i * 32 * kLane >= E) break;  // (the same for the whole warp)
-      const bool any = block_of(i) < E;
-      float v[kLane], b[kLane];
-      turn.load(x + at, block_of(i), E, any, v);
-      if (a != nullptr) {
-        turn.load(a + at, block_of(i), E, any, b);
-#pragma unroll
-        for (int e = 0; e < kLane; ++e) v[e] += b[e];
-      }
-      raw[i].pack(v);
+      float v[kLane];
       raw[i].get(v);
-      if (h_out != nullptr) turn.store(h_out + at, block_of(i), E, any, v);
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) ss = fmaf(v[e], v[e], ss);
     }
-  }
+    Raw<T> mine[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float v[kLane];
-    raw[i].get(v);
-#pragma unroll
-    for (int e = 0; e < kLane; ++e) ss = fmaf(v[e], v[e], ss);
-  }
-  const float rstd = rsqrtf(warp_sum(ss) / (float)E + eps);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (i * 32 * kLane >= E) break;
-    const int col = col_of(i);
-    float y[kLane], g[kLane];
-    if constexpr (VEC) {
-      Raw<T> gain = {};
-      if (col < E) gain.load(w, col, E);
-      gain.get(g);
-    } else {
-      turn.load(w, block_of(i), E, block_of(i) < E, g);
+    for (int i = 0; i < NV; ++i) mine[i] = raw[i];
+    if (AHEAD && row + step < rows) {
+      load(raw, x + at + step * E);
+      if (a != nullptr) load(more, a + at + step * E);
     }
-    raw[i].get(y);
+    if (h_out != nullptr) {
 #pragma unroll
-    for (int e = 0; e < kLane; ++e) y[e] = col + e < E ? y[e] * rstd * g[e] : 0.f;  // (past the end 0 * rstd would be NaN where rstd is)
-    const uint32_t byte = scale_byte(max8(top_of(y)));
-    if (col < E) {
-      store16(q + row * ld_q, col, E, y, inverse_scale(byte));
-      if ((lane & 7) == 0) scales[row * ld_s + col / kBlock] = (uint8_t)byte;
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (VEC) {
+          if (col_of(i) < E) mine[i].store(h_out + at, col_of(i), E);
+        } else {
+          if (i * 32 * kLane >= E) break;  // (the same for the whole warp)
+          float v[kLane];
+          mine[i].get(v);
+          store_any(s_turn[threadIdx.x >> 5], lane, h_out + at, (i * 4 + (lane >> 3)) * kBlock, E, col_of(i) / kBlock * kBlock < E, v);
+        }
+      }
     }
+    const float rstd = rsqrtf(warp_sum(ss) / (float)E + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i * 32 * kLane >= E) break;
+      const int col = col_of(i);
+      float y[kLane], g[kLane];
+      if constexpr (AHEAD) {
+        gain[i].get(g);
+      } else {
+        Raw<T> one = {};
+        if (col < E) {
+          if constexpr (VEC) one.load(w, col, E);
+          else one.load_any(w, col, E);
+        }
+        one.get(g);
+      }
+      mine[i].get(y);
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) y[e] = col + e < E ? y[e] * rstd * g[e] : 0.f;  // (past the end 0 * rstd would be NaN where rstd is)
+      const uint32_t byte = scale_byte(max8(top_of(y)));
+      if (col < E) {
+        store16(q + row * ld_q, col, E, y, inverse_scale(byte));
+        if ((lane & 7) == 0) scales[row * ld_s + col / kBlock] = (uint8_t)byte;
+      }
+    }
+    if constexpr (!AHEAD) break;
   }
 }
 
@@ -272,18 +305,14 @@ int check_input(const char* what, const void* p, int64_t ld, int32_t width, int3
   return MVPA_OK;
 }
 
-unsigned units_grid(int64_t rows, int width) {
-  return (unsigned)((rows * ((width + kBlock - 1) / kBlock) + kThreads / 8 - 1) / (kThreads / 8));
-}
-
 template <typename T>
 int run_quantize(const void* x, int64_t ld_x, void* q, int64_t ld_q, void* scales, int64_t ld_s, int64_t rows, int width, int tall,
                  cudaStream_t s) {
   const bool vec = vectors<T>(x, ld_x);
   if (tall == 1) {
-    const unsigned grid = units_grid(rows, width);
-    MVPA_CUDA_CHECK(launch_dependent(1, vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, grid, kThreads, 0, s,
-                                     (const T*)x, ld_x, (uint8_t*)q, ld_q, (uint8_t*)scales, ld_s, rows, width));
+    const Units g(rows, width);
+    MVPA_CUDA_CHECK(launch_dependent(1, vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, g.grid(), kThreads, 0, s,
+                                     (const T*)x, ld_x, (uint8_t*)q, ld_q, (uint8_t*)scales, ld_s, g));
   } else {
     const dim3 grid((width + kBlock - 1) / kBlock, (unsigned)((rows + kBlock - 1) / kBlock));
     MVPA_CUDA_CHECK(launch_dependent(1, vec ? quantize_blocks_kernel<T, true> : quantize_blocks_kernel<T, false>, grid, kThreads, 0, s,
@@ -298,9 +327,9 @@ template <typename T>
 int run_silu_mul(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* scales, int64_t ld_s, int64_t rows,
                  int width, cudaStream_t s) {
   const bool vec = vectors<T>(gate, ld_in) && aligned16(up);
-  MVPA_CUDA_CHECK(launch_dependent(1, vec ? silu_mul_fp8_kernel<T, true> : silu_mul_fp8_kernel<T, false>, units_grid(rows, width),
-                                   kThreads, 0, s, (const T*)gate, (const T*)up, ld_in, (uint8_t*)q, ld_q, (uint8_t*)scales, ld_s, rows,
-                                   width));
+  const Units g(rows, width);
+  MVPA_CUDA_CHECK(launch_dependent(1, vec ? silu_mul_fp8_kernel<T, true> : silu_mul_fp8_kernel<T, false>, g.grid(), kThreads, 0, s,
+                                   (const T*)gate, (const T*)up, ld_in, (uint8_t*)q, ld_q, (uint8_t*)scales, ld_s, g));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
@@ -310,9 +339,10 @@ template <typename T, int NV>
 int run_rmsnorm(const void* x, const void* add, const void* w, void* h_out, void* q, int64_t ld_q, void* scales, int64_t ld_s,
                 int64_t rows, int E, float eps, cudaStream_t s) {
   const bool vec = vectors<T>(x, E) && aligned16(w) && (add == nullptr || aligned16(add)) && (h_out == nullptr || aligned16(h_out));
-  const unsigned grid = (unsigned)((rows + kWarpsPerCta - 1) / kWarpsPerCta);
-  MVPA_CUDA_CHECK(launch_dependent(1, vec ? rmsnorm_fp8_kernel<T, NV, true> : rmsnorm_fp8_kernel<T, NV, false>, grid,
-                                   kWarpsPerCta * 32, 0, s, (const T*)x, (const T*)add, (const T*)w, (T*)h_out, (uint8_t*)q, ld_q,
+  const int64_t want = (rows + kNormWarps - 1) / kNormWarps;
+  const int64_t most = kNormAhead<T, NV, true> && vec ? (int64_t)device_sm_count() * kNormCtas<T, NV, true> : want;
+  MVPA_CUDA_CHECK(launch_dependent(1, vec ? rmsnorm_fp8_kernel<T, NV, true> : rmsnorm_fp8_kernel<T, NV, false>,
+                                   (unsigned)(want < most ? want : most), kNormWarps * 32, 0, s, (const T*)x, (const T*)add, (const T*)w, (T*)h_out, (uint8_t*)q, ld_q,
                                    (uint8_t*)scales, ld_s, rows, E, eps));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
@@ -325,6 +355,7 @@ int run_rmsnorm_any(const void* x, const void* add, const void* w, void* h_out, 
   const int nv = (E + 32 * kLane - 1) / (32 * kLane);
   if (nv <= 1) return run_rmsnorm<T, 1>(x, add, w, h_out, q, ld_q, scales, ld_s, rows, E, eps, s);
   if (nv <= 2) return run_rmsnorm<T, 2>(x, add, w, h_out, q, ld_q, scales, ld_s, rows, E, eps, s);
+  if (nv <= 3) return run_rmsnorm<T, 3>(x, add, w, h_out, q, ld_q, scales, ld_s, rows, E, eps, s);
   if (nv <= 4) return run_rmsnorm<T, 4>(x, add, w, h_out, q, ld_q, scales, ld_s, rows, E, eps, s);
   if constexpr (sizeof(T) == 4) return MVPA_ERR_UNSUPPORTED;  // (refused by the caller: rows of at most 2048)
   else return run_rmsnorm<T, 8>(x, add, w, h_out, q, ld_q, scales, ld_s, rows, E, eps, s);
