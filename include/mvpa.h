@@ -302,7 +302,7 @@ int mvpa_rmsnorm_fp8(const void* x, const void* add, const void* weight, void* s
                      int32_t dtype, void* cuda_stream);
 
 /* silu(gate) * up as a pair, from fp32 in one rounding (mvpa_silu_mul rounds silu to the element type
- * in between). */
+ * in between); e^-|gate| below 2^-126 counts as zero. */
 int mvpa_silu_mul_fp8(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* scales,
                       int64_t ld_s, int64_t rows, int32_t width, int32_t dtype, void* cuda_stream);
 
@@ -310,8 +310,9 @@ int mvpa_silu_mul_fp8(const void* gate, const void* up, int64_t ld_in, void* q, 
  * out = A B^T:  out[m, n] = sum_kb a_scales[m, kb] b_scales[n / 128, kb] sum_{k in kb} a[m, k] b[n, k].
  * a (M, K) and b (N, K) in e4m3, bases and rows (ld_a, ld_b) on 16-byte boundaries; scales MVPA_E8M0 or
  * MVPA_F32 (both the same), any strides in elements; out (M, N) MVPA_BF16 or MVPA_F32, leading dimension
- * ld_out.  A block's products are summed in fp32, scaled by the fp32 product of the two scales and summed
- * over the blocks in fp32, in an order that depends on the sizes alone; K = 0 gives zeros.  `status` (may be
+ * ld_out.  All sums are in fp32, in an order that depends on the sizes alone, and rounded once.  A block's
+ * products are scaled by the two scales' product, which for a few rows (up to 32) and for fp32 scales is
+ * formed in fp32: it must not overflow there.  K = 0 gives zeros.  `status` (may be
  * NULL): 64 ints, zeroed by the caller, of which the first is non-zero afterwards if one of the kernel's
  * bounded waits ran out (the results are then NaN); mvpa_workspace_status(status, 256, stream) reads it.
  */

@@ -869,8 +869,9 @@ using namespace mvpa;
 extern "C" int mvpa_matmul_fp8(const void* a, int64_t ld_a, const void* a_scales, int64_t a_stride_m, int64_t a_stride_k, const void* b,
                                int64_t ld_b, const void* b_scales, int64_t b_stride_n, int64_t b_stride_k, int32_t scale_dtype, void* out,
                                int64_t ld_out, int64_t M, int32_t N, int32_t K, int32_t out_dtype, int32_t* status, void* cuda_stream) {
-  if (M < 0 || N < 0 || K < 0 || M > 0x7fffffff) {
-    set_error("mvpa_matmul_fp8: M, N and K must not be negative, M below 2^31 (got %lld, %d, %d)", (long long)M, N, K);
+  constexpr int kMost = 0x7fffffff - 1024;  // (the first place past the last tile is a 32-bit coordinate)
+  if (M < 0 || N < 0 || K < 0 || M > kMost || N > kMost || K > kMost) {
+    set_error("mvpa_matmul_fp8: M, N and K must not be negative, and at most %d (got %lld, %d, %d)", kMost, (long long)M, N, K);
     return MVPA_ERR_SHAPE;
   }
   if ((out_dtype != MVPA_F32 && out_dtype != MVPA_BF16) || (scale_dtype != MVPA_F32 && scale_dtype != MVPA_E8M0)) {

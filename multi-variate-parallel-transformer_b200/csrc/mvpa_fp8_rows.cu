@@ -211,13 +211,16 @@ __global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnor
         raw[i].pack(v);  // (rounds to T)
       }
     }
-    float ss = 0.f;
+    float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float v[kLane];
       raw[i].get(v);
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) ss = fmaf(v[e], v[e], ss);
+      for (int e = 0; e < kLane; e += 2) {
+        squares.x = fmaf(v[e], v[e], squares.x);
+        squares.y = fmaf(v[e + 1], v[e + 1], squares.y);
+      }
     }
     Raw<T> mine[NV];
 #pragma unroll
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnor
         }
       }
     }
-    const float rstd = rsqrtf(warp_sum(ss) / (float)E + eps);
+    const float rstd = rsqrtf(warp_sum(squares.x + squares.y) / (float)E + eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (i * 32 * kLane >= E) break;
@@ -257,7 +260,12 @@ __global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnor
       }
       mine[i].get(y);
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) y[e] = col + e < E ? y[e] * rstd * g[e] : 0.f;  // (past the end 0 * rstd would be NaN where rstd is)
+      for (int e = 0; e < kLane; ++e) y[e] = y[e] * rstd * g[e];
+      if (col + kLane > E) {  // (past the end 0 * rstd is NaN where rstd is)
+#pragma unroll
+        for (int e = 0; e < kLane; ++e)
+          if (col + e >= E) y[e] = 0.f;
+      }
       const uint32_t byte = scale_byte(max8(top_of(y)));
       if (col < E) {
         store16(q + row * ld_q, col, E, y, inverse_scale(byte));

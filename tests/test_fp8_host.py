@@ -69,7 +69,7 @@ def _matmul(a=P, ld_a=128, sa=P, b=P, ld_b=128, sb=P, sdt=3, out=P, ld_out=64, M
 
 def test_matmul_refusals():
     assert _matmul(M=0) == 0 and _matmul(N=0) == 0
-    assert _matmul(M=-1) == -1 and _matmul(K=-1) == -1 and _matmul(M=1 << 31) == -1
+    assert _matmul(M=-1) == -1 and _matmul(K=-1) == -1 and _matmul(M=1 << 31) == -1 and _matmul(K=0x7fffffff, ld_a=1 << 31, ld_b=1 << 31) == -1
     assert _matmul(odt=2) == -2 and _matmul(sdt=1) == -2
     assert _matmul(out=None) == -3 and _matmul(out=P + 1) == -3 and _matmul(ld_out=63) == -3 and _matmul(out=P + 2, odt=0) == -3
     assert _matmul(a=P + 8) == -3 and _matmul(ld_a=136) == -3 and _matmul(ld_b=112) == -3 and _matmul(b=None) == -3
