@@ -685,6 +685,70 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// branches_fp8(q, scales, w_in q, w_in scales, w_out q, w_out scales, bias, r_time, r_chan, window, B, T, C, H, Hkv, D, status): the fused
+//   inference block with its projections in 8 bits (`MVPFormerBlock.fused_branches_fp8`), in the type of `bias`; or None
+PyObject* branches_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 17)) return nullptr;
+  const bool status = a[16] == Py_True;
+  Tensor in[9];
+  for (int i = 0; i < 9; ++i)
+    if (a[i] == Py_None || !take(a[i], in[i])) Py_RETURN_NONE;
+  const Tensor &xq = in[0], &xs = in[1], &iq = in[2], &is = in[3], &oq = in[4], &os = in[5], &bias = in[6], &rt = in[7], &rc = in[8];
+  if (!fp8_inputs({&xq, &xs, &iq, &is, &oq, &os, &bias, &rt, &rc})) Py_RETURN_NONE;
+  int64_t v[7];
+  for (int i = 0; i < 7; ++i) v[i] = PyLong_AsLongLong(a[9 + i]);
+  if (PyErr_Occurred()) return nullptr;
+  Dims d;
+  d.B = v[1]; d.T = v[2]; d.C = v[3]; d.H = v[4]; d.Hkv = v[5]; d.D = v[6];
+  d.N = d.T * d.C; d.KV = d.Hkv * d.D; d.rows = d.B * d.N; d.E = d.H * d.D;
+  const int64_t ld_x = matrix_ld(xq), ld_i = matrix_ld(iq), ld_o = matrix_ld(oq);
+  const int64_t I = iq.dim() == 2 ? (iq.size(0) - d.E - 2 * d.KV) / 2 : 0, es = bias.element_size(), K = d.E + I, kb = blocks_of(K);
+  const auto pair_of = [](const Tensor& q, const Tensor& s, int64_t rows, int64_t width, int64_t tall) {
+    return q.scalar_type() == at::kFloat8_e4m3fn && s.scalar_type() == at::kFloat8_e8m0fnu && q.sizes() == at::IntArrayRef({rows, width}) &&
+           s.sizes() == at::IntArrayRef({(rows + tall - 1) / tall, blocks_of(width)});
+  };
+  if (I <= 0 || d.KV <= 0 || d.rows <= 0 || ld_x == 0 || ld_i == 0 || ld_o == 0 || d.E % kFp8Block != 0 || !bf16_or_fp32(bias) ||
+      d.E + 2 * (d.KV + I) > INT32_MAX || !pair_of(xq, xs, d.rows, d.E, 1) || !pair_of(iq, is, d.E + 2 * (d.KV + I), d.E, kFp8Block) ||
+      !pair_of(oq, os, d.E, K, kFp8Block) || bias.numel() != 3 * d.KV || d.D * es % 16 != 0 || rt.numel() != d.T * d.KV ||
+      rc.numel() != d.C * d.KV || rt.dim() < 2 || rc.dim() < 2 || rt.size(-2) != d.T || rc.size(-2) != d.C)
+    Py_RETURN_NONE;
+  // (the attention reads q, k and v in place: the product's rows have to start on 16-byte boundaries)
+  if ((d.E + 2 * (d.KV + I)) * es % 16 != 0) Py_RETURN_NONE;
+  for (const Tensor* t : {&bias, &rt, &rc})
+    if (!t->is_contiguous() || t->scalar_type() != bias.scalar_type() || !aligned16(t->const_data_ptr())) Py_RETURN_NONE;
+  Tensor out;
+  {
+    const Body body(xq);
+    const auto options = bias.options().requires_grad(false);
+    const Tensor word = status ? at::zeros({64}, options.dtype(at::kInt)) : Tensor();
+    int32_t* w = status ? word.data_ptr<int32_t>() : nullptr;
+    const int dt = dtype_code(bias);
+    const auto product = [&](const Tensor& a, int64_t ld_a, const Tensor& sa, const Tensor& b, int64_t ld_b, const Tensor& sb) {
+      Tensor o = at::empty({a.size(0), b.size(0)}, options);
+      check(api.matmul_fp8(a.const_data_ptr(), ld_a, sa.const_data_ptr(), sa.stride(0), sa.stride(1), b.const_data_ptr(), ld_b,
+                           sb.const_data_ptr(), sb.stride(0), sb.stride(1), MVPA_E8M0, o.data_ptr(), o.size(1), a.size(0), (int32_t)b.size(0),
+                           (int32_t)a.size(1), dt, w, stream_of(a)), "mvpa_matmul_fp8");
+      return o;
+    };
+    const Tensor big = product(xq, ld_x, xs, iq, ld_i, is);  // (rows, E + 2 KV + 2 I)
+    const Tensor att = at::empty({d.rows, d.E}, options);
+    launch_fwd(d.problem(dt, 1.0 / std::sqrt((double)d.D), (int)v[0]), columns(big, 0, d.N, d.D), columns(big, d.E, d.N, d.D),
+               columns(big, d.E + d.KV, d.N, d.D), part(bias, 0), part(bias, d.KV), part(bias, 2 * d.KV), rt, rc, columns(att, 0, d.N, d.D),
+               nullptr, status);
+    const int64_t ld = (K + 15) / 16 * 16, g0 = d.E + 2 * d.KV;
+    const Tensor q = at::empty({d.rows, ld}, options.dtype(at::kFloat8_e4m3fn)), scales = at::empty({d.rows, kb}, options.dtype(at::kFloat8_e8m0fnu));
+    uint8_t *qp = static_cast<uint8_t*>(q.data_ptr()), *sp = static_cast<uint8_t*>(scales.data_ptr());
+    check(api.quantize_fp8(att.const_data_ptr(), d.E, qp, ld, sp, kb, d.rows, (int32_t)d.E, 1, dt, stream_of(xq)), "mvpa_quantize_fp8");
+    check(api.silu_mul_fp8(part(big, g0), part(big, g0 + I), big.stride(0), qp + d.E, ld, sp + d.E / kFp8Block, kb, d.rows, (int32_t)I, dt,
+                           stream_of(xq)), "mvpa_silu_mul_fp8");
+    out = product(K == ld ? q : q.narrow(1, 0, K), ld, scales, oq, ld_o, os);
+    if (status) check(api.fwd_status(w, 256, stream_of(xq)), "mvpa_matmul_fp8 kernel");  // synchronises the stream
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // init(path of libmvpa_b200.so, which is already loaded; the class of the mode that a default device is)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 2)) return nullptr;
@@ -715,7 +779,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init), FAST(attend), FAST(forward), FAST(backward), FAST(plain), FAST(block_forward),
                          FAST(block_backward), FAST(branches), FAST(quantize_fp8), FAST(rmsnorm_fp8), FAST(silu_mul_fp8),
-                         FAST(matmul_fp8), {nullptr, nullptr, 0, nullptr}};
+                         FAST(matmul_fp8), FAST(branches_fp8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "mvpa_host_b200", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -182,6 +182,11 @@ class MVPFormerBlock(torch.nn.Module):
         I = self.mlp.gate_proj.out_features
         N, KV, rows = T * C, Hkv * D, B * T * C
         w_in, w_out = self.fused_weights_fp8()
+        if mvpa_host.usable(pair[0]):
+            out = mvpa_host.module().branches_fp8(*pair, *w_in, *w_out, a.attn_bias.detach().to(dtype), r_time.to(dtype), r_chan.to(dtype),
+                                                  10, B, T, C, H, Hkv, D, attn_mod._CHECK_STATUS)
+            if out is not None:
+                return out
         big = mvpa_ops.matmul_fp8(*pair, *w_in, dtype=dtype)             # (rows, E + 2 KV + 2 I)
         head = lambda c, heads: big[:, c:c + heads * D].view(B, N, heads, D).permute(0, 2, 1, 3)
         att = torch.empty((rows, E), dtype=dtype, device=big.device)

@@ -56,6 +56,17 @@ def test_block_against_the_definitions(cuda, dtype, inner):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("inner", [352, 200, 201])
+def test_native_call_and_python_path_agree(cuda, dtype, inner, monkeypatch):
+    import mvpa_host
+    m, x = _model(dtype, inner=inner).enable_fp8(), _embeds(dtype)
+    with torch.no_grad():
+        native = m(inputs_embeds=x).last_hidden_state.clone()
+        monkeypatch.setattr(mvpa_host, "usable", lambda t: False)
+        assert torch.equal(m(inputs_embeds=x).last_hidden_state, native)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_model_near_itself_in_16_bits(cuda, dtype):
     m, x = _model(dtype), _embeds(dtype)
     with torch.no_grad():
