@@ -2,9 +2,11 @@
 //
 //   out[m, n] = sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in block kb} a[m, k] b[n, k]
 //
-// The inner sums are tcgen05 products (kind::f8f6f4, fp32 accumulators in TMEM); a block's product leaves TMEM once, is scaled
-// and added up in fp32 registers, while the tensor cores work on the next block in the other half of TMEM.  Any fp32 scales
-// therefore serve, not only powers of two, and no sum is longer than 128 products before it is scaled.
+// The inner sums are tcgen05 products of e4m3 with fp32 accumulators in TMEM.  Three kernels, by the number of tokens and the type
+// of the scales (run_matmul has the rule):
+//   few     up to 32 tokens: the weights' rows are the product's M side
+//   many    fp32 scales: a block's product leaves TMEM once, is scaled and added up in fp32 registers, so that any numbers serve
+//   scaled  scales that are powers of two (e8m0): the tensor cores apply them, and a tile's sum stays in TMEM over the whole of K
 #include <type_traits>
 
 #include "fp8.cuh"
@@ -852,6 +854,9 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
 
 template <typename Out, typename S>
 int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
+  // From 33 tokens on the pairs are faster (e8m0, us, pairs of CTAs / few rows with as many columns as there are tokens, up to 128 a
+  // CTA): 132 x 4736 x 768 7.3 / 21.3, 257 x 2048 x 7680 18.5 / 34, 33 x 5000 x 2000 9.4 / 11.2; below, few rows: 22 x 768 x 2496
+  // 9.5 / 6.5, 22 x 2048 x 7680 18 / 13, 22 x 15360 x 2048 13.9 / 8.4 (22 x 4736 x 768: 7.0 / 7.1).
   if (g.M > 32) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
   const int nt = g.M <= 16 ? 16 : 32;
   CUtensorMap map_w, map_x;
