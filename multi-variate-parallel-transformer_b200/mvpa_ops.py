@@ -317,7 +317,7 @@ def quantize_fp8(x, block_rows=1, out=None):
     `block_rows=128` every block of 128 x 128 one (weights).  `out=(q, scales)` writes into the caller's tensors, which may be
     column blocks of wider ones."""
     if _host.usable(x):
-        pair = _host.module().quantize_fp8(x, block_rows, *(out or (None, None)))
+        pair = _host.module().quantize_fp8(x, block_rows, None, None) if out is None else _host.module().quantize_fp8(x, block_rows, *out)
         if pair is not None:
             return pair
     _fp8_inputs("quantize_fp8", x)
@@ -339,7 +339,7 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None):
     dimensions as rows.  h is rounded to x's type, as in `rmsnorm`, and written to `sum_out` (which may be `x`); the normalised
     row goes from fp32 to e4m3 in one rounding.  E up to 4096 in bf16, 2048 in fp32."""
     if _host.usable(x):
-        pair = _host.module().rmsnorm_fp8(x, weight, eps, add, sum_out, *(out or (None, None)))
+        pair = _host.module().rmsnorm_fp8(x, weight, eps, add, sum_out, None, None) if out is None else _host.module().rmsnorm_fp8(x, weight, eps, add, sum_out, *out)
         if pair is not None:
             return pair
     extra = [t for t in (add, sum_out) if t is not None]
@@ -365,7 +365,7 @@ def silu_mul_fp8(gate, up, out=None):
     """silu(gate) * up in 8 bits: (q, scales).  gate, up (rows, width) with unit inner stride (column blocks of a wider buffer
     are fine).  From fp32 to e4m3 in one rounding; `silu_mul` rounds silu(gate) to the type in between, as eager PyTorch does."""
     if _host.usable(gate):
-        pair = _host.module().silu_mul_fp8(gate, up, *(out or (None, None)))
+        pair = _host.module().silu_mul_fp8(gate, up, None, None) if out is None else _host.module().silu_mul_fp8(gate, up, *out)
         if pair is not None:
             return pair
     _fp8_inputs("silu_mul_fp8", gate, up)
