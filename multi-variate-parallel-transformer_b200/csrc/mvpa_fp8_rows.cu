@@ -282,8 +282,9 @@ bool vectors(const void* p, int64_t ld) { return aligned16(p) && ld * (int64_t)s
 
 int check(const char* what, int64_t rows, int32_t width, int32_t dtype, const void* q, int64_t ld_q, const void* scales,
           int64_t ld_s) {
-  if (rows < 0 || width < 0) {
-    set_error("%s: negative sizes (%lld rows of %d)", what, (long long)rows, width);
+  constexpr int kMost = 0x7fffffff - 1024;  // (rows and columns past the last block are still 32-bit numbers)
+  if (rows < 0 || width < 0 || width > kMost) {
+    set_error("%s: sizes must not be negative and a row at most %d wide (%lld rows of %d)", what, kMost, (long long)rows, width);
     return MVPA_ERR_SHAPE;
   }
   if (dtype != MVPA_F32 && dtype != MVPA_BF16) {
@@ -299,7 +300,7 @@ int check(const char* what, int64_t rows, int32_t width, int32_t dtype, const vo
     set_error("%s: the scales' leading dimension is shorter than a row's blocks", what);
     return MVPA_ERR_SHAPE;
   }
-  if (rows > (int64_t)0x7fffffff * 8 / ((width + kBlock - 1) / kBlock)) {
+  if (rows > kMost || rows > (int64_t)0x7fffffff * 8 / ((width + kBlock - 1) / kBlock)) {
     set_error("%s: too many rows (%lld)", what, (long long)rows);
     return MVPA_ERR_SHAPE;
   }

@@ -121,6 +121,8 @@ _SHIPPED = tuple(block_grad.shipped(cls) for cls in (RMSNorm, MVPFormerGQAFlashA
 
 
 class MVPFormerBlock(torch.nn.Module):
+    _fused_fp8 = None      # (of the class: modules pickled before there was an 8-bit path have neither of their own)
+
     def __init__(self, config, layer_idx=None):
         super().__init__()
         self.ln_1 = RMSNorm(config.hidden_size, eps=config.layer_norm_epsilon)
@@ -128,7 +130,6 @@ class MVPFormerBlock(torch.nn.Module):
         self.ln_2 = RMSNorm(config.hidden_size, eps=config.layer_norm_epsilon)   # unused, as in the reference
         self.mlp = LlamaMLP(config)
         self._fused = None
-        self._fused_fp8 = None
 
     def forward(self, hidden_states, positional_embedding, channel_embedding, layer_past=None, attention_mask=None,
                 head_mask=None, encoder_hidden_states=None, encoder_attention_mask=None, use_cache=False,
@@ -263,6 +264,8 @@ class MVPFormerBlock(torch.nn.Module):
 
 
 class MVPFormerModel(torch.nn.Module):
+    _fp8 = False
+
     def __init__(self, config, gradient_checkpointing=False):
         super().__init__()
         self.config = config
@@ -279,7 +282,6 @@ class MVPFormerModel(torch.nn.Module):
         self.gradient_checkpointing = gradient_checkpointing
         self._rel = None
         self._use_graph, self._graphs = False, {}
-        self._fp8 = False
         std = config.initializer_range                                     # `_init_weights` (`:179-188`)
         for m in self.modules():
             if isinstance(m, (torch.nn.Linear, torch.nn.Embedding)):

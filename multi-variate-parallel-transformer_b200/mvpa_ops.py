@@ -393,7 +393,7 @@ def matmul_fp8(a, a_scales, b, b_scales, out=None, dtype=torch.bfloat16):
         if done is not None:
             return done if out is None else out
     what = "matmul_fp8"
-    _fp8_inputs(what, a, a_scales, b, b_scales)
+    _fp8_inputs(what, a, a_scales, b, b_scales, *(() if out is None else (out,)))
     ld_a, ld_b = _fp8_rows(what, a, "a"), _fp8_rows(what, b, "b")
     (M, K), N = a.shape, b.shape[0]
     kb = -(-K // FP8_BLOCK)
@@ -405,8 +405,8 @@ def matmul_fp8(a, a_scales, b, b_scales, out=None, dtype=torch.bfloat16):
                            f"b {tuple(b.shape)} with scales {tuple(b_scales.shape)}")
     if out is None:
         out = torch.empty((M, N), dtype=dtype, device=a.device)
-    elif out.shape != (M, N) or out.device != a.device:
-        raise RuntimeError(f"matmul_fp8: out must be {(M, N)} on {a.device}, got {tuple(out.shape)} on {out.device}")
+    elif out.shape != (M, N):
+        raise RuntimeError(f"matmul_fp8: out must be {(M, N)}, got {tuple(out.shape)}")
     ld_out = _fp8_rows(what, out, "out")
     status = torch.zeros(64, dtype=torch.int32, device=a.device) if _attn._CHECK_STATUS else None
     with _nat.on_device(a.device):

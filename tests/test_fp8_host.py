@@ -46,6 +46,7 @@ def test_quantize_refusals():
     assert _quantize(x=None) == -3 and _quantize(x=P + 1) == -3 and _quantize(ld_x=100) == -3
     assert _quantize(rows=1 << 40) == -1 and "too many" in nat.last_error()
     assert _quantize(rows=(65535 * 128) + 1, block=128) == -1
+    assert _quantize(width=0x7fffffff, ld_x=1 << 31, ld_q=1 << 31, ld_s=1 << 24) == -1 and _quantize(rows=1 << 31) == -1
 
 
 def _norm(x=P, add=None, w=P, h=None, q=P, ld_q=128, s=P, ld_s=1, rows=2, width=128, dtype=1):

@@ -171,3 +171,16 @@ def test_default_device_and_inference_mode(cuda):
         again = ops.quantize_fp8(x.clone())
     for p in (got, again):
         assert torch.equal(p[0].float(), want[0].float()) and torch.equal(p[1].float(), want[1].float())
+
+
+def test_outputs_that_require_a_gradient_are_refused(cuda):
+    a, sa, b, sb = _pairs(3, 64, 128)
+    leaf = torch.zeros(3, 64, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.matmul_fp8(a, sa, b, sb, out=leaf)
+    x = torch.randn(3, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.rmsnorm_fp8(x, torch.ones(64, device="cuda"), 1e-5, sum_out=leaf)
+    with torch.no_grad():
+        ops.matmul_fp8(a, sa, b, sb, out=leaf)
+    assert bool(leaf.detach().ne(0).any())
