@@ -287,12 +287,16 @@ constexpr int kManyThreads = 384;
 // matrix, and lets the warp go on.  Stored from registers a tile of 256 x 256 held its warps for 4200 cycles of 20000.
 struct OutRing {
   uint32_t smem;
+  bool two;  // places, or one
   uint32_t which = 0;
-  // Where the next 128 bytes of columns go; the store before the last has been read.
+  // Where the next 128 bytes of columns go; the store that was there has been read.
   __device__ __forceinline__ uint32_t next(int lane) {
-    if (lane == 0) ptx::tma_store_wait_read<1>();
+    if (lane == 0) {
+      if (two) ptx::tma_store_wait_read<1>();
+      else ptx::tma_store_wait_read<0>();
+    }
     __syncwarp();
-    which ^= 1;
+    which ^= two ? 1 : 0;
     return smem + which * 4096;
   }
   __device__ __forceinline__ static void put(uint32_t at, int lane, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     const int row = (int)rank * 128 + (warp & 3) * 32 + lane, half = (warp - 4) >> 2;
     const uint32_t at_tmem = tmem + ((uint32_t)(warp & 3) << 21) + half * 128;
     const uint32_t tempty[2] = {ptx::cluster_map(ptx::smem_u32(&s_tempty[0]), 0), ptx::cluster_map(ptx::smem_u32(&s_tempty[1]), 0)};
-    OutRing ring = {stages + C::kStages * C::kStageBytes + (warp - 4) * 8192};
+    OutRing ring = {stages + C::kStages * C::kStageBytes + (warp - 4) * 8192, true};
     Ring<2> buf;
     for (uint32_t t = pair; t < tiles; t += pairs) {
       const Tile at = tile_at<256>(t, tiles_n, tiles_m);
@@ -566,19 +570,20 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 // blocks at once.  (For each block, four bytes alike, the three copies took the tensor cores' time as well, 100 cycles for 384 of
 // products: 470 us for 16384 x 15360 x 2048.)
 //
-// Warps: 0 and 2 load tokens and weights, 1 issues, 3 lays the scales out in shared memory, 4 to 7 take the sums home.
+// Warps: 0 and 2 load tokens and weights, 1 issues, 3 lays the scales out in shared memory, 4 to 11 take the sums home, every
+// other 128 bytes of columns each.
 struct ScaledRows {
   static constexpr int kTileN = 192, kHalfN = kTileN / 2;
   static constexpr int kStages = 6;
   static constexpr int kGroup = 4, kGroups = 3;   // blocks that share a word of scales; such groups on their way
   static constexpr int kOperandBytes = 128 * 128 + kHalfN * 128;
   static constexpr int kScaleBytes = 512 + 1024;  // 128 tokens; two groups of 128 weight rows
-  static constexpr int kOutBytes = 4 * 2 * 32 * 128;
+  static constexpr int kOutBytes = (8 + 4) * 32 * 128;  // two places for the warps that have more columns, one for the others
   static constexpr uint32_t kTmemScales = 2 * kTileN, kTmemScaleCols = 16;
   static constexpr size_t kSmem = 1024 + kStages * kOperandBytes + kGroups * kScaleBytes + kOutBytes;
   static_assert(kTmemScales + kGroups * kTmemScaleCols <= 512 && kOperandBytes % 1024 == 0, "");
 };
-constexpr int kScaledThreads = 256;
+constexpr int kScaledThreads = 384;
 
 template <typename Out>
 __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -611,7 +616,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       }
       for (int i = 0; i < 2; ++i) {
         ptx::mbar_init(&s_tfull[i], 1);
-        ptx::mbar_init(&s_tempty[i], 8);
+        ptx::mbar_init(&s_tempty[i], 16);
       }
       ptx::mbar_fence_init();
       s_dead = 0;
@@ -757,9 +762,9 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_sfull[group.at]), 0));
     }
   } else if (warp >= 4) {
-    const int quad = warp - 4;
+    const int quad = warp & 3, group = (warp - 4) >> 2;
     const uint32_t at_tmem = tmem + ((uint32_t)quad << 21);
-    OutRing ring = {outs + quad * 8192};
+    OutRing ring = {outs + (group == 0 ? quad * 8192 : 4 * 8192 + quad * 4096), group == 0};
     Ring<2> buf;
     for (uint32_t t = pair; t < tiles; t += pairs, buf.step()) {
       const Tile at = tile_at<C::kTileN>(t, tiles_n, tiles_m);
@@ -770,12 +775,12 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       const int y = at.m0 + (int)rank * 128 + quad * 32;
       constexpr int kCols = 128 / sizeof(Out);
 #pragma unroll 1
-      for (int c = 0; c < C::kTileN; c += kCols) {
+      for (int c = group * kCols; c < C::kTileN; c += 2 * kCols) {
         uint32_t r[kCols];
         if constexpr (kCols == 64) ptx::tmem_ld64(from + c, r);
         else ptx::tmem_ld32(from + c, r);
         ptx::tmem_ld_wait();
-        if (c + kCols == C::kTileN) {
+        if (c + 2 * kCols >= C::kTileN) {
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_tempty[buf.at]), 0));
