@@ -23,7 +23,8 @@ struct MatmulArgs {
   void* out;
   int64_t ld_out, M;
   int N, KB, per;  // blocks along K, blocks per split
-  int out_tma;     // out's rows are on 16-byte boundaries
+  int splits;      // pairs of CTAs that share a tile
+  int out_tma;     // out's rows start on 16-byte boundaries (1), and end on them too (2)
   int* status;
 };
 
@@ -43,10 +44,10 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, float v) {
   static_cast<Out*>(out)[i] = from_f32<Out>(v);
 }
 
-// The float at `p`'s place in the shared memory of the cluster's CTA `rank`.
-__device__ __forceinline__ float peer_load(const float* p, uint32_t rank) {
+// The float at this place in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_map(ptx::smem_u32(p), rank)) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_map(at, rank)) : "memory");
   return v;
 }
 
@@ -62,6 +63,32 @@ cudaError_t grant_smem(size_t bytes) {
   const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (set == cudaSuccess && device < 64) granted |= (uint64_t)1 << device;
   return set;
+}
+
+// How many clusters of `ctas` CTAs along x (up to eight) the current device holds at once; asked once per device (and thread).
+template <auto kernel>
+cudaError_t resident_clusters(int ctas, int threads, size_t smem, int* clusters) {
+  static thread_local int known[64][9] = {};  // (one more than the number; 0: not asked yet)
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 64 && known[device][ctas] != 0) {
+    *clusters = known[device][ctas] - 1;
+    return cudaSuccess;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas * 64);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg);
+  if (e == cudaSuccess && device < 64) known[device][ctas] = *clusters + 1;
+  return e;
 }
 
 // ---- few rows: 128 weight rows x NT tokens a CTA ----------------------------------------------------------------------------
@@ -230,7 +257,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
     if (inside) {
       for (int j = blockIdx.z; j < NT && m0 + j < g.M; j += splits) {
         float v = 0.f;
-        for (int z = 0; z < splits; ++z) v += peer_load(part + j * 128 + row, z);
+        for (int z = 0; z < splits; ++z) v += peer_load(ptx::smem_u32(part + j * 128 + row), z);
         store_out<Out>(g.out, at + j * g.ld_out, v);
       }
     }
@@ -283,8 +310,8 @@ struct ManyRows {
 constexpr int kManyThreads = 384;
 
 // Results on their way out: a warp puts 32 tokens x 128 bytes of columns into shared memory (in the 128-byte swizzle: a token's
-// 16-byte pieces go to eight different places) and leaves them to the TMA, which writes whole lines, skips what lies past the
-// matrix, and lets the warp go on.  Stored from registers a tile of 256 x 256 held its warps for 4200 cycles of 20000.
+// 16-byte pieces go to eight different places) and leaves them to the TMA, which writes whole lines, skips rows and pieces of
+// 16 bytes past the matrix, and lets the warp go on.  Stored from registers a tile of 256 x 256 held its warps for 4200 cycles of 20000.
 struct OutRing {
   uint32_t smem;
   bool two;  // places, or one
@@ -303,7 +330,9 @@ struct OutRing {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((piece ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
   }
-  // The same without the TMA, for rows that do not start on 16-byte boundaries: lanes along the columns, a row at a time.
+  // Whether the TMA may store `cols` columns from `n` on: it writes whole pieces of 16 bytes, past a row's end too.
+  __device__ __forceinline__ static bool whole(const MatmulArgs& g, int n, int cols) { return g.out_tma == 2 || (g.out_tma == 1 && n + cols <= g.N); }
+  // The same without the TMA, for other rows and their ends: lanes along the columns, a row at a time.
   template <typename Out>
   __device__ __forceinline__ static void write(uint32_t at, int lane, Out* out, int64_t ld, int rows, int cols) {
     constexpr int kCols = 128 / sizeof(Out);
@@ -364,34 +393,34 @@ struct Ring {
 };
 
 // One operand's tiles on their way in: a warp of each CTA loads its CTA's `rows` rows a block; the loads of both count at the barrier
-// of the CTA of rank 0, which the tokens' warp there tells how many bytes to expect.  (One lane that issued both operands' loads
+// of the pair's first CTA, which the tokens' warp there tells how many bytes to expect.  (One lane that issued both operands' loads
 // from a branch of its own needed some 450 cycles a block, more than the products of it.)
 template <int kStages, int kTileN, int kBytes, typename Wait>
 __device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t to, bool tokens, int rows, uint64_t* full, uint64_t* empty,
-                                             uint32_t pair, uint32_t pairs, uint32_t tiles_n, uint32_t tiles_m, const MatmulArgs& g,
+                                             uint32_t pair, uint32_t pairs, uint32_t tiles_n, uint32_t tiles_m, int kb0, int nkb, int* status,
                                              const Wait& wait) {
-  const uint32_t el = ptx::elect_one(), rank = ptx::cluster_rank(), tiles = tiles_n * tiles_m;
-  const uint32_t there = ptx::cluster_map(ptx::smem_u32(full), 0);
+  const uint32_t el = ptx::elect_one(), rank = ptx::cluster_rank(), half = rank & 1, tiles = tiles_n * tiles_m;
+  const uint32_t there = ptx::cluster_map(ptx::smem_u32(full), rank - half);
   Ring<kStages> st;
   uint32_t loads = 0;
   bool on = true;
   for (uint32_t t = pair; t < tiles && on; t += pairs) {
     const Tile at = tile_at<kTileN>(t, tiles_n, tiles_m);
-    const int y = (tokens ? at.m0 : at.n0) + (int)rank * rows;
-    for (int kb = 0; kb < g.KB; ++kb, ++loads, st.step()) {
+    const int y = (tokens ? at.m0 : at.n0) + (int)half * rows;
+    for (int kb = 0; kb < nkb; ++kb, ++loads, st.step()) {
       if (!wait(empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
         on = false;
         break;
       }
-      if (tokens && rank == 0 && el) ptx::mbar_arrive_expect_tx(&full[st.at], 2 * kBytes);
+      if (tokens && half == 0 && el) ptx::mbar_arrive_expect_tx(&full[st.at], 2 * kBytes);
       __syncwarp();
-      ptx::tma_load_2d_pair_w(el, to + st.at * kBytes, map, there + 8 * st.at, kb * 128, y);
+      ptx::tma_load_2d_pair_w(el, to + st.at * kBytes, map, there + 8 * st.at, (kb0 + kb) * 128, y);
     }
   }
-  if (tokens && rank == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one at the end)
+  if (tokens && half == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one at the end)
     const uint32_t n = min(loads, (uint32_t)kStages);
     for (uint32_t k = loads - n; k != loads; ++k)
-      if (!ptx::mbar_wait(&full[k % kStages], (k / kStages) & 1, g.status, kGiveUpDrain)) break;
+      if (!ptx::mbar_wait(&full[k % kStages], (k / kStages) & 1, status, kGiveUpDrain)) break;
   }
 }
 
@@ -449,7 +478,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 || warp == 2) {  // tokens, weights
       load_operand<C::kStages, 256, C::kStageBytes>(warp == 0 ? &map_x : &map_w, stages + (warp == 0 ? 0 : 128 * 128), warp == 0, 128, s_full,
-                                                    s_empty, pair, pairs, tiles_n, tiles_m, g, wait);
+                                                    s_empty, pair, pairs, tiles_n, tiles_m, 0, g.KB, g.status, wait);
     } else if (warp == 1 && rank == 0) {
       const uint32_t el = ptx::elect_one();
       constexpr uint32_t idesc = ptx::make_idesc_e4m3(256, 256);
@@ -465,8 +494,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
         if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
         ptx::tc_fence_after();
         ptx::mma_f8_ss_x4_pair_w(el, tmem + buf.at * 256, a, b, idesc);
-        ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_tfull[buf.at]));
-        ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_empty[st.at]));
+        ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_tfull[buf.at]));
+        ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_empty[st.at]));
         last = st.at;
         last_parity = st.parity;
       }
@@ -545,7 +574,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
           else
             OutRing::put(to, lane, k, __float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
         }
-        if (g.out_tma) OutRing::send(to, lane, &map_o, n0 + c, y);
+        if (OutRing::whole(g, n0 + c, kCols)) OutRing::send(to, lane, &map_o, n0 + c, y);
         else OutRing::write(to, lane, static_cast<Out*>(g.out) + y * g.ld_out + n0 + c, g.ld_out, (int)min(g.M - y, (int64_t)32), g.N - n0 - c);
       }
     }
@@ -570,6 +599,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 // blocks at once.  (For each block, four bytes alike, the three copies took the tensor cores' time as well, 100 cycles for 384 of
 // products: 470 us for 16384 x 15360 x 2048.)
 //
+// A long K and so few tiles that most pairs would have none: the pairs of a cluster share the blocks of a tile and add their sums up
+// through distributed shared memory, in the order of the blocks.
+//
 // Warps: 0 and 2 load tokens and weights, 1 issues, 3 lays the scales out in shared memory, 4 to 11 take the sums home, every
 // other 128 bytes of columns each.
 struct ScaledRows {
@@ -581,11 +613,12 @@ struct ScaledRows {
   static constexpr int kOutBytes = (8 + 4) * 32 * 128;  // two places for the warps that have more columns, one for the others
   static constexpr uint32_t kTmemScales = 2 * kTileN, kTmemScaleCols = 16;
   static constexpr size_t kSmem = 1024 + kStages * kOperandBytes + kGroups * kScaleBytes + kOutBytes;
+  static_assert(kTileN * 128 * 4 <= kStages * kOperandBytes, "the sums of a split wait in the stages' memory");
   static_assert(kTmemScales + kGroups * kTmemScaleCols <= 512 && kOperandBytes % 1024 == 0, "");
 };
 constexpr int kScaledThreads = 384;
 
-template <typename Out>
+template <typename Out, bool SPLIT>
 __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                           const __grid_constant__ CUtensorMap map_x,
                                                                           const __grid_constant__ CUtensorMap map_o, const MatmulArgs g) {
@@ -598,8 +631,11 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
   const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t outs = stages + C::kStages * C::kOperandBytes, scales = outs + C::kOutBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_rank();
-  const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t half = ptx::cluster_rank() & 1, first_rank = SPLIT ? ptx::cluster_rank() - half : 0, split = first_rank >> 1;
+  const uint32_t splits = SPLIT ? (uint32_t)g.splits : 1;
+  const uint32_t pair = blockIdx.x / (2 * splits), pairs = gridDim.x / (2 * splits);  // (SPLIT: a cluster's pairs have one tile)
+  const int kb_first = SPLIT ? (int)split * g.per : 0, nkb = SPLIT ? min(g.KB - kb_first, g.per) : g.KB;
+  const uint16_t both = (uint16_t)(3u << first_rank);
   const uint32_t tiles_n = (uint32_t)(g.N + C::kTileN - 1) / C::kTileN, tiles_m = (uint32_t)((g.M + 255) / 256), tiles = tiles_n * tiles_m;
   if (warp == 0) {
     ptx::prefetch_tensormap(&map_w);
@@ -643,9 +679,10 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
 
   if (warp == 0 || warp == 2) {  // tokens, weights
     load_operand<C::kStages, C::kTileN, C::kOperandBytes>(warp == 0 ? &map_x : &map_w, stages + (warp == 0 ? 0 : 128 * 128), warp == 0,
-                                                          warp == 0 ? 128 : C::kHalfN, s_full, s_empty, pair, pairs, tiles_n, tiles_m, g, wait);
+                                                          warp == 0 ? 128 : C::kHalfN, s_full, s_empty, pair, pairs, tiles_n, tiles_m, kb_first,
+                                                          nkb, g.status, wait);
   } else if (warp == 1) {
-    if (rank == 0) {
+    if (half == 0) {
       // (The loop has to be shorter than a block's 384 cycles of products: four blocks unrolled, their barriers by address, and each
       // block's barrier looked at while the products of the one before are issued.)
       const uint32_t el = ptx::elect_one();
@@ -661,7 +698,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
         if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
         const uint32_t d = tmem + buf.at * C::kTileN;
         bool there = false;
-        for (int kb0 = 0; kb0 < g.KB && on; kb0 += C::kGroup, group.step()) {
+        for (int kb0 = 0; kb0 < nkb && on; kb0 += C::kGroup, group.step()) {
           if (!wait(s_sfull[group.at], group.parity, kGiveUpFull)) {
             on = false;
             break;
@@ -673,7 +710,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
           ptx::tmem_copy_scales_pair_w(el, sb + 4, s + 1024);
 #pragma unroll
           for (uint32_t byte = 0; byte < C::kGroup; ++byte) {
-            if (kb0 + (int)byte >= g.KB) break;
+            if (kb0 + (int)byte >= nkb) break;
             if (!there && !wait(s_full[st.at], st.parity, kGiveUpFull)) {
               on = false;
               break;
@@ -681,23 +718,23 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
             ptx::tc_fence_after();
             const ptx::DescHalves a = {first.lo + st.at * (C::kOperandBytes >> 4), first.hi}, b = {a.lo + (128 * 128 >> 4), first.hi};
             ptx::mma_mxf8_ss_x4_pair_w(el, d, a, b, idesc | (byte << 4) | (byte << 29), sa, sb, kb0 > 0 || byte > 0);
-            ptx::mma_commit_pair_w(el, empty + 8 * st.at);
+            ptx::mma_commit_pair_w(el, both, empty + 8 * st.at);
             last = st.at;
             last_parity = st.parity;
             any = true;
             st.step();
             there = ptx::mbar_test_wait_a(full + 8 * st.at, st.parity);
           }
-          ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_sempty[group.at]));
+          ptx::mma_commit_pair_w(el, both, ptx::smem_u32(&s_sempty[group.at]));
         }
-        if (on) ptx::mma_commit_pair_w(el, ptx::smem_u32(&s_tfull[buf.at]));
+        if (on) ptx::mma_commit_pair_w(el, both, ptx::smem_u32(&s_tfull[buf.at]));
       }
       if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
     }
   } else if (warp == 3) {
     // Word j of lane l: the scales of row 32 j + l over a group of blocks, a byte each.  Four words for this CTA's 128 tokens; six for
     // the tile's 192 weight rows, whose groups of 32 lie in one block of 128 each (lane j loads the word of rows 32 j).
-    const uint8_t *sa = static_cast<const uint8_t*>(g.sa), *sb = static_cast<const uint8_t*>(g.sb);
+    const uint8_t *sa = static_cast<const uint8_t*>(g.sa) + kb_first * g.sa_k, *sb = static_cast<const uint8_t*>(g.sb) + kb_first * g.sb_k;
     const auto words = [](const void* p, int64_t rows, int64_t k) {  // four blocks' scales are an aligned word
       return k == 1 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)rows) & 3) == 0;
     };
@@ -709,18 +746,18 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       const Tile at = tile_at<C::kTileN>(t < tiles ? t : pair, tiles_n, tiles_m);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t m = at.m0 + (int)rank * 128 + 32 * j + lane;
+        const int64_t m = at.m0 + (int)half * 128 + 32 * j + lane;
         row[j] = t < tiles && m < g.M ? sa + m * g.sa_m : nullptr;
       }
       const int n = at.n0 + 32 * lane;
       weights = t < tiles && lane < 6 && n < g.N ? sb + (int64_t)(n / 128) * g.sb_n : nullptr;
     };
     const auto fetch = [&](const uint8_t* p, int64_t k, bool word, uint32_t (&v)[C::kGroup]) {  // (v[0] alone where it is a word)
-      if (word && kb + C::kGroup <= g.KB) {
+      if (word && kb + C::kGroup <= nkb) {
         v[0] = p != nullptr ? *reinterpret_cast<const uint32_t*>(p + kb) : 0u;
       } else {
 #pragma unroll
-        for (int i = 0; i < C::kGroup; ++i) v[i] = p != nullptr && kb + i < g.KB ? p[(kb + i) * k] : 0u;
+        for (int i = 0; i < C::kGroup; ++i) v[i] = p != nullptr && kb + i < nkb ? p[(kb + i) * k] : 0u;
       }
     };
     const auto joined = [&](const uint32_t (&v)[C::kGroup], bool word) { return word ? v[0] : v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24; };
@@ -734,7 +771,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
     settle();
     load();
     for (; t < tiles; group.step()) {
-      const bool whole = kb + C::kGroup <= g.KB;
+      const bool whole = kb + C::kGroup <= nkb;
       uint32_t w[4], v[6];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = joined(token[j], word_a && whole);
@@ -742,7 +779,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
 #pragma unroll
       for (int j = 0; j < 6; ++j) v[j] = __shfl_sync(0xffffffffu, mine, j);
       kb += C::kGroup;
-      if (kb >= g.KB) {
+      if (kb >= nkb) {
         kb = 0;
         t += pairs;
         settle();
@@ -759,7 +796,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       put(to + 1024, v[4], v[5], 0, 0);
       ptx::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_sfull[group.at]), 0));
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_sfull[group.at]), first_rank));
     }
   } else if (warp >= 4) {
     const int quad = warp & 3, group = (warp - 4) >> 2;
@@ -772,7 +809,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       __syncwarp();
       ptx::tc_fence_after();
       const uint32_t from = at_tmem + buf.at * C::kTileN;
-      const int y = at.m0 + (int)rank * 128 + quad * 32;
+      const int y = at.m0 + (int)half * 128 + quad * 32;
       constexpr int kCols = 128 / sizeof(Out);
 #pragma unroll 1
       for (int c = group * kCols; c < C::kTileN; c += 2 * kCols) {
@@ -783,11 +820,17 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
         if (c + 2 * kCols >= C::kTileN) {
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_tempty[buf.at]), 0));
+          if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_tempty[buf.at]), first_rank));
         }
         if (*dead) {
 #pragma unroll
           for (int j = 0; j < kCols; ++j) r[j] = 0x7fffffffu;
+        }
+        if constexpr (SPLIT) {  // (the products that read the stages are finished)
+#pragma unroll
+          for (int j = 0; j < kCols; ++j)
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(stages + ((c + j) * 128 + quad * 32 + lane) * 4), "r"(r[j]) : "memory");
+          continue;
         }
         if (y >= g.M || at.n0 + c >= g.N) continue;  // (the same for the whole warp: a store does not begin past the matrix)
         const uint32_t to = ring.next(lane);
@@ -802,13 +845,47 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
           }
         }
         const int n = at.n0 + c;
-        if (g.out_tma) OutRing::send(to, lane, &map_o, n, y);
+        if (OutRing::whole(g, n, kCols)) OutRing::send(to, lane, &map_o, n, y);
         else OutRing::write(to, lane, static_cast<Out*>(g.out) + y * g.ld_out + n, g.ld_out, (int)min(g.M - y, (int64_t)32), g.N - n);
       }
     }
     if (lane == 0) ptx::tma_store_wait_all();
   }
   __syncwarp();
+  if constexpr (SPLIT) {
+    ptx::cluster_sync();
+    // Each split has its share of the columns, a thread eight columns of a token at a time.
+    const Tile at = tile_at<C::kTileN>(pair, tiles_n, tiles_m);
+    const int row = (warp & 3) * 32 + lane, share = C::kTileN / (int)splits;
+    const int64_t m = at.m0 + (int)half * 128 + row;
+    for (int c = (int)split * share + (warp >> 2) * 8; c < (int)(split + 1) * share && m < g.M; c += kScaledThreads / 128 * 8) {
+      const int n = at.n0 + c;
+      if (n >= g.N) break;
+      float v[8] = {};
+      for (uint32_t z = 0; z < splits; ++z) {
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = peer_load(stages + ((c + j) * 128 + row) * 4, 2 * z + half);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += p[j];
+      }
+      Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n;
+      if (g.out_tma && n + 8 <= g.N) {  // (rows on 16-byte boundaries)
+        if constexpr (sizeof(Out) == 2) {
+          *reinterpret_cast<uint4*>(out) = make_uint4(ptx::pack_bf16(v[0], v[1]), ptx::pack_bf16(v[2], v[3]), ptx::pack_bf16(v[4], v[5]),
+                                                      ptx::pack_bf16(v[6], v[7]));
+        } else {
+          reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + j < g.N) out[j] = from_f32<Out>(v[j]);
+      }
+    }
+    __syncwarp();
+  }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::cluster_sync();  // neither CTA's memory goes while the other's products or barriers use it
@@ -836,6 +913,7 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
   int rc = encode_bytes(&map_w, b, g.N, K, ld_b, kTileN / 2);
   if (rc == MVPA_OK) rc = encode_bytes(&map_x, a, g.M, K, ld_a, 128);
   g.out_tma = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ld_out * (int64_t)sizeof(Out) % 16 == 0;
+  if (g.out_tma && (int64_t)g.N * (int)sizeof(Out) % 16 == 0) g.out_tma = 2;
   if (rc == MVPA_OK && g.out_tma) {
     const uint64_t dims[2] = {(uint64_t)g.N, (uint64_t)g.M}, strides[1] = {(uint64_t)g.ld_out * sizeof(Out)};
     const uint32_t box[2] = {128 / sizeof(Out), 32};
@@ -844,9 +922,25 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
   if (rc != MVPA_OK) return rc;
   const dim3 grid(2 * (unsigned)(tiles < pairs ? tiles : pairs));
   if constexpr (kScaled) {
-    constexpr auto kernel = matmul_scaled_kernel<Out>;
-    MVPA_CUDA_CHECK(grant_smem<kernel>(ScaledRows::kSmem));
-    MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, grid, kScaledThreads, ScaledRows::kSmem, s, map_w, map_x, map_o, g));
+    // Two or four pairs to a tile, as long as all clusters are resident at once: a cluster of eight costs some 2 us more than one of
+    // two, a block 0.2 us.  us with 1 / 2 / 4 pairs: 132 x 2048 x 7680 18.5 / 15.7 / 12.8, 550 x 2048 x 7680 19.2 / 17.0 / two rounds,
+    // 550 x 768 x 4096 12.5 / 12.8 / 11.2; 550 x 768 x 2496 (20 blocks) 10.1 / 11.7 / 10.4.
+    constexpr auto whole = matmul_scaled_kernel<Out, false>, parts = matmul_scaled_kernel<Out, true>;
+    for (int n : {4, 2}) {
+      int most = 0;
+      if (g.splits > 1 || g.KB < 64 - 8 * n) continue;
+      MVPA_CUDA_CHECK(grant_smem<parts>(ScaledRows::kSmem));
+      MVPA_CUDA_CHECK(resident_clusters<parts>(2 * n, kScaledThreads, ScaledRows::kSmem, &most));
+      if (tiles <= most) g.splits = n;
+    }
+    g.per = (g.KB + g.splits - 1) / g.splits;
+    if (g.splits > 1) {
+      MVPA_CUDA_CHECK(launch_dependent(dim3(2 * g.splits), parts, dim3(2 * (unsigned)tiles * g.splits), kScaledThreads, ScaledRows::kSmem, s,
+                                       map_w, map_x, map_o, g));
+    } else {
+      MVPA_CUDA_CHECK(grant_smem<whole>(ScaledRows::kSmem));
+      MVPA_CUDA_CHECK(launch_dependent(dim3(2), whole, grid, kScaledThreads, ScaledRows::kSmem, s, map_w, map_x, map_o, g));
+    }
   } else {
     constexpr auto kernel = matmul_many_kernel<Out, S>;
     MVPA_CUDA_CHECK(grant_smem<kernel>(ManyRows::kSmem));
@@ -909,7 +1003,7 @@ extern "C" int mvpa_matmul_fp8(const void* a, int64_t ld_a, const void* a_scales
     set_error("mvpa_matmul_fp8: the scales are NULL or not aligned to their elements");
     return MVPA_ERR_ALIGNMENT;
   }
-  MatmulArgs g = {a_scales, b_scales, a_stride_m, a_stride_k, b_stride_n, b_stride_k, out, ld_out, M, N, (int)(((int64_t)K + 127) / 128), 0, 0, status};
+  MatmulArgs g = {a_scales, b_scales, a_stride_m, a_stride_k, b_stride_n, b_stride_k, out, ld_out, M, N, (int)(((int64_t)K + 127) / 128), 0, 1, 0, status};
   if (out_dtype == MVPA_BF16)
     return scale_dtype == MVPA_E8M0 ? run_matmul<__nv_bfloat16, uint8_t>(a, ld_a, b, ld_b, K, g, s)
                                     : run_matmul<__nv_bfloat16, float>(a, ld_a, b, ld_b, K, g, s);

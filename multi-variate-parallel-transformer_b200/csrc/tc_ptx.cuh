@@ -380,7 +380,7 @@ __device__ __forceinline__ void mma_f8_ss_x4_w(uint32_t el, uint32_t d_tmem, Des
       "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el)
       : "memory");
 }
-// ---- pairs: one product over two CTAs of a cluster (cta_group::2), issued by the CTA of rank 0 ----
+// ---- pairs: one product over two CTAs of a cluster (cta_group::2: ranks 2 i and 2 i + 1), issued by the first ----
 // M = 256: each CTA stages its 128 rows of A and its half of B's rows, and holds its 128 rows of D in its own TMEM.
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -422,11 +422,12 @@ __device__ __forceinline__ void tma_load_2d_pair_w(uint32_t el, uint32_t smem_ds
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(el)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit_pair_w(uint32_t el, uint32_t bar) {  // the barrier of this place in both CTAs
+// The barrier of this place in each CTA of the cluster whose bit is set.
+__device__ __forceinline__ void mma_commit_pair_w(uint32_t el, uint16_t ctas, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred pe;\n\t.reg .b16 both;\n\tsetp.ne.b32 pe, %1, 0;\n\tmov.b16 both, 3;\n\t"
-      "@pe tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar),
-      "r"(el)
+      "{\n\t.reg .pred pe;\n\tsetp.ne.b32 pe, %1, 0;\n\t"
+      "@pe tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(bar),
+      "r"(el), "h"(ctas)
       : "memory");
 }
 __device__ __forceinline__ void mma_f8_ss_x4_pair_w(uint32_t el, uint32_t d_tmem, DescHalves a, DescHalves b, uint32_t idesc) {

@@ -184,3 +184,44 @@ def test_outputs_that_require_a_gradient_are_refused(cuda):
     with torch.no_grad():
         ops.matmul_fp8(a, sa, b, sb, out=leaf)
     assert bool(leaf.detach().ne(0).any())
+
+
+@pytest.mark.parametrize("M,N,K", [(33, 500, 4096), (100, 300, 4097), (257, 193, 5000), (600, 700, 6200), (1000, 1500, 6200), (200, 2100, 8191),
+                                   (300, 64, 7680), (3000, 700, 6145)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_long_sums_of_whole_numbers(cuda, M, N, K, dtype):
+    """Long K with few tiles, where several pairs of CTAs share a tile's blocks: small whole numbers, whose sums (below 2^24) are
+    exact in fp32, into aligned and odd column blocks; the same bits again."""
+    g = torch.Generator().manual_seed(M + N + K)
+    a, b = (torch.randint(-8, 9, (r, (K + 15) // 16 * 16), generator=g).float().cuda().to(torch.float8_e4m3fn)[:, :K] for r in (M, N))
+    kb = -(-K // 128)
+    sa, sb = (torch.exp2(torch.randint(0, 3, (n, kb), generator=g).float()).cuda().to(torch.float8_e8m0fnu) for n in (M, -(-N // 128)))
+    want = (ref.value(a, sa) @ ref.value(b, sb, 128).t()).to(dtype)
+    for offset, ld in ((0, (N + 7) // 8 * 8), (3, N + 9)):
+        whole = torch.full((M + 1, offset + ld), 5.0, dtype=dtype, device="cuda")
+        out = whole[:M, offset:offset + N]
+        for _ in range(2):
+            ops.matmul_fp8(a, sa, b, sb, out=out)
+            assert torch.equal(out, want)
+        out.fill_(5.0)
+        assert bool((whole == 5).all())
+    sa[M // 2, kb - 1] = float("nan")
+    out = ops.matmul_fp8(a, sa, b, sb, dtype=dtype)
+    assert bool(out[M // 2].isnan().all()) and int(out.isnan().sum()) == N
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fp32_scales", [False, True])
+@pytest.mark.parametrize("M,N", [(1, 5), (20, 131), (40, 3), (200, 100), (300, 700), (2500, 1030), (2500, 1033)])
+def test_rows_that_end_inside_sixteen_bytes(cuda, M, N, dtype, fp32_scales):
+    """Results whose rows start on 16-byte boundaries and end anywhere: what stands behind them stays."""
+    a, sa, b, sb = _pairs(M, N, 256, seed=3)
+    if fp32_scales:
+        sa, sb = sa.float() * 1.25, sb.float() * 0.75
+    ld = (N + 7) // 8 * 8 + 8
+    whole = torch.full((M + 1, ld), 5.0, dtype=dtype, device="cuda")
+    out = whole[:M, :N]
+    ops.matmul_fp8(a, sa, b, sb, out=out)
+    assert torch.equal(out, ops.matmul_fp8(a, sa, b, sb, dtype=dtype))
+    out.fill_(5.0)
+    assert bool((whole == 5).all())
