@@ -304,6 +304,7 @@ struct ManyRows {
   static constexpr int kStages = 5;
   static constexpr int kOutBytes = 8 * 2 * 32 * 128;  // a warp's tokens x 128 bytes of columns, twice
   static constexpr size_t kSmem = 1024 + kStages * kStageBytes + kOutBytes;
+  static_assert(256 * 128 * 4 <= kStages * kStageBytes, "the sums of a split wait in the stages' memory");
 };
 // Four warps that load and issue, eight that add up.  Registers: 384 x 168 at launch, of which the four keep 56 a thread and the
 // eight take 216 (128 x 56 + 256 x 216 = 62464 of 64512).
@@ -392,6 +393,42 @@ struct Ring {
   }
 };
 
+// A tile whose blocks several pairs have summed, a token's columns in the shared memory of the CTA of each pair that holds its rows
+// (sums[column][row]): each pair has its share of the columns, a thread eight of a token at a time, and adds in the order of the
+// blocks.  `group` of `groups`: which 128 threads of the CTA's these are.
+template <typename Out>
+__device__ __forceinline__ void add_splits(uint32_t sums, uint32_t splits, uint32_t split, int columns, uint32_t half, int row, int group,
+                                           int groups, const Tile& at, const MatmulArgs& g) {
+  const int share = columns / (int)splits;
+  const int64_t m = at.m0 + (int)half * 128 + row;
+  for (int c = (int)split * share + group * 8; c < (int)(split + 1) * share && m < g.M; c += groups * 8) {
+    const int n = at.n0 + c;
+    if (n >= g.N) break;
+    float v[8] = {};
+    for (uint32_t z = 0; z < splits; ++z) {
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = peer_load(sums + ((c + j) * 128 + row) * 4, 2 * z + half);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += p[j];
+    }
+    Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n;
+    if (g.out_tma && n + 8 <= g.N) {  // (rows on 16-byte boundaries)
+      if constexpr (sizeof(Out) == 2) {
+        *reinterpret_cast<uint4*>(out) =
+            make_uint4(ptx::pack_bf16(v[0], v[1]), ptx::pack_bf16(v[2], v[3]), ptx::pack_bf16(v[4], v[5]), ptx::pack_bf16(v[6], v[7]));
+      } else {
+        reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < g.N) out[j] = from_f32<Out>(v[j]);
+    }
+  }
+}
+
 // One operand's tiles on their way in: a warp of each CTA loads its CTA's `rows` rows a block; the loads of both count at the barrier
 // of the pair's first CTA, which the tokens' warp there tells how many bytes to expect.  (One lane that issued both operands' loads
 // from a branch of its own needed some 450 cycles a block, more than the products of it.)
@@ -424,7 +461,7 @@ __device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t to
   }
 }
 
-template <typename Out, typename S>
+template <typename Out, typename S, bool SPLIT>
 __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                       const __grid_constant__ CUtensorMap map_x,
                                                                       const __grid_constant__ CUtensorMap map_o, const MatmulArgs g) {
@@ -435,8 +472,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
   __shared__ int s_dead;
   const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_rank();
-  const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t rank = ptx::cluster_rank() & 1, first_rank = SPLIT ? ptx::cluster_rank() - rank : 0, split = first_rank >> 1;
+  const uint32_t splits = SPLIT ? (uint32_t)g.splits : 1;
+  const uint32_t pair = blockIdx.x / (2 * splits), pairs = gridDim.x / (2 * splits);  // (SPLIT: a cluster's pairs have one tile)
+  const int kb_first = SPLIT ? (int)split * g.per : 0, nkb = SPLIT ? min(g.KB - kb_first, g.per) : g.KB;
+  const uint16_t both = (uint16_t)(3u << first_rank);
   const uint32_t tiles_n = (uint32_t)(g.N + 255) / 256, tiles_m = (uint32_t)((g.M + 255) / 256), tiles = tiles_n * tiles_m;
   if (warp == 0) {
     ptx::prefetch_tensormap(&map_w);
@@ -478,14 +518,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 || warp == 2) {  // tokens, weights
       load_operand<C::kStages, 256, C::kStageBytes>(warp == 0 ? &map_x : &map_w, stages + (warp == 0 ? 0 : 128 * 128), warp == 0, 128, s_full,
-                                                    s_empty, pair, pairs, tiles_n, tiles_m, 0, g.KB, g.status, wait);
+                                                    s_empty, pair, pairs, tiles_n, tiles_m, kb_first, nkb, g.status, wait);
     } else if (warp == 1 && rank == 0) {
       const uint32_t el = ptx::elect_one();
       constexpr uint32_t idesc = ptx::make_idesc_e4m3(256, 256);
       Ring<C::kStages> st;
       Ring<2> buf;
       uint32_t last = 0, last_parity = 0;
-      const uint32_t mine = pair < tiles ? ((tiles - pair + pairs - 1) / pairs) * (uint32_t)g.KB : 0;
+      const uint32_t mine = pair < tiles ? ((tiles - pair + pairs - 1) / pairs) * (uint32_t)nkb : 0;
       uint32_t i = 0;
       for (; i < mine; ++i, st.step(), buf.step()) {
         const uint32_t x = stages + st.at * C::kStageBytes;
@@ -494,18 +534,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
         if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
         ptx::tc_fence_after();
         ptx::mma_f8_ss_x4_pair_w(el, tmem + buf.at * 256, a, b, idesc);
-        ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_tfull[buf.at]));
-        ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_empty[st.at]));
+        ptx::mma_commit_pair_w(el, both, ptx::smem_u32(&s_tfull[buf.at]));
+        ptx::mma_commit_pair_w(el, both, ptx::smem_u32(&s_empty[st.at]));
         last = st.at;
         last_parity = st.parity;
       }
       if (i > 0) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
     }
+    if constexpr (SPLIT) {
+      __syncwarp();
+      ptx::cluster_sync();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int row = (int)rank * 128 + (warp & 3) * 32 + lane, half = (warp - 4) >> 2;
     const uint32_t at_tmem = tmem + ((uint32_t)(warp & 3) << 21) + half * 128;
-    const uint32_t tempty[2] = {ptx::cluster_map(ptx::smem_u32(&s_tempty[0]), 0), ptx::cluster_map(ptx::smem_u32(&s_tempty[1]), 0)};
+    const uint32_t tempty[2] = {ptx::cluster_map(ptx::smem_u32(&s_tempty[0]), first_rank), ptx::cluster_map(ptx::smem_u32(&s_tempty[1]), first_rank)};
     OutRing ring = {stages + C::kStages * C::kStageBytes + (warp - 4) * 8192, true};
     Ring<2> buf;
     for (uint32_t t = pair; t < tiles; t += pairs) {
@@ -513,11 +557,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
       const int64_t m = at.m0 + row;
       const int n0 = at.n0 + half * 128;
       const bool mine = m < g.M && n0 < g.N;
-      const S* pa = static_cast<const S*>(g.sa) + m * g.sa_m;
-      const S* pb = static_cast<const S*>(g.sb) + (int64_t)(n0 / 128) * g.sb_n;
+      const S* pa = static_cast<const S*>(g.sa) + m * g.sa_m + kb_first * g.sa_k;
+      const S* pb = static_cast<const S*>(g.sb) + (int64_t)(n0 / 128) * g.sb_n + kb_first * g.sb_k;
       const auto scales_of = [&](int kb) {
         Scales<S> v = {};
-        if (mine && kb < g.KB) v = {pa[kb * g.sa_k], pb[kb * g.sb_k]};
+        if (mine && kb < nkb) v = {pa[kb * g.sa_k], pb[kb * g.sb_k]};
         return v;
       };
       float2 acc[64];
@@ -525,7 +569,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
       for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.f, 0.f);
       Scales<S> now = scales_of(0), next = scales_of(1);
 #pragma unroll 1
-      for (int kb = 0; kb < g.KB; ++kb, buf.step()) {
+      for (int kb = 0; kb < nkb; ++kb, buf.step()) {
         const Scales<S> after = scales_of(kb + 2);
         wait(s_tfull[buf.at], buf.parity, kGiveUpTmemFull);
         __syncwarp();
@@ -559,6 +603,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j].x = acc[j].y = __uint_as_float(0x7fffffffu);
       }
+      if constexpr (SPLIT) {  // (the products that read the stages are finished)
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(stages + ((half * 128 + c) * 128 + (warp & 3) * 32 + lane) * 4),
+                       "r"(__float_as_uint(c & 1 ? acc[c / 2].y : acc[c / 2].x))
+                       : "memory");
+        continue;
+      }
       constexpr int kCols = 128 / sizeof(Out);
       const int y = at.m0 + row - lane;
 #pragma unroll
@@ -579,6 +631,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
       }
     }
     if (lane == 0) ptx::tma_store_wait_all();
+    if constexpr (SPLIT) {
+      __syncwarp();
+      ptx::cluster_sync();
+      add_splits<Out>(stages, splits, split, 256, rank, (warp & 3) * 32 + lane, half, 2, tile_at<256>(pair, tiles_n, tiles_m), g);
+    }
   }
   __syncwarp();
   ptx::tc_fence_before();
@@ -854,36 +911,8 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
   __syncwarp();
   if constexpr (SPLIT) {
     ptx::cluster_sync();
-    // Each split has its share of the columns, a thread eight columns of a token at a time.
-    const Tile at = tile_at<C::kTileN>(pair, tiles_n, tiles_m);
-    const int row = (warp & 3) * 32 + lane, share = C::kTileN / (int)splits;
-    const int64_t m = at.m0 + (int)half * 128 + row;
-    for (int c = (int)split * share + (warp >> 2) * 8; c < (int)(split + 1) * share && m < g.M; c += kScaledThreads / 128 * 8) {
-      const int n = at.n0 + c;
-      if (n >= g.N) break;
-      float v[8] = {};
-      for (uint32_t z = 0; z < splits; ++z) {
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = peer_load(stages + ((c + j) * 128 + row) * 4, 2 * z + half);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += p[j];
-      }
-      Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n;
-      if (g.out_tma && n + 8 <= g.N) {  // (rows on 16-byte boundaries)
-        if constexpr (sizeof(Out) == 2) {
-          *reinterpret_cast<uint4*>(out) = make_uint4(ptx::pack_bf16(v[0], v[1]), ptx::pack_bf16(v[2], v[3]), ptx::pack_bf16(v[4], v[5]),
-                                                      ptx::pack_bf16(v[6], v[7]));
-        } else {
-          reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (n + j < g.N) out[j] = from_f32<Out>(v[j]);
-      }
-    }
+    add_splits<Out>(stages, splits, split, C::kTileN, half, (warp & 3) * 32 + lane, warp >> 2, kScaledThreads / 128,
+                    tile_at<C::kTileN>(pair, tiles_n, tiles_m), g);
     __syncwarp();
   }
   ptx::tc_fence_before();
@@ -898,6 +927,11 @@ int encode_bytes(CUtensorMap* map, const void* base, int64_t rows, int64_t width
   const uint32_t box[2] = {128, (uint32_t)box_rows};
   return encode_sw128(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 2, dims, strides, box);
 }
+
+template <auto k>
+struct Kernel {
+  static constexpr auto value = k;
+};
 
 template <typename Out, typename S>
 int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, MatmulArgs g, cudaStream_t s) {
@@ -920,32 +954,36 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
     rc = encode_sw128(&map_o, sizeof(Out) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.out, 2, dims, strides, box);
   }
   if (rc != MVPA_OK) return rc;
-  const dim3 grid(2 * (unsigned)(tiles < pairs ? tiles : pairs));
-  if constexpr (kScaled) {
-    // Two or four pairs to a tile, as long as all clusters are resident at once: a cluster of eight costs some 2 us more than one of
-    // two, a block 0.2 us.  us with 1 / 2 / 4 pairs: 132 x 2048 x 7680 18.5 / 15.7 / 12.8, 550 x 2048 x 7680 19.2 / 17.0 / two rounds,
-    // 550 x 768 x 4096 12.5 / 12.8 / 11.2; 550 x 768 x 2496 (20 blocks) 10.1 / 11.7 / 10.4.
-    constexpr auto whole = matmul_scaled_kernel<Out, false>, parts = matmul_scaled_kernel<Out, true>;
+  const auto run = [&](auto whole, auto parts, int threads, size_t smem, int most4, int most2) {
+    // Four or two pairs to a tile, as long as all clusters are resident at once (15 of eight CTAs, 33 of four).  A cluster of eight costs
+    // some 2 us more than one of two; a block 0.2 us with scales that are powers of two, 0.4 with others.  us with 1 / 2 / 4 pairs, powers of
+    // two: 132 x 2048 x 7680 18.5 / 15.7 / 12.8, 550 x 2048 x 7680 19.2 / 17.0 / two rounds, 550 x 768 x 4096 12.5 / 12.8 / 11.2;
+    // 550 x 768 x 2496 (20 blocks) 10.1 / 11.7 / 10.4; others, 1 / 4 pairs: 132 x 2048 x 7680 30.2 / 14.8, 550 x 768 x 2496 12.8 / 10.3,
+    // and with 2 pairs 64 x 8000 x 8000 31.3 / 21.9.
+    constexpr auto one = decltype(whole)::value, some = decltype(parts)::value;
     for (int n : {4, 2}) {
       int most = 0;
-      if (g.splits > 1 || g.KB < 64 - 8 * n) continue;
-      MVPA_CUDA_CHECK(grant_smem<parts>(ScaledRows::kSmem));
-      MVPA_CUDA_CHECK(resident_clusters<parts>(2 * n, kScaledThreads, ScaledRows::kSmem, &most));
+      if (g.splits > 1 || g.KB < (n == 4 ? most4 : most2)) continue;
+      MVPA_CUDA_CHECK(grant_smem<some>(smem));
+      MVPA_CUDA_CHECK(resident_clusters<some>(2 * n, threads, smem, &most));
       if (tiles <= most) g.splits = n;
     }
     g.per = (g.KB + g.splits - 1) / g.splits;
     if (g.splits > 1) {
-      MVPA_CUDA_CHECK(launch_dependent(dim3(2 * g.splits), parts, dim3(2 * (unsigned)tiles * g.splits), kScaledThreads, ScaledRows::kSmem, s,
-                                       map_w, map_x, map_o, g));
+      const dim3 grid(2 * (unsigned)tiles * g.splits);
+      MVPA_CUDA_CHECK(launch_dependent(dim3(2 * g.splits), some, grid, threads, smem, s, map_w, map_x, map_o, g));
     } else {
-      MVPA_CUDA_CHECK(grant_smem<whole>(ScaledRows::kSmem));
-      MVPA_CUDA_CHECK(launch_dependent(dim3(2), whole, grid, kScaledThreads, ScaledRows::kSmem, s, map_w, map_x, map_o, g));
+      const dim3 grid(2 * (unsigned)(tiles < pairs ? tiles : pairs));
+      MVPA_CUDA_CHECK(grant_smem<one>(smem));
+      MVPA_CUDA_CHECK(launch_dependent(dim3(2), one, grid, threads, smem, s, map_w, map_x, map_o, g));
     }
-  } else {
-    constexpr auto kernel = matmul_many_kernel<Out, S>;
-    MVPA_CUDA_CHECK(grant_smem<kernel>(ManyRows::kSmem));
-    MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, grid, kManyThreads, ManyRows::kSmem, s, map_w, map_x, map_o, g));
-  }
+    return MVPA_OK;
+  };
+  if constexpr (kScaled)
+    rc = run(Kernel<matmul_scaled_kernel<Out, false>>(), Kernel<matmul_scaled_kernel<Out, true>>(), kScaledThreads, ScaledRows::kSmem, 32, 48);
+  else
+    rc = run(Kernel<matmul_many_kernel<Out, S, false>>(), Kernel<matmul_many_kernel<Out, S, true>>(), kManyThreads, ManyRows::kSmem, 16, 24);
+  if (rc != MVPA_OK) return rc;
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;

@@ -225,3 +225,25 @@ def test_rows_that_end_inside_sixteen_bytes(cuda, M, N, dtype, fp32_scales):
     assert torch.equal(out, ops.matmul_fp8(a, sa, b, sb, dtype=dtype))
     out.fill_(5.0)
     assert bool((whole == 5).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(33, 500, 2048), (100, 300, 2049), (300, 259, 5000), (600, 700, 6200), (1000, 1500, 6200), (200, 2100, 3200)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_long_sums_with_other_scales(cuda, M, N, K, dtype):
+    """The same with fp32 scales, small whole numbers that are no powers of two."""
+    g = torch.Generator().manual_seed(M + N + K)
+    a, b = (torch.randint(-4, 5, (r, (K + 15) // 16 * 16), generator=g).float().cuda().to(torch.float8_e4m3fn)[:, :K] for r in (M, N))
+    kb = -(-K // 128)
+    sa, sb = (torch.randint(1, 6, (n, kb), generator=g).float().cuda() for n in (M, -(-N // 128)))
+    want = (ref.value(a, sa) @ ref.value(b, sb, 128).t()).to(dtype)      # below 2^24
+    for offset, ld in ((0, (N + 7) // 8 * 8), (3, N + 9)):
+        whole = torch.full((M + 1, offset + ld), 5.0, dtype=dtype, device="cuda")
+        out = whole[:M, offset:offset + N]
+        for _ in range(2):
+            ops.matmul_fp8(a, sa, b, sb, out=out)
+            assert torch.equal(out, want)
+        out.fill_(5.0)
+        assert bool((whole == 5).all())
+    sa[M // 2, kb - 1] = float("nan")
+    out = ops.matmul_fp8(a, sa, b, sb, dtype=dtype)
+    assert bool(out[M // 2].isnan().all()) and int(out.isnan().sum()) == N
