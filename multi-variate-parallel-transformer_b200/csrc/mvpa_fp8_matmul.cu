@@ -395,15 +395,16 @@ struct Ring {
 
 // A tile whose blocks several pairs have summed, a token's columns in the shared memory of the CTA of each pair that holds its rows
 // (sums[column][row]): each pair has its share of the columns, a thread eight of a token at a time, and adds in the order of the
-// blocks.  `group` of `groups`: which 128 threads of the CTA's these are.
+// blocks.  `group` of `groups`: which 128 threads of the CTA's these are; `turn`: 1 KB of the warp's own, by way of which rows that do
+// not start on 16-byte boundaries are written eight columns of four rows at a time.
 template <typename Out>
-__device__ __forceinline__ void add_splits(uint32_t sums, uint32_t splits, uint32_t split, int columns, uint32_t half, int row, int group,
-                                           int groups, const Tile& at, const MatmulArgs& g) {
-  const int share = columns / (int)splits;
+__device__ __forceinline__ void add_splits(uint32_t sums, uint32_t turn, uint32_t splits, uint32_t split, int columns, uint32_t half, int row,
+                                           int group, int groups, const Tile& at, const MatmulArgs& g) {
+  const int share = columns / (int)splits, lane = row & 31;
   const int64_t m = at.m0 + (int)half * 128 + row;
-  for (int c = (int)split * share + group * 8; c < (int)(split + 1) * share && m < g.M; c += groups * 8) {
+  for (int c = (int)split * share + group * 8; c < (int)(split + 1) * share; c += groups * 8) {
     const int n = at.n0 + c;
-    if (n >= g.N) break;
+    if (n >= g.N || m - lane >= g.M) break;  // (the same for the whole warp)
     float v[8] = {};
     for (uint32_t z = 0; z < splits; ++z) {
       float p[8];
@@ -412,8 +413,9 @@ __device__ __forceinline__ void add_splits(uint32_t sums, uint32_t splits, uint3
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += p[j];
     }
-    Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n;
     if (g.out_tma && n + 8 <= g.N) {  // (rows on 16-byte boundaries)
+      Out* out = static_cast<Out*>(g.out) + m * g.ld_out + n;
+      if (m >= g.M) continue;
       if constexpr (sizeof(Out) == 2) {
         *reinterpret_cast<uint4*>(out) =
             make_uint4(ptx::pack_bf16(v[0], v[1]), ptx::pack_bf16(v[2], v[3]), ptx::pack_bf16(v[4], v[5]), ptx::pack_bf16(v[6], v[7]));
@@ -421,11 +423,20 @@ __device__ __forceinline__ void add_splits(uint32_t sums, uint32_t splits, uint3
         reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
         reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (n + j < g.N) out[j] = from_f32<Out>(v[j]);
+      continue;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + (lane * 8 + ((j + lane) & 7)) * 4), "f"(v[j]) : "memory");
+    __syncwarp();
+    const int col = lane & 7;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = k * 4 + (lane >> 3);
+      float w;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w) : "r"(turn + (r * 8 + ((col + r) & 7)) * 4) : "memory");
+      if (m - lane + r < g.M && n + col < g.N) static_cast<Out*>(g.out)[(m - lane + r) * g.ld_out + n + col] = from_f32<Out>(w);
+    }
+    __syncwarp();
   }
 }
 
@@ -634,7 +645,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
     if constexpr (SPLIT) {
       __syncwarp();
       ptx::cluster_sync();
-      add_splits<Out>(stages, splits, split, 256, rank, (warp & 3) * 32 + lane, half, 2, tile_at<256>(pair, tiles_n, tiles_m), g);
+      add_splits<Out>(stages, ring.smem, splits, split, 256, rank, (warp & 3) * 32 + lane, half, 2, tile_at<256>(pair, tiles_n, tiles_m), g);
     }
   }
   __syncwarp();
@@ -911,7 +922,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
   __syncwarp();
   if constexpr (SPLIT) {
     ptx::cluster_sync();
-    add_splits<Out>(stages, splits, split, C::kTileN, half, (warp & 3) * 32 + lane, warp >> 2, kScaledThreads / 128,
+    add_splits<Out>(stages, outs + warp * 4096, splits, split, C::kTileN, half, (warp & 3) * 32 + lane, warp >> 2, kScaledThreads / 128,
                     tile_at<C::kTileN>(pair, tiles_n, tiles_m), g);
     __syncwarp();
   }
