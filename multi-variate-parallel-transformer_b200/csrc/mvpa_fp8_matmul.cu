@@ -670,10 +670,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 // A long K and so few tiles that most pairs would have none: the pairs of a cluster share the blocks of a tile and add their sums up
 // through distributed shared memory, in the order of the blocks.
 //
+// Where 192 columns a tile would leave pairs without one, tiles of 64: a multiprocessor takes some 150 bytes in a nanosecond, so a
+// block of 256 x 64 is there after 0.14 us and one of 256 x 192 after 0.19.
+//
 // Warps: 0 and 2 load tokens and weights, 1 issues, 3 lays the scales out in shared memory, 4 to 11 take the sums home, every
 // other 128 bytes of columns each.
+template <int TN>
 struct ScaledRows {
-  static constexpr int kTileN = 192, kHalfN = kTileN / 2;
+  static constexpr int kTileN = TN, kHalfN = kTileN / 2;
   static constexpr int kStages = 6;
   static constexpr int kGroup = 4, kGroups = 3;   // blocks that share a word of scales; such groups on their way
   static constexpr int kOperandBytes = 128 * 128 + kHalfN * 128;
@@ -686,11 +690,12 @@ struct ScaledRows {
 };
 constexpr int kScaledThreads = 384;
 
-template <typename Out, bool SPLIT>
+template <typename Out, bool SPLIT, int TN>
 __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                           const __grid_constant__ CUtensorMap map_x,
                                                                           const __grid_constant__ CUtensorMap map_o, const MatmulArgs g) {
-  using C = ScaledRows;
+  using C = ScaledRows<TN>;
+  constexpr int kWords = TN / 32;  // groups of 32 weight rows
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2], s_sfull[C::kGroups],
       s_sempty[C::kGroups];
@@ -775,7 +780,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
           const uint32_t sa = tmem + C::kTmemScales + group.at * C::kTmemScaleCols, sb = sa + 4, s = scales + group.at * C::kScaleBytes;
           ptx::tmem_copy_scales_pair_w(el, sa, s);
           ptx::tmem_copy_scales_pair_w(el, sb, s + 512);
-          ptx::tmem_copy_scales_pair_w(el, sb + 4, s + 1024);
+          if constexpr (TN > 128) ptx::tmem_copy_scales_pair_w(el, sb + 4, s + 1024);
 #pragma unroll
           for (uint32_t byte = 0; byte < C::kGroup; ++byte) {
             if (kb0 + (int)byte >= nkb) break;
@@ -800,8 +805,8 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
     }
   } else if (warp == 3) {
-    // Word j of lane l: the scales of row 32 j + l over a group of blocks, a byte each.  Four words for this CTA's 128 tokens; six for
-    // the tile's 192 weight rows, whose groups of 32 lie in one block of 128 each (lane j loads the word of rows 32 j).
+    // Word j of lane l: the scales of row 32 j + l over a group of blocks, a byte each.  Four words for this CTA's 128 tokens, and
+    // those of the tile's weight rows, whose groups of 32 lie in one block of 128 each (lane j loads the word of rows 32 j).
     const uint8_t *sa = static_cast<const uint8_t*>(g.sa) + kb_first * g.sa_k, *sb = static_cast<const uint8_t*>(g.sb) + kb_first * g.sb_k;
     const auto words = [](const void* p, int64_t rows, int64_t k) {  // four blocks' scales are an aligned word
       return k == 1 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)rows) & 3) == 0;
@@ -818,7 +823,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
         row[j] = t < tiles && m < g.M ? sa + m * g.sa_m : nullptr;
       }
       const int n = at.n0 + 32 * lane;
-      weights = t < tiles && lane < 6 && n < g.N ? sb + (int64_t)(n / 128) * g.sb_n : nullptr;
+      weights = t < tiles && lane < kWords && n < g.N ? sb + (int64_t)(n / 128) * g.sb_n : nullptr;
     };
     const auto fetch = [&](const uint8_t* p, int64_t k, bool word, uint32_t (&v)[C::kGroup]) {  // (v[0] alone where it is a word)
       if (word && kb + C::kGroup <= nkb) {
@@ -840,12 +845,12 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
     load();
     for (; t < tiles; group.step()) {
       const bool whole = kb + C::kGroup <= nkb;
-      uint32_t w[4], v[6];
+      uint32_t w[4], v[8] = {};
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = joined(token[j], word_a && whole);
       const uint32_t mine = joined(weight, word_b && whole);
 #pragma unroll
-      for (int j = 0; j < 6; ++j) v[j] = __shfl_sync(0xffffffffu, mine, j);
+      for (int j = 0; j < kWords; ++j) v[j] = __shfl_sync(0xffffffffu, mine, j);
       kb += C::kGroup;
       if (kb >= nkb) {
         kb = 0;
@@ -861,7 +866,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       };
       put(to, w[0], w[1], w[2], w[3]);
       put(to + 512, v[0], v[1], v[2], v[3]);
-      put(to + 1024, v[4], v[5], 0, 0);
+      if constexpr (TN > 128) put(to + 1024, v[4], v[5], v[6], v[7]);
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_sfull[group.at]), first_rank));
@@ -879,6 +884,8 @@ __global__ void __launch_bounds__(kScaledThreads, 1) matmul_scaled_kernel(const 
       const uint32_t from = at_tmem + buf.at * C::kTileN;
       const int y = at.m0 + (int)half * 128 + quad * 32;
       constexpr int kCols = 128 / sizeof(Out);
+      if (group * kCols >= C::kTileN && lane == 0)  // (no columns for these warps)
+        ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_tempty[buf.at]), first_rank));
 #pragma unroll 1
       for (int c = group * kCols; c < C::kTileN; c += 2 * kCols) {
         uint32_t r[kCols];
@@ -947,9 +954,15 @@ struct Kernel {
 template <typename Out, typename S>
 int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, MatmulArgs g, cudaStream_t s) {
   constexpr bool kScaled = sizeof(S) == 1;
-  constexpr int kTileN = kScaled ? ScaledRows::kTileN : 256;
-  const int64_t tiles = (int64_t)((g.N + kTileN - 1) / kTileN) * ((g.M + 255) / 256);
   const int64_t pairs = device_sm_count() / 2;
+  const auto tiles_of = [&](int width) { return (int64_t)((g.N + width - 1) / width) * ((g.M + 255) / 256); };
+  // Narrow tiles where each has a pair of its own, unless K is long and four pairs can share a wide one (15 clusters of eight CTAs are
+  // resident at once).  us, narrow / wide, alone or shared: 550 x 768 x 2496 7.1 / 8.8, 300 x 300 x 300 5.1 / 6.3, 550 x 768 x 4096
+  // 8.8 / 10.6, 500 x 2048 x 7680 13.8 / 16.1; 132 x 4736 x 768 (as many narrow tiles as pairs) 6.6 / 6.2; 132 x 2048 x 7680
+  // 12.9 / 12.2, 256 x 1500 x 6000 14.8 / 12.2, 100 x 500 x 8000 17.4 / 11.9.
+  const bool narrow = kScaled && 3 * tiles_of(192) <= pairs && !(g.KB >= 40 && tiles_of(192) <= 15);
+  const int kTileN = !kScaled ? 256 : narrow ? 64 : 192;
+  const int64_t tiles = tiles_of(kTileN);
   if (tiles * g.KB > 0x7fffffff) {
     set_error("mvpa_matmul_fp8: more than 2^31 blocks of 256 x %d x 128", kTileN);
     return MVPA_ERR_UNSUPPORTED;
@@ -990,10 +1003,18 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
     }
     return MVPA_OK;
   };
-  if constexpr (kScaled)
-    rc = run(Kernel<matmul_scaled_kernel<Out, false>>(), Kernel<matmul_scaled_kernel<Out, true>>(), kScaledThreads, ScaledRows::kSmem, 32, 48);
-  else
+  if constexpr (kScaled) {
+    if (narrow) {
+      constexpr auto kernel = matmul_scaled_kernel<Out, false, 64>;
+      MVPA_CUDA_CHECK(grant_smem<kernel>(ScaledRows<64>::kSmem));
+      MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)tiles), kScaledThreads, ScaledRows<64>::kSmem, s, map_w, map_x, map_o, g));
+    } else {
+      rc = run(Kernel<matmul_scaled_kernel<Out, false, 192>>(), Kernel<matmul_scaled_kernel<Out, true, 192>>(), kScaledThreads,
+               ScaledRows<192>::kSmem, 40, 48);
+    }
+  } else {
     rc = run(Kernel<matmul_many_kernel<Out, S, false>>(), Kernel<matmul_many_kernel<Out, S, true>>(), kManyThreads, ManyRows::kSmem, 16, 24);
+  }
   if (rc != MVPA_OK) return rc;
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
