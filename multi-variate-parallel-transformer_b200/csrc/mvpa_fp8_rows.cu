@@ -165,6 +165,12 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const T* __re
 // registers from too many warps (65536 x 768: 86 us for 65): there and for longer rows each warp has one row.
 constexpr int kNormWarps = 4;
 
+// 1 / sqrt(x): the library's, within two units, and a step of Newton's where that is finite and not zero.
+__device__ __forceinline__ float inverse_root(float x) {
+  const float r = rsqrtf(x), e = fmaf(-x * r, r, 1.f);
+  return fabsf(e) < 0.5f ? fmaf(0.5f * r, e, r) : r;
+}
+
 template <typename T, int NV, bool VEC>
 constexpr bool kNormAhead = VEC && sizeof(T) == 4 && NV <= 2;
 template <typename T, int NV, bool VEC>
@@ -211,16 +217,14 @@ __global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnor
         raw[i].pack(v);  // (rounds to T)
       }
     }
-    float2 squares = make_float2(0.f, 0.f);
+    float squares = 0.f;  // (short chains: what the sum loses moves every value of the row towards its next step)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float v[kLane];
+      float v[kLane], s[4];
       raw[i].get(v);
 #pragma unroll
-      for (int e = 0; e < kLane; e += 2) {
-        squares.x = fmaf(v[e], v[e], squares.x);
-        squares.y = fmaf(v[e + 1], v[e + 1], squares.y);
-      }
+      for (int e = 0; e < kLane; ++e) s[e & 3] = e < 4 ? v[e] * v[e] : fmaf(v[e], v[e], s[e & 3]);
+      squares += (s[0] + s[1]) + (s[2] + s[3]);
     }
     Raw<T> mine[NV];
 #pragma unroll
@@ -242,7 +246,7 @@ __global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnor
         }
       }
     }
-    const float rstd = rsqrtf(warp_sum(squares.x + squares.y) / (float)E + eps);
+    const float rstd = inverse_root(warp_sum(squares) / (float)E + eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (i * 32 * kLane >= E) break;
@@ -259,8 +263,13 @@ __global__ void __launch_bounds__(kNormWarps * 32, kNormCtas<T, NV, VEC>) rmsnor
         one.get(g);
       }
       mine[i].get(y);
+      // One rounding on the way to e4m3: the product with the weight is exact in fp32 for bf16; for fp32 its remainder goes along.
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) y[e] = y[e] * rstd * g[e];
+      for (int e = 0; e < kLane; ++e) {
+        const float p = y[e] * g[e];
+        if constexpr (sizeof(T) == 2) y[e] = p * rstd;
+        else y[e] = fmaf(p, rstd, fmaf(y[e], g[e], -p) * rstd);
+      }
       if (col + kLane > E) {  // (past the end 0 * rstd is NaN where rstd is)
 #pragma unroll
         for (int e = 0; e < kLane; ++e)
