@@ -317,7 +317,8 @@ struct OutRing {
   uint32_t smem;
   bool two;  // places, or one
   uint32_t which = 0;
-  // Where the next 128 bytes of columns go; the store that was there has been read.
+  // Where the next 128 bytes of columns go; the store that was there has been read.  (With two places all groups but the newest are
+  // waited for, so each use of a place has to be one group: send() commits its store, write() an empty group.)
   __device__ __forceinline__ uint32_t next(int lane) {
     if (lane == 0) {
       if (two) ptx::tma_store_wait_read<1>();
@@ -357,6 +358,7 @@ struct OutRing {
         for (int c = 0; c < kEach; ++c)
           if (r0 + r < rows && lane + 32 * c < cols) reinterpret_cast<Word*>(out)[(r0 + r) * ld + lane + 32 * c] = v[r][c];
     }
+    if (lane == 0) ptx::tma_store_commit();
     __syncwarp();
   }
   __device__ __forceinline__ static void send(uint32_t at, int lane, const CUtensorMap* map, int x, int y) {

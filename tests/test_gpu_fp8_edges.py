@@ -247,3 +247,29 @@ def test_long_sums_with_other_scales(cuda, M, N, K, dtype):
     sa[M // 2, kb - 1] = float("nan")
     out = ops.matmul_fp8(a, sa, b, sb, dtype=dtype)
     assert bool(out[M // 2].isnan().all()) and int(out.isnan().sum()) == N
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fp32_scales", [False, True])
+@pytest.mark.parametrize("M,N", [(8192, 1100), (8192, 1033), (20000, 1030)])
+@pytest.mark.parametrize("K", [128, 768])
+def test_row_ends_of_many_tiles(cuda, M, N, K, dtype, fp32_scales):
+    """Rows on 16-byte boundaries that end inside one, with several tiles to a pair of CTAs: a row's last columns, which are stored
+    one by one, and the tiles before and after, which the TMA stores, leave through the same shared memory.  Whole numbers, whose sums
+    (at most 768 * 16 * 25 < 2^24) are exact in fp32."""
+    g = torch.Generator().manual_seed(M + N + K)
+    a, b = (torch.randint(-4, 5, (r, K), generator=g).float().cuda().to(torch.float8_e4m3fn) for r in (M, N))
+    shapes = (M, K // 128), (-(-N // 128), K // 128)
+    if fp32_scales:
+        sa, sb = (torch.randint(1, 6, n, generator=g).float().cuda() for n in shapes)
+    else:
+        sa, sb = (torch.exp2(torch.randint(0, 3, n, generator=g).float()).cuda().to(torch.float8_e8m0fnu) for n in shapes)
+    want = (ref.value(a, sa) @ ref.value(b, sb, 128).t()).to(dtype)
+    whole = torch.full((M + 1, (N + 7) // 8 * 8), 5.0, dtype=dtype, device="cuda")
+    out = whole[:M, :N]
+    for _ in range(8):
+        out.fill_(7.0)
+        ops.matmul_fp8(a, sa, b, sb, out=out)
+        assert torch.equal(out, want)
+    out.fill_(5.0)
+    assert bool((whole == 5).all())
