@@ -15,6 +15,7 @@ import torch
 
 import mvpa_ops
 from models import BrainEncoder
+from models.prepared import prepared
 
 
 class _Weight(torch.nn.Module):
@@ -38,17 +39,18 @@ class WaveEncoder(BrainEncoder):
         self.dwt_size = total
         self.ln = _Weight(self.dwt_size, 1e-5)
         self.proj = torch.nn.Linear(self.dwt_size, size_output, bias=False)
-        self._padded = None                             # (version, zero-padded copy of proj.weight)
+        self._padded = None                             # (zero-padded copy of proj.weight, see `prepared`)
 
     def _proj_padded(self):
         w = self.proj.weight
         k = (self.dwt_size + 31) // 32 * 32
-        tag = (w._version, w.data_ptr(), w.dtype)
-        if self._padded is None or self._padded[0] != tag:
+
+        def pad():
             wp = torch.zeros((w.shape[0], k), dtype=w.dtype, device=w.device)
             wp[:, :self.dwt_size] = w.detach()
-            self._padded = (tag, wp)
-        return self._padded[1]
+            return (wp,)
+
+        return prepared(self, "_padded", (w._version, w.data_ptr(), w.dtype), pad)[0]
 
     @torch.no_grad()
     def block(self, x: torch.Tensor) -> torch.Tensor:

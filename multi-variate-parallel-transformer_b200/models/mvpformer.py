@@ -38,6 +38,7 @@ import mvpa_ops
 from attentions import attn as attn_mod, flash_mvpa_into
 from layers import MVPFormerGQAFlashAttention
 from models import BrainDecider, block_grad
+from models.prepared import prepared
 
 
 class MVPFormerConfig:
@@ -162,16 +163,14 @@ class MVPFormerBlock(torch.nn.Module):
     def fused_weights(self):
         """[q | k v | gate up] (rows) and [c_proj | down_proj] (columns), concatenated once per weight version."""
         ws, tag = self._projections()
-        if self._fused is None or self._fused[0] != tag:
-            self._fused = (tag, *self._concatenated(ws))
-        return self._fused[1], self._fused[2]
+        return prepared(self, "_fused", tag, lambda: self._concatenated(ws))
 
     def fused_weights_fp8(self):
         """The same two matrices in 8 bits, ((q, scales), (q, scales)), quantised once per weight version."""
         ws, tag = self._projections()
-        if self._fused_fp8 is None or self._fused_fp8[0] != tag:
-            self._fused_fp8 = (tag, *(mvpa_ops.quantize_fp8(w, block_rows=mvpa_ops.FP8_BLOCK) for w in self._concatenated(ws)))
-        return self._fused_fp8[1], self._fused_fp8[2]
+        in_8_bits = lambda: sum((mvpa_ops.quantize_fp8(w, block_rows=mvpa_ops.FP8_BLOCK) for w in self._concatenated(ws)), ())
+        made = prepared(self, "_fused_fp8", tag, in_8_bits)
+        return made[:2], made[2:]
 
     @torch.no_grad()
     def fused_branches_fp8(self, pair, r_time, r_chan, B, T, C, dtype):
@@ -290,11 +289,9 @@ class MVPFormerModel(torch.nn.Module):
     def _rel_weights(self):
         ws = [b.attn.position_net.weight for b in self.h] + [b.attn.channel_net.weight for b in self.h]
         tag = tuple((w._version, w.data_ptr(), w.dtype) for w in ws)
-        if self._rel is None or self._rel[0] != tag:
-            L = len(self.h)
-            self._rel = (tag, torch.cat([w.detach() for w in ws[:L]], dim=0).contiguous(),
-                         torch.cat([w.detach() for w in ws[L:]], dim=0).contiguous())
-        return self._rel[1], self._rel[2]
+        L = len(self.h)
+        return prepared(self, "_rel", tag, lambda: (torch.cat([w.detach() for w in ws[:L]], dim=0).contiguous(),
+                                                    torch.cat([w.detach() for w in ws[L:]], dim=0).contiguous()))
 
     def forward(self, input_ids=None, past_key_values=None, attention_mask=None, token_type_ids=None,
                 position_ids=None, channel_ids=None, head_mask=None, inputs_embeds=None, encoder_hidden_states=None,

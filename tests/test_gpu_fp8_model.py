@@ -6,7 +6,7 @@ import torch
 import fp8_oracle as ref
 import models
 import mvpa_ops as ops
-from attentions import flash_mvpa
+from attentions import attn, flash_mvpa
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -112,3 +112,38 @@ def test_model_refusals(cuda):
     m = _model(BF16).enable_fp8()
     with pytest.raises(NotImplementedError, match="8 bits"):
         m.forward_time_sharded(torch.zeros(4, 256, device="cuda", dtype=BF16), 2, 2)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_weights_prepared_on_one_stream_are_read_on_another(cuda, fp8):
+    """The first call makes the concatenated (and quantised) weights on its stream, behind other work; a call on another stream right
+    after it finds them finished."""
+    m, x = _model(BF16).enable_fp8(fp8), _embeds(BF16)
+    with torch.no_grad():
+        want = _model(BF16).enable_fp8(fp8)(inputs_embeds=x).last_hidden_state
+        torch.cuda.synchronize()
+        one, two = torch.cuda.Stream(), torch.cuda.Stream()
+        got = []
+        for stream in (one, two, one):
+            with torch.cuda.stream(stream):
+                if not got:
+                    torch.cuda._sleep(20_000_000)                        # some 10 ms
+                got.append(m(inputs_embeds=x).last_hidden_state)
+        torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_capture_without_a_call_before_it_keeps_nothing(cuda, fp8, monkeypatch):
+    """Weights that a capture makes exist only after a replay: calls outside the graph make their own."""
+    monkeypatch.setattr(attn, "_CHECK_STATUS", False)                    # (reading a status word back is not for captures)
+    m, x = _model(BF16).enable_fp8(fp8), _embeds(BF16)
+    with torch.no_grad():
+        want = _model(BF16).enable_fp8(fp8)(inputs_embeds=x).last_hidden_state
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=side):
+            captured = m(inputs_embeds=x).last_hidden_state
+        assert torch.equal(m(inputs_embeds=x).last_hidden_state, want)
+        graph.replay()
+        assert torch.equal(captured, want)

@@ -159,3 +159,52 @@ def test_scratch_sizes_are_asked_for_on_the_tensors_device(monkeypatch):
     x = torch.zeros(3, 8)
     mvpa_ops.rmsnorm_bwd(x, x[0], x, 1e-5)
     assert asked == [x.device, x.device]
+
+
+class _OnDevice:
+    """Stands for a CUDA tensor: remembers the streams that its memory has to wait for."""
+    is_cuda, device = True, torch.device("cuda", 0)
+
+    def __init__(self):
+        self.streams = []
+
+    def record_stream(self, stream):
+        self.streams.append(stream.cuda_stream)
+
+
+def test_what_is_made_of_the_weights_is_finished_before_another_stream_finds_it(monkeypatch):
+    """Concatenated and quantised weights: the stream that makes them is waited for before they are kept, other streams that read
+    them are noted, and inside a capture nothing is kept."""
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+    block = models.MVPFormerBlock(models.MVPFormerConfig(n_embd=64, n_layer=1, n_head=4, n_head_kv=2, n_inner=96))
+    state = {"stream": 7, "capturing": False}
+    waited = []
+
+    def current_stream(device=None):
+        at = state["stream"]
+        return SimpleNamespace(cuda_stream=at, synchronize=lambda: waited.append((at, getattr(block, state["kept"]) is None)))
+
+    monkeypatch.setattr(torch.cuda, "current_stream", current_stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: state["stream"], raising=False)
+    monkeypatch.setattr(block, "_concatenated", lambda ws: (_OnDevice(), _OnDevice()))
+    monkeypatch.setattr(models.mvpformer.mvpa_ops, "quantize_fp8", lambda w, block_rows: (_OnDevice(), _OnDevice()))
+    flat = lambda made: [t for m in made for t in (m if isinstance(m, tuple) else (m,))]
+    for make, kept in ((block.fused_weights, "_fused"), (block.fused_weights_fp8, "_fused_fp8")):
+        state.update(stream=7, capturing=True, kept=kept)
+        captured = flat(make())
+        assert not waited and flat(make())[0] is not captured[0]
+        state.update(capturing=False)
+        first = flat(make())
+        assert waited == [(7, True)]                    # before anything is kept
+        assert flat(make())[0] is first[0] and len(waited) == 1 and all(t.streams == [] for t in first)
+        for stream in (8, 8, 9, 7):
+            state.update(stream=stream)
+            assert flat(make())[0] is first[0]
+        assert len(waited) == 1 and all(t.streams == [8, 9] for t in first)
+        with torch.no_grad():
+            block.mlp.up_proj.weight.mul_(2.0)
+        assert flat(make())[0] is not first[0] and len(waited) == 2
+        waited.clear()
