@@ -15,7 +15,7 @@ import torch
 
 import mvpa_ops
 from models import BrainEncoder
-from models.prepared import prepared
+from models.prepared import Prepares, prepared
 
 
 class _Weight(torch.nn.Module):
@@ -27,7 +27,9 @@ class _Weight(torch.nn.Module):
         self.eps = eps
 
 
-class WaveEncoder(BrainEncoder):
+class WaveEncoder(Prepares, BrainEncoder):
+    _prepared = ("_padded",)
+
     def __init__(self, size_input: int, size_output: int, wavelet: str = "db4", gradient_checkpointing: bool = False):
         super().__init__()
         if wavelet != "db4":

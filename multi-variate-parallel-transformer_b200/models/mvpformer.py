@@ -38,7 +38,7 @@ import mvpa_ops
 from attentions import attn as attn_mod, flash_mvpa_into
 from layers import MVPFormerGQAFlashAttention
 from models import BrainDecider, block_grad
-from models.prepared import prepared
+from models.prepared import Prepares, prepared
 
 
 class MVPFormerConfig:
@@ -121,8 +121,8 @@ class LlamaMLP(torch.nn.Module):
 _SHIPPED = tuple(block_grad.shipped(cls) for cls in (RMSNorm, MVPFormerGQAFlashAttention, LlamaMLP))
 
 
-class MVPFormerBlock(torch.nn.Module):
-    _fused_fp8 = None      # (of the class: modules pickled before there was an 8-bit path have neither of their own)
+class MVPFormerBlock(Prepares, torch.nn.Module):
+    _prepared = ("_fused", "_fused_fp8")
 
     def __init__(self, config, layer_idx=None):
         super().__init__()
@@ -130,7 +130,7 @@ class MVPFormerBlock(torch.nn.Module):
         self.attn = MVPFormerGQAFlashAttention(config, layer_idx=layer_idx)
         self.ln_2 = RMSNorm(config.hidden_size, eps=config.layer_norm_epsilon)   # unused, as in the reference
         self.mlp = LlamaMLP(config)
-        self._fused = None
+        self._fused = self._fused_fp8 = None
 
     def forward(self, hidden_states, positional_embedding, channel_embedding, layer_past=None, attention_mask=None,
                 head_mask=None, encoder_hidden_states=None, encoder_attention_mask=None, use_cache=False,
@@ -262,8 +262,9 @@ class MVPFormerBlock(torch.nn.Module):
         return F.linear(cat, w_out)
 
 
-class MVPFormerModel(torch.nn.Module):
-    _fp8 = False
+class MVPFormerModel(Prepares, torch.nn.Module):
+    _prepared = ("_rel",)
+    _fp8 = False           # (of the class: modules pickled before there was an 8-bit path have none of their own)
 
     def __init__(self, config, gradient_checkpointing=False):
         super().__init__()

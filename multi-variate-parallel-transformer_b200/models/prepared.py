@@ -31,3 +31,15 @@ def prepared(owner, name, tag, make):
                 t.record_stream(stream)
             streams.add(handle)
     return made
+
+
+class Prepares:
+    """Mixin of modules that keep such tensors, under the names in `_prepared`: copies and pickles go without, since in another
+    process other weights can have the same versions and places."""
+    _prepared = ()
+
+    def __getstate__(self):
+        return {**self.__dict__, **dict.fromkeys(self._prepared)}
+
+    def __setstate__(self, state):
+        super().__setstate__({**state, **dict.fromkeys(self._prepared)})

@@ -208,3 +208,29 @@ def test_what_is_made_of_the_weights_is_finished_before_another_stream_finds_it(
             block.mlp.up_proj.weight.mul_(2.0)
         assert flat(make())[0] is not first[0] and len(waited) == 2
         waited.clear()
+
+
+def test_copies_and_pickles_prepare_their_own_weights(monkeypatch):
+    """In another process a changed weight can have the version and the place that a kept concatenation was made for."""
+    import copy
+    import pickle
+    monkeypatch.setattr(models.MVPFormerBlock, "_projections", lambda self: ((
+        self.attn.q_attn.weight, self.attn.c_attn.weight, self.mlp.gate_proj.weight, self.mlp.up_proj.weight,
+        self.attn.c_proj.weight, self.mlp.down_proj.weight), "the same"))
+    config = models.MVPFormerConfig(n_embd=64, n_layer=1, n_head=4, n_head_kv=2, n_inner=96)
+    block = models.MVPFormerBlock(config)
+    encoder, model = models.WaveEncoder(256, 64), models.MVPFormerModel(config)
+    kept = block.fused_weights()[1]
+    encoder._proj_padded(), model._rel_weights()
+    with torch.no_grad():
+        block.mlp.down_proj.weight.mul_(2.0)
+    want = torch.cat([block.attn.c_proj.weight, block.mlp.down_proj.weight], 1)
+    assert block.fused_weights()[1] is kept and not torch.equal(kept, want)
+    for again in (copy.deepcopy, lambda m: pickle.loads(pickle.dumps(m))):
+        assert torch.equal(again(block).fused_weights()[1], want)
+        assert again(encoder)._padded is None and again(model)._rel is None
+    assert block.fused_weights()[1] is kept and encoder._padded is not None
+    old = {k: v for k, v in block.__dict__.items() if k != "_fused_fp8"}                 # pickled by another version
+    other = models.MVPFormerBlock.__new__(models.MVPFormerBlock)
+    other.__setstate__({**old, "_fused": ("the same", kept, kept)})
+    assert torch.equal(other.fused_weights()[1], want) and other._fused_fp8 is None
