@@ -355,9 +355,9 @@ class MVPFormerModel(Prepares, torch.nn.Module):
                 with torch.cuda.graph(g):
                     static_out = self.forward_time_sharded(static_in, T, C, group, transport)
                 _ms.PeerKV.forget_events()                 # ... nor those of the capture outside it
-                entry = (g, static_in, static_out)
+                entry = (g, static_in, static_out, self._kept())
                 self._graphs[key] = entry
-            g, static_in, static_out = entry
+            g, static_in, static_out = entry[:3]
             static_in.copy_(embeds_local)
             g.replay()
             return static_out
@@ -411,6 +411,10 @@ class MVPFormerModel(Prepares, torch.nn.Module):
         self._graphs = {}
         return self
 
+    def _kept(self):
+        """The prepared weights as they are now."""
+        return [self._rel] + [(b._fused_fp8 if self._fp8 else b._fused) for b in self.h]
+
     def reset_cuda_graphs(self):
         self._graphs = {}
 
@@ -435,8 +439,8 @@ class MVPFormerModel(Prepares, torch.nn.Module):
                     static_out = self._fused_forward(static_in, pos, chan)
             finally:
                 attn_mod._CHECK_STATUS = check
-            # the graph reads these buffers on every replay: the index tensors stay alive with it
-            entry = (graph, static_in, static_out, pos, chan)
+            # the graph reads these buffers on every replay: the index tensors and the prepared weights stay alive with it
+            entry = (graph, static_in, static_out, pos, chan, self._kept())
             self._graphs[key] = entry
         graph, static_in, static_out = entry[:3]
         static_in.copy_(hidden)

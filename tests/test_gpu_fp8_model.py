@@ -147,3 +147,24 @@ def test_a_capture_without_a_call_before_it_keeps_nothing(cuda, fp8, monkeypatch
         assert torch.equal(m(inputs_embeds=x).last_hidden_state, want)
         graph.replay()
         assert torch.equal(captured, want)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_graph_keeps_the_weights_that_it_reads(cuda, fp8):
+    """Graphs are for frozen weights; one that is replayed after some have changed all the same reads those that were prepared for
+    it, also when another shape's capture has prepared them anew and their old memory could have gone to something else."""
+    m, x, y = _model(BF16).enable_fp8(fp8), _embeds(BF16), _embeds(BF16, T=5)
+    with torch.no_grad():
+        m.enable_cuda_graph()
+        want = m(inputs_embeds=x).last_hidden_state.clone()
+        kept = [t.data_ptr() for entry in m._kept() for t in entry[1]]
+        for block in m.h:
+            block.mlp.down_proj.weight.mul_(2.0)
+            block.attn.position_net.weight.mul_(2.0)
+        other = m(inputs_embeds=y).last_hidden_state.clone()
+        others = torch.full((1 << 20,), 0x7f, dtype=torch.uint8, device="cuda"), [torch.full((n,), 3e38, device="cuda") for n in range(1000, 200000, 1999)]
+        assert not set(kept) & {t.data_ptr() for entry in m._kept() for t in entry[1]}
+        assert torch.equal(m(inputs_embeds=x).last_hidden_state, want)
+        fresh = m.enable_cuda_graph(False)(inputs_embeds=y).last_hidden_state
+    del others
+    assert torch.equal(fresh, other)

@@ -234,3 +234,36 @@ def test_copies_and_pickles_prepare_their_own_weights(monkeypatch):
     other = models.MVPFormerBlock.__new__(models.MVPFormerBlock)
     other.__setstate__({**old, "_fused": ("the same", kept, kept)})
     assert torch.equal(other.fused_weights()[1], want) and other._fused_fp8 is None
+
+
+def test_a_graph_is_kept_with_the_weights_that_it_reads(monkeypatch):
+    """The prepared weights of a capture live as long as its graph, whatever is prepared after it."""
+    import weakref
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+    m = models.MVPFormerModel(models.MVPFormerConfig(n_embd=64, n_layer=2, n_head=4, n_head_kv=2, n_inner=96, n_positions=4, n_channels=4)).eval()
+    stream = SimpleNamespace(wait_stream=lambda other: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: stream)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda device=None: stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: nullcontext())
+    monkeypatch.setattr(torch.cuda, "graph", lambda g: nullcontext())
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: SimpleNamespace(replay=lambda: None))
+
+    def forward(hidden, pos, chan):
+        for t in (m._rel_weights(), *(b.fused_weights() for b in m.h)):
+            read.extend(weakref.ref(w) for w in t)
+        return hidden
+
+    monkeypatch.setattr(m, "_fused_forward", forward)
+    m.enable_cuda_graph()
+    with torch.no_grad():
+        read = []
+        m(inputs_embeds=torch.zeros(1, 3, 4, 64))
+        first, read = read, []
+        for p in m.parameters():
+            p.mul_(2.0)
+        m(inputs_embeds=torch.zeros(1, 4, 4, 64))
+        assert all(r() is not None for r in first)
+        assert not {id(r()) for r in first} & {id(r()) for r in read}
+        m.reset_cuda_graphs()
+        assert all(r() is None for r in first)
