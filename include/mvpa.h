@@ -302,7 +302,7 @@ int mvpa_rmsnorm_fp8(const void* x, const void* add, const void* weight, void* s
                      int32_t dtype, void* cuda_stream);
 
 /* silu(gate) * up as a pair, from fp32 in one rounding (mvpa_silu_mul rounds silu to the element type
- * in between); e^-|gate| below 2^-126 counts as zero. */
+ * in between). */
 int mvpa_silu_mul_fp8(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* scales,
                       int64_t ld_s, int64_t rows, int32_t width, int32_t dtype, void* cuda_stream);
 

@@ -48,12 +48,14 @@ __device__ __forceinline__ Unit unit_of(const Units& g) {
   return t;
 }
 
-__device__ __forceinline__ void write_unit(const Unit& t, const float (&y)[kLane], uint8_t* q, int64_t ld_q, uint8_t* scales,
-                                           int64_t ld_s, int width) {
+// (-> the scale's byte)
+__device__ __forceinline__ uint32_t write_unit(const Unit& t, const float (&y)[kLane], uint8_t* q, int64_t ld_q, uint8_t* scales,
+                                               int64_t ld_s, int width) {
   const uint32_t byte = scale_byte(max8(top_of(y)));
-  if (!t.any) return;
+  if (!t.any) return byte;
   if (t.col < width) store16(q + t.row * ld_q, t.col, width, y, inverse_scale(byte));
   if ((threadIdx.x & 7) == 0) scales[t.row * ld_s + t.block] = (uint8_t)byte;
+  return byte;
 }
 
 // A lane's values of one block.
@@ -79,27 +81,52 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
   write_unit(t, y, q, ld_q, scales, ld_s, g.width);
 }
 
-// silu(g) u = g / (1 + e^-g) u of two numbers, from e = e^-|g| <= 1 so that nothing overflows: 1 / (1 + e), or e / (1 + e) where
-// g < 0.  e = 2^(-|g| log2 e): the product in two parts, since 2^x turns an error of x into a relative one (log2 e = kHi + kLo),
-// and 2^(hi + lo) = 2^hi (1 + lo ln 2) as |lo| < 2^-16; the reciprocal is an estimate and one step of Newton's.  As exact as the
-// quotient by library functions, in 20 instructions a value for 40, most of them on pairs: the gate was bound by their number.
-// e below 2^-126 counts as zero (g < -87); past 200 nothing changes any more, and the bound keeps the products finite.
+// silu(g) u = g / (1 + e^-g) u of two numbers.  e^-g = 2^(-g log2 e): the product in two parts, since 2^x turns an error of x into a
+// relative one (log2 e = kHi + kLo), and 2^(hi + lo) = 2^hi (1 + lo ln 2) as |lo| < 2^-16; the reciprocal is an estimate and one
+// step of Newton's.  As exact as the quotient by library functions, in less than half of their instructions, most of them on pairs:
+// the gate is bound by their number.  It is 8 e^-g that is computed, so that for g < -86.6 it overflows before the reciprocal could
+// leave the normal numbers: infinity has no reciprocal by Newton, and the result is NaN (as it is where g log2 e overflows).
+// Blocks that come out NaN are looked at again by silu_mul_any.
 __device__ __forceinline__ float2 silu_mul(float2 g, float2 u) {
   constexpr float kHi = 1.44269504f, kLo = 1.92596299e-8f, kLn2 = 0.693147181f;
   const auto both = [](float x) { return make_float2(x, x); };
-  const float2 a = make_float2(fminf(fabsf(g.x), 200.f), fminf(fabsf(g.y), 200.f));
-  const float2 hi = ptx::fmul2(a, both(-kHi));
-  const float2 low = ptx::ffma2(a, both(-kHi), make_float2(-hi.x, -hi.y));
-  const float2 lo = ptx::ffma2(a, both(-kLo), low);
-  const float2 p = make_float2(ptx::ex2(hi.x), ptx::ex2(hi.y));
-  const float2 e = ptx::ffma2(p, ptx::fmul2(lo, both(kLn2)), p);
-  const float2 d = ptx::fadd2(e, both(1.f));
+  const float2 hi = ptx::fmul2(g, both(-kHi)), low = ptx::ffma2(g, both(-kHi), make_float2(-hi.x, -hi.y));
+  const float2 lo = ptx::ffma2(g, both(-kLo), low);
+  const float2 p = ptx::fmul2(make_float2(ptx::ex2(hi.x), ptx::ex2(hi.y)), both(8.f));
+  const float2 d = ptx::ffma2(ptx::ffma2(p, ptx::fmul2(lo, both(kLn2)), p), both(0.125f), both(1.f));
   float2 r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
   r = ptx::ffma2(r, ptx::ffma2(make_float2(-d.x, -d.y), r, both(1.f)), r);
-  const float2 top = make_float2(g.x < 0.f ? e.x : 1.f, g.y < 0.f ? e.y : 1.f);
-  return ptx::fmul2(ptx::fmul2(g, ptx::fmul2(top, r)), u);
+  return ptx::fmul2(ptx::fmul2(g, r), u);
+}
+// The same for any g.  Below -86, 1 / (1 + e^-g) is e^g to more places than fp32 has, as small as it may be beside a large u: in
+// four parts, which leave the normal numbers where the product does and not before.  Above 86 it is 1.
+__device__ __forceinline__ float silu_mul_any(float g, float u) {
+  if (g > 86.f) return g * u;
+  if (!(g < -86.f)) return silu_mul(make_float2(g, g), make_float2(u, u)).x;
+  const float part = expf(0.25f * g);
+  return u * part * part * (g * part) * part;
+}
+
+// A warp's units once more, written where `again`: value by value and apart from the kernel, whose registers (32 a thread for aligned
+// bf16, which is what lets its warps fill a multiprocessor) it does not add to.
+template <typename T>
+__device__ __noinline__ void silu_mul_again(bool again, const T* gate, const T* up, int64_t ld_in, uint8_t* q, int64_t ld_q, uint8_t* scales,
+                                            int64_t ld_s, const Units g) {
+  const Unit t = unit_of(g);
+  const int n = again && t.any ? min(g.width - t.col, kLane) : 0;
+  gate += t.row * ld_in + t.col;
+  up += t.row * ld_in + t.col;
+  q += t.row * ld_q + t.col;
+  uint32_t top = 0;
+#pragma unroll 1
+  for (int e = 0; e < n; ++e) top = max(top, __float_as_uint(fabsf(silu_mul_any(to_f32<T>(gate[e]), to_f32<T>(up[e])))));
+  const uint32_t byte = scale_byte(max8(top));
+  const float inverse = inverse_scale(byte);
+#pragma unroll 1
+  for (int e = 0; e < n; ++e) q[e] = (uint8_t)e4m3x2(silu_mul_any(to_f32<T>(gate[e]), to_f32<T>(up[e])) * inverse, 0.f);
+  if (n > 0 && (threadIdx.x & 7) == 0) scales[t.row * ld_s + t.block] = (uint8_t)byte;
 }
 
 // silu(gate) * up, in fp32 from the inputs to the step to e4m3.
@@ -119,7 +146,8 @@ __global__ void __launch_bounds__(kThreads) silu_mul_fp8_kernel(const T* __restr
     y[e] = v.x;
     y[e + 1] = v.y;
   }
-  write_unit(t, y, q, ld_q, scales, ld_s, g.width);
+  const bool again = write_unit(t, y, q, ld_q, scales, ld_s, g.width) == 255u;
+  if (__any_sync(0xffffffffu, again)) silu_mul_again<T>(again, gate, up, ld_in, q, ld_q, scales, ld_s, g);
 }
 
 // One CTA per block of 128 x 128: eight lanes a row, 32 rows at a time, four times; the values wait in registers for the

@@ -342,3 +342,41 @@ def test_refusals(cuda):
     ]:
         with pytest.raises(RuntimeError, match=words):
             call()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("width,shift", [(128, 0), (300, 0), (300, 3), (1001, 1)])
+def test_gate_between_its_smallest_values(cuda, dtype, width, shift):
+    """Gates between -300 and -60, whose e^g leaves fp32's normal numbers, beside factors that bring the product back: blocks of
+    such values alone and blocks with ordinary ones among them, at any alignment."""
+    g = _gen(width, shift)
+    rows = 24
+    gate = -60.0 - 240.0 * torch.rand(rows, width + shift, generator=g)
+    gate[:4] = -87.0 - torch.linspace(-1.0, 2.0, width + shift)                     # both sides of -87
+    gate[4:8].mul_(0.5)
+    gate[8:12, ::3] = torch.randn(4, len(range(0, width + shift, 3)), generator=g) * 20
+    gate = gate.to(dtype).cuda()[:, shift:]
+    # |silu(gate) u| between 1e-30 and 1 where fp32 has such a u, and u at fp32's (bf16's) largest below
+    size = 10.0 ** (-30.0 * torch.rand(rows, width, generator=g).double().cuda())
+    up = (size / (gate.double() * torch.sigmoid(gate.double())).abs().clamp(min=1e-300)).clamp(max=3e38)
+    up = (up * torch.randint(0, 2, (rows, width), generator=g).cuda().mul(2).sub(1)).to(dtype)
+    wide = torch.zeros(rows, width + shift, dtype=dtype, device="cuda")
+    up = wide[:, shift:].copy_(up)
+    q, s = ops.silu_mul_fp8(gate, up)
+    # e^(g / 4) four times, each within a unit (2^-23), and four products of half a unit (2^-24) each: 12 * 2^-24.  Values and
+    # products of them below 2^-126 are off by up to 2^-150 each time: blocks whose largest value is above 2^-100 do not see that.
+    y = _gate64(gate, up)
+    seen = (ref.tops(y) > 2.0 ** -100).repeat_interleave(128, 1)[:, :width]
+    assert bool(seen[:12].all())
+    ref.check_pair(q, s, y, 16 * 2.0 ** -24)
+
+
+def test_gate_of_infinite_and_missing_numbers(cuda):
+    """-inf, NaN and infinite factors in the places that e^g makes zero: as the formula has them."""
+    inf, nan = float("inf"), float("nan")
+    g = torch.tensor([[-inf, 1.0], [nan, -100.0], [-100.0, 1.0], [-1e30, 2.0], [-100.0, nan], [-300.0, 3.0]], device="cuda")
+    u = torch.tensor([[1.0, 1.0], [1.0, 1.0], [inf, 1.0], [1e30, 1.0], [1.0, 1.0], [0.0, 1.0]], device="cuda")
+    q, s = ops.silu_mul_fp8(g, u)
+    assert s.float().isnan().flatten().tolist() == [True, True, True, False, True, False]
+    assert bool(q[[0, 1, 2, 4]].float().isnan().all()) and not bool(q[[3, 5]].float().isnan().any())
+    assert q[[3, 5], 0].float().tolist() == [0.0, 0.0]
