@@ -91,7 +91,7 @@ cudaError_t resident_clusters(int ctas, int threads, size_t smem, int* clusters)
   return e;
 }
 
-// ---- few rows: 128 weight rows x NT tokens a CTA ----------------------------------------------------------------------------
+// ---- few rows: 128 weight rows x all of up to NT tokens a CTA ----------------------------------------------------------------------------
 // The weights are the product's M side, so that one token fills 1/16 of a tile and not 1/128; the tile is transposed in TMEM
 // (lane = weight row, column = token).  The blocks along K are split over the CTAs of a cluster where there are too few tiles to
 // fill the multiprocessors; their sums meet through distributed shared memory in a fixed order.
@@ -117,7 +117,6 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * 128;
-  const int64_t m0 = (int64_t)blockIdx.y * NT;
   const int kb0 = blockIdx.z * g.per, nkb = min(g.KB - kb0, g.per);
   if (warp == 0) {
     ptx::prefetch_tensormap(&map_w);
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
         uint8_t* w = stages + st * C::kStageBytes;
         ptx::mbar_arrive_expect_tx(&s_full[st], C::kStageBytes);
         ptx::tma_load_2d(w, &map_w, &s_full[st], (kb0 + i) * 128, n0);
-        ptx::tma_load_2d(w + 128 * 128, &map_x, &s_full[st], (kb0 + i) * 128, (int)m0);
+        ptx::tma_load_2d(w + 128 * 128, &map_x, &s_full[st], (kb0 + i) * 128, 0);
       }
       for (int k = i < C::kStages ? 0 : i - C::kStages; k < i; ++k)  // no copy is in flight when the CTA ends
         if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
@@ -192,8 +191,8 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
   } else {
     const int quad = warp & 3, t = threadIdx.x - 64;  // a warp reads the TMEM lanes of its place among four
     const uint32_t at = tmem + ((uint32_t)quad << 21);
-    const bool mine = t < NT && m0 + t < g.M;
-    const int64_t ia = (m0 + t) * g.sa_m, ib = (int64_t)blockIdx.x * g.sb_n;
+    const bool mine = t < NT && t < g.M;
+    const int64_t ia = t * g.sa_m, ib = (int64_t)blockIdx.x * g.sb_n;
     const S *pa = static_cast<const S*>(g.sa) + ia, *pb = static_cast<const S*>(g.sb) + ib;
     const auto scales_of = [&](int i) {
       Scales<S> v = {};
@@ -239,12 +238,12 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
   const int row = (warp & 3) * 32 + lane, splits = gridDim.z;
   const bool sums = warp >= 2, inside = sums && n0 + row < g.N;
   const float poison = *dead ? __uint_as_float(0x7fffffffu) : 0.f;
-  const int64_t at = m0 * g.ld_out + n0 + row;
+  const int64_t at = n0 + row;
   if (splits == 1) {
     if (inside) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        if (m0 + j < g.M) store_out<Out>(g.out, at + j * g.ld_out, acc[j] + poison);
+        if (j < g.M) store_out<Out>(g.out, at + j * g.ld_out, acc[j] + poison);
     }
   } else {
     float* part = reinterpret_cast<float*>(stages);  // (every product that read the stages is finished)
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
     __syncwarp();
     ptx::cluster_sync();
     if (inside) {
-      for (int j = blockIdx.z; j < NT && m0 + j < g.M; j += splits) {
+      for (int j = blockIdx.z; j < NT && j < g.M; j += splits) {
         float v = 0.f;
         for (int z = 0; z < splits; ++z) v += peer_load(ptx::smem_u32(part + j * 128 + row), z);
         store_out<Out>(g.out, at + j * g.ld_out, v);
@@ -273,22 +272,16 @@ __global__ void __launch_bounds__(192) matmul_few_kernel(const __grid_constant__
 template <int NT, typename Out, typename S>
 int run_few(const CUtensorMap& map_w, const CUtensorMap& map_x, MatmulArgs g, cudaStream_t s) {
   using C = FewRows<NT>;
-  const int tiles_n = (g.N + 127) / 128;
-  const int64_t tiles_m = (g.M + NT - 1) / NT;
-  if (tiles_m > 65535) {
-    set_error("mvpa_matmul_fp8: too many rows (%lld)", (long long)g.M);
-    return MVPA_ERR_UNSUPPORTED;
-  }
+  const int64_t tiles = (g.N + 127) / 128, sms = device_sm_count();
   // Up to two CTAs on a multiprocessor (their stages take half of its memory each), with a few blocks each: one token x 15360 x 2048
   // takes 8.1 us in 120 CTAs and 6.7 in 240, x 2048 x 7680 23.4 in 16 CTAs, 8.8 in 64 and 5.9 in 128.
   int splits = 1;
-  const int64_t tiles = tiles_n * tiles_m, sms = device_sm_count();
   while (splits < 8 && ((tiles * splits * 2 <= sms && g.KB >= 4 * splits) || (tiles * splits <= sms && g.KB >= 8 * splits))) splits *= 2;
   g.per = (g.KB + splits - 1) / splits;
   splits = (g.KB + g.per - 1) / g.per;
   constexpr auto kernel = matmul_few_kernel<NT, Out, S>;
   MVPA_CUDA_CHECK(grant_smem<kernel>(C::kSmem));
-  MVPA_CUDA_CHECK(launch_dependent(splits, kernel, dim3(tiles_n, (unsigned)tiles_m, splits), 192, C::kSmem, s, map_w, map_x, g));
+  MVPA_CUDA_CHECK(launch_dependent(splits, kernel, dim3((unsigned)tiles, 1, splits), 192, C::kSmem, s, map_w, map_x, g));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
