@@ -98,11 +98,12 @@ cudaError_t resident_clusters(int ctas, int threads, size_t smem, int* clusters)
 template <int NT>
 struct FewRows {
   static constexpr int kStageBytes = 128 * 128 + NT * 128;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = NT == 16 ? 6 : 5;  // (as many as let two CTAs share a multiprocessor)
   static constexpr int kBuffers = 4;  // products on their way home
   static constexpr int kTmemCols = kBuffers * NT;
   static constexpr size_t kSmem = 1024 + kStages * kStageBytes;
   static_assert(kStages * kStageBytes >= NT * 128 * 4, "the sums of a split wait in the stages' memory");
+  static_assert(2 * (kSmem + 2048) <= 228 * 1024, "two CTAs, with what the system and the kernel's own variables take of each");
 };
 
 template <int NT, typename Out, typename S>
@@ -274,7 +275,9 @@ int run_few(const CUtensorMap& map_w, const CUtensorMap& map_x, MatmulArgs g, cu
   using C = FewRows<NT>;
   const int64_t tiles = (g.N + 127) / 128, sms = device_sm_count();
   // Up to two CTAs on a multiprocessor (their stages take half of its memory each), with a few blocks each: one token x 15360 x 2048
-  // takes 8.1 us in 120 CTAs and 6.7 in 240, x 2048 x 7680 23.4 in 16 CTAs, 8.8 in 64 and 5.9 in 128.
+  // takes 8.1 us in 120 CTAs and 6.7 in 240, x 2048 x 7680 23.4 in 16 CTAs, 8.8 in 64 and 5.9 in 128.  For 17 to 32 tokens that takes
+  // five stages: with six one CTA fits, and what was split for two runs in two turns (22 rows, six / five stages, us: 15360 x 2048
+  // 15.9 / 9.6, 2048 x 7680 12.3 / 7.3, 4096 x 4096 14.3 / 6.6, 9500 x 6000 28.0 / 16.6; unsplit in six 8.5 / - / 7.3 / 20.0).
   int splits = 1;
   while (splits < 8 && ((tiles * splits * 2 <= sms && g.KB >= 4 * splits) || (tiles * splits <= sms && g.KB >= 8 * splits))) splits *= 2;
   g.per = (g.KB + splits - 1) / splits;

@@ -273,3 +273,20 @@ def test_row_ends_of_many_tiles(cuda, M, N, K, dtype, fp32_scales):
         assert torch.equal(out, want)
     out.fill_(5.0)
     assert bool((whole == 5).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 15360, 2048), (22, 2048, 7680), (32, 600, 6144), (31, 129, 641), (1, 2048, 7680), (16, 9500, 1024)])
+@pytest.mark.parametrize("fp32_scales", [False, True])
+def test_few_rows_of_whole_numbers(cuda, M, N, K, fp32_scales):
+    """Up to 32 rows, alone and split along K, more blocks than stages: whole numbers whose sums (below 7680 * 16 * 25 < 2^24) are
+    exact in fp32, and the same bits again."""
+    g = torch.Generator().manual_seed(M + N + K)
+    a, b = (torch.randint(-4, 5, (r, (K + 15) // 16 * 16), generator=g).float().cuda().to(torch.float8_e4m3fn)[:, :K] for r in (M, N))
+    kb = -(-K // 128)
+    if fp32_scales:
+        sa, sb = (torch.randint(1, 6, (n, kb), generator=g).float().cuda() for n in (M, -(-N // 128)))
+    else:
+        sa, sb = (torch.exp2(torch.randint(0, 3, (n, kb), generator=g).float()).cuda().to(torch.float8_e8m0fnu) for n in (M, -(-N // 128)))
+    want = (ref.value(a, sa) @ ref.value(b, sb, 128).t()).float()
+    for _ in range(3):
+        assert torch.equal(ops.matmul_fp8(a, sa, b, sb, dtype=F32), want)
