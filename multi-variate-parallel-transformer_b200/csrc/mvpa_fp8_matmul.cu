@@ -952,13 +952,22 @@ struct Kernel {
 template <typename Out, typename S>
 int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, MatmulArgs g, cudaStream_t s) {
   constexpr bool kScaled = sizeof(S) == 1;
+  constexpr int kLongScaled = 40;  // blocks from which on four pairs may share a tile
   const int64_t pairs = device_sm_count() / 2;
   const auto tiles_of = [&](int width) { return (int64_t)((g.N + width - 1) / width) * ((g.M + 255) / 256); };
   // Narrow tiles where each has a pair of its own, unless K is long and four pairs can share a wide one (15 clusters of eight CTAs are
   // resident at once).  us, narrow / wide, alone or shared: 550 x 768 x 2496 7.1 / 8.8, 300 x 300 x 300 5.1 / 6.3, 550 x 768 x 4096
   // 8.8 / 10.6, 500 x 2048 x 7680 13.8 / 16.1; 132 x 4736 x 768 (as many narrow tiles as pairs) 6.6 / 6.2; 132 x 2048 x 7680
   // 12.9 / 12.2, 256 x 1500 x 6000 14.8 / 12.2, 100 x 500 x 8000 17.4 / 11.9.
-  const bool narrow = kScaled && 3 * tiles_of(192) <= pairs && !(g.KB >= 40 && tiles_of(192) <= 15);
+  int fours = 0;  // clusters of four pairs
+  if constexpr (kScaled) {
+    if (g.KB >= kLongScaled) {
+      constexpr auto shared = matmul_scaled_kernel<Out, true, 192>;
+      MVPA_CUDA_CHECK(grant_smem<shared>(ScaledRows<192>::kSmem));
+      MVPA_CUDA_CHECK(resident_clusters<shared>(8, kScaledThreads, ScaledRows<192>::kSmem, &fours));
+    }
+  }
+  const bool narrow = kScaled && 3 * tiles_of(192) <= pairs && tiles_of(192) > fours;
   const int kTileN = !kScaled ? 256 : narrow ? 64 : 192;
   const int64_t tiles = tiles_of(kTileN);
   if (tiles * g.KB > 0x7fffffff) {
@@ -1008,7 +1017,7 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
       MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)tiles), kScaledThreads, ScaledRows<64>::kSmem, s, map_w, map_x, map_o, g));
     } else {
       rc = run(Kernel<matmul_scaled_kernel<Out, false, 192>>(), Kernel<matmul_scaled_kernel<Out, true, 192>>(), kScaledThreads,
-               ScaledRows<192>::kSmem, 40, 48);
+               ScaledRows<192>::kSmem, kLongScaled, 48);
     }
   } else {
     rc = run(Kernel<matmul_many_kernel<Out, S, false>>(), Kernel<matmul_many_kernel<Out, S, true>>(), kManyThreads, ManyRows::kSmem, 16, 24);
