@@ -312,7 +312,7 @@ int mvpa_silu_mul_fp8(const void* gate, const void* up, int64_t ld_in, void* q, 
  * MVPA_F32 (both the same), any strides in elements; out (M, N) MVPA_BF16 or MVPA_F32, leading dimension
  * ld_out.  All sums are in fp32, in an order that depends on the sizes alone, and rounded once.  A block's
  * products are scaled by the two scales' product, which for a few rows (up to 32) and for fp32 scales is
- * formed in fp32: it must not overflow there.  K = 0 gives zeros.  `status` (may be
+ * formed in fp32: it must not overflow there, and counts as zero below 2^-150.  K = 0 gives zeros.  `status` (may be
  * NULL): 64 ints, zeroed by the caller, of which the first is non-zero afterwards if one of the kernel's
  * bounded waits ran out (the results are then NaN); mvpa_workspace_status(status, 256, stream) reads it.
  */

@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) matmul_many_kernel(const __gr
 // a tile's sum stays in TMEM over the whole of K and comes home once.  In matmul_many_kernel a block's product has to be fetched
 // before the block after the next can start - 512 cycles of products, then some 1400 to hear of them, fetch them in both CTAs and
 // say so - which leaves the tensor cores idle half of the time.  Tiles of 256 tokens x 192 weight rows: two of them and the scales
-// of five blocks fill TMEM, so that a tile leaves while the next one is summed.
+// of three groups of four blocks take 432 of TMEM's 512 columns, and a tile leaves while the next one is summed.
 //
 // A word of TMEM has room for four scales, and a product names the byte that it wants: they are laid out and copied for four
 // blocks at once.  (For each block, four bytes alike, the three copies took the tensor cores' time as well, 100 cycles for 384 of
@@ -955,10 +955,10 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
   constexpr int kLongScaled = 40;  // blocks from which on four pairs may share a tile
   const int64_t pairs = device_sm_count() / 2;
   const auto tiles_of = [&](int width) { return (int64_t)((g.N + width - 1) / width) * ((g.M + 255) / 256); };
-  // Narrow tiles where each has a pair of its own, unless K is long and four pairs can share a wide one (15 clusters of eight CTAs are
-  // resident at once).  us, narrow / wide, alone or shared: 550 x 768 x 2496 7.1 / 8.8, 300 x 300 x 300 5.1 / 6.3, 550 x 768 x 4096
-  // 8.8 / 10.6, 500 x 2048 x 7680 13.8 / 16.1; 132 x 4736 x 768 (as many narrow tiles as pairs) 6.6 / 6.2; 132 x 2048 x 7680
-  // 12.9 / 12.2, 256 x 1500 x 6000 14.8 / 12.2, 100 x 500 x 8000 17.4 / 11.9.
+  // Narrow tiles where each has a pair of its own, unless K is long and four pairs can share a wide one (on this device 15 clusters of
+  // eight CTAs are resident at once).  us, narrow / wide with one, two, four pairs a tile: 300 x 300 x 300 5.2 / 6.3, 9.3, 8.9; 550 x 768 x
+  // 2496 7.1 / 8.8, 10.7, 9.9; 550 x 768 x 4096 8.8 / 11.4, 11.9, 10.6; 500 x 2048 x 7680 (22 wide tiles) 13.9 / 17.6, 16.1, -; 132 x 2048
+  // x 7680 12.9 / 17.2, 14.8, 12.2; 256 x 1500 x 6000 14.8 / 20.3, 15.8, 12.2; 100 x 500 x 8000 17.5 / 19.4, 15.7, 12.0.
   int fours = 0;  // clusters of four pairs
   if constexpr (kScaled) {
     if (g.KB >= kLongScaled) {
@@ -986,11 +986,10 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
   }
   if (rc != MVPA_OK) return rc;
   const auto run = [&](auto whole, auto parts, int threads, size_t smem, int most4, int most2) {
-    // Four or two pairs to a tile, as long as all clusters are resident at once (15 of eight CTAs, 33 of four).  A cluster of eight costs
-    // some 2 us more than one of two; a block 0.2 us with scales that are powers of two, 0.4 with others.  us with 1 / 2 / 4 pairs, powers of
-    // two: 132 x 2048 x 7680 18.5 / 15.7 / 12.8, 550 x 2048 x 7680 19.2 / 17.0 / two rounds, 550 x 768 x 4096 12.5 / 12.8 / 11.2;
-    // 550 x 768 x 2496 (20 blocks) 10.1 / 11.7 / 10.4; others, 1 / 4 pairs: 132 x 2048 x 7680 30.2 / 14.8, 550 x 768 x 2496 12.8 / 10.3,
-    // and with 2 pairs 64 x 8000 x 8000 31.3 / 21.9.
+    // Four or two pairs to a tile, as long as all clusters are resident at once (15 of eight CTAs, 33 of four).  us with 1 / 2 / 4 pairs:
+    // scales that are powers of two, above and 550 x 2048 x 7680 (33 tiles) 18.0 / 16.7 / -; others, 300 x 300 x 300 (3 blocks) 6.5 /
+    // 11.2 / 9.5, 550 x 768 x 2496 13.1 / 13.4 / 10.7, 132 x 2048 x 7680 30.6 / 21.4 / 15.2, 550 x 768 x 4096 18.5 / 15.8 / 12.0, 64 x
+    // 8000 x 8000 (32 tiles) 32.5 / 22.3 / -.
     constexpr auto one = decltype(whole)::value, some = decltype(parts)::value;
     for (int n : {4, 2}) {
       int most = 0;
@@ -1030,9 +1029,11 @@ int run_many(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, Ma
 
 template <typename Out, typename S>
 int run_matmul(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int K, const MatmulArgs& g, cudaStream_t s) {
-  // From 33 tokens on the pairs are faster (e8m0, us, pairs of CTAs / few rows with as many columns as there are tokens, up to 128 a
-  // CTA): 132 x 4736 x 768 7.3 / 21.3, 257 x 2048 x 7680 18.5 / 34, 33 x 5000 x 2000 9.4 / 11.2; below, few rows: 22 x 768 x 2496
-  // 9.5 / 6.5, 22 x 2048 x 7680 18 / 13, 22 x 15360 x 2048 13.9 / 8.4 (22 x 4736 x 768: 7.0 / 7.1).
+  // Up to 32 tokens the weights' bytes bound a product, which is what the kernel for few rows is made for.  us, few rows / pairs of
+  // CTAs, e8m0 scales: 22 x 15360 x 2048 9.5 / 12.1, 32 x 15360 x 2048 10.4 / 12.0, 32 x 2048 x 7680 7.6 / 10.5, 32 x 768 x 2496 6.0 / 6.7,
+  // 32 x 5000 x 2000 7.5 / 7.9, 32 x 4096 x 4096 6.9 / 9.3; where K is short the pairs catch up sooner (4736 x 768: 16 rows 5.1 / 5.6, 32
+  // rows 7.1 / 5.6).  Its time grows with the columns that a thread adds up (one row 7.1, 16 rows 8.5, 32 rows 10.4 at 15360 x 2048), so
+  // it ends there.
   if (g.M > 32) return run_many<Out, S>(a, ld_a, b, ld_b, K, g, s);
   const int nt = g.M <= 16 ? 16 : 32;
   CUtensorMap map_w, map_x;
