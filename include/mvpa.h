@@ -277,6 +277,25 @@ int mvpa_contrastive_logits(const void* pred, const void* enc, const int32_t* ne
                             float* logits, int32_t B, int32_t T, int32_t C, int32_t E, int32_t K,
                             float temperature, int32_t dtype, void* cuda_stream);
 
+/*
+ * The gated projection of the MLP, bf16: h = silu(x Wg^T) * (x Wu^T), x (M, E) with leading dimension ld_x, w_gate and w_up (I, E)
+ * contiguous, h (M, I) with leading dimension ld_h; what `LlamaMLP` does before its down projection (`models/mvpformer.py:114,146`)
+ * in one kernel.  Both products and the activation are in fp32, rounded once.  `gate` and `up` ((M, I) contiguous, or both NULL)
+ * receive the two products, rounded to bf16, for the backward pass.  E and I are multiples of 8; bases and rows lie on 16-byte
+ * boundaries.  `status` (may be NULL): as for mvpa_matmul_fp8.
+ */
+int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const void* w_up, void* h, int64_t ld_h, void* gate, void* up,
+                      int64_t M, int32_t E, int32_t I, int32_t* status, void* cuda_stream);
+
+/*
+ * Its gradients from dh (M, I; leading dimension ld_dh) and what the forward saved: dx = dg Wg + du Wu (M, E) unless dx is NULL,
+ * dw_gate = dg^T x and dw_up = du^T x (I, E) unless they are NULL; all contiguous, sums in fp32, in an order that depends on the sizes
+ * alone, rounded once.  `dgate` and `dup` ((M, I), contiguous) receive dg and du in bf16, the operands of those products.
+ */
+int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* gate, const void* up, const void* x, int64_t ld_x, const void* w_gate,
+                          const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up, int64_t M, int32_t E, int32_t I,
+                          int32_t* status, void* cuda_stream);
+
 /* ---- the block in 8 bits ----------------------------------------------------------------------
  * A row in 8 bits is a pair: q in e4m3, and one scale for each block of 128 neighbours (the row's last
  * block as long as the row leaves it); a weight has one scale for each block of 128 x 128.  The pair

@@ -1,0 +1,415 @@
+// The gated projection of the MLP in one kernel, and its gradients, in bf16:
+//
+//   h = silu(g) u,  g = x Wg^T,  u = x Wu^T                    x (M, E), Wg and Wu (I, E)
+//   dg = dh u s (1 + g (1 - s)),  du = dh g s,  s = 1 / (1 + e^-g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+//
+// Three matrix products of one shape of kernel: a pair of CTAs (cta_group::2) forms 256 rows x 256 columns of sums in TMEM, fp32, from
+// blocks of 64 along the summed axis that the TMA stages in shared memory.
+//   forward        the first CTA brings 128 rows of Wg and the second the same rows of Wu, so that a thread that holds a token's row of
+//                  sums finds g and u of one feature 128 columns apart: h leaves from fp32 in one rounding, and g and u go to memory
+//                  (rounded to bf16) only where a backward pass will want them.
+//   input          dg and du are the left operand one after the other, Wg and Wu, whose rows lie along the columns of the result
+//                  (MN-major), the right one: the sum of both products is formed in TMEM.
+//   weights        both operands have the summed axis, the tokens, outermost (MN-major).
+// dg and du are rounded to bf16 between the kernels: the products take 16-bit operands, and each of their sums is over hundreds of
+// terms, whose roundings (2^-9 each) leave the sum as exact as its own rounding to bf16 does.
+#include "block_rows.cuh"
+#include "tc_pairs.cuh"
+#include "tc_tma_host.cuh"
+
+namespace mvpa {
+namespace {
+
+enum : int { kForward = 0, kForwardSave = 1, kInput = 2, kWeights = 3 };
+
+struct GatedMaps {
+  CUtensorMap a[2], b[2], out[3];
+};
+struct GatedArgs {
+  uint32_t tiles_m, tiles_n;
+  uint32_t part;     // tiles along M of one part (kWeights: dWg, then dWu)
+  int blocks;        // blocks along the summed axis in a segment (kInput: dg Wg, then du Wu)
+  int segments;
+  int rows, cols;    // of the results
+  int* status;
+};
+
+constexpr int kGatedThreads = 384;
+constexpr int kGatedStages = 5, kGatedStageBytes = 2 * 128 * 128;
+constexpr int kGatedOutBytes = 8 * 2 * 4096;  // a warp's 32 rows x 64 columns on their way out, twice
+constexpr size_t kGatedSmem = 1024 + kGatedStages * kGatedStageBytes + kGatedOutBytes;
+
+enum : int { kGiveUpEmpty = 81, kGiveUpFull = 82, kGiveUpTmemEmpty = 83, kGiveUpTmemFull = 84, kGiveUpDrain = 85 };
+
+// silu(g) u = g u / (1 + e^-g), for any g.  With a = e^(-|g| / 4) (which leaves the normal numbers below |g| = 349, where the product
+// with any u rounds to zero) the factor of a negative g is a^4 / (1 + a^4), taken into the product in four parts, so that nothing
+// underflows that the result does not.  Errors: an ulp or two of a, four times over, 2^-19 against the 2^-9 of the result's rounding.
+struct Sigmoid {
+  float part, r;  // e^(-|g| / 4) where g < 0, else 1;  1 / (1 + e^-|g|)
+  float other;    // 1 - s
+  __device__ __forceinline__ explicit Sigmoid(float g) {
+    const float a = ptx::ex2(fabsf(g) * (-0.25f * kLog2e)), a2 = a * a, e = a2 * a2;
+    r = __fdividef(1.f, 1.f + e);
+    part = g < 0.f ? a : 1.f;
+    other = g < 0.f ? r : e * r;
+  }
+  // a b s
+  __device__ __forceinline__ float times(float a, float b) const { return (a * part * part) * (b * part * part) * r; }
+};
+
+template <int MODE>
+__global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs g) {
+  constexpr bool kGate = MODE <= kForwardSave, kRowsA = MODE == kWeights, kRowsB = MODE >= kInput;  // (rows along M / N: MN-major)
+  constexpr int kTileN = kGate ? 128 : 256;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_full[kGatedStages], s_empty[kGatedStages], s_tfull[2], s_tempty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_dead;  // a wait ran out: nothing waits any more, and the results are NaN
+  const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t half = ptx::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = g.tiles_m * g.tiles_n;
+  const int blocks = g.blocks * g.segments;
+  if (warp == 0) {
+    ptx::prefetch_tensormap(&maps.a[0]);
+    ptx::prefetch_tensormap(&maps.b[0]);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < kGatedStages; ++i) {
+        ptx::mbar_init(&s_full[i], 1);
+        ptx::mbar_init(&s_empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(&s_tfull[i], 1);
+        ptx::mbar_init(&s_tempty[i], 16);
+      }
+      ptx::mbar_fence_init();
+      s_dead = 0;
+    }
+    __syncwarp();
+    ptx::tmem_alloc_pair(&s_tmem, 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* dead = &s_dead;
+  const auto wait = [&](uint64_t& bar, uint32_t parity, int code) {
+    if (ptx::mbar_test_wait(&bar, parity)) return true;
+    if (*dead) return false;
+    if (ptx::mbar_wait(&bar, parity, g.status, code)) return true;
+    *dead = 1;
+    return false;
+  };
+  ptx::griddep_launch();
+  ptx::griddep_wait();
+
+  if (warp == 0 || warp == 2) {  // left operand, right operand: a warp of each CTA loads its CTA's 128 rows (or columns) a block
+    const bool left = warp == 0;
+    const uint32_t el = ptx::elect_one(), there = ptx::cluster_map(ptx::smem_u32(s_full), 0);
+    Ring<kGatedStages> st;
+    uint32_t loads = 0;
+    bool on = true;
+    for (uint32_t t = pair; t < tiles && on; t += pairs) {
+      const Tile at = tile_at<kTileN>(t, g.tiles_n, g.tiles_m);
+      const uint32_t part = (uint32_t)at.m0 / 256 >= g.part ? 1 : 0;
+      const int row = left ? at.m0 - (int)(part * g.part * 256) + (int)half * 128 : kGate ? at.n0 : at.n0 + (int)half * 128;
+      for (int kb = 0; kb < blocks; ++kb, ++loads, st.step()) {
+        if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
+          on = false;
+          break;
+        }
+        if (left && half == 0 && el) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * kGatedStageBytes);
+        __syncwarp();
+        const int seg = kb >= g.blocks ? 1 : 0, k = (kb - seg * g.blocks) * 64;
+        const uint32_t to = stages + st.at * kGatedStageBytes + (left ? 0 : 128 * 128), bar = there + 8 * st.at;
+        const CUtensorMap* map = left ? &maps.a[kRowsA ? part : seg] : &maps.b[kGate ? half : kRowsA ? 0 : seg];
+        if (left ? kRowsA : kRowsB) {
+          ptx::tma_load_2d_pair_w(el, to, map, bar, row, k);
+          ptx::tma_load_2d_pair_w(el, to + 64 * 128, map, bar, row + 64, k);
+        } else {
+          ptx::tma_load_2d_pair_w(el, to, map, bar, k, row);
+        }
+      }
+    }
+    if (left && half == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one at the end)
+      const uint32_t n = min(loads, (uint32_t)kGatedStages);
+      for (uint32_t k = loads - n; k != loads; ++k)
+        if (!ptx::mbar_wait(&s_full[k % kGatedStages], (k / kGatedStages) & 1, g.status, kGiveUpDrain)) break;
+    }
+  } else if (warp == 1) {
+    if (half == 0) {
+      const uint32_t el = ptx::elect_one();
+      constexpr uint32_t idesc = ptx::make_idesc_bf16_ab(256, 256, kRowsA, kRowsB);
+      constexpr uint32_t kStepA = kRowsA ? 128 : 2, kStepB = kRowsB ? 128 : 2;
+      const ptx::DescHalves a0 = ptx::make_desc_halves_sw128(stages, kRowsA ? 64 * 128 : 16, 1024),
+                            b0 = ptx::make_desc_halves_sw128(stages + 128 * 128, kRowsB ? 64 * 128 : 16, 1024);
+      Ring<kGatedStages> st;
+      Ring<2> buf;
+      uint32_t last = 0, last_parity = 0;
+      bool on = true, any = false;
+      for (uint32_t t = pair; t < tiles && on; t += pairs, buf.step()) {
+        if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
+        ptx::tc_fence_after();
+        for (int kb = 0; kb < blocks; ++kb, st.step()) {
+          if (!wait(s_full[st.at], st.parity, kGiveUpFull)) {
+            on = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t off = st.at * (kGatedStageBytes >> 4);
+          ptx::mma_f16_ss_x4_pair_w(el, tmem + buf.at * 256, {a0.lo + off, a0.hi}, {b0.lo + off, b0.hi}, kStepA, kStepB, idesc, kb > 0);
+          ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_empty[st.at]));
+          last = st.at;
+          last_parity = st.parity;
+          any = true;
+        }
+        if (on) ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_tfull[buf.at]));
+      }
+      if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
+    }
+  } else if (warp >= 4) {
+    // Eight warps take the sums home: a thread one row, every other 64 columns.  A warp puts 32 rows x 64 columns into shared memory in
+    // the 128-byte swizzle and leaves them to the TMA, which skips what lies past the matrix.
+    const int quad = warp & 3, group = (warp - 4) >> 2;
+    const uint32_t outs = stages + kGatedStages * kGatedStageBytes + (warp - 4) * 8192, at_tmem = tmem + ((uint32_t)quad << 21);
+    uint32_t which = 0;
+    const auto place = [&]() {
+      if (lane == 0) ptx::tma_store_wait_read<1>();
+      __syncwarp();
+      which ^= 1;
+      return outs + which * 4096;
+    };
+    const auto put = [&](uint32_t to, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + lane * 128 + ((piece ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d)
+                   : "memory");
+    };
+    const auto send = [&](uint32_t from, const CUtensorMap* map, int x, int y) {
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        ptx::tma_store_2d(map, from, x, y);
+        ptx::tma_store_commit();
+      }
+    };
+    Ring<2> buf;
+    for (uint32_t t = pair; t < tiles; t += pairs, buf.step()) {
+      const Tile at = tile_at<kTileN>(t, g.tiles_n, g.tiles_m);
+      const uint32_t part = (uint32_t)at.m0 / 256 >= g.part ? 1 : 0;
+      const int y = at.m0 - (int)(part * g.part * 256) + (int)half * 128 + quad * 32;
+      wait(s_tfull[buf.at], buf.parity, kGiveUpTmemFull);
+      __syncwarp();
+      ptx::tc_fence_after();
+      const uint32_t from = at_tmem + buf.at * 256;
+      const uint32_t poison = *dead ? 0x7fffffffu : 0u;
+      const auto release = [&]() {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&s_tempty[buf.at]), 0));
+      };
+      const auto words = [&](const uint32_t (&r)[32], uint32_t to, int piece) {  // 32 sums as they are, rounded
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const auto two = [&](int i) {
+            return ptx::pack_bf16(__uint_as_float(r[k * 8 + 2 * i] | poison), __uint_as_float(r[k * 8 + 2 * i + 1] | poison));
+          };
+          put(to, piece + k, two(0), two(1), two(2), two(3));
+        }
+      };
+      if constexpr (kGate) {
+        const int x = at.n0 + group * 64;
+        const bool inside = y < g.rows && x < g.cols;  // (the same for the whole warp: a store does not begin past the matrix)
+        if constexpr (MODE == kForwardSave) {
+          for (int which_sum = 0; which_sum < 2; ++which_sum) {
+            const uint32_t to = place();
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+              uint32_t r[32];
+              ptx::tmem_ld32(from + which_sum * 128 + group * 64 + c, r);
+              ptx::tmem_ld_wait();
+              words(r, to, c / 8);
+            }
+            if (inside) send(to, &maps.out[1 + which_sum], x, y);
+            else if (lane == 0) ptx::tma_store_commit();  // (each use of a place is a group)
+          }
+        }
+        const uint32_t to = place();
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t rg[32], ru[32];
+          ptx::tmem_ld32(from + group * 64 + c, rg);
+          ptx::tmem_ld32(from + 128 + group * 64 + c, ru);
+          ptx::tmem_ld_wait();
+          if (c == 32) release();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float gate = __uint_as_float(rg[j]);
+            rg[j] = __float_as_uint(Sigmoid(gate).times(gate, __uint_as_float(ru[j])));
+          }
+          words(rg, to, c / 8);
+        }
+        if (inside) send(to, &maps.out[0], x, y);
+        else if (lane == 0) ptx::tma_store_commit();
+      } else {
+#pragma unroll
+        for (int c = 0; c < 256; c += 128) {
+          const int x = at.n0 + c + group * 64;
+          const uint32_t to = place();
+          uint32_t r0[32], r1[32];
+          ptx::tmem_ld32(from + c + group * 64, r0);
+          ptx::tmem_ld32(from + c + group * 64 + 32, r1);
+          ptx::tmem_ld_wait();
+          if (c == 128) release();
+          words(r0, to, 0);
+          words(r1, to, 4);
+          if (y < g.rows && x < g.cols) send(to, &maps.out[part], x, y);
+          else if (lane == 0) ptx::tma_store_commit();
+        }
+      }
+    }
+    if (lane == 0) ptx::tma_store_wait_all();
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();  // neither CTA's memory goes while the other's products or barriers use it
+  ptx::tc_fence_after();
+  if (warp == 1) ptx::tmem_dealloc_pair(tmem, 512);
+}
+
+// dg and du from dh and the forward's g and u, in fp32, rounded once.  Bound by memory: 10 bytes an element.
+__global__ void __launch_bounds__(256) gate_bwd_kernel(const __nv_bfloat16* __restrict__ dh, int64_t ld_dh, const __nv_bfloat16* __restrict__ gate,
+                                                       const __nv_bfloat16* __restrict__ up, __nv_bfloat16* __restrict__ dgate,
+                                                       __nv_bfloat16* __restrict__ dup, int64_t rows, int width) {
+  using V = Vec<__nv_bfloat16>;
+  ptx::griddep_launch();
+  ptx::griddep_wait();
+  const int per_row = width / V::N;
+  const int64_t total = rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / per_row, c = (i - row * per_row) * V::N;
+    float x[V::N], u[V::N], d[V::N];
+    V::load(gate + i * V::N, x);
+    V::load(up + i * V::N, u);
+    V::load(dh + row * ld_dh + c, d);
+#pragma unroll
+    for (int e = 0; e < V::N; ++e) {
+      const Sigmoid s(x[e]);
+      const float dg = s.times(d[e], u[e]) * fmaf(x[e], s.other, 1.f);
+      u[e] = s.times(d[e], x[e]);
+      x[e] = dg;
+    }
+    V::store(dgate + i * V::N, x);
+    V::store(dup + i * V::N, u);
+  }
+}
+
+// A matrix of bf16, in boxes of 64 columns.
+int encode(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)ld * 2};
+  const uint32_t box[2] = {64, (uint32_t)box_rows};
+  return encode_bf16_sw128(map, base, 2, dims, strides, box);
+}
+
+template <int MODE>
+int run_gated(const GatedMaps& maps, GatedArgs g, cudaStream_t s) {
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, pairs = device_sm_count() / 2;
+  if (tiles * g.blocks * g.segments > 0x7fffffff) {
+    set_error("mvpa_gated_linear: more than 2^31 blocks of 256 x 256 x 64");
+    return MVPA_ERR_UNSUPPORTED;
+  }
+  constexpr auto kernel = gated_kernel<MODE>;
+  MVPA_CUDA_CHECK(grant_smem<kernel>(kGatedSmem));
+  MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kGatedThreads, kGatedSmem, s, maps, g));
+  count_launch();
+  MVPA_CUDA_CHECK(cudaGetLastError());
+  return MVPA_OK;
+}
+
+uint32_t tiles_of(int64_t n, int each) { return (uint32_t)((n + each - 1) / each); }
+
+int check_sizes(const char* what, int64_t M, int32_t E, int32_t I) {
+  constexpr int kMost = 0x7fffffff - 1024;  // (the first place past the last tile is a 32-bit coordinate)
+  if (M < 1 || E < 1 || I < 1 || M > kMost || E > kMost || I > kMost || E % 8 != 0 || I % 8 != 0) {
+    set_error("%s: M, E and I must lie between 1 and %d, E and I be multiples of 8 (got %lld, %d, %d)", what, kMost, (long long)M, E, I);
+    return MVPA_ERR_SHAPE;
+  }
+  return MVPA_OK;
+}
+bool rows_fit(const void* p, int64_t ld, int64_t width) {
+  return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld >= width && ld % 8 == 0;
+}
+
+}  // namespace
+}  // namespace mvpa
+
+using namespace mvpa;
+
+extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const void* w_up, void* h, int64_t ld_h, void* gate, void* up,
+                                 int64_t M, int32_t E, int32_t I, int32_t* status, void* cuda_stream) {
+  const int rc0 = check_sizes("mvpa_gated_linear", M, E, I);
+  if (rc0 != MVPA_OK) return rc0;
+  if (!rows_fit(x, ld_x, E) || !rows_fit(w_gate, E, E) || !rows_fit(w_up, E, E) || !rows_fit(h, ld_h, I) ||
+      (gate == nullptr) != (up == nullptr) || (gate != nullptr && (!rows_fit(gate, I, I) || !rows_fit(up, I, I)))) {
+    set_error("mvpa_gated_linear: x, the weights, h, gate and up must be 16-byte aligned with rows of a multiple of 16 bytes, not shorter than "
+              "their widths; gate and up are given both or neither");
+    return MVPA_ERR_ALIGNMENT;
+  }
+  GatedMaps maps = {};
+  int rc = encode(&maps.a[0], x, M, E, ld_x, 128);
+  if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, 128);
+  if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 128);
+  if (rc == MVPA_OK) rc = encode(&maps.out[0], h, M, I, ld_h, 32);
+  if (rc == MVPA_OK && gate != nullptr) rc = encode(&maps.out[1], gate, M, I, I, 32);
+  if (rc == MVPA_OK && gate != nullptr) rc = encode(&maps.out[2], up, M, I, I, 32);
+  if (rc != MVPA_OK) return rc;
+  const uint32_t tm = tiles_of(M, 256);
+  const GatedArgs g = {tm, tiles_of(I, 128), tm, (int)tiles_of(E, 64), 1, (int)M, I, status};
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  return gate != nullptr ? run_gated<kForwardSave>(maps, g, s) : run_gated<kForward>(maps, g, s);
+}
+
+extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* gate, const void* up, const void* x, int64_t ld_x,
+                                     const void* w_gate, const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up,
+                                     int64_t M, int32_t E, int32_t I, int32_t* status, void* cuda_stream) {
+  const int rc0 = check_sizes("mvpa_gated_linear_bwd", M, E, I);
+  if (rc0 != MVPA_OK) return rc0;
+  if (!rows_fit(dh, ld_dh, I) || !rows_fit(gate, I, I) || !rows_fit(up, I, I) || !rows_fit(dgate, I, I) || !rows_fit(dup, I, I) ||
+      (dx != nullptr && (!rows_fit(w_gate, E, E) || !rows_fit(w_up, E, E) || !rows_fit(dx, E, E))) || (dw_gate == nullptr) != (dw_up == nullptr) ||
+      (dw_gate != nullptr && (!rows_fit(x, ld_x, E) || !rows_fit(dw_gate, E, E) || !rows_fit(dw_up, E, E)))) {
+    set_error("mvpa_gated_linear_bwd: every matrix must be 16-byte aligned with rows of a multiple of 16 bytes, not shorter than its width; "
+              "dw_gate and dw_up are wanted both or neither");
+    return MVPA_ERR_ALIGNMENT;
+  }
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  using B = const __nv_bfloat16*;
+  const int64_t ctas = (M * (I / 8) + 255) / 256, most = (int64_t)device_sm_count() * 16;
+  MVPA_CUDA_CHECK(launch_dependent(1, gate_bwd_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, s, (B)dh, ld_dh, (B)gate, (B)up,
+                                   (__nv_bfloat16*)dgate, (__nv_bfloat16*)dup, M, (int)I));
+  count_launch();
+  MVPA_CUDA_CHECK(cudaGetLastError());
+  int rc = MVPA_OK;
+  if (dx != nullptr) {
+    GatedMaps maps = {};
+    rc = encode(&maps.a[0], dgate, M, I, I, 128);
+    if (rc == MVPA_OK) rc = encode(&maps.a[1], dup, M, I, I, 128);
+    if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, 64);
+    if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 64);
+    if (rc == MVPA_OK) rc = encode(&maps.out[0], dx, M, E, E, 32);
+    const uint32_t tm = tiles_of(M, 256);
+    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, tiles_of(E, 256), tm, (int)tiles_of(I, 64), 2, (int)M, E, status}, s);
+  }
+  if (rc == MVPA_OK && dw_gate != nullptr) {
+    GatedMaps maps = {};
+    rc = encode(&maps.a[0], dgate, M, I, I, 64);
+    if (rc == MVPA_OK) rc = encode(&maps.a[1], dup, M, I, I, 64);
+    if (rc == MVPA_OK) rc = encode(&maps.b[0], x, M, E, ld_x, 64);
+    if (rc == MVPA_OK) rc = encode(&maps.out[0], dw_gate, I, E, E, 32);
+    if (rc == MVPA_OK) rc = encode(&maps.out[1], dw_up, I, E, E, 32);
+    const uint32_t tm = tiles_of(I, 256);
+    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, tiles_of(E, 256), tm, (int)tiles_of(M, 64), 1, I, E, status}, s);
+  }
+  return rc;
+}

@@ -447,6 +447,26 @@ __device__ __forceinline__ void mma_f8_ss_x4_pair_w(uint32_t el, uint32_t d_tmem
       "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el)
       : "memory");
 }
+// Four consecutive K-steps of 16 for 16-bit operands, `a_step` and `b_step` units of 16 bytes apart (2 in rows of K, 128 where rows
+// lie along M or N); the first one overwrites D if `accumulate` is 0.
+__device__ __forceinline__ void mma_f16_ss_x4_pair_w(uint32_t el, uint32_t d_tmem, DescHalves a, DescHalves b, uint32_t a_step, uint32_t b_step,
+                                                     uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p0, p1, pe;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+      "setp.ne.b32 p0, %9, 0;\n\t"
+      "setp.eq.b32 p1, 0, 0;\n\t"
+      "setp.ne.b32 pe, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t mov.b64 db, {%3, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p0;\n\t"
+      "add.u32 la, %1, %7;\n\t add.u32 lb, %3, %8;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p1;\n\t"
+      "add.u32 la, la, %7;\n\t add.u32 lb, lb, %8;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p1;\n\t"
+      "add.u32 la, la, %7;\n\t add.u32 lb, lb, %8;\n\t mov.b64 da, {la, %2};\n\t mov.b64 db, {lb, %4};\n\t"
+      "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p1;\n\t}" ::"r"(d_tmem),
+      "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(el), "r"(a_step), "r"(b_step), "r"(accumulate)
+      : "memory");
+}
 // ---- the same with a scale (e8m0) for each row's 32 neighbours along K, read from TMEM (kind::mxf8f6f4) ----
 // A matrix of up to 128 rows has its scales in four columns of TMEM: row r in lane r % 32 of column r / 32, in the byte of the
 // word that the instruction descriptor names (A's in bits [29,31), B's in [4,6)), in each quarter of the lanes.  Shared memory

@@ -33,7 +33,8 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
 ]
 FAST_MATH = "--use_fast_math"        # everywhere but in the files below, whose results are not rounded to 16 bits afterwards
-PRECISE = ("mvpa_rows_f32.cu", "mvpa_fp8_rows.cu", "mvpa_fp8_matmul.cu")   # (8-bit: every value lies next to some rounding border)
+PRECISE = ("mvpa_rows_f32.cu", "mvpa_fp8_rows.cu", "mvpa_fp8_matmul.cu",   # (8-bit: every value lies next to some rounding border)
+           "mvpa_gated.cu")
 
 MVPA_F32, MVPA_BF16, MVPA_F16, MVPA_E8M0 = 0, 1, 2, 3
 
@@ -145,7 +146,7 @@ EXPORTS = ("mvpa_fwd", "mvpa_bwd", "mvpa_fwd_workspace_bytes", "mvpa_bwd_workspa
            "mvpa_selftest_wait_timeout", "mvpa_rmsnorm", "mvpa_silu_mul", "mvpa_wave_encode_size",
            "mvpa_wave_encode", "mvpa_channel_mean", "mvpa_contrastive_logits", "mvpa_peer_gather", "mvpa_peer_signal",
            "mvpa_peer_wait", "mvpa_rmsnorm_bwd", "mvpa_rmsnorm_bwd_workspace_bytes", "mvpa_silu_mul_bwd", "mvpa_quantize_fp8",
-           "mvpa_rmsnorm_fp8", "mvpa_silu_mul_fp8", "mvpa_matmul_fp8")
+           "mvpa_rmsnorm_fp8", "mvpa_silu_mul_fp8", "mvpa_matmul_fp8", "mvpa_gated_linear", "mvpa_gated_linear_bwd")
 ABI_VERSION = 3   # mvpa_abi_version() of the header this shim was written against
 
 
@@ -210,6 +211,10 @@ def lib() -> ctypes.CDLL:
         L.mvpa_silu_mul_fp8.argtypes = [vp, vp, i64, vp, i64, vp, i64, i64, i32, i32, vp]
         L.mvpa_matmul_fp8.restype = ctypes.c_int
         L.mvpa_matmul_fp8.argtypes = [vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, i32, vp, i64, i64, i32, i32, i32, vp, vp]
+        L.mvpa_gated_linear.restype = ctypes.c_int
+        L.mvpa_gated_linear.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, i64, i32, i32, vp, vp]
+        L.mvpa_gated_linear_bwd.restype = ctypes.c_int
+        L.mvpa_gated_linear_bwd.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, vp]
         L.mvpa_wave_encode_size.restype = i32
         L.mvpa_wave_encode_size.argtypes = [i32, ctypes.POINTER(i32), i32]
         L.mvpa_wave_encode.restype = ctypes.c_int

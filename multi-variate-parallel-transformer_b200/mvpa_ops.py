@@ -188,6 +188,86 @@ def swiglu(gate, up):
     return torch.nn.functional.silu(gate) * up
 
 
+def _status_word(device):
+    """The kernels' status word, or None unless calls look at it."""
+    return torch.zeros(64, dtype=torch.int32, device=device) if _attn._CHECK_STATUS else None
+
+
+def _look_at(status, what, like):
+    if status is not None:      # debugging aid: synchronises the stream
+        _nat.check(_nat.lib().mvpa_workspace_status(status.data_ptr(), 256, _stream(like)), f"{what} kernel")
+
+
+def _gated_kernel(x, w_gate, w_up, save):
+    """(h, gate, up) by the kernel, the last two None unless `save`; x (rows, E)."""
+    (rows, E), I = x.shape, w_gate.shape[0]
+    h = torch.empty((rows, I), dtype=x.dtype, device=x.device)
+    gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
+    with _nat.on_device(x.device):
+        status = _status_word(x.device)
+        st = _nat.lib().mvpa_gated_linear(x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(), I,
+                                          gate.data_ptr() if save else None, up.data_ptr() if save else None, rows, E, I,
+                                          None if status is None else status.data_ptr(), _stream(x))
+        _nat.check(st, "mvpa_gated_linear")
+        _look_at(status, "mvpa_gated_linear", x)
+    return h, gate, up
+
+
+def _gated_kernel_bwd(dh, gate, up, x, w_gate, w_up, need_x, need_w):
+    """(dx, dw_gate, dw_up) by the kernels, None where not needed; x (rows, E)."""
+    (rows, E), I = x.shape, w_gate.shape[0]
+    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    dx = torch.empty((rows, E), dtype=x.dtype, device=x.device) if need_x else None
+    dw_gate, dw_up = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need_w else (None, None)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    with _nat.on_device(x.device):
+        status = _status_word(x.device)
+        st = _nat.lib().mvpa_gated_linear_bwd(dh.data_ptr(), I, gate.data_ptr(), up.data_ptr(), x.data_ptr(), E, w_gate.data_ptr(),
+                                              w_up.data_ptr(), dgate.data_ptr(), dup.data_ptr(), ptr(dx), ptr(dw_gate), ptr(dw_up), rows,
+                                              E, I, ptr(status), _stream(x))
+        _nat.check(st, "mvpa_gated_linear_bwd")
+        _look_at(status, "mvpa_gated_linear_bwd", x)
+    return dx, dw_gate, dw_up
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up):
+        h, gate, up = _gated_kernel(x.view(-1, x.shape[-1]), w_gate, w_up, any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, w_gate, w_up, gate, up)
+        return h if x.dim() == 2 else h.reshape(*x.shape[:-1], w_gate.shape[0])
+
+    @staticmethod
+    def backward(ctx, dh):
+        x, w_gate, w_up, gate, up = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        E, I = x.shape[-1], w_gate.shape[0]
+        if not torch.is_grad_enabled() and _plain(dh.contiguous(), x, w_gate, w_up, gate, up):
+            dx, dw_gate, dw_up = _gated_kernel_bwd(dh.contiguous().view(-1, I), gate, up, x.view(-1, E), w_gate, w_up, need[0],
+                                                   need[1] or need[2])
+            return dx.view(x.shape) if need[0] else None, dw_gate if need[1] else None, dw_up if need[2] else None
+        # a graph of the gradient is wanted (or a transform is active): the same formula in torch operations
+        x2, d = x.reshape(-1, E), dh.reshape(-1, I).float()
+        g, u = torch.nn.functional.linear(x2, w_gate).float(), torch.nn.functional.linear(x2, w_up).float()
+        s = torch.sigmoid(g)
+        dg, du = (d * u * (s * (1 + g * (1 - s)))).to(x.dtype), (d * (g * s)).to(x.dtype)
+        return (dg @ w_gate + du @ w_up).view(x.shape), dg.t() @ x2, du.t() @ x2
+
+
+def gated_linear(x, w_gate, w_up):
+    """Differentiable silu(x w_gate^T) * (x w_up^T) for x (..., E) and weights (I, E): the MLP up to its down projection.  bf16 with E
+    and I multiples of 8: one kernel forward, with both products and the activation in fp32, rounded once; the backward is one for the
+    gate and one for each matrix product (the gradient of x, that of both weights), from the two products, which the forward keeps in
+    bf16 where a gradient is wanted.  Everything else, and calls under autocast, by torch operations."""
+    if (not torch.is_autocast_enabled("cuda") and x.dtype == torch.bfloat16 and x.dim() > 1 and w_gate.dim() == 2 and w_gate.shape == w_up.shape
+            and x.shape[-1] == w_gate.shape[1] and x.shape[-1] % 8 == 0 and w_gate.shape[0] % 8 == 0):
+        if not x.is_contiguous():
+            x = x.contiguous()
+        if _plain(x, w_gate, w_up):
+            return _GatedLinear.apply(x, w_gate, w_up)
+    return swiglu(torch.nn.functional.linear(x, w_gate), torch.nn.functional.linear(x, w_up))
+
+
 @functools.lru_cache(maxsize=None)
 def db4_filters():
     """Decomposition filters (dec_lo, dec_hi) of the Daubechies wavelet with four vanishing moments, eight

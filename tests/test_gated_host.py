@@ -1,0 +1,52 @@
+"""CPU: the gated projection's definition against differences, and what the C entry points refuse before they touch a GPU."""
+import ctypes
+
+import torch
+
+import gated_oracle as ref
+import mvpa_native as nat
+
+
+def _inputs(M, E, I, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    return rand(M, E), rand(I, E) * E ** -0.5, rand(I, E) * E ** -0.5, rand(M, I)
+
+
+def test_gradients_against_differences():
+    x, wg, wu, dh = ins = _inputs(5, 7, 6)
+    grads = ref.gradients(*ins)
+    step = 2.0 ** -17                       # error of a central difference: step^2 |f'''| / 6 ~ 1e-11, roundings 1e-16 / step ~ 1e-11
+    for i, grad in enumerate(grads):
+        for at in range(grad.numel()):
+            moved = [t.clone() for t in (x, wg, wu)]
+            value = []
+            for sign in (1, -1):
+                moved[i].view(-1)[at] = ins[i].view(-1)[at] + sign * step
+                value.append((ref.forward(*moved) * dh).sum())
+            assert abs((value[0] - value[1]) / (2 * step) - grad.view(-1)[at]) < 1e-8
+
+
+def test_gradients_against_autograd():
+    x, wg, wu, dh = _inputs(4, 9, 3, 1)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    auto = torch.autograd.grad(ref.forward(*leaves), leaves, dh)
+    for a, b in zip(auto, ref.gradients(x.detach(), wg.detach(), wu.detach(), dh)):
+        torch.testing.assert_close(a, b, rtol=1e-12, atol=1e-13)
+
+
+def test_entry_points_refuse():
+    lib = nat.lib()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    fwd = lambda x=p, ld_x=64, wg=p, wu=p, h=p, ld_h=64, g=None, u=None, M=4, E=64, I=64: lib.mvpa_gated_linear(
+        x, ld_x, wg, wu, h, ld_h, g, u, M, E, I, None, None)
+    bwd = lambda dh=p, ld=64, g=p, u=p, x=p, dg=p, du=p, dx=p, dwg=p, dwu=p, M=4, E=64, I=64: lib.mvpa_gated_linear_bwd(
+        dh, ld, g, u, x, 64, p, p, dg, du, dx, dwg, dwu, M, E, I, None, None)
+    shape = (dict(M=0), dict(E=0), dict(I=0), dict(E=60), dict(I=4), dict(M=-1), dict(M=2 ** 31))
+    for bad in shape:
+        assert fwd(**bad) == bwd(**bad) == -1 and "multiples of 8" in nat.last_error(), bad
+    for bad in (dict(x=p + 2), dict(ld_x=63), dict(ld_x=56), dict(wg=None), dict(wu=p + 8), dict(h=None), dict(ld_h=68), dict(g=p), dict(u=p)):
+        assert fwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad
+    for bad in (dict(dh=None), dict(ld=60), dict(g=None), dict(du=p + 4), dict(dwg=None), dict(dx=p + 2), dict(x=None)):
+        assert bwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad

@@ -1,0 +1,224 @@
+"""GPU: the gated projection and its gradients against their definition in 64 bits, at the sizes, layouts and values where they can
+go wrong."""
+import threading
+
+import pytest
+import torch
+
+import gated_oracle as ref
+import mvpa_native as nat
+import mvpa_ops as ops
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _inputs(M, E, I, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed + 1000 * M + E + 7 * I)
+    rand = lambda *s: torch.randn(*s, generator=g)
+    x = (rand(M, E) * spread).to(BF16).cuda()
+    wg, wu = ((rand(I, E) * E ** -0.5).to(BF16).cuda() for _ in range(2))
+    return x, wg, wu, (rand(M, I) * 0.1).to(BF16).cuda()
+
+
+def _check(got, x, wg, wu, dh):
+    ins = [t.double() for t in (x, wg, wu, dh)]
+    want = (ref.forward(*ins[:3]), *ref.gradients(*ins))
+    for name, a, b, bound in zip(("h", "dx", "dwg", "dwu"), got, want, ref.bounds(*ins)):
+        worst = ((a.double() - b).abs() - bound).max().item()
+        assert worst <= 1e-38, (name, worst)
+
+
+def _all(x, wg, wu, dh):
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    h = ops.gated_linear(*leaves)
+    return (h.detach(), *torch.autograd.grad(h, leaves, dh))
+
+
+# one of everything; tiles, blocks and boxes that end on their borders, one before and one after; a model's sizes
+@pytest.mark.parametrize("M,E,I", [(1, 8, 8), (1, 768, 1728), (22, 768, 1728), (255, 64, 128), (256, 64, 136), (257, 72, 120), (64, 248, 256),
+                                   (65, 256, 264), (512, 520, 1024), (700, 1000, 1368), (1500, 2048, 776), (40, 64, 20000), (20000, 16, 24),
+                                   (3, 2048, 5632)])
+def test_against_64_bits(cuda, M, E, I):
+    ins = _inputs(M, E, I)
+    launched = nat.lib().mvpa_launch_count()
+    got = _all(*ins)
+    assert nat.lib().mvpa_launch_count() - launched == 4        # the kernels, not torch's operations
+    _check(got, *ins)
+    with torch.no_grad():
+        assert torch.equal(ops.gated_linear(*ins[:3]), got[0])  # what is kept for the backward changes no bit
+
+
+def test_same_bits_from_run_to_run(cuda):
+    ins = _inputs(3000, 768, 1728)
+    first = _all(*ins)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, _all(*ins)))
+
+
+@pytest.mark.parametrize("need", [(True, False, False), (False, True, False), (False, False, True), (True, False, True), (False, True, True)])
+def test_gradients_of_some(cuda, need):
+    ins = _inputs(300, 264, 200)
+    whole = _all(*ins)
+    leaves = [t.detach().requires_grad_(n) for t, n in zip(ins, need)]
+    h = ops.gated_linear(*leaves)
+    wanted = [t for t, n in zip(leaves, need) if n]
+    got = iter(torch.autograd.grad(h, wanted, ins[3]))
+    for n, grad in zip(need, whole[1:]):
+        assert not n or torch.equal(next(got), grad)
+
+
+def test_leading_dimensions_and_strides(cuda):
+    x, wg, wu, dh = _inputs(120, 64, 72)
+    whole = _all(x, wg, wu, dh)
+    got = _all(x.view(2, 3, 20, 64), wg, wu, dh.view(2, 3, 20, 72))
+    assert got[0].shape == (2, 3, 20, 72) and got[1].shape == (2, 3, 20, 64)
+    assert all(torch.equal(a.view(b.shape), b) for a, b in zip(got, whole))
+    wide = torch.zeros(120, 200, dtype=BF16, device="cuda")
+    wide[:, 8:72] = x
+    again = _all(wide[:, 8:72], wg, wu, dh)
+    assert all(torch.equal(a, b) for a, b in zip(again, whole))
+    # an incoming gradient of another layout, and one that is broadcast
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    turned = dh.t().contiguous().t()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(ops.gated_linear(*leaves), leaves, turned), whole[1:]))
+    ones = _all(x, wg, wu, torch.ones_like(dh))
+    ops.gated_linear(*leaves).sum().backward()
+    assert all(torch.equal(t.grad, b) for t, b in zip(leaves, ones[1:]))
+
+
+@pytest.mark.parametrize("M,E,I,dtype", [(5, 9, 16, BF16), (5, 16, 9, BF16), (6, 16, 24, torch.float32), (0, 16, 24, BF16), (4, 16, 8, torch.float16)])
+def test_other_sizes_and_types_by_torch(cuda, M, E, I, dtype):
+    ins = [t.to(dtype) for t in _inputs(M, E, I)]
+    got = _all(*ins)
+    leaves = [t.detach().requires_grad_() for t in ins[:3]]
+    h = torch.nn.functional.silu(leaves[0] @ leaves[1].t()) * (leaves[0] @ leaves[2].t())
+    want = (h.detach(), *torch.autograd.grad(h, leaves, ins[3]))
+    for a, b in zip(got, want):
+        assert a.dtype == dtype and a.shape == b.shape
+        torch.testing.assert_close(a, b, rtol=2 * torch.finfo(dtype).eps, atol=4 * torch.finfo(dtype).eps)
+
+
+def test_unaligned_rows_by_torch(cuda):
+    x, wg, wu, dh = _inputs(9, 64, 72)
+    flat = torch.zeros(9 * 64 + 1, dtype=BF16, device="cuda")
+    moved = flat[1:].view(9, 64)
+    moved.copy_(x)
+    _check(_all(x, wg, wu, dh), x, wg, wu, dh)
+    torch.testing.assert_close(ops.gated_linear(moved, wg, wu), ops.gated_linear(x, wg, wu), rtol=2 ** -6, atol=2 ** -6)
+
+
+def _gates(values, ups, dhs):
+    """Gates and ups that are exactly these numbers: x holds them beside ones and zeros."""
+    n = len(values)
+    x = torch.zeros(n, 8)
+    x[:, 0], x[:, 1] = torch.tensor(values), torch.tensor(ups)
+    wg, wu = torch.zeros(8, 8), torch.zeros(8, 8)
+    wg[:, 0] = 1
+    wu[:, 1] = 1
+    return [t.to(BF16).cuda() for t in (x, wg, wu, torch.tensor(dhs)[:, None].expand(n, 8))]
+
+
+def test_gates_of_any_size(cuda):
+    """Factors far below the smallest number beside a large up, gates that saturate, the largest numbers."""
+    gates = [-1e4, -190.0, -180.0, -120.0, -100.0, -90.0, -87.5, -86.0, -40.0, -1.0, -1e-30, 0.0, 1e-30, 1.0, 20.0, 88.0, 90.0, 200.0, 3e38, -3e38]
+    for up in (1.0, -3e38, 1e-20):
+        x, wg, wu, dh = _gates(gates, [up] * len(gates), [1e-3] * len(gates))
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+        h = ops.gated_linear(*leaves)
+        dx = torch.autograd.grad(h, leaves[0], dh)[0]
+        g64, u64 = x.double()[:, :1], x.double()[:, 1:2]
+        s = torch.sigmoid(g64)
+        want = (g64 * s * u64).expand(-1, 8)
+        small = 2.0 ** -133                                      # half of bf16's smallest step
+        over = want.abs() > 3.39e38
+        assert bool(h.double()[over].isinf().all()) and bool((h.double()[over].sign() == want[over].sign()).all())
+        assert bool(((h.double() - want).abs() <= (ref.HALF + ref.GATE) * want.abs() + small)[~over].all()), up
+        du = (8 * dh.double()[:, :1] * g64 * s)[:, 0]            # the second column of dx: the sum of eight equal du
+        off = (dx.double()[:, 1] - du).abs()
+        assert bool((off <= 2.1 * (ref.HALF + ref.GATE) * du.abs() + 16 * small).all()), up
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_not_finite(cuda, bad):
+    """A row that holds an infinity or a NaN concerns itself alone in h and dx, and every weight's gradient that it touches."""
+    x, wg, wu, dh = _inputs(300, 64, 40)
+    whole = _all(x, wg, wu, dh)
+    y = x.clone()
+    y[131, 5] = bad
+    h, dx, dwg, _ = _all(y, wg, wu, dh)
+    others = torch.arange(300, device="cuda") != 131
+    assert torch.equal(h[others], whole[0][others]) and torch.equal(dx[others], whole[1][others])
+    assert not bool(h[131].isfinite().all()) and not bool(dwg[:, 5].isfinite().all())
+
+
+def test_second_derivative(cuda):
+    x, wg, wu, dh = _inputs(6, 16, 24)
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    dx = torch.autograd.grad(ops.gated_linear(*leaves), leaves[0], dh, create_graph=True)[0]
+    got = torch.autograd.grad(dx.float().square().sum(), leaves)
+    deep = [t.detach().double().requires_grad_() for t in leaves]
+    dx64 = torch.autograd.grad(ref.forward(*deep), deep[0], dh.double(), create_graph=True)[0]
+    want = torch.autograd.grad(dx64.square().sum(), deep)
+    for a, b in zip(got, want):     # a chain of some ten steps in bf16, relative to the largest
+        assert (a.double() - b).abs().max() <= 16 * ref.HALF * b.abs().max()
+
+
+def test_graph_capture_of_a_step(cuda):
+    """Forward and backward in one captured graph, replayed on new inputs."""
+    x, wg, wu, dh = _inputs(500, 264, 136)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, wg, wu)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    step = lambda: (lambda h: (h.detach(), *torch.autograd.grad(h, leaves, dh)))(ops.gated_linear(*leaves))
+    check, ops._attn._CHECK_STATUS = ops._attn._CHECK_STATUS, False
+    try:
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+    finally:
+        ops._attn._CHECK_STATUS = check
+    x2 = _inputs(500, 264, 136, seed=5)[0]
+    with torch.no_grad():
+        leaves[0].copy_(x2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, _all(x2, wg, wu, dh)))
+
+
+def test_streams_and_threads(cuda):
+    """Four threads on streams of their own, many calls each, with results that no other call changes."""
+    cases = [_inputs(200 + 100 * i, 256, 136, seed=i) for i in range(4)]
+    alone = [_all(*c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _all(*cases[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, alone[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_offsets_past_32_bits(cuda):
+    M, E, I = 420000, 16, 5632                                   # M I > 2^31 elements
+    x, wg, wu, _ = _inputs(64, E, I)
+    x = x.repeat(M // 64 + 1, 1)[:M].contiguous()
+    dh = torch.zeros(M, I, dtype=BF16, device="cuda")
+    dh[-64:] = 0.1
+    h, dx, dwg, dwu = _all(x, wg, wu, dh)
+    last = x[-64:].contiguous()
+    small = _all(last, wg, wu, dh[-64:].contiguous())
+    assert torch.equal(h[-64:], small[0]) and torch.equal(dx[-64:], small[1])
+    assert not bool(dx[:-64].any())
+    _check((h[-64:], dx[-64:], dwg, dwu), last, wg, wu, dh[-64:])
