@@ -340,6 +340,46 @@ int mvpa_matmul_fp8(const void* a, int64_t ld_a, const void* a_scales, int64_t a
                     int32_t scale_dtype, void* out, int64_t ld_out, int64_t M, int32_t N, int32_t K,
                     int32_t out_dtype, int32_t* status, void* cuda_stream);
 
+/* ---- weights in 4 bits --------------------------------------------------------------------------
+ * A weight (N, K) in 4 bits: q, two values a byte, the first one in its low half (base and rows, ld_q bytes, on 16-byte boundaries;
+ * nothing past (K + 1) / 2 bytes of a row is read or written); one scale for each group of 32, 64 or 128 neighbours in a row, the
+ * last group as long as the row leaves it, MVPA_F32 or MVPA_BF16, (N, ceil(K / group)) with leading dimension ld_s; and, or NULL,
+ * one zero for each group, a byte from 0 to 15.  It stands for (q - zero) * scale, with zero = 8 where there are none.
+ * These have no counterpart in the reference, whose block is bf16 throughout. */
+typedef struct mvpa_int4 {
+  const void* q;
+  const void* scales;
+  const void* zeros;
+  int64_t ld_q, ld_s, ld_z;
+} mvpa_int4;
+
+/*
+ * w (N, K), leading dimension ld_w, MVPA_F32 or MVPA_BF16, to 4 bits with scales of its type; into the memory that `to` names.
+ *   to->zeros NULL   scale = max|y| / 7 rounded to the type,  q = 8 + clamp(round(y / scale), -8, 7)
+ *   else             scale = (hi - lo) / 15 rounded to the type,  zero = clamp(round(-lo / scale), 0, 15),
+ *                    q = clamp(round(y / scale) + zero, 0, 15)  for lo = min(0, min y), hi = max(0, max y)
+ * Quotients are exact before they are rounded, halves to even.  A group whose scale rounds to zero stands for zeros, one that
+ * holds an infinity or a NaN has the scale NaN.  Zero rows or columns are no work and no error.
+ */
+int mvpa_quantize_int4(const void* w, int64_t ld_w, const mvpa_int4* to, int64_t N, int32_t K, int32_t group,
+                       int32_t dtype, void* cuda_stream);
+
+/* The values that a weight stands for, (N, K) in out_dtype with leading dimension ld_out: the product in fp32, rounded once. */
+int mvpa_dequantize_int4(const mvpa_int4* w, int32_t scale_dtype, void* out, int64_t ld_out, int64_t N, int32_t K,
+                         int32_t group, int32_t out_dtype, void* cuda_stream);
+
+/*
+ * out = x W^T, or with `up` (may be NULL) out = silu(x W^T) * (x Up^T); x (M, K) and out (M, N) MVPA_F32 or MVPA_BF16, both `dtype`,
+ * any alignment to their elements (16-byte aligned rows of x are read faster).  Whole numbers q - zero and x are multiplied exactly (an
+ * fp32 x in three parts) and added in fp32 over a group; the groups' sums are scaled and added in fp32, in an order that depends on the
+ * sizes alone, and rounded once.  K = 0 gives zeros.  `workspace`: 16-byte aligned, of at least
+ * mvpa_matmul_int4_workspace_bytes(...) bytes, which may be 0.  `status` (may be NULL): as for mvpa_matmul_fp8.
+ */
+size_t mvpa_matmul_int4_workspace_bytes(const void* x, int64_t ld_x, int64_t M, int32_t K, int32_t dtype);
+int mvpa_matmul_int4(const void* x, int64_t ld_x, const mvpa_int4* w, const mvpa_int4* up, int32_t scale_dtype, void* out,
+                     int64_t ld_out, int64_t M, int32_t N, int32_t K, int32_t group, int32_t dtype, void* workspace,
+                     size_t workspace_bytes, int32_t* status, void* cuda_stream);
+
 /* Text of the last error raised on this host thread ("" if none).
  * Stands where the reference raises RuntimeError / assert
  * (`attentions/attn.py:1034-1045, 1339, 1344`). */

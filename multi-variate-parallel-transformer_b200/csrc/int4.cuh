@@ -1,0 +1,51 @@
+// What the 4-bit kernels share.  A weight (N, K) in 4 bits: q, two values a byte, the first in its low half, rows of bytes on 16-byte
+// boundaries; a scale for each group of 32, 64 or 128 neighbours in a row (the last group as long as the row leaves it), fp32 or
+// bf16; and, or not, a zero for each group, a byte from 0 to 15.  It stands for (q - zero) * scale, zero = 8 where there are none.
+#pragma once
+#include "fp8.cuh"
+
+namespace mvpa {
+namespace {
+
+struct Int4Weight {
+  const uint8_t* q;
+  const void* scales;
+  const uint8_t* zeros;  // or NULL
+  int64_t ld_q, ld_s, ld_z;
+  int scale_f32;
+  __device__ __forceinline__ float scale(int64_t row, int group) const {
+    return scale_f32 ? static_cast<const float*>(scales)[row * ld_s + group]
+                     : __bfloat162float(static_cast<const __nv_bfloat16*>(scales)[row * ld_s + group]);
+  }
+  __device__ __forceinline__ uint32_t zero(int64_t row, int group) const { return zeros != nullptr ? zeros[row * ld_z + group] : 8u; }
+};
+
+// Eight values of a word as pairs of bf16, (0, 4), (1, 5), (2, 6), (3, 7): a nibble in the low bits of 128's mantissa is 128 + q, from
+// which 128 + zero (`minus`, twice) is taken.  Whole numbers from -15 to 15: exact.
+__device__ __forceinline__ uint32_t int4_minus(uint32_t zero) { return 0x43004300u | zero | zero << 16; }
+__device__ __forceinline__ void int4_pairs(uint32_t w, uint32_t minus, uint32_t (&p)[4]) {
+  const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&minus);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), m);
+    p[i] = *reinterpret_cast<const uint32_t*>(&d);
+  }
+}
+
+// An fp32 number as three bf16 whose sum it is, exactly (but for what lies below 2^-133): eight bits of the mantissa each, cut off.  An
+// infinity or a NaN is the first of them alone.
+struct Thirds {
+  uint32_t hi, mid, lo;  // bf16 in the upper half of a word
+  __device__ __forceinline__ explicit Thirds(float x) {
+    const uint32_t b = __float_as_uint(x);
+    const bool finite = (b & 0x7fffffffu) < 0x7f800000u;
+    hi = (b & 0xffff0000u) | ((b & 0x7fffffffu) > 0x7f800000u ? 0x00400000u : 0u);
+    const float r = finite ? x - __uint_as_float(hi) : 0.f;
+    mid = __float_as_uint(r) & 0xffff0000u;
+    lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
+  }
+};
+
+}  // namespace
+}  // namespace mvpa

@@ -15,6 +15,7 @@
 // dg and du are rounded to bf16 between the kernels: the products take 16-bit operands, and each of their sums is over hundreds of
 // terms, whose roundings (2^-9 each) leave the sum as exact as its own rounding to bf16 does.
 #include "block_rows.cuh"
+#include "silu.cuh"
 #include "tc_pairs.cuh"
 #include "tc_tma_host.cuh"
 
@@ -41,22 +42,6 @@ constexpr int kGatedOutBytes = 8 * 2 * 4096;  // a warp's 32 rows x 64 columns o
 constexpr size_t kGatedSmem = 1024 + kGatedStages * kGatedStageBytes + kGatedOutBytes;
 
 enum : int { kGiveUpEmpty = 81, kGiveUpFull = 82, kGiveUpTmemEmpty = 83, kGiveUpTmemFull = 84, kGiveUpDrain = 85 };
-
-// silu(g) u = g u / (1 + e^-g), for any g.  With a = e^(-|g| / 4) (which leaves the normal numbers below |g| = 349, where the product
-// with any u rounds to zero) the factor of a negative g is a^4 / (1 + a^4), taken into the product in four parts, so that nothing
-// underflows that the result does not.  Errors: an ulp or two of a, four times over, 2^-19 against the 2^-9 of the result's rounding.
-struct Sigmoid {
-  float part, r;  // e^(-|g| / 4) where g < 0, else 1;  1 / (1 + e^-|g|)
-  float other;    // 1 - s
-  __device__ __forceinline__ explicit Sigmoid(float g) {
-    const float a = ptx::ex2(fabsf(g) * (-0.25f * kLog2e)), a2 = a * a, e = a2 * a2;
-    r = __fdividef(1.f, 1.f + e);
-    part = g < 0.f ? a : 1.f;
-    other = g < 0.f ? r : e * r;
-  }
-  // a b s
-  __device__ __forceinline__ float times(float a, float b) const { return (a * part * part) * (b * part * part) * r; }
-};
 
 template <int MODE>
 __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs g) {

@@ -52,7 +52,7 @@ struct TensorMapSlot {
 constexpr int kTensorMapSlots = 64;
 
 inline int encode_sw128(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims,
-                        const uint64_t* strides_bytes, const uint32_t* box);
+                        const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 // bf16 tensor of `rank` dims (dims[0] innermost, contiguous), byte strides for dims 1..rank-1,
 // box of `box` elements, 128-byte swizzle, zero fill outside the tensor.
@@ -83,9 +83,9 @@ inline int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const
   return rc;
 }
 
-// The same for any element type, encoded anew.
+// The same for any element type (and, where one is named, another swizzle), encoded anew.
 inline int encode_sw128(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims,
-                        const uint64_t* strides_bytes, const uint32_t* box) {
+                        const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle) {
   // The driver call needs a current context, and a thread's first runtime call is what binds one: make that call here,
   // whatever the caller has done on this thread so far (autograd runs backwards on threads of its own).
   int device = 0;
@@ -106,7 +106,7 @@ inline int encode_sw128(CUtensorMap* map, CUtensorMapDataType type, const void* 
     if (i > 0) gstr[i - 1] = strides_bytes[i - 1];
   }
   CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr,
-                  bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d (rank %d, dims %llu %llu %llu, box %u %u %u)",

@@ -34,7 +34,7 @@ NVCC_FLAGS = [
 ]
 FAST_MATH = "--use_fast_math"        # everywhere but in the files below, whose results are not rounded to 16 bits afterwards
 PRECISE = ("mvpa_rows_f32.cu", "mvpa_fp8_rows.cu", "mvpa_fp8_matmul.cu",   # (8-bit: every value lies next to some rounding border)
-           "mvpa_gated.cu")
+           "mvpa_gated.cu", "mvpa_int4_rows.cu", "mvpa_int4_matmul.cu")
 
 MVPA_F32, MVPA_BF16, MVPA_F16, MVPA_E8M0 = 0, 1, 2, 3
 
@@ -140,13 +140,19 @@ class Tensor(ctypes.Structure):
                 ("stride_h", ctypes.c_int64), ("stride_n", ctypes.c_int64)]
 
 
+class Int4(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p), ("ld_q", ctypes.c_int64),
+                ("ld_s", ctypes.c_int64), ("ld_z", ctypes.c_int64)]
+
+
 EXPORTS = ("mvpa_fwd", "mvpa_bwd", "mvpa_fwd_workspace_bytes", "mvpa_bwd_workspace_bytes",
            "mvpa_last_error_string", "mvpa_launch_count", "mvpa_abi_version",
            "mvpa_workspace_status", "mvpa_fwd_noalloc", "mvpa_bwd_status", "mvpa_noalloc_status",
            "mvpa_selftest_wait_timeout", "mvpa_rmsnorm", "mvpa_silu_mul", "mvpa_wave_encode_size",
            "mvpa_wave_encode", "mvpa_channel_mean", "mvpa_contrastive_logits", "mvpa_peer_gather", "mvpa_peer_signal",
            "mvpa_peer_wait", "mvpa_rmsnorm_bwd", "mvpa_rmsnorm_bwd_workspace_bytes", "mvpa_silu_mul_bwd", "mvpa_quantize_fp8",
-           "mvpa_rmsnorm_fp8", "mvpa_silu_mul_fp8", "mvpa_matmul_fp8", "mvpa_gated_linear", "mvpa_gated_linear_bwd")
+           "mvpa_rmsnorm_fp8", "mvpa_silu_mul_fp8", "mvpa_matmul_fp8", "mvpa_gated_linear", "mvpa_gated_linear_bwd",
+           "mvpa_quantize_int4", "mvpa_dequantize_int4", "mvpa_matmul_int4_workspace_bytes", "mvpa_matmul_int4")
 ABI_VERSION = 3   # mvpa_abi_version() of the header this shim was written against
 
 
@@ -215,6 +221,15 @@ def lib() -> ctypes.CDLL:
         L.mvpa_gated_linear.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, i64, i32, i32, vp, vp]
         L.mvpa_gated_linear_bwd.restype = ctypes.c_int
         L.mvpa_gated_linear_bwd.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, vp]
+        I4 = ctypes.POINTER(Int4)
+        L.mvpa_quantize_int4.restype = ctypes.c_int
+        L.mvpa_quantize_int4.argtypes = [vp, i64, I4, i64, i32, i32, i32, vp]
+        L.mvpa_dequantize_int4.restype = ctypes.c_int
+        L.mvpa_dequantize_int4.argtypes = [I4, i32, vp, i64, i64, i32, i32, i32, vp]
+        L.mvpa_matmul_int4_workspace_bytes.restype = ctypes.c_size_t
+        L.mvpa_matmul_int4_workspace_bytes.argtypes = [vp, i64, i64, i32, i32]
+        L.mvpa_matmul_int4.restype = ctypes.c_int
+        L.mvpa_matmul_int4.argtypes = [vp, i64, I4, I4, i32, vp, i64, i64, i32, i32, i32, i32, vp, ctypes.c_size_t, vp, vp]
         L.mvpa_wave_encode_size.restype = i32
         L.mvpa_wave_encode_size.argtypes = [i32, ctypes.POINTER(i32), i32]
         L.mvpa_wave_encode.restype = ctypes.c_int

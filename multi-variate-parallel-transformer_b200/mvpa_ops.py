@@ -497,3 +497,115 @@ def matmul_fp8(a, a_scales, b, b_scales, out=None, dtype=torch.bfloat16):
         if status is not None:  # debugging aid: synchronises the stream
             _nat.check(_nat.lib().mvpa_workspace_status(status.data_ptr(), 256, _stream(a)), "mvpa_matmul_fp8 kernel")
     return out
+
+
+# ---- weights in 4 bits ----
+# A weight (N, K) in 4 bits is (q, scales) or (q, scales, zeros): q (N, ceil(K / 2)) uint8, two values a byte, the first in its low
+# half, whose rows start on 16-byte boundaries; scales (N, ceil(K / group)), one for each group of 32, 64 or 128 neighbours in a row;
+# zeros, uint8 from 0 to 15, one for each scale.  It stands for (q - zero) * scale, zero = 8 where there are none.
+
+INT4_GROUPS = (32, 64, 128)
+
+
+def _int4_weight(what, q, scales, zeros, N, K, group):
+    """The weight for the C entry points; N and K from its shape where they are None."""
+    if group not in INT4_GROUPS:
+        raise RuntimeError(f"{what}: group is 32, 64 or 128, got {group}")
+    if q.dtype != torch.uint8 or scales.dtype not in (torch.bfloat16, torch.float32) or (zeros is not None and zeros.dtype != torch.uint8):
+        raise RuntimeError(f"{what}: q and zeros are uint8, scales bfloat16 or float32, got {q.dtype}, {scales.dtype}"
+                           + ("" if zeros is None else f", {zeros.dtype}"))
+    ld_q, ld_s = _fp8_rows(what, q, "q"), _fp8_rows(what, scales, "scales")
+    ld_z = 0 if zeros is None else _fp8_rows(what, zeros, "zeros")
+    groups = -(-K // group)
+    if q.shape != (N, (K + 1) // 2) or scales.shape != (N, groups) or (zeros is not None and zeros.shape != (N, groups)):
+        raise RuntimeError(f"{what}: shapes do not go together: q {tuple(q.shape)}, scales {tuple(scales.shape)}"
+                           + ("" if zeros is None else f", zeros {tuple(zeros.shape)}") + f" for {N} rows of {K} in groups of {group}")
+    return _nat.Int4(q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), ld_q, ld_s, ld_z)
+
+
+def quantize_int4(w, group=128, zeros=False):
+    """A weight w (N, K), bf16 or fp32, in 4 bits: (q, scales), or with `zeros` (q, scales, zeros); scales in w's type.  Without zeros
+    scale = max|w| / 7 over a group, values -8 to 7; with them scale = (hi - lo) / 15 for lo = min(0, min w) and hi = max(0, max w), and
+    the zero is -lo / scale, rounded.  Quotients are exact before they are rounded, halves to even.  A group whose scale rounds to zero
+    stands for zeros, one that holds an infinity or a NaN has the scale NaN."""
+    what = "quantize_int4"
+    _fp8_inputs(what, w)
+    if group not in INT4_GROUPS:
+        raise RuntimeError(f"{what}: group is 32, 64 or 128, got {group}")
+    ld, (N, K) = _fp8_rows(what, w, "w"), w.shape
+    half, groups = (K + 1) // 2, -(-K // group)
+    q = torch.empty((N, (half + 15) // 16 * 16), dtype=torch.uint8, device=w.device)[:, :half]
+    scales = torch.empty((N, groups), dtype=w.dtype, device=w.device)
+    z = torch.empty((N, groups), dtype=torch.uint8, device=w.device) if zeros else None
+    code = _code(w)
+    with _nat.on_device(w.device):
+        st = _nat.lib().mvpa_quantize_int4(w.data_ptr(), ld, ctypes.byref(_int4_weight(what, q, scales, z, N, K, group)), N, K, group, code,
+                                           _stream(w))
+    _nat.check(st, "mvpa_quantize_int4")
+    return (q, scales, z) if zeros else (q, scales)
+
+
+def dequantize_int4(q, scales, zeros=None, width=None, group=128, dtype=None):
+    """The values (N, width) that a weight in 4 bits stands for, in `dtype` (the scales' type unless given).  `width` is K, which for an
+    odd K the shape of q does not tell; 2 * q.shape[1] unless given."""
+    what = "dequantize_int4"
+    _fp8_inputs(what, q, scales, *(() if zeros is None else (zeros,)))
+    if q.dim() != 2:
+        raise RuntimeError(f"{what}: q must be a matrix, got shape {tuple(q.shape)}")
+    N, K = q.shape[0], 2 * q.shape[1] if width is None else int(width)
+    weight = _int4_weight(what, q, scales, zeros, N, K, group)
+    out = torch.empty((N, K), dtype=scales.dtype if dtype is None else dtype, device=q.device)
+    code = _code(out)
+    with _nat.on_device(q.device):
+        st = _nat.lib().mvpa_dequantize_int4(ctypes.byref(weight), _code(scales), out.data_ptr(), K, N, K, group, code, _stream(q))
+    _nat.check(st, "mvpa_dequantize_int4")
+    return out
+
+
+def _int4_product(what, x, weight, up, group, out):
+    tensors = [t for t in (*weight, *(() if up is None else up)) if t is not None]
+    _fp8_inputs(what, x, *tensors, *(() if out is None else (out,)))
+    if x.dim() == 0:
+        raise RuntimeError(f"{what}: x must have a last dimension")
+    K, N = x.shape[-1], weight[0].shape[0] if weight[0].dim() else 0
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if x2.dim() == 2 and x2.stride(1) != 1 and K > 1:
+        x2 = x2.contiguous()
+    first = _int4_weight(what, *weight, *(() if len(weight) == 3 else (None,)), N, K, group)
+    second = None if up is None else _int4_weight(what, *up, *(() if len(up) == 3 else (None,)), N, K, group)
+    if up is not None and up[1].dtype != weight[1].dtype:
+        raise RuntimeError(f"{what}: the scales of both weights are of one type, got {weight[1].dtype} and {up[1].dtype}")
+    code, ld_x, M = _code(x), _fp8_rows(what, x2, "x"), x2.shape[0]
+    made = out is None
+    if made:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    elif out.shape != (M, N) or out.dtype != x.dtype:
+        raise RuntimeError(f"{what}: out must be {(M, N)} {x.dtype}, got {tuple(out.shape)} {out.dtype}")
+    ld_out = _fp8_rows(what, out, "out")
+    lib = _nat.lib()
+    with _nat.on_device(x.device):
+        nbytes = lib.mvpa_matmul_int4_workspace_bytes(x2.data_ptr(), ld_x, M, K, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        status = _status_word(x.device)
+        st = lib.mvpa_matmul_int4(x2.data_ptr(), ld_x, ctypes.byref(first), None if second is None else ctypes.byref(second),
+                                  _code(weight[1]), out.data_ptr(), ld_out, M, N, K, group, code, None if ws is None else ws.data_ptr(),
+                                  nbytes, None if status is None else status.data_ptr(), _stream(x))
+        _nat.check(st, "mvpa_matmul_int4")
+        _look_at(status, "mvpa_matmul_int4", x)
+    return out.view(*x.shape[:-1], N) if made and x.dim() != 2 else out
+
+
+def matmul_int4(x, q, scales, zeros=None, group=128, out=None):
+    """x @ W.T for a weight W (N, K) in 4 bits and x (..., K), bf16 or fp32; the result in x's type, or in `out` (rows, N), which may be a
+    column block of a wider buffer.  No weight is rounded: whole numbers are multiplied and added in fp32 over a group, the groups' sums
+    scaled and added in fp32, rounded once."""
+    return _int4_product("matmul_int4", x, (q, scales, zeros), None, group, out)
+
+
+def gated_linear_int4(x, gate, up, group=128, out=None):
+    """silu(x @ G.T) * (x @ U.T) for weights G and U (N, K) in 4 bits, `gate` and `up` each (q, scales) or (q, scales, zeros): `gated_linear`
+    for inference, in one kernel, from x to the result in fp32 and rounded once."""
+    what = "gated_linear_int4"
+    if len(gate) not in (2, 3) or len(up) not in (2, 3):
+        raise RuntimeError(f"{what}: gate and up are (q, scales) or (q, scales, zeros)")
+    return _int4_product(what, x, tuple(gate), tuple(up), group, out)
