@@ -280,11 +280,12 @@ int mvpa_contrastive_logits(const void* pred, const void* enc, const int32_t* ne
 /*
  * The gated projection of the MLP, bf16: h = silu(x Wg^T) * (x Wu^T), x (M, E) with leading dimension ld_x, w_gate and w_up (I, E)
  * contiguous, h (M, I) with leading dimension ld_h; what `LlamaMLP` does before its down projection (`models/mvpformer.py:114,146`)
- * in one kernel.  Both products and the activation are in fp32, rounded once.  `gate` and `up` ((M, I) contiguous, or both NULL)
- * receive the two products, rounded to bf16, for the backward pass.  E and I are multiples of 8; bases and rows lie on 16-byte
- * boundaries.  `status` (may be NULL): as for mvpa_matmul_fp8.
+ * in one kernel.  Both products and the activation are in fp32, rounded once.  `saved` (16-byte aligned, of
+ * mvpa_gated_linear_saved_bytes(M, I) bytes, or NULL) receives 24 bits of each product for the backward pass.  E and I are multiples of
+ * 8; bases and rows lie on 16-byte boundaries.  `status` (may be NULL): as for mvpa_matmul_fp8.
  */
-int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const void* w_up, void* h, int64_t ld_h, void* gate, void* up,
+size_t mvpa_gated_linear_saved_bytes(int64_t M, int32_t I);
+int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const void* w_up, void* h, int64_t ld_h, void* saved,
                       int64_t M, int32_t E, int32_t I, int32_t* status, void* cuda_stream);
 
 /*
@@ -292,7 +293,7 @@ int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const voi
  * dw_gate = dg^T x and dw_up = du^T x (I, E) unless they are NULL; all contiguous, sums in fp32, in an order that depends on the sizes
  * alone, rounded once.  `dgate` and `dup` ((M, I), contiguous) receive dg and du in bf16, the operands of those products.
  */
-int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* gate, const void* up, const void* x, int64_t ld_x, const void* w_gate,
+int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* saved, const void* x, int64_t ld_x, const void* w_gate,
                           const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up, int64_t M, int32_t E, int32_t I,
                           int32_t* status, void* cuda_stream);
 

@@ -8,7 +8,9 @@
 // blocks of 64 along the summed axis that the TMA stages in shared memory.
 //   forward        the first CTA brings 128 rows of Wg and the second the same rows of Wu, so that a thread that holds a token's row of
 //                  sums finds g and u of one feature 128 columns apart: h leaves from fp32 in one rounding, and g and u go to memory
-//                  (rounded to bf16) only where a backward pass will want them.
+//                  only where a backward pass will want them: 24 bits of each, the upper half of the fp32 number and the byte after it,
+//                  in matrices of their own.  (In bf16 their roundings are half of the gradients' error: 0.0031 of the gradients' size
+//                  against 0.0024, of which 0.0017 is the results' own rounding.)
 //   input          dg and du are the left operand one after the other, Wg and Wu, whose rows lie along the columns of the result
 //                  (MN-major), the right one: the sum of both products is formed in TMEM.
 //   weights        both operands have the summed axis, the tokens, outermost (MN-major).
@@ -25,7 +27,7 @@ namespace {
 enum : int { kForward = 0, kForwardSave = 1, kInput = 2, kWeights = 3 };
 
 struct GatedMaps {
-  CUtensorMap a[2], b[2], out[3];
+  CUtensorMap a[2], b[2], out[5];
 };
 struct GatedArgs {
   uint32_t tiles_m, tiles_n;
@@ -207,17 +209,37 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
         const int x = at.n0 + group * 64;
         const bool inside = y < g.rows && x < g.cols;  // (the same for the whole warp: a store does not begin past the matrix)
         if constexpr (MODE == kForwardSave) {
-          for (int which_sum = 0; which_sum < 2; ++which_sum) {
-            const uint32_t to = place();
+#pragma unroll 1
+          for (int sum = 0; sum < 2; ++sum) {  // g, then u: the numbers' upper halves, and the byte after
+            if (lane == 0) ptx::tma_store_wait_read<0>();  // (both places at once)
+            __syncwarp();
+            const uint32_t upper = outs + (which ^ 1) * 4096, lower = outs + which * 4096;
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
               uint32_t r[32];
-              ptx::tmem_ld32(from + which_sum * 128 + group * 64 + c, r);
+              ptx::tmem_ld32(from + sum * 128 + group * 64 + c, r);
               ptx::tmem_ld_wait();
-              words(r, to, c / 8);
+              uint32_t b[8];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] |= poison;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const auto two = [&](int i) { return __byte_perm(r[k * 8 + 2 * i], r[k * 8 + 2 * i + 1], 0x7632); };
+                put(upper, c / 8 + k, two(0), two(1), two(2), two(3));
+              }
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                b[k] = __byte_perm(__byte_perm(r[4 * k], r[4 * k + 1], 0x0051), __byte_perm(r[4 * k + 2], r[4 * k + 3], 0x0051), 0x5410);
+#pragma unroll
+              for (int k = 0; k < 2; ++k)  // (rows of 64 bytes, in the 64-byte swizzle)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(lower + lane * 64 + (((c / 16 + k) ^ ((lane >> 1) & 3)) << 4)),
+                             "r"(b[4 * k]), "r"(b[4 * k + 1]), "r"(b[4 * k + 2]), "r"(b[4 * k + 3])
+                             : "memory");
             }
-            if (inside) send(to, &maps.out[1 + which_sum], x, y);
-            else if (lane == 0) ptx::tma_store_commit();  // (each use of a place is a group)
+            if (inside) {
+              send(upper, &maps.out[1 + sum], x, y);
+              send(lower, &maps.out[3 + sum], x, y);
+            }  // (the next use of a place is of the upper one, whose group is not the newest)
           }
         }
         const uint32_t to = place();
@@ -264,10 +286,37 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
   if (warp == 1) ptx::tmem_dealloc_pair(tmem, 512);
 }
 
-// dg and du from dh and the forward's g and u, in fp32, rounded once.  Bound by memory: 10 bytes an element.
-__global__ void __launch_bounds__(256) gate_bwd_kernel(const __nv_bfloat16* __restrict__ dh, int64_t ld_dh, const __nv_bfloat16* __restrict__ gate,
-                                                       const __nv_bfloat16* __restrict__ up, __nv_bfloat16* __restrict__ dgate,
-                                                       __nv_bfloat16* __restrict__ dup, int64_t rows, int width) {
+// What the forward keeps, in one piece of memory: the upper halves of g and of u, (M, I) each, then the bytes after, with rows on 16-byte
+// boundaries.
+struct Saved {
+  uint8_t *upper[2], *lower[2];
+  int64_t ld;  // of the bytes
+  Saved(void* p, int64_t M, int64_t I) : ld((I + 15) / 16 * 16) {
+    uint8_t* at = static_cast<uint8_t*>(p);
+    for (int i = 0; i < 2; ++i) {
+      upper[i] = at + i * M * I * 2;
+      lower[i] = at + 2 * M * I * 2 + i * M * ld;
+    }
+  }
+  static size_t bytes(int64_t M, int64_t I) { return (size_t)M * ((size_t)I * 4 + (size_t)(I + 15) / 16 * 16 * 2); }
+};
+
+// Eight numbers of 24 bits.
+__device__ __forceinline__ void load24(const uint8_t* upper, const uint8_t* lower, float (&f)[8]) {
+  const uint4 h = *reinterpret_cast<const uint4*>(upper);
+  const uint2 l = *reinterpret_cast<const uint2*>(lower);
+  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = i < 2 ? l.x : l.y;
+    f[2 * i] = __uint_as_float(__byte_perm(w[i], b, i & 1 ? 0x1060 : 0x1040) & 0xffffff00u);
+    f[2 * i + 1] = __uint_as_float(__byte_perm(w[i], b, i & 1 ? 0x3270 : 0x3250) & 0xffffff00u);
+  }
+}
+
+// dg and du from dh and the forward's g and u, in fp32, rounded once.  Bound by memory: 12 bytes an element.
+__global__ void __launch_bounds__(256) gate_bwd_kernel(const __nv_bfloat16* __restrict__ dh, int64_t ld_dh, const Saved kept,
+                                                       __nv_bfloat16* __restrict__ dgate, __nv_bfloat16* __restrict__ dup, int64_t rows, int width) {
   using V = Vec<__nv_bfloat16>;
   ptx::griddep_launch();
   ptx::griddep_wait();
@@ -276,8 +325,8 @@ __global__ void __launch_bounds__(256) gate_bwd_kernel(const __nv_bfloat16* __re
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / per_row, c = (i - row * per_row) * V::N;
     float x[V::N], u[V::N], d[V::N];
-    V::load(gate + i * V::N, x);
-    V::load(up + i * V::N, u);
+    load24(kept.upper[0] + i * 16, kept.lower[0] + row * kept.ld + c, x);
+    load24(kept.upper[1] + i * 16, kept.lower[1] + row * kept.ld + c, u);
     V::load(dh + row * ld_dh + c, d);
 #pragma unroll
     for (int e = 0; e < V::N; ++e) {
@@ -332,14 +381,16 @@ bool rows_fit(const void* p, int64_t ld, int64_t width) {
 
 using namespace mvpa;
 
-extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const void* w_up, void* h, int64_t ld_h, void* gate, void* up,
+extern "C" size_t mvpa_gated_linear_saved_bytes(int64_t M, int32_t I) { return M < 1 || I < 1 ? 0 : Saved::bytes(M, I); }
+
+extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const void* w_up, void* h, int64_t ld_h, void* saved,
                                  int64_t M, int32_t E, int32_t I, int32_t* status, void* cuda_stream) {
   const int rc0 = check_sizes("mvpa_gated_linear", M, E, I);
   if (rc0 != MVPA_OK) return rc0;
   if (!rows_fit(x, ld_x, E) || !rows_fit(w_gate, E, E) || !rows_fit(w_up, E, E) || !rows_fit(h, ld_h, I) ||
-      (gate == nullptr) != (up == nullptr) || (gate != nullptr && (!rows_fit(gate, I, I) || !rows_fit(up, I, I)))) {
-    set_error("mvpa_gated_linear: x, the weights, h, gate and up must be 16-byte aligned with rows of a multiple of 16 bytes, not shorter than "
-              "their widths; gate and up are given both or neither");
+      (reinterpret_cast<uintptr_t>(saved) & 15) != 0) {
+    set_error("mvpa_gated_linear: x, the weights, h and saved must be 16-byte aligned with rows of a multiple of 16 bytes, not shorter than "
+              "their widths");
     return MVPA_ERR_ALIGNMENT;
   }
   GatedMaps maps = {};
@@ -347,32 +398,40 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
   if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, 128);
   if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 128);
   if (rc == MVPA_OK) rc = encode(&maps.out[0], h, M, I, ld_h, 32);
-  if (rc == MVPA_OK && gate != nullptr) rc = encode(&maps.out[1], gate, M, I, I, 32);
-  if (rc == MVPA_OK && gate != nullptr) rc = encode(&maps.out[2], up, M, I, I, 32);
+  if (saved != nullptr) {
+    const Saved kept(saved, M, I);
+    for (int i = 0; i < 2 && rc == MVPA_OK; ++i) {
+      rc = encode(&maps.out[1 + i], kept.upper[i], M, I, I, 32);
+      const uint64_t dims[2] = {(uint64_t)I, (uint64_t)M}, strides[1] = {(uint64_t)kept.ld};
+      const uint32_t box[2] = {64, 32};
+      if (rc == MVPA_OK)
+        rc = encode_sw128(&maps.out[3 + i], CU_TENSOR_MAP_DATA_TYPE_UINT8, kept.lower[i], 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    }
+  }
   if (rc != MVPA_OK) return rc;
   const uint32_t tm = tiles_of(M, 256);
   const GatedArgs g = {tm, tiles_of(I, 128), tm, (int)tiles_of(E, 64), 1, (int)M, I, status};
   cudaStream_t s = (cudaStream_t)cuda_stream;
-  return gate != nullptr ? run_gated<kForwardSave>(maps, g, s) : run_gated<kForward>(maps, g, s);
+  return saved != nullptr ? run_gated<kForwardSave>(maps, g, s) : run_gated<kForward>(maps, g, s);
 }
 
-extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* gate, const void* up, const void* x, int64_t ld_x,
-                                     const void* w_gate, const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up,
-                                     int64_t M, int32_t E, int32_t I, int32_t* status, void* cuda_stream) {
+extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* saved, const void* x, int64_t ld_x, const void* w_gate,
+                                     const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up, int64_t M, int32_t E,
+                                     int32_t I, int32_t* status, void* cuda_stream) {
   const int rc0 = check_sizes("mvpa_gated_linear_bwd", M, E, I);
   if (rc0 != MVPA_OK) return rc0;
-  if (!rows_fit(dh, ld_dh, I) || !rows_fit(gate, I, I) || !rows_fit(up, I, I) || !rows_fit(dgate, I, I) || !rows_fit(dup, I, I) ||
-      (dx != nullptr && (!rows_fit(w_gate, E, E) || !rows_fit(w_up, E, E) || !rows_fit(dx, E, E))) || (dw_gate == nullptr) != (dw_up == nullptr) ||
+  if (!rows_fit(dh, ld_dh, I) || saved == nullptr || (reinterpret_cast<uintptr_t>(saved) & 15) != 0 || !rows_fit(dgate, I, I) ||
+      !rows_fit(dup, I, I) || (dx != nullptr && (!rows_fit(w_gate, E, E) || !rows_fit(w_up, E, E) || !rows_fit(dx, E, E))) ||
+      (dw_gate == nullptr) != (dw_up == nullptr) ||
       (dw_gate != nullptr && (!rows_fit(x, ld_x, E) || !rows_fit(dw_gate, E, E) || !rows_fit(dw_up, E, E)))) {
     set_error("mvpa_gated_linear_bwd: every matrix must be 16-byte aligned with rows of a multiple of 16 bytes, not shorter than its width; "
               "dw_gate and dw_up are wanted both or neither");
     return MVPA_ERR_ALIGNMENT;
   }
   cudaStream_t s = (cudaStream_t)cuda_stream;
-  using B = const __nv_bfloat16*;
   const int64_t ctas = (M * (I / 8) + 255) / 256, most = (int64_t)device_sm_count() * 16;
-  MVPA_CUDA_CHECK(launch_dependent(1, gate_bwd_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, s, (B)dh, ld_dh, (B)gate, (B)up,
-                                   (__nv_bfloat16*)dgate, (__nv_bfloat16*)dup, M, (int)I));
+  MVPA_CUDA_CHECK(launch_dependent(1, gate_bwd_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, s, (const __nv_bfloat16*)dh, ld_dh,
+                                   Saved(const_cast<void*>(saved), M, I), (__nv_bfloat16*)dgate, (__nv_bfloat16*)dup, M, (int)I));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   int rc = MVPA_OK;

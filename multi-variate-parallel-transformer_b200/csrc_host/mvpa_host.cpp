@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -48,6 +49,13 @@ struct Api {
   decltype(&mvpa_rmsnorm_fp8) rmsnorm_fp8;
   decltype(&mvpa_silu_mul_fp8) silu_mul_fp8;
   decltype(&mvpa_matmul_fp8) matmul_fp8;
+  decltype(&mvpa_gated_linear) gated_linear;
+  decltype(&mvpa_gated_linear_bwd) gated_linear_bwd;
+  decltype(&mvpa_gated_linear_saved_bytes) gated_saved_bytes;
+  decltype(&mvpa_quantize_int4) quantize_int4;
+  decltype(&mvpa_dequantize_int4) dequantize_int4;
+  decltype(&mvpa_matmul_int4) matmul_int4;
+  decltype(&mvpa_matmul_int4_workspace_bytes) int4_workspace_bytes;
 } api;
 
 PyObject* device_mode = nullptr;  // torch.utils._device.DeviceContext
@@ -752,6 +760,249 @@ PyObject* branches_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the gated projection (`mvpa_ops.gated_linear`) ----
+
+// x (..., E), w_gate and w_up (I, E) as the kernels read them: bf16, contiguous, 16-byte aligned, E and I multiples of 8, not empty.
+struct Gated {
+  Tensor x, wg, wu;
+  int64_t rows, E, I;
+  bool take(PyObject* const* a) {
+    for (int i = 0; i < 3; ++i)
+      if (!THPVariable_CheckExact(a[i])) return false;
+    x = THPVariable_Unpack(a[0]);
+    wg = THPVariable_Unpack(a[1]);
+    wu = THPVariable_Unpack(a[2]);
+    if (!ordinary(x) || x.scalar_type() != at::kBFloat16 || x.dim() < 2 || x.numel() == 0 || !ordinary(wg) || wg.dim() != 2 || function_modes() ||
+        watched())
+      return false;
+    E = x.size(-1);
+    I = wg.size(0);
+    rows = x.numel() / E;
+    return E % 8 == 0 && I % 8 == 0 && I > 0 && E <= INT32_MAX && I <= INT32_MAX && fits(x, x, at::kBFloat16, x.sizes()) &&
+           fits(wg, x, at::kBFloat16, {I, E}) && fits(wu, x, at::kBFloat16, {I, E});
+  }
+  Tensor like_x(int64_t width) const {  // (..., width)
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = width;
+    return at::empty(sizes, x.options().requires_grad(false));
+  }
+  Tensor word(bool status) const { return status ? at::zeros({64}, x.options().dtype(at::kInt).requires_grad(false)) : Tensor(); }
+  void look_at(const Tensor& w, const char* what) const {  // synchronises the stream
+    if (w.defined()) check(api.fwd_status(w.data_ptr(), 256, stream_of(x)), what);
+  }
+  Tensor forward(Tensor* saved, bool status) const {
+    Tensor h = like_x(I);
+    if (saved) *saved = scratch(api.gated_saved_bytes(rows, (int32_t)I), x);
+    const Tensor w = word(status);
+    check(api.gated_linear(x.const_data_ptr(), E, wg.const_data_ptr(), wu.const_data_ptr(), h.data_ptr(), I, saved ? saved->data_ptr() : nullptr,
+                           rows, (int32_t)E, (int32_t)I, w.defined() ? w.data_ptr<int32_t>() : nullptr, stream_of(x)), "mvpa_gated_linear");
+    look_at(w, "mvpa_gated_linear kernel");
+    return h;
+  }
+};
+
+// gated_linear(x, w_gate, w_up, status): a call that no gradient flows through -> h or None
+PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 4)) return nullptr;
+  Gated g;
+  if (!g.take(a) || at::autocast::is_autocast_enabled(at::kCUDA) ||
+      (c10::GradMode::is_enabled() && (g.x.requires_grad() || g.wg.requires_grad() || g.wu.requires_grad())))
+    Py_RETURN_NONE;
+  Tensor h;
+  {
+    const Body body(g.x);
+    h = g.forward(nullptr, a[3] == Py_True);
+  }
+  return THPVariable_Wrap(std::move(h));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_forward(x, w_gate, w_up, save, status) -> (h, saved or None) or None
+PyObject* gated_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 5)) return nullptr;
+  Gated g;
+  if (!g.take(a)) Py_RETURN_NONE;
+  Tensor h, saved;
+  {
+    const Body body(g.x);
+    h = g.forward(a[3] == Py_True ? &saved : nullptr, a[4] == Py_True);
+  }
+  return wrap({std::move(h), std::move(saved)});
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_backward(dh, x, w_gate, w_up, saved, need, status) -> the three gradients (None where the bit of `need` is clear), or None
+PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 7)) return nullptr;
+  Gated g;
+  if (!THPVariable_CheckExact(a[0]) || !THPVariable_CheckExact(a[4]) || !g.take(a + 1)) Py_RETURN_NONE;
+  const Tensor &dh = THPVariable_Unpack(a[0]), &saved = THPVariable_Unpack(a[4]);
+  std::vector<int64_t> sizes = g.x.sizes().vec();
+  sizes.back() = g.I;
+  if (!ordinary(dh) || dh.scalar_type() != at::kBFloat16 || dh.device() != g.x.device() || dh.sizes() != at::IntArrayRef(sizes) ||
+      !fits(saved, g.x, at::kByte, {(int64_t)api.gated_saved_bytes(g.rows, (int32_t)g.I)}))
+    Py_RETURN_NONE;
+  const int64_t need = PyLong_AsLongLong(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  std::vector<Tensor> grad(3);
+  {
+    const Body body(g.x);
+    const Tensor d = dh.is_contiguous() && aligned16(dh.const_data_ptr()) ? dh : dh.clone(at::MemoryFormat::Contiguous);
+    const Tensor dg = at::empty({2, g.rows, g.I}, g.x.options().requires_grad(false)), w = g.word(a[6] == Py_True);
+    if (need & 1) grad[0] = g.like_x(g.E);
+    Tensor dwg, dwu;
+    if (need & 6) {
+      dwg = at::empty_like(g.wg);
+      dwu = at::empty_like(g.wu);
+    }
+    const auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(api.gated_linear_bwd(d.const_data_ptr(), g.I, saved.const_data_ptr(), g.x.const_data_ptr(), g.E, g.wg.const_data_ptr(),
+                               g.wu.const_data_ptr(), dg.data_ptr(), const_cast<char*>(part(dg, g.rows * g.I)), ptr(grad[0]), ptr(dwg), ptr(dwu),
+                               g.rows, (int32_t)g.E, (int32_t)g.I, w.defined() ? w.data_ptr<int32_t>() : nullptr, stream_of(g.x)),
+          "mvpa_gated_linear_bwd");
+    g.look_at(w, "mvpa_gated_linear_bwd kernel");
+    if (need & 2) grad[1] = std::move(dwg);
+    if (need & 4) grad[2] = std::move(dwu);
+  }
+  return wrap(std::move(grad));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- weights in 4 bits (`mvpa_ops.quantize_int4` and its neighbours): as for 8 bits ----
+
+// (q, scales, zeros or None) of N rows of K values.
+struct Int4 {
+  Tensor q, scales, zeros;
+  mvpa_int4 c = {};
+  bool take(PyObject* const* a) { return a[0] != Py_None && a[1] != Py_None && take_(a[0], q) && take_(a[1], scales) && take_(a[2], zeros); }
+  bool fits(int64_t N, int64_t K, int64_t group) {
+    const int64_t groups = (K + group - 1) / group;
+    if (q.scalar_type() != at::kByte || !bf16_or_fp32(scales) || q.sizes() != at::IntArrayRef({N, (K + 1) / 2}) ||
+        scales.sizes() != at::IntArrayRef({N, groups}))
+      return false;
+    c.ld_q = matrix_ld(q);
+    c.ld_s = matrix_ld(scales);
+    if (zeros.defined()) {
+      if (zeros.scalar_type() != at::kByte || zeros.sizes() != at::IntArrayRef({N, groups})) return false;
+      c.ld_z = matrix_ld(zeros);
+      if (c.ld_z == 0) return false;
+    }
+    c.q = q.const_data_ptr();
+    c.scales = scales.const_data_ptr();
+    c.zeros = zeros.defined() ? zeros.const_data_ptr() : nullptr;
+    return c.ld_q != 0 && c.ld_s != 0;
+  }
+
+ private:
+  static bool take_(PyObject* a, Tensor& t) {  // (None leaves the tensor undefined)
+    if (a == Py_None) return true;
+    if (!THPVariable_CheckExact(a)) return false;
+    t = THPVariable_Unpack(a);
+    return true;
+  }
+};
+bool group_of(PyObject* a, int64_t* group) {
+  if (!PyLong_CheckExact(a)) return false;
+  int overflow = 0;
+  *group = PyLong_AsLongLongAndOverflow(a, &overflow);
+  return *group == 32 || *group == 64 || *group == 128;
+}
+
+// quantize_int4(w, group, zeros) -> (q, scales[, zeros]) or None
+PyObject* quantize_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 3)) return nullptr;
+  Tensor w;
+  int64_t group;
+  if (a[0] == Py_None || !take(a[0], w) || !group_of(a[1], &group) || (a[2] != Py_True && a[2] != Py_False) || !fp8_inputs({&w}) ||
+      !bf16_or_fp32(w))
+    Py_RETURN_NONE;
+  const int64_t ld = matrix_ld(w);
+  if (ld == 0 || w.size(1) > INT32_MAX - 1024) Py_RETURN_NONE;
+  const int64_t N = w.size(0), K = w.size(1), groups = (K + group - 1) / group, half = (K + 1) / 2, ld_q = (half + 15) / 16 * 16;
+  Tensor q, scales, zeros;
+  {
+    const Body body(w);
+    q = fresh({N, half}, {ld_q, 1}, at::kByte, w);
+    scales = fresh({N, groups}, {groups, 1}, w.scalar_type(), w);
+    if (a[2] == Py_True) zeros = fresh({N, groups}, {groups, 1}, at::kByte, w);
+    const mvpa_int4 to = {q.data_ptr(), scales.data_ptr(), zeros.defined() ? zeros.data_ptr() : nullptr, ld_q, groups, groups};
+    check(api.quantize_int4(w.const_data_ptr(), ld, &to, N, (int32_t)K, (int32_t)group, dtype_code(w), stream_of(w)), "mvpa_quantize_int4");
+  }
+  if (zeros.defined()) return wrap({std::move(q), std::move(scales), std::move(zeros)});
+  return wrap({std::move(q), std::move(scales)});
+  END_HANDLE_TH_ERRORS
+}
+
+// dequantize_int4(q, scales, zeros or None, width, group, out is fp32) -> the values or None
+PyObject* dequantize_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 6)) return nullptr;
+  Int4 w;
+  int64_t group;
+  if (!w.take(a) || !PyLong_CheckExact(a[3]) || !group_of(a[4], &group) || !fp8_inputs({&w.q, &w.scales, &w.zeros})) Py_RETURN_NONE;
+  int overflow = 0;
+  const int64_t K = PyLong_AsLongLongAndOverflow(a[3], &overflow);
+  if (overflow || K <= 0 || K > INT32_MAX - 1024 || w.q.dim() != 2 || !w.fits(w.q.size(0), K, group)) Py_RETURN_NONE;
+  Tensor out;
+  {
+    const Body body(w.q);
+    out = fresh({w.q.size(0), K}, {K, 1}, a[5] == Py_True ? at::kFloat : at::kBFloat16, w.q);
+    check(api.dequantize_int4(&w.c, dtype_code(w.scales), out.data_ptr(), K, w.q.size(0), (int32_t)K, (int32_t)group, dtype_code(out),
+                              stream_of(w.q)), "mvpa_dequantize_int4");
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// matmul_int4(x, q, scales, zeros or None, and the same three of the second weight of a gate, or None three times, group, out or None,
+//   status) -> out or None
+PyObject* matmul_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 10)) return nullptr;
+  const bool status = a[9] == Py_True, two = a[4] != Py_None;
+  Tensor x, out;
+  Int4 w, up;
+  int64_t group;
+  if (a[0] == Py_None || !take(a[0], x) || !w.take(a + 1) || (two && !up.take(a + 4)) || !group_of(a[7], &group) || !take(a[8], out) ||
+      !fp8_inputs({&x, &w.q, &w.scales, &w.zeros, &up.q, &up.scales, &up.zeros, &out}) || !bf16_or_fp32(x) || x.dim() < 1 || x.numel() == 0 ||
+      w.q.dim() != 2 || w.q.numel() == 0)
+    Py_RETURN_NONE;
+  const int64_t K = x.size(-1), M = x.numel() / K, N = w.q.size(0);
+  int64_t ld = K;
+  if (x.dim() == 2) ld = matrix_ld(x);
+  else if (!x.is_contiguous()) ld = 0;
+  if (ld == 0 || K > INT32_MAX - 1024 || !w.fits(N, K, group) || (two && (!up.fits(N, K, group) || up.scales.scalar_type() != w.scales.scalar_type())))
+    Py_RETURN_NONE;
+  if (out.defined() && (out.sizes() != at::IntArrayRef({M, N}) || out.scalar_type() != x.scalar_type() || matrix_ld(out) == 0)) Py_RETURN_NONE;
+  {
+    const Body body(x);
+    const int dt = dtype_code(x);
+    int64_t ld_out = N;
+    if (out.defined()) {
+      ld_out = matrix_ld(out);
+    } else if (x.dim() == 2) {
+      out = fresh({M, N}, {N, 1}, x.scalar_type(), x);
+    } else {
+      std::vector<int64_t> sizes = x.sizes().vec();
+      sizes.back() = N;
+      out = at::empty(sizes, x.options().requires_grad(false));
+    }
+    const size_t bytes = api.int4_workspace_bytes(x.const_data_ptr(), ld, M, (int32_t)K, dt);
+    const Tensor ws = bytes ? fresh({(int64_t)bytes}, {1}, at::kByte, x) : Tensor();
+    const Tensor word = status ? at::zeros({64}, x.options().dtype(at::kInt).requires_grad(false)) : Tensor();
+    check(api.matmul_int4(x.const_data_ptr(), ld, &w.c, two ? &up.c : nullptr, dtype_code(w.scales), out.data_ptr(), ld_out, M, (int32_t)N,
+                          (int32_t)K, (int32_t)group, dt, bytes ? ws.data_ptr() : nullptr, bytes, status ? word.data_ptr<int32_t>() : nullptr,
+                          stream_of(x)), "mvpa_matmul_int4");
+    if (status) check(api.fwd_status(word.data_ptr<int32_t>(), 256, stream_of(x)), "mvpa_matmul_int4 kernel");  // synchronises the stream
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // init(path of libmvpa_b200.so, which is already loaded; the class of the mode that a default device is)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 2)) return nullptr;
@@ -775,6 +1026,10 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(api.last_error, "mvpa_last_error_string");
   get(api.quantize_fp8, "mvpa_quantize_fp8"); get(api.rmsnorm_fp8, "mvpa_rmsnorm_fp8");
   get(api.silu_mul_fp8, "mvpa_silu_mul_fp8"); get(api.matmul_fp8, "mvpa_matmul_fp8");
+  get(api.gated_linear, "mvpa_gated_linear"); get(api.gated_linear_bwd, "mvpa_gated_linear_bwd");
+  get(api.gated_saved_bytes, "mvpa_gated_linear_saved_bytes");
+  get(api.quantize_int4, "mvpa_quantize_int4"); get(api.dequantize_int4, "mvpa_dequantize_int4");
+  get(api.matmul_int4, "mvpa_matmul_int4"); get(api.int4_workspace_bytes, "mvpa_matmul_int4_workspace_bytes");
   if (missing) { PyErr_Format(PyExc_ImportError, "%s has no %s", p, missing); return nullptr; }
   Py_RETURN_NONE;
 }
@@ -782,7 +1037,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init), FAST(attend), FAST(forward), FAST(backward), FAST(plain), FAST(block_forward),
                          FAST(block_backward), FAST(branches), FAST(quantize_fp8), FAST(rmsnorm_fp8), FAST(silu_mul_fp8),
-                         FAST(matmul_fp8), FAST(branches_fp8), {nullptr, nullptr, 0, nullptr}};
+                         FAST(matmul_fp8), FAST(branches_fp8), FAST(gated_linear), FAST(gated_forward), FAST(gated_backward),
+                         FAST(quantize_int4), FAST(dequantize_int4), FAST(matmul_int4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "mvpa_host_b200", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -199,32 +199,32 @@ def _look_at(status, what, like):
 
 
 def _gated_kernel(x, w_gate, w_up, save):
-    """(h, gate, up) by the kernel, the last two None unless `save`; x (rows, E)."""
+    """(h, what the backward wants of it, or None unless `save`) by the kernel; x (rows, E)."""
     (rows, E), I = x.shape, w_gate.shape[0]
     h = torch.empty((rows, I), dtype=x.dtype, device=x.device)
-    gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
+    lib = _nat.lib()
+    saved = torch.empty(lib.mvpa_gated_linear_saved_bytes(rows, I), dtype=torch.uint8, device=x.device) if save else None
     with _nat.on_device(x.device):
         status = _status_word(x.device)
-        st = _nat.lib().mvpa_gated_linear(x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(), I,
-                                          gate.data_ptr() if save else None, up.data_ptr() if save else None, rows, E, I,
-                                          None if status is None else status.data_ptr(), _stream(x))
+        st = lib.mvpa_gated_linear(x.data_ptr(), E, w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(), I, saved.data_ptr() if save else None,
+                                   rows, E, I, None if status is None else status.data_ptr(), _stream(x))
         _nat.check(st, "mvpa_gated_linear")
         _look_at(status, "mvpa_gated_linear", x)
-    return h, gate, up
+    return h, saved
 
 
-def _gated_kernel_bwd(dh, gate, up, x, w_gate, w_up, need_x, need_w):
+def _gated_kernel_bwd(dh, x, w_gate, w_up, saved, need_x, need_w):
     """(dx, dw_gate, dw_up) by the kernels, None where not needed; x (rows, E)."""
     (rows, E), I = x.shape, w_gate.shape[0]
-    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    dgate, dup = torch.empty_like(dh), torch.empty_like(dh)
     dx = torch.empty((rows, E), dtype=x.dtype, device=x.device) if need_x else None
     dw_gate, dw_up = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need_w else (None, None)
     ptr = lambda t: None if t is None else t.data_ptr()
     with _nat.on_device(x.device):
         status = _status_word(x.device)
-        st = _nat.lib().mvpa_gated_linear_bwd(dh.data_ptr(), I, gate.data_ptr(), up.data_ptr(), x.data_ptr(), E, w_gate.data_ptr(),
-                                              w_up.data_ptr(), dgate.data_ptr(), dup.data_ptr(), ptr(dx), ptr(dw_gate), ptr(dw_up), rows,
-                                              E, I, ptr(status), _stream(x))
+        st = _nat.lib().mvpa_gated_linear_bwd(dh.data_ptr(), I, saved.data_ptr(), x.data_ptr(), E, w_gate.data_ptr(), w_up.data_ptr(),
+                                              dgate.data_ptr(), dup.data_ptr(), ptr(dx), ptr(dw_gate), ptr(dw_up), rows, E, I, ptr(status),
+                                              _stream(x))
         _nat.check(st, "mvpa_gated_linear_bwd")
         _look_at(status, "mvpa_gated_linear_bwd", x)
     return dx, dw_gate, dw_up
@@ -233,19 +233,26 @@ def _gated_kernel_bwd(dh, gate, up, x, w_gate, w_up, need_x, need_w):
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up):
-        h, gate, up = _gated_kernel(x.view(-1, x.shape[-1]), w_gate, w_up, any(ctx.needs_input_grad))
-        ctx.save_for_backward(x, w_gate, w_up, gate, up)
-        return h if x.dim() == 2 else h.reshape(*x.shape[:-1], w_gate.shape[0])
+        need = any(ctx.needs_input_grad)
+        native = _host.module().gated_forward(x, w_gate, w_up, need, _attn._CHECK_STATUS) if _host.usable(x) else None
+        h, saved = native or _gated_kernel(x.view(-1, x.shape[-1]), w_gate, w_up, need)
+        ctx.save_for_backward(x, w_gate, w_up, saved)
+        return h if h.dim() == x.dim() else h.reshape(*x.shape[:-1], w_gate.shape[0])
 
     @staticmethod
     def backward(ctx, dh):
-        x, w_gate, w_up, gate, up = ctx.saved_tensors
+        x, w_gate, w_up, saved = ctx.saved_tensors
         need = ctx.needs_input_grad
         E, I = x.shape[-1], w_gate.shape[0]
-        if not torch.is_grad_enabled() and _plain(dh.contiguous(), x, w_gate, w_up, gate, up):
-            dx, dw_gate, dw_up = _gated_kernel_bwd(dh.contiguous().view(-1, I), gate, up, x.view(-1, E), w_gate, w_up, need[0],
-                                                   need[1] or need[2])
-            return dx.view(x.shape) if need[0] else None, dw_gate if need[1] else None, dw_up if need[2] else None
+        if not torch.is_grad_enabled():
+            if _host.usable(dh):
+                native = _host.module().gated_backward(dh, x, w_gate, w_up, saved, need[0] + 2 * need[1] + 4 * need[2], _attn._CHECK_STATUS)
+                if native is not None:
+                    return native
+            d = dh.contiguous()
+            if _plain(d, x, w_gate, w_up) and saved.device == x.device and saved.is_contiguous() and saved.data_ptr() % 16 == 0:
+                dx, dw_gate, dw_up = _gated_kernel_bwd(d.view(-1, I), x.view(-1, E), w_gate, w_up, saved, need[0], need[1] or need[2])
+                return dx.view(x.shape) if need[0] else None, dw_gate if need[1] else None, dw_up if need[2] else None
         # a graph of the gradient is wanted (or a transform is active): the same formula in torch operations
         x2, d = x.reshape(-1, E), dh.reshape(-1, I).float()
         g, u = torch.nn.functional.linear(x2, w_gate).float(), torch.nn.functional.linear(x2, w_up).float()
@@ -257,8 +264,12 @@ class _GatedLinear(torch.autograd.Function):
 def gated_linear(x, w_gate, w_up):
     """Differentiable silu(x w_gate^T) * (x w_up^T) for x (..., E) and weights (I, E): the MLP up to its down projection.  bf16 with E
     and I multiples of 8: one kernel forward, with both products and the activation in fp32, rounded once; the backward is one for the
-    gate and one for each matrix product (the gradient of x, that of both weights), from the two products, which the forward keeps in
-    bf16 where a gradient is wanted.  Everything else, and calls under autocast, by torch operations."""
+    gate and one for each matrix product (the gradient of x, that of both weights), from the two products, of which the forward keeps
+    24 bits each where a gradient is wanted.  Everything else, and calls under autocast, by torch operations."""
+    if _host.usable(x):
+        h = _host.module().gated_linear(x, w_gate, w_up, _attn._CHECK_STATUS)     # (an ordinary call that no gradient flows through)
+        if h is not None:
+            return h
     if (not torch.is_autocast_enabled("cuda") and x.dtype == torch.bfloat16 and x.dim() > 1 and w_gate.dim() == 2 and w_gate.shape == w_up.shape
             and x.shape[-1] == w_gate.shape[1] and x.shape[-1] % 8 == 0 and w_gate.shape[0] % 8 == 0):
         if not x.is_contiguous():
@@ -528,6 +539,10 @@ def quantize_int4(w, group=128, zeros=False):
     scale = max|w| / 7 over a group, values -8 to 7; with them scale = (hi - lo) / 15 for lo = min(0, min w) and hi = max(0, max w), and
     the zero is -lo / scale, rounded.  Quotients are exact before they are rounded, halves to even.  A group whose scale rounds to zero
     stands for zeros, one that holds an infinity or a NaN has the scale NaN."""
+    if _host.usable(w):
+        made = _host.module().quantize_int4(w, group, zeros)
+        if made is not None:
+            return made
     what = "quantize_int4"
     _fp8_inputs(what, w)
     if group not in INT4_GROUPS:
@@ -548,6 +563,11 @@ def quantize_int4(w, group=128, zeros=False):
 def dequantize_int4(q, scales, zeros=None, width=None, group=128, dtype=None):
     """The values (N, width) that a weight in 4 bits stands for, in `dtype` (the scales' type unless given).  `width` is K, which for an
     odd K the shape of q does not tell; 2 * q.shape[1] unless given."""
+    if _host.usable(q) and (dtype is None or dtype is torch.bfloat16 or dtype is torch.float32):
+        made = _host.module().dequantize_int4(q, scales, zeros, 2 * q.shape[-1] if width is None else width, group,
+                                              scales.dtype is torch.float32 if dtype is None else dtype is torch.float32)
+        if made is not None:
+            return made
     what = "dequantize_int4"
     _fp8_inputs(what, q, scales, *(() if zeros is None else (zeros,)))
     if q.dim() != 2:
@@ -599,6 +619,10 @@ def matmul_int4(x, q, scales, zeros=None, group=128, out=None):
     """x @ W.T for a weight W (N, K) in 4 bits and x (..., K), bf16 or fp32; the result in x's type, or in `out` (rows, N), which may be a
     column block of a wider buffer.  No weight is rounded: whole numbers are multiplied and added in fp32 over a group, the groups' sums
     scaled and added in fp32, rounded once."""
+    if _host.usable(x):
+        done = _host.module().matmul_int4(x, q, scales, zeros, None, None, None, group, out, _attn._CHECK_STATUS)
+        if done is not None:
+            return done if out is None else out
     return _int4_product("matmul_int4", x, (q, scales, zeros), None, group, out)
 
 
@@ -608,4 +632,9 @@ def gated_linear_int4(x, gate, up, group=128, out=None):
     what = "gated_linear_int4"
     if len(gate) not in (2, 3) or len(up) not in (2, 3):
         raise RuntimeError(f"{what}: gate and up are (q, scales) or (q, scales, zeros)")
+    if _host.usable(x):
+        done = _host.module().matmul_int4(x, *(gate if len(gate) == 3 else (*gate, None)), *(up if len(up) == 3 else (*up, None)), group, out,
+                                          _attn._CHECK_STATUS)
+        if done is not None:
+            return done if out is None else out
     return _int4_product(what, x, tuple(gate), tuple(up), group, out)

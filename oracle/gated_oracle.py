@@ -6,6 +6,7 @@ import torch
 
 HALF = 2.0 ** -8
 CUT = 2.0 ** -23
+KEPT = 2.0 ** -15          # the 24 bits of a product that wait for the backward, cut off
 GATE = 2.0 ** -18          # silu from fp32 sums: estimates of e^x and 1/x, taken to the fourth power at worst
 
 
@@ -30,7 +31,7 @@ def bounds(x, wg, wu, dh):
     eg, eu = (E * CUT * (x.abs() @ w.abs().t()) for w in (wg, wu))
     h, f = g * s * u, s * (1 + g * (1 - s))
     bh = 1.1 * eg * u.abs() + (g * s).abs() * eu + 1.1 * eg * eu + (HALF + GATE) * h.abs()
-    eg, eu = eg + HALF * (g.abs() + eg), eu + HALF * (u.abs() + eu)       # as they are kept for the backward
+    eg, eu = eg + KEPT * (g.abs() + eg), eu + KEPT * (u.abs() + eu)       # as they are kept for the backward
     dg, du = dh * u * f, dh * g * s
     bg = dh.abs() * (0.5 * eg * (u.abs() + eu) + f.abs() * eu)
     bu = dh.abs() * 1.1 * eg

@@ -39,14 +39,15 @@ def test_entry_points_refuse():
     lib = nat.lib()
     buf = ctypes.create_string_buffer(1 << 16)
     p = (ctypes.addressof(buf) + 15) & ~15
-    fwd = lambda x=p, ld_x=64, wg=p, wu=p, h=p, ld_h=64, g=None, u=None, M=4, E=64, I=64: lib.mvpa_gated_linear(
-        x, ld_x, wg, wu, h, ld_h, g, u, M, E, I, None, None)
-    bwd = lambda dh=p, ld=64, g=p, u=p, x=p, dg=p, du=p, dx=p, dwg=p, dwu=p, M=4, E=64, I=64: lib.mvpa_gated_linear_bwd(
-        dh, ld, g, u, x, 64, p, p, dg, du, dx, dwg, dwu, M, E, I, None, None)
+    fwd = lambda x=p, ld_x=64, wg=p, wu=p, h=p, ld_h=64, saved=None, M=4, E=64, I=64: lib.mvpa_gated_linear(
+        x, ld_x, wg, wu, h, ld_h, saved, M, E, I, None, None)
+    bwd = lambda dh=p, ld=64, saved=p, x=p, dg=p, du=p, dx=p, dwg=p, dwu=p, M=4, E=64, I=64: lib.mvpa_gated_linear_bwd(
+        dh, ld, saved, x, 64, p, p, dg, du, dx, dwg, dwu, M, E, I, None, None)
+    assert lib.mvpa_gated_linear_saved_bytes(5, 24) == 5 * (2 * 48 + 2 * 32) and lib.mvpa_gated_linear_saved_bytes(0, 24) == 0
     shape = (dict(M=0), dict(E=0), dict(I=0), dict(E=60), dict(I=4), dict(M=-1), dict(M=2 ** 31))
     for bad in shape:
         assert fwd(**bad) == bwd(**bad) == -1 and "multiples of 8" in nat.last_error(), bad
-    for bad in (dict(x=p + 2), dict(ld_x=63), dict(ld_x=56), dict(wg=None), dict(wu=p + 8), dict(h=None), dict(ld_h=68), dict(g=p), dict(u=p)):
+    for bad in (dict(x=p + 2), dict(ld_x=63), dict(ld_x=56), dict(wg=None), dict(wu=p + 8), dict(h=None), dict(ld_h=68), dict(saved=p + 8)):
         assert fwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad
-    for bad in (dict(dh=None), dict(ld=60), dict(g=None), dict(du=p + 4), dict(dwg=None), dict(dx=p + 2), dict(x=None)):
+    for bad in (dict(dh=None), dict(ld=60), dict(saved=None), dict(du=p + 4), dict(dwg=None), dict(dx=p + 2), dict(x=None)):
         assert bwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad
