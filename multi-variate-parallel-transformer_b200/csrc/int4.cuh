@@ -27,7 +27,8 @@ __device__ __forceinline__ void int4_pairs(uint32_t w, uint32_t minus, uint32_t 
   const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&minus);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    uint32_t v;  // (w >> 4 i) & 0x000f000f | 0x43004300 in one operation: both constants in registers, or the compiler makes it two
+    asm("{\n\t.reg .b32 mask, one;\n\tmov.b32 mask, 0x000f000f;\n\tmov.b32 one, 0x43004300;\n\tlop3.b32 %0, %1, mask, one, 0xea;\n\t}" : "=r"(v) : "r"(w >> (4 * i)));
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), m);
     p[i] = *reinterpret_cast<const uint32_t*>(&d);
   }

@@ -4,8 +4,9 @@
 //
 // The whole numbers q - zero are exact in bf16, so the inner sums are products of bf16 on the tensor cores with fp32 sums, and a group's
 // sum is scaled in fp32: no weight is rounded.  An fp32 x goes in as the three bf16 that it is the sum of.  Two kernels:
-//   few     up to 8 tokens: a warp forms 16 weight rows x 8 tokens from registers alone
-//   many    128 weight rows x up to 128 tokens a CTA: the weights are the product's M side, unpacked into TMEM on their way
+//   few     up to 16 tokens: a warp forms 2 x 16 weight rows x 8 or 16 tokens from registers
+//   many    128 weight rows x up to 256 tokens a CTA: the weights are the product's M side, unpacked into TMEM on their way
+#include <algorithm>
 #include <type_traits>
 
 #include "int4.cuh"
@@ -26,9 +27,9 @@ struct Int4Args {
   void* out;
   int64_t ld_out, M;
   int N, K, group, groups, chunks;  // chunks of 128 along K
-  int per, splits;                  // many: chunks of a split
+  int per, splits;                  // chunks of a split
   uint32_t tiles_m, tiles_n;
-  int vec;                          // few: rows of x on 16-byte boundaries
+  int64_t plane;                    // few: elements between the parts of x
   int* status;
 };
 
@@ -40,87 +41,33 @@ __device__ __forceinline__ float gate_of(float g, float u) {
   else return Sigmoid(g).times(g, u);
 }
 
+__device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_map(at, rank)) : "memory");
+  return v;
+}
+
 // ---- few rows ---------------------------------------------------------------------------------------------------------------------------
-// Bound by the weights' bytes.  A CTA has 16 weight rows, its warps every kWarps-th chunk of 128 columns; a lane's nibbles go through
-// registers straight into the products of mma.sync (m16n8k16: with 8 tokens its rate is far above what the weights' arrival asks for, and
-// nothing waits in shared memory).  Which columns stand at which place along K of a product is free as long as both operands agree:
-// lane t of a row's four takes 16, 8 or 4 neighbouring bytes, so that all columns of one product lie in one group.
+// Bound by the weights' bytes, and next to that by the instructions that unpack them.  A warp forms 16 weight rows x all tokens over a
+// chunk of 128 columns at a time, with mma.sync (m16n8k16: with these few tokens its rate is far above what the weights' arrival asks
+// for, and the unpacked weights never leave the registers).  Which columns stand at which place along K of a product is free as long as
+// both operands agree: lane t of a row's four takes 16, 8 or 4 neighbouring bytes, so that all columns of one product lie in one group.
+//
+// A CTA's eight warps are WR stretches of 16 rows x WK chunks side by side.  Weights and tokens come by cp.async, kDepth - 1 turns ahead:
+// what hides the memory's latency is bytes on their way, and those that wait in registers cost warps.  The scales of a CTA's rows are
+// loaded once.  A long K is split over the CTAs of a cluster, whose sums meet through distributed shared memory in a fixed order.
 constexpr int kFewWarps = 8;
 
-template <int G>
-__device__ __forceinline__ int word_column(int t, int i) {  // the first column, in its chunk, of word i of lane t
-  if constexpr (G == 128) return t * 32 + i * 8;
-  else if constexpr (G == 64) return (i >> 1) * 64 + t * 16 + (i & 1) * 8;
-  else return i * 32 + t * 8;
+// 16 bytes to shared memory, of which the first `bytes` come from memory and the others are zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-
-// Four words of a row's chunk; what lies past the row reads as zero.
-template <int G>
-__device__ __forceinline__ void load_words(const uint8_t* row, int chunk, int t, int bytes, uint32_t (&w)[4]) {
-  const uint8_t* p = row + (int64_t)chunk * (kChunk / 2);
-  if ((chunk + 1) * (int64_t)(kChunk / 2) <= bytes) {
-    if constexpr (G == 128) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + t * 16);
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else if constexpr (G == 64) {
-      const uint2 a = *reinterpret_cast<const uint2*>(p + t * 8), b = *reinterpret_cast<const uint2*>(p + 32 + t * 8);
-      w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(p + i * 16 + t * 4);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = word_column<G>(t, i) / 2, left = bytes - chunk * (kChunk / 2) - at;
-    w[i] = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (b < left) w[i] |= (uint32_t)p[at + b] << (8 * b);
-  }
+template <int N>
+__device__ __forceinline__ void load_shared(uint32_t at, uint32_t* v) {
+  if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at) : "memory");
+  else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(at) : "memory");
 }
-
-// Eight neighbouring columns of a token as the right operand of two products, in the order of int4_pairs; in 16 bits, or in three parts.
-template <typename T>
-struct Columns {
-  static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-  uint32_t b[kParts][4];
-  __device__ __forceinline__ void load(const T* row, int64_t col, int K, bool any, bool vec) {
-    constexpr int W = 8 * (int)sizeof(T) / 4;
-    uint32_t v[W] = {};
-    if (any && col < K) {
-      if (vec && col + 8 <= K) {
-#pragma unroll
-        for (int i = 0; i < W; i += 4) {
-          const uint4 r = *reinterpret_cast<const uint4*>(row + col + i * 4 / (int)sizeof(T));
-          v[i] = r.x; v[i + 1] = r.y; v[i + 2] = r.z; v[i + 3] = r.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (col + e >= K) continue;
-          if constexpr (sizeof(T) == 4) v[e] = reinterpret_cast<const uint32_t*>(row)[col + e];
-          else v[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[col + e] << (16 * (e & 1));
-        }
-      }
-    }
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Thirds a(__uint_as_float(v[i])), c(__uint_as_float(v[i + 4]));
-        b[0][i] = __byte_perm(a.hi, c.hi, 0x7632);
-        b[kParts - 2][i] = __byte_perm(a.mid, c.mid, 0x7632);
-        b[kParts - 1][i] = __byte_perm(a.lo, c.lo, 0x7632);
-      }
-    } else {
-      b[0][0] = __byte_perm(v[0], v[2], 0x5410);
-      b[0][1] = __byte_perm(v[0], v[2], 0x7632);
-      b[0][2] = __byte_perm(v[1], v[3], 0x5410);
-      b[0][3] = __byte_perm(v[1], v[3], 0x7632);
-    }
-  }
-};
 
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -128,106 +75,277 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int G, int W>
+// Each warp has two sets of 16 weight rows: a gate's two weights (W = 2), or two stretches of one.
+template <int W, int NT, int PARTS>
+struct Few {
+  static constexpr int WR = 2, WK = kFewWarps / WR, kTokens = NT * 8, kRows = WR * 16;  // (of a set)
+  static constexpr int kDepth = 3;
+  static constexpr int kXBytes = WK * PARTS * kTokens * 256, kWBytes = kFewWarps * 2 * 1024;  // [wk][part][token]; [warp][set][row]
+  static constexpr int kStageBytes = kXBytes + kWBytes;
+  static constexpr int kSums = 2 * kTokens * kRows, kSumBytes = WK * kSums * 4;               // wait in the stages' memory
+  static constexpr int kBytes = kDepth * kStageBytes > kSumBytes ? kDepth * kStageBytes : kSumBytes;
+  static constexpr int kLeft = 220 * 1024 - kBytes, kMostScales = (kLeft < 48 * 1024 ? kLeft : 48 * 1024) / 8;  // of a CTA's rows, eight bytes each
+};
+
+// Where piece `p` (16 bytes) of token `m`'s row of a chunk lies: pieces change places so that the lanes of a load of 16 bytes, two tokens
+// and the four words of a row that they read together, meet no bank twice.
+template <int G>
+__device__ __forceinline__ int token_piece(int m, int p) {
+  return G == 128 ? p ^ ((p >> 3) & 1) ^ ((m & 1) << 1) : G == 64 ? p ^ (m & 1) : p ^ ((m & 1) << 2);
+}
+
+template <typename T, int G, int W, int NT, int PARTS>
 __global__ void __launch_bounds__(kFewWarps * 32) int4_few_kernel(const Int4Args g) {
-  constexpr int kGroups = kChunk / G;  // of a chunk
-  __shared__ float s_sum[kFewWarps][W][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3, token = lane >> 2;
-  const int n0 = blockIdx.x * 16, bytes = (g.K + 1) / 2;
-  const int row[2] = {min(n0 + (lane >> 2), g.N - 1), min(n0 + (lane >> 2) + 8, g.N - 1)};  // (rows past the last one are not written)
-  const T* x = static_cast<const T*>(g.x) + (token < g.M ? token : 0) * g.ld_x;
+  using C = Few<W, NT, PARTS>;
+  constexpr int kThreads = kFewWarps * 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t base = ptx::smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3, line = lane >> 2;
+  const int wr = warp % C::WR, wk = warp / C::WR;
+  const int n0 = blockIdx.x * C::kRows * (W == 1 ? 2 : 1), bytes = (g.K + 1) / 2;
+  const auto row_of = [&](int s, int row) { return (int64_t)min(n0 + (W == 1 ? s * C::kRows : 0) + row, g.N - 1); };  // (past the last: not written)
+  const int c0 = (int)blockIdx.z * g.per, nc = min(g.chunks - c0, g.per), turns = (nc + C::WK - 1) / C::WK;
   ptx::griddep_launch();
   ptx::griddep_wait();
-  float acc[W][4] = {};
-  uint32_t q[W][2][4];
-  const auto fetch = [&](int c) {
+
+  // What a thread brings each turn (WK chunks): two pieces of 16 bytes of each set of its warp's weight rows, and pieces of the tokens' rows.
+  const int whole = min((g.K >> 7) - c0, nc) / C::WK;  // turns whose columns all exist
+  const uint8_t* w_from[2][2];
 #pragma unroll
-    for (int w = 0; w < W; ++w)
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) load_words<G>(g.w[w].q + row[r] * g.w[w].ld_q, c, t, bytes, q[w][r]);
-  };
-  if (warp < g.chunks) fetch(warp);
-#pragma unroll 1
-  for (int c = warp; c < g.chunks; c += kFewWarps) {
-    uint32_t now[W][2][4];
+    for (int r = 0; r < 2; ++r) {
+      const Int4Weight& w = g.w[W == 2 ? s : 0];
+      w_from[s][r] = w.q + row_of(s, wr * 16 + r * 8 + line) * w.ld_q + (c0 + wk) * (int64_t)(kChunk / 2) + t * 16;
+    }
+  const uint32_t w_to = base + C::kXBytes + warp * 2048 + line * 64 + ((t ^ ((line >> 1) & 3)) << 4);  // (in the order of a 64-byte swizzle)
+  const auto fetch_w = [&](int turn, uint32_t to) {
+    if (turn >= turns) return;
+    const int left = turn < whole ? 16 : max(0, min(16, min(bytes, (c0 + nc) * (kChunk / 2)) - (c0 + turn * C::WK + wk) * (kChunk / 2) - t * 16));
 #pragma unroll
-    for (int w = 0; w < W; ++w)
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) now[w][r][i] = q[w][r][i];
-    if (c + kFewWarps < g.chunks) fetch(c + kFewWarps);
-    float part[W][4];
-    float scale[W][2];
-    uint32_t minus[W][2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // words; 4 / kGroups of them to a group
-      constexpr int kEach = 4 / kGroups;
-      const int group = c * kGroups + i / kEach;
-      if (group >= g.groups) break;  // (the same for the whole warp)
-      if (i % kEach == 0) {
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            scale[w][r] = g.w[w].scale(row[r], group);
-            minus[w][r] = int4_minus(g.w[w].zero(row[r], group));
-            part[w][r] = part[w][r + 2] = 0.f;
-          }
+      for (int r = 0; r < 2; ++r) {
+        copy16(w_to + s * 1024 + r * 512 + to, left > 0 ? w_from[s][r] : g.w[0].q, left);
+        w_from[s][r] += C::WK * (kChunk / 2);
       }
-      Columns<T> b;
-      b.load(x, (int64_t)c * kChunk + word_column<G>(t, i), g.K, token < g.M, g.vec);
+  };
+  // (Rows of tokens that do not exist stay as they are: a token's sums are its own.)
+  constexpr int kMine = C::kXBytes / 16 / kThreads;
+  static_assert(C::kXBytes / 16 % kThreads == 0, "");
+  const int p = threadIdx.x & 15;
+  const uint8_t* x_from[kMine];
+  uint32_t x_to[kMine];
+  const auto fetch_x = [&](int turn, uint32_t to) {
+    if (turn >= turns) return;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        uint32_t a[2][4];
-        int4_pairs(now[w][0][i], minus[w][0], a[0]);
-        int4_pairs(now[w][1][i], minus[w][1], a[1]);
+    for (int j = 0; j < kMine; ++j) {
+      if (x_from[j] == nullptr) continue;
+      const int k = c0 + turn * C::WK + ((threadIdx.x >> 4) + j * (kThreads / 16)) / C::kTokens / PARTS;
+      const int left = turn < whole ? 8 : max(0, min(8, min(g.K, (c0 + nc) * kChunk) - k * kChunk - p * 8));
+      copy16(x_to[j] + to, left > 0 ? x_from[j] : static_cast<const uint8_t*>(g.x), left * 2);
+      x_from[j] += C::WK * kChunk * 2;
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < C::kDepth - 1; ++i) fetch_w(i, i * C::kStageBytes);  // (the weights first: everything else can hide behind them)
 #pragma unroll
-        for (int p = 0; p < Columns<T>::kParts; ++p) {
-          mma_16x8x16(part[w], a[0][0], a[1][0], a[0][1], a[1][1], b.b[p][0], b.b[p][1]);
-          mma_16x8x16(part[w], a[0][2], a[1][2], a[0][3], a[1][3], b.b[p][2], b.b[p][3]);
+  for (int j = 0; j < kMine; ++j) {
+    const int row = (threadIdx.x >> 4) + j * (kThreads / 16), m = row % C::kTokens, part = row / C::kTokens % PARTS, k = row / C::kTokens / PARTS;
+    x_from[j] = m < g.M ? static_cast<const uint8_t*>(g.x) + (part * g.plane + m * g.ld_x + (int64_t)(c0 + k) * kChunk + p * 8) * 2 : nullptr;
+    x_to[j] = base + row * 256 + token_piece<G>(m, p) * 16;
+  }
+#pragma unroll 1
+  for (int i = 0; i < C::kDepth - 1; ++i) {
+    fetch_x(i, i * C::kStageBytes);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  // The scales of the CTA's rows over its chunks, and what their zeros ask to be taken from a nibble: [set][row][group].  Four loads of a
+  // thread at once: one after the other they take longer than everything else.
+  constexpr int kGroups = kChunk / G, kEach = 4 / kGroups;  // groups of a chunk, words of a group
+  const int g0 = c0 * kGroups, ng = min(g.groups - g0, nc * kGroups);
+  const uint32_t s_scale = base + C::kBytes;
+  {
+    constexpr int kAtOnce = 4, kSide = kThreads > 2 * C::kRows ? kThreads / (2 * C::kRows) : 1;  // threads of a row
+#pragma unroll 1
+    for (int row = threadIdx.x / kSide; row < 2 * C::kRows; row += kThreads / kSide) {
+      const Int4Weight& w = g.w[W == 2 ? row / C::kRows : 0];
+      const int64_t n = row_of(row / C::kRows, row % C::kRows);
+#pragma unroll 1
+      for (int k0 = threadIdx.x % kSide; k0 < ng; k0 += kAtOnce * kSide) {
+        float scale[kAtOnce];
+        uint32_t zero[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int k = g0 + min(k0 + j * kSide, ng - 1);
+          scale[j] = w.scale(n, k);
+          zero[j] = w.zero(n, k);
         }
-        if (i % kEach == kEach - 1) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[w][j] = fmaf(scale[w][j / 2], part[w][j], acc[w][j]);
-        }
+        for (int j = 0; j < kAtOnce; ++j)
+          if (k0 + j * kSide < ng)
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(s_scale + (row * ng + k0 + j * kSide) * 8), "f"(scale[j]), "r"(int4_minus(zero[j])) : "memory");
       }
     }
   }
+
+  // Lane t's word i of a row's chunk is word (i of t's four), (of t's two in half i / 2) or (t of the four in quarter i).
+  uint32_t x_at[4];
 #pragma unroll
-  for (int w = 0; w < W; ++w)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s_sum[warp][w][(lane & 3) * 2 * 16 + (j & 1) * 16 + (lane >> 2) + (j >> 1) * 8] = acc[w][j];  // [token][row]
-  __syncthreads();
-  if (threadIdx.x >= 128) return;
-  const int m = threadIdx.x / 16, n = n0 + threadIdx.x % 16;
-  if (m >= g.M || n >= g.N) return;
-  float v[W];
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    v[w] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kFewWarps; ++k) v[w] += s_sum[k][w][threadIdx.x];
+  for (int i = 0; i < 4; ++i) {
+    const int word = G == 128 ? t * 4 + i : G == 64 ? (i >> 1) * 8 + t * 2 + (i & 1) : i * 4 + t;
+    x_at[i] = base + (wk * PARTS * C::kTokens + line) * 256 + token_piece<G>(line, word) * 16;
   }
-  static_cast<T*>(g.out)[m * g.ld_out + n] = from_f32<T>(W == 2 ? gate_of<T>(v[0], v[W - 1]) : v[0]);
+  const uint32_t w_at = base + C::kXBytes + warp * 2048 + line * 64, turned = (line >> 1) & 3;
+  uint32_t my_scale[2][2];  // [set][row]
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) my_scale[s][r] = s_scale + (s * C::kRows + wr * 16 + r * 8 + line) * ng * 8;
+  float acc[2][NT][4] = {};
+  uint32_t from = 0;
+#pragma unroll 1
+  for (int turn = 0; turn < turns; ++turn) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(C::kDepth - 2) : "memory");
+    __syncthreads();
+    {
+      const uint32_t to = from == 0 ? (C::kDepth - 1) * C::kStageBytes : from - C::kStageBytes;
+      fetch_w(turn + C::kDepth - 1, to);
+      fetch_x(turn + C::kDepth - 1, to);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    const int c = turn * C::WK + wk;  // (of the CTA's)
+    if (c < nc) {
+      uint32_t word[2][2][4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t at = w_at + s * 1024 + r * 512 + from;
+          if constexpr (G == 128) {
+            load_shared<4>(at + ((t ^ turned) << 4), word[s][r]);
+          } else if constexpr (G == 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) load_shared<2>(at + (((h * 2 + (t >> 1)) ^ turned) << 4) + (t & 1) * 8, word[s][r] + 2 * h);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_shared<1>(at + ((i ^ turned) << 4) + t * 4, word[s][r] + i);
+          }
+        }
+      float part[2][NT][4];
+      uint32_t sm[2][2][2];  // scale, minus
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i % kEach == 0) {
+          const int k = (kGroups == 1 ? c : min(c * kGroups + i / kEach, ng - 1)) * 8;  // (past the last group: columns of zeros)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            load_shared<2>(my_scale[s][0] + k, sm[s][0]);
+            load_shared<2>(my_scale[s][1] + k, sm[s][1]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) part[s][j][0] = part[s][j][1] = part[s][j][2] = part[s][j][3] = 0.f;
+          }
+        }
+        uint32_t a[2][2][4];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) int4_pairs(word[s][r][i], sm[s][r][1], a[s][r]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) {
+            uint32_t v[4];
+            load_shared<4>(x_at[i] + (q * C::kTokens + j * 8) * 256 + from, v);
+            const uint32_t b0 = __byte_perm(v[0], v[2], 0x5410), b1 = __byte_perm(v[0], v[2], 0x7632), b2 = __byte_perm(v[1], v[3], 0x5410),
+                           b3 = __byte_perm(v[1], v[3], 0x7632);  // (columns 0 and 4, 1 and 5, as int4_pairs leaves them)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              mma_16x8x16(part[s][j], a[s][0][0], a[s][1][0], a[s][0][1], a[s][1][1], b0, b1);
+              mma_16x8x16(part[s][j], a[s][0][2], a[s][1][2], a[s][0][3], a[s][1][3], b2, b3);
+            }
+          }
+        if (i % kEach == kEach - 1) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[s][j][e] = fmaf(__uint_as_float(sm[s][e / 2][0]), part[s][j][e], acc[s][j][e]);
+        }
+      }
+    }
+    from = from == (C::kDepth - 1) * C::kStageBytes ? 0 : from + C::kStageBytes;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* s_sum = reinterpret_cast<float*>(smem);  // [wk][set][token][row]
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s_sum[((wk * 2 + s) * C::kTokens + j * 8 + t * 2 + (e & 1)) * C::kRows + wr * 16 + line + (e >> 1) * 8] = acc[s][j][e];
+  __syncthreads();
+  if (g.splits > 1) {
+    if constexpr (C::WK > 1) {
+      for (int i = threadIdx.x; i < C::kSums; i += kThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < C::WK; ++k) v += s_sum[k * C::kSums + i];
+        s_sum[i] = v;
+      }
+    }
+    __syncwarp();
+    ptx::cluster_sync();
+  }
+  constexpr int kHalf = C::kTokens * C::kRows;
+  for (int i = threadIdx.x + blockIdx.z * kThreads; i < (W == 2 ? 1 : 2) * kHalf; i += kThreads * g.splits) {
+    const int m = i % kHalf / C::kRows, n = n0 + (i / kHalf) * C::kRows + i % C::kRows;
+    if (m >= g.M || n >= g.N) continue;
+    float v[W] = {};
+    if (g.splits > 1) {
+      for (int z = 0; z < g.splits; ++z)
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[w] += peer_load(base + (w * kHalf + i) * 4, z);
+    } else {
+#pragma unroll
+      for (int k = 0; k < C::WK; ++k)
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[w] += s_sum[k * C::kSums + w * kHalf + i];
+    }
+    static_cast<T*>(g.out)[m * g.ld_out + n] = from_f32<T>(W == 2 ? gate_of<T>(v[0], v[W - 1]) : v[0]);
+  }
+  if (g.splits > 1) {
+    __syncwarp();
+    ptx::cluster_sync();  // nobody's memory goes while it is read
+  }
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------------------------
-// 128 weight rows x NT tokens a CTA.  Warps: 0 loads a chunk of 128 columns of both operands (TMA), 2 to 5 unpack the weights, a row a
-// thread, into TMEM, 1 issues a group's products, whose left operand is that part of TMEM, and the warps from 6 on fetch a group's sums,
-// scale them and add them up in registers.  The CTAs are resident and take their tiles one after the other; few tiles: the chunks are
-// split over the CTAs of a cluster, whose sums meet through distributed shared memory in a fixed order.
+// 128 weight rows x NT tokens a CTA.  Warps: 0 loads a chunk of 128 columns of both operands (TMA), 1 issues a group's products, whose left
+// operand is weights unpacked into TMEM, for 128 tokens at a time, 4 to 11 unpack, a row a thread, four warps every other chunk, and 12 to 19
+// fetch a group's sums, scale them and add them up in registers.  A chunk takes four unpacking warps some 1500 cycles from its arrival to
+// the product, half of them instructions, and the products of 256 tokens 1024: two sets of unpackers and four places in TMEM for what they
+// unpack keep up with that (with one set of eight warps, half a row each, and two places: 2200 x 15360 x 2048 185 us).    The CTAs are resident and take their tiles one
+// after the other; few tiles: the chunks are split over the CTAs of a cluster, whose sums meet through distributed shared memory in a
+// fixed order.
 template <int NT, int W, int PARTS>
 struct Many {
   static constexpr int kWBytes = 128 * 64, kXBytes = NT * 256;  // of a chunk: 128 rows x 64 bytes; two halves of NT rows x 128 bytes
   static constexpr int kStageBytes = PARTS * kXBytes + W * kWBytes;
-  static constexpr bool kTwo = NT <= 32;  // two CTAs share a multiprocessor
-  static constexpr int kBudget = (kTwo ? 100 : 208) * 1024;
-  static constexpr int kStages = kBudget / kStageBytes < 8 ? kBudget / kStageBytes : 8;
-  static constexpr int kSums = NT == 128 ? 2 : 4, kTmemA = kSums * NT;  // columns: groups' sums; two chunks of one weight
-  static constexpr int kTmemCols = kTmemA + 128 > 256 ? 512 : 256;
-  static constexpr int kAdders = NT >= 64 ? 8 : 4, kColumns = NT / (kAdders / 4);
-  static constexpr int kThreads = (6 + kAdders) * 32;
+  static constexpr int kBudget = 216 * 1024, kStages = kBudget / kStageBytes < 8 ? kBudget / kStageBytes : 8;
+  static constexpr int kSub = NT < 128 ? NT : 128, kSubs = NT / kSub;   // tokens of one product, products of a tile
+  static constexpr int kSums = kSub == 128 ? 2 : 4, kTmemA = 256, kA = 4;  // columns: groups' sums; chunks of one weight
+  static constexpr int kThreads = 20 * 32;
+  // Two products of a tile: each has four of the adding warps and a place for its sums to itself.  One: four warps take half of its columns.
+  static constexpr int kColumns = kSubs == 2 ? kSub : kSub / 2;         // a thread's of a product
+  // Registers: 640 x 96 at launch.  Up to 32 sums of a thread fit in that.  For more the first four warps keep 24, the unpackers 48, and the
+  // adders take 176: 128 x 24 + 256 x 48 + 256 x 176 = 60416 of 61440.
+  static constexpr bool kWide = W * kColumns > 32;
+  static_assert(kSubs == 1 || (kSubs == 2 && kSums == 2 && W == 1), "");
   static constexpr size_t kSmem = 1024 + kStages * kStageBytes;
   static_assert(kStages >= 2 && W * NT * 128 * 4 <= kStages * kStageBytes, "the sums of a split wait in the stages' memory");
 };
@@ -238,25 +356,19 @@ struct Int4Maps {
 
 enum : int { kGiveUpEmpty = 91, kGiveUpFull = 92, kGiveUpAEmpty = 93, kGiveUpAFull = 94, kGiveUpSumEmpty = 95, kGiveUpSumFull = 96, kGiveUpDrain = 97 };
 
-__device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_map(at, rank)) : "memory");
-  return v;
-}
-
-template <int NT, typename T, int W, bool SPLIT>
-__global__ void __launch_bounds__((Many<NT, W, sizeof(T) == 4 ? 3 : 1>::kThreads), (NT <= 32 ? 2 : 1))
+template <int NT, typename T, int W>
+__global__ void __launch_bounds__((Many<NT, W, sizeof(T) == 4 ? 3 : 1>::kThreads), 1)
 int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
   constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
   using C = Many<NT, W, PARTS>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_afull[2], s_aempty[2], s_sfull[C::kSums], s_sempty[C::kSums];
+  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_afull[C::kA], s_aempty[C::kA], s_sfull[C::kSums], s_sempty[C::kSums];
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;  // a wait ran out: nothing waits any more, and the results are NaN
   const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tiles = g.tiles_m * g.tiles_n;
-  const int c0 = SPLIT ? (int)blockIdx.z * g.per : 0, nc = SPLIT ? min(g.chunks - c0, g.per) : g.chunks;
+  const int c0 = (int)blockIdx.z * g.per, nc = min(g.chunks - c0, g.per);
   const int each = kChunk / g.group;  // groups of a chunk
   if (warp == 0) {
     ptx::prefetch_tensormap(&maps.x);
@@ -267,19 +379,19 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
         ptx::mbar_init(&s_full[i], 1);
         ptx::mbar_init(&s_empty[i], 1 + 4);  // the products that read x, and the four warps that read the weights
       }
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < C::kA; ++i) {
         ptx::mbar_init(&s_afull[i], 4);
         ptx::mbar_init(&s_aempty[i], 1);
       }
       for (int i = 0; i < C::kSums; ++i) {
         ptx::mbar_init(&s_sfull[i], 1);
-        ptx::mbar_init(&s_sempty[i], C::kAdders);
+        ptx::mbar_init(&s_sempty[i], C::kSubs == 2 ? 4 : 8);
       }
       ptx::mbar_fence_init();
       s_dead = 0;
     }
     __syncwarp();
-    ptx::tmem_alloc(&s_tmem, C::kTmemCols);
+    ptx::tmem_alloc(&s_tmem, 512);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
@@ -297,83 +409,98 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
   ptx::griddep_launch();
   ptx::griddep_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
-      Ring<C::kStages> st;
-      uint32_t loads = 0;
-      bool on = true;
-      for (uint32_t t = blockIdx.x; t < tiles && on; t += gridDim.x) {
-        const int m0 = (int)(t % g.tiles_m) * NT, n0 = (int)(t / g.tiles_m) * 128;
-        for (int c = c0; c < c0 + nc; ++c, ++loads, st.step()) {
-          if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
-            on = false;
-            break;
-          }
-          uint8_t* to = smem_raw + (stages - ptx::smem_u32(smem_raw)) + st.at * C::kStageBytes;
-          ptx::mbar_arrive_expect_tx(&s_full[st.at], C::kStageBytes);
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              ptx::tma_load_3d(to + p * C::kXBytes + h * NT * 128, &maps.x, &s_full[st.at], c * kChunk + h * 64, m0, p);
-#pragma unroll
-          for (int w = 0; w < W; ++w) ptx::tma_load_2d(to + PARTS * C::kXBytes + w * C::kWBytes, &maps.w[w], &s_full[st.at], c * (kChunk / 2), n0);
-        }
-      }
-      const uint32_t n = min(loads, (uint32_t)C::kStages);
-      for (uint32_t k = loads - n; k != loads; ++k)  // no copy is in flight when the CTA ends
-        if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
-    }
-  } else if (warp == 1) {
-    const uint32_t el = ptx::elect_one();
-    constexpr uint32_t idesc = ptx::make_idesc_bf16(128, NT, 0);
-    Ring<C::kStages> st;
-    Ring<2> a;
-    Ring<C::kSums> sum;
-    uint32_t last = 0, last_parity = 0;
-    bool on = true, any = false;
-    for (uint32_t t = blockIdx.x; t < tiles && on; t += gridDim.x) {
-      for (int c = c0; c < c0 + nc && on; ++c, st.step()) {
-        if (!wait(s_full[st.at], st.parity, kGiveUpFull)) {
-          on = false;
-          break;
-        }
-        const ptx::DescHalves x = ptx::make_desc_halves_sw128(stages + st.at * C::kStageBytes, 16, 1024);
-        const int here = min(each, g.groups - c * each);
-        for (int w = 0; w < W && on; ++w, a.step()) {
-          if (!wait(s_afull[a.at], a.parity, kGiveUpAFull)) {
-            on = false;
-            break;
-          }
-          for (int k = 0; k < here; ++k, sum.step()) {
-            if (!wait(s_sempty[sum.at], sum.parity ^ 1, kGiveUpSumEmpty)) {
+  if (warp < 4) {
+    if constexpr (C::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+    if (warp == 0) {
+      if (lane == 0) {
+        Ring<C::kStages> st;
+        uint32_t loads = 0;
+        bool on = true;
+        for (uint32_t t = blockIdx.x; t < tiles && on; t += gridDim.x) {
+          const int m0 = (int)(t % g.tiles_m) * NT, n0 = (int)(t / g.tiles_m) * 128;
+          for (int c = c0; c < c0 + nc; ++c, ++loads, st.step()) {
+            if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
               on = false;
               break;
             }
-            ptx::tc_fence_after();
-            for (int s = k * (g.group / 16); s < (k + 1) * (g.group / 16); ++s) {  // steps of 16 columns
+            uint8_t* to = smem_raw + (stages - ptx::smem_u32(smem_raw)) + st.at * C::kStageBytes;
+            ptx::mbar_arrive_expect_tx(&s_full[st.at], C::kStageBytes);
 #pragma unroll
-              for (int p = 0; p < PARTS; ++p)
-                ptx::mma_ts_w(el, tmem + sum.at * NT, tmem + C::kTmemA + a.at * 64 + s * 8, x, p * C::kXBytes + (s >> 2) * NT * 128 + (s & 3) * 32,
-                              idesc, s > k * (g.group / 16) || p > 0);
-            }
-            ptx::mma_commit_w(el, ptx::smem_u32(&s_sfull[sum.at]));
+            for (int w = 0; w < W; ++w) ptx::tma_load_2d(to + PARTS * C::kXBytes + w * C::kWBytes, &maps.w[w], &s_full[st.at], c * (kChunk / 2), n0);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                ptx::tma_load_3d(to + p * C::kXBytes + h * NT * 128, &maps.x, &s_full[st.at], c * kChunk + h * 64, m0, p);
           }
-          ptx::mma_commit_w(el, ptx::smem_u32(&s_aempty[a.at]));
         }
-        if (!on) break;
-        ptx::mma_commit_w(el, ptx::smem_u32(&s_empty[st.at]));
-        last = st.at;
-        last_parity = st.parity;
-        any = true;
+        const uint32_t n = min(loads, (uint32_t)C::kStages);
+        for (uint32_t k = loads - n; k != loads; ++k)  // no copy is in flight when the CTA ends
+          if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
       }
+    } else if (warp == 1) {
+      const uint32_t el = ptx::elect_one();
+      constexpr uint32_t idesc = ptx::make_idesc_bf16(128, C::kSub, 0);
+      Ring<C::kStages> st;
+      Ring<C::kA> a;
+      Ring<C::kSums> sum;
+      uint32_t last = 0, last_parity = 0;
+      bool on = true, any = false;
+      for (uint32_t t = blockIdx.x; t < tiles && on; t += gridDim.x) {
+        for (int c = c0; c < c0 + nc && on; ++c, st.step()) {
+          if (!wait(s_full[st.at], st.parity, kGiveUpFull)) {
+            on = false;
+            break;
+          }
+          const ptx::DescHalves x = ptx::make_desc_halves_sw128(stages + st.at * C::kStageBytes, 16, 1024);
+          const int here = min(each, g.groups - c * each);
+          for (int w = 0; w < W && on; ++w, a.step()) {
+            if (!wait(s_afull[a.at], a.parity, kGiveUpAFull)) {
+              on = false;
+              break;
+            }
+            for (int k = 0; k < here && on; ++k) {
+              for (int sub = 0; sub < C::kSubs; ++sub, sum.step()) {
+                if (!wait(s_sempty[sum.at], sum.parity ^ 1, kGiveUpSumEmpty)) {
+                  on = false;
+                  break;
+                }
+                ptx::tc_fence_after();
+                // (Few instructions: this warp's loop has to be shorter than the products that it issues.)
+                const uint32_t d = tmem + sum.at * C::kSub, left = tmem + C::kTmemA + a.at * 64, right = x.lo + sub * (128 * 128 >> 4);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                  const uint32_t part = right + p * (C::kXBytes >> 4);
+                  if (each == 1) {
+                    ptx::mma_ts_x4_w(el, d, left, part, x.hi, 2, idesc, p > 0);
+                    ptx::mma_ts_x4_w(el, d, left + 32, part + (NT * 128 >> 4), x.hi, 2, idesc, 1);
+                  } else if (each == 2) {
+                    ptx::mma_ts_x4_w(el, d, left + k * 32, part + k * (NT * 128 >> 4), x.hi, 2, idesc, p > 0);
+                  } else {
+                    ptx::mma_ts_x2_w(el, d, left + k * 16, part + (k >> 1) * (NT * 128 >> 4) + (k & 1) * 4, x.hi, 2, idesc, p > 0);
+                  }
+                }
+                ptx::mma_commit_w(el, ptx::smem_u32(&s_sfull[sum.at]));
+              }
+            }
+            ptx::mma_commit_w(el, ptx::smem_u32(&s_aempty[a.at]));
+          }
+          if (!on) break;
+          ptx::mma_commit_w(el, ptx::smem_u32(&s_empty[st.at]));
+          last = st.at;
+          last_parity = st.parity;
+          any = true;
+        }
+      }
+      if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
     }
-    if (any) ptx::mbar_wait(&s_empty[last], last_parity, g.status, kGiveUpDrain);
-  } else if (warp < 6) {
-    const int quad = warp & 3, row = quad * 32 + lane;  // a warp reaches the TMEM lanes of its place among four
+  } else if (warp < 12) {
+    if constexpr (C::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    const int quad = warp & 3, set = (warp - 4) >> 2, row = quad * 32 + lane;  // a warp reaches the TMEM lanes of its place among four
     const uint32_t at_tmem = tmem + C::kTmemA + ((uint32_t)quad << 21);
     Ring<C::kStages> st;
-    Ring<2> a;
+    Ring<C::kA> a;
+    int turn = 0;  // chunks so far, over all tiles
     for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
       const int n = min((int)(t / g.tiles_m) * 128 + row, g.N - 1);
       const auto zeros_of = [&](int c, uint32_t (&z)[W]) {  // a chunk's, a byte each
@@ -387,42 +514,39 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
         }
       };
       uint32_t next[W];
-      zeros_of(c0, next);
-      for (int c = c0; c < c0 + nc; ++c, st.step()) {
+      zeros_of(c0 + ((turn ^ set) & 1), next);
+      for (int c = c0; c < c0 + nc; ++c, ++turn, st.step()) {
+        wait(s_full[st.at], st.parity, kGiveUpFull);  // (each one's: a pass over the ring that is not waited for would make the next look done)
+        if (((turn ^ set) & 1) != 0) {  // the other set's
+#pragma unroll
+          for (int w = 0; w < W; ++w) a.step();
+          continue;
+        }
         uint32_t zeros[W];
 #pragma unroll
         for (int w = 0; w < W; ++w) zeros[w] = next[w];
-        zeros_of(c + 1, next);
-        wait(s_full[st.at], st.parity, kGiveUpFull);
-        const uint32_t tile = stages + st.at * C::kStageBytes + PARTS * C::kXBytes;
+        zeros_of(c + 2, next);
+        const uint32_t tile = stages + st.at * C::kStageBytes + PARTS * C::kXBytes + row * 64, turned = (row >> 1) & 3;
 #pragma unroll
         for (int w = 0; w < W; ++w, a.step()) {
           wait(s_aempty[a.at], a.parity ^ 1, kGiveUpAEmpty);
           __syncwarp();
           ptx::tc_fence_after();
-          uint32_t r[32];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t minus = int4_minus((zeros[w] >> (8 * (i * 32 / g.group))) & 255u);
+            uint32_t v[4], r[16];
+            load_shared<4>(tile + w * C::kWBytes + ((i ^ turned) << 4), v);
 #pragma unroll
-            for (int piece = 0; piece < 2; ++piece) {
-              const int i = half * 2 + piece;
-              uint32_t v[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                           : "r"(tile + w * C::kWBytes + row * 64 + ((i ^ ((row >> 1) & 3)) << 4)));
-              const uint32_t minus = int4_minus((zeros[w] >> (8 * (i * 32 / g.group))) & 255u);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint32_t p[4];
-                int4_pairs(v[j], minus, p);
-                uint32_t* o = r + piece * 16 + j * 4;
-                o[0] = __byte_perm(p[0], p[1], 0x5410);
-                o[1] = __byte_perm(p[2], p[3], 0x5410);
-                o[2] = __byte_perm(p[0], p[1], 0x7632);
-                o[3] = __byte_perm(p[2], p[3], 0x7632);
-              }
+            for (int j = 0; j < 4; ++j) {
+              uint32_t p[4];
+              int4_pairs(v[j], minus, p);
+              r[j * 4] = __byte_perm(p[0], p[1], 0x5410);
+              r[j * 4 + 1] = __byte_perm(p[2], p[3], 0x5410);
+              r[j * 4 + 2] = __byte_perm(p[0], p[1], 0x7632);
+              r[j * 4 + 3] = __byte_perm(p[2], p[3], 0x7632);
             }
-            ptx::tmem_st32(at_tmem + a.at * 64 + half * 32, r);
+            ptx::tmem_st16(at_tmem + a.at * 64 + i * 16, r);
           }
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
@@ -435,46 +559,41 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
       }
     }
   } else {
-    const int quad = warp & 3, first = ((warp - 6) >> 2) * C::kColumns, row = quad * 32 + lane;
-    const uint32_t at_tmem = tmem + ((uint32_t)quad << 21) + first;
+    if constexpr (C::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int quad = warp & 3, set = (warp - 12) >> 2, first = set * C::kColumns, row = quad * 32 + lane;  // (columns of the tile)
+    const uint32_t at_tmem = tmem + ((uint32_t)quad << 21) + (C::kSubs == 2 ? 0 : first);
     Ring<C::kSums> sum;
+    if (C::kSubs == 2 && set == 1) sum.step();
     for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
       const int m0 = (int)(t % g.tiles_m) * NT, n0 = (int)(t / g.tiles_m) * 128, n = min(n0 + row, g.N - 1);
-      float acc[W][C::kColumns];
+      float2 acc[W][C::kColumns / 2];
 #pragma unroll
       for (int w = 0; w < W; ++w)
 #pragma unroll
-        for (int j = 0; j < C::kColumns; ++j) acc[w][j] = 0.f;
-      float next[W][4];
-      const auto scales_of = [&](int c) {
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) next[w][k] = k < each && c < c0 + nc && c * each + k < g.groups ? g.w[w].scale(n, c * each + k) : 0.f;
-      };
-      scales_of(c0);
+        for (int j = 0; j < C::kColumns / 2; ++j) acc[w][j] = make_float2(0.f, 0.f);
+      float next = g.w[0].scale(n, c0 * each);  // (one group ahead)
       for (int c = c0; c < c0 + nc; ++c) {
-        float scale[W][4];
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) scale[w][k] = next[w][k];
-        scales_of(c + 1);
         const int here = min(each, g.groups - c * each);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k >= here) break;
+#pragma unroll 1
+          for (int k = 0; k < here; ++k) {
+            const float2 scale = make_float2(next, next);
+            {
+              const bool same = k + 1 < here;  // the next sums' weight and chunk
+              const int w1 = same ? w : w + 1 < W ? w + 1 : 0, c1 = same || w + 1 < W ? c : c + 1, k1 = same ? k + 1 : 0;
+              if (c1 < c0 + nc) next = g.w[w1].scale(n, c1 * each + k1);
+            }
             wait(s_sfull[sum.at], sum.parity, kGiveUpSumFull);
             __syncwarp();
             ptx::tc_fence_after();
+            const uint32_t from = at_tmem + sum.at * C::kSub;
             constexpr int P = C::kColumns < 32 ? 16 : 32;
 #pragma unroll
             for (int j0 = 0; j0 < C::kColumns; j0 += P) {
               uint32_t r[P];
-              if constexpr (P == 32) ptx::tmem_ld32(at_tmem + sum.at * NT + j0, r);
-              else ptx::tmem_ld16(at_tmem + sum.at * NT + j0, r);
+              if constexpr (P == 32) ptx::tmem_ld32(from + j0, r);
+              else ptx::tmem_ld16(from + j0, r);
               ptx::tmem_ld_wait();
               if (j0 + P == C::kColumns) {
                 ptx::tc_fence_before();
@@ -482,38 +601,46 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
                 if (lane == 0) ptx::mbar_arrive(&s_sempty[sum.at]);
               }
 #pragma unroll
-              for (int j = 0; j < P; ++j) acc[w][j0 + j] = fmaf(__uint_as_float(r[j]), scale[w][k], acc[w][j0 + j]);
+              for (int j = 0; j < P / 2; ++j)
+                acc[w][j0 / 2 + j] = ptx::ffma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), scale, acc[w][j0 / 2 + j]);
             }
-            sum.step();
+#pragma unroll
+            for (int i = 0; i < C::kSubs; ++i) sum.step();
           }
         }
       }
       const float poison = *dead ? __uint_as_float(0x7fffffffu) : 0.f;
-      if constexpr (SPLIT) {  // (every product that read the stages is finished)
+      const auto at = [&](int w, int j) { return (j & 1 ? acc[w][j / 2].y : acc[w][j / 2].x) + poison; };
+      if (g.splits > 1) {  // (every product that read the stages is finished)
 #pragma unroll
         for (int w = 0; w < W; ++w)
 #pragma unroll
           for (int j = 0; j < C::kColumns; ++j)
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(stages + ((w * NT + first + j) * 128 + row) * 4), "f"(acc[w][j] + poison) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(stages + ((w * NT + first + j) * 128 + row) * 4), "f"(at(w, j)) : "memory");
       } else if (n0 + row < g.N) {
         T* out = static_cast<T*>(g.out) + (int64_t)(m0 + first) * g.ld_out + n0 + row;
 #pragma unroll
         for (int j = 0; j < C::kColumns; ++j)
-          if (m0 + first + j < g.M) out[j * g.ld_out] = from_f32<T>((W == 2 ? gate_of<T>(acc[0][j], acc[W - 1][j]) : acc[0][j]) + poison);
+          if (m0 + first + j < g.M) out[j * g.ld_out] = from_f32<T>(W == 2 ? gate_of<T>(at(0, j), at(W - 1, j)) : at(0, j));
       }
     }
   }
-  if constexpr (SPLIT) {
+  if (g.splits > 1) {
     __syncwarp();
     ptx::cluster_sync();
     const int m0 = (int)(blockIdx.x % g.tiles_m) * NT, n0 = (int)(blockIdx.x / g.tiles_m) * 128, splits = g.splits;
-    for (int i = threadIdx.x; i < NT * 128; i += C::kThreads) {
+    for (int i = (int)blockIdx.z * C::kThreads + threadIdx.x; i < NT * 128; i += C::kThreads * splits) {
       const int j = i >> 7, row = i & 127;
-      if (j % splits != (int)blockIdx.z || m0 + j >= g.M || n0 + row >= g.N) continue;
-      float v[W] = {};
-      for (int z = 0; z < splits; ++z)
+      if (m0 + j >= g.M || n0 + row >= g.N) continue;
+      float v[W] = {}, part[W][8];
 #pragma unroll
-        for (int w = 0; w < W; ++w) v[w] += peer_load(stages + ((w * NT + j) * 128 + row) * 4, z);
+      for (int z = 0; z < 8; ++z)  // (all on their way before the first is added)
+#pragma unroll
+        for (int w = 0; w < W; ++w) part[w][z] = z < splits ? peer_load(stages + ((w * NT + j) * 128 + row) * 4, z) : 0.f;
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[w] += part[w][z];
       static_cast<T*>(g.out)[(int64_t)(m0 + j) * g.ld_out + n0 + row] = from_f32<T>(W == 2 ? gate_of<T>(v[0], v[W - 1]) : v[0]);
     }
     __syncwarp();
@@ -523,7 +650,7 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  if (warp == 1) ptx::tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == 1) ptx::tmem_dealloc(tmem, 512);
 }
 
 // x as the TMA can read it: bf16 with rows on 16-byte boundaries, an fp32 one in its three parts, a matrix each.
@@ -544,8 +671,7 @@ __global__ void __launch_bounds__(256) int4_lay_out_kernel(const T* __restrict__
   }
 }
 
-constexpr int kFewTokens = 8;
-
+constexpr int kFewTokens = 16;
 bool in_place(const void* x, int64_t ld_x, int32_t dtype) {
   return dtype == MVPA_BF16 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld_x % 8 == 0;
 }
@@ -567,36 +693,62 @@ int run_many(const void* x, int64_t ld_x, int64_t plane, Int4Args g, cudaStream_
     const int rc = encode_sw128(&maps.w[w], CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w[w].q, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc != MVPA_OK) return rc;
   }
-  const int64_t tm = (g.M + NT - 1) / NT, tn = (g.N + 127) / 128, tiles = tm * tn, room = (int64_t)device_sm_count() * (C::kTwo ? 2 : 1);
+  const int64_t tm = (g.M + NT - 1) / NT, tn = (g.N + 127) / 128, tiles = tm * tn, room = device_sm_count();
   if (tiles * g.chunks > 0x7fffffff) {
     set_error("mvpa_matmul_int4: more than 2^31 blocks of 128 x %d x 128", NT);
     return MVPA_ERR_UNSUPPORTED;
   }
   g.tiles_m = (uint32_t)tm;
   g.tiles_n = (uint32_t)tn;
+  // As many CTAs to a tile as are resident for all tiles at once (clusters of eight: 15 on this device), with two chunks each at least.
+  constexpr auto kernel = int4_many_kernel<NT, T, W>;
+  MVPA_CUDA_CHECK(grant_smem<kernel>(C::kSmem));
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= room && g.chunks >= 4 * splits) splits *= 2;
+  for (int n = 8; n > 1 && splits == 1; n /= 2) {
+    int most = 0;
+    if (g.chunks < 2 * n || tiles * n > room) continue;
+    MVPA_CUDA_CHECK(resident_clusters<kernel>(n, C::kThreads, C::kSmem, &most));
+    if (tiles <= most) splits = n;
+  }
   g.per = (g.chunks + splits - 1) / splits;
   g.splits = (g.chunks + g.per - 1) / g.per;
-  if (g.splits > 1) {
-    constexpr auto kernel = int4_many_kernel<NT, T, W, true>;
-    MVPA_CUDA_CHECK(grant_smem<kernel>(C::kSmem));
-    MVPA_CUDA_CHECK(launch_dependent(g.splits, kernel, dim3((unsigned)tiles, 1, g.splits), C::kThreads, C::kSmem, s, maps, g));
-  } else {
-    constexpr auto kernel = int4_many_kernel<NT, T, W, false>;
-    MVPA_CUDA_CHECK(grant_smem<kernel>(C::kSmem));
-    MVPA_CUDA_CHECK(launch_dependent(1, kernel, (unsigned)(tiles < room ? tiles : room), C::kThreads, C::kSmem, s, maps, g));
-  }
+  const dim3 grid((unsigned)(g.splits > 1 || tiles < room ? tiles : room), 1, g.splits);
+  MVPA_CUDA_CHECK(launch_dependent((unsigned)g.splits, kernel, grid, C::kThreads, C::kSmem, s, maps, g));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
 }
 
-template <typename T, int W>
-int run_few(const Int4Args& g, cudaStream_t s) {
-  const unsigned grid = (unsigned)((g.N + 15) / 16);
-  const auto kernel = g.group == 128 ? int4_few_kernel<T, 128, W> : g.group == 64 ? int4_few_kernel<T, 64, W> : int4_few_kernel<T, 32, W>;
-  MVPA_CUDA_CHECK(launch_dependent(1, kernel, grid, kFewWarps * 32, 0, s, g));
+// -> whether this kernel can do it (a CTA's scales have to fit in shared memory).
+template <typename T, int W, int NT>
+int run_few(const void* x, int64_t ld_x, int64_t plane, Int4Args g, cudaStream_t s, bool* done) {
+  constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+  using C = Few<W, NT, PARTS>;
+  constexpr int kRows = C::kRows * (W == 1 ? 2 : 1);
+  const int64_t tiles = (g.N + kRows - 1) / kRows, room = (int64_t)device_sm_count() * 2;
+  const auto scales = [&](int splits) {
+    const int64_t per = (g.chunks + splits - 1) / splits;
+    return 2 * C::kRows * std::min<int64_t>(per * (kChunk / g.group), g.groups);
+  };
+  int splits = 1;
+  while (splits < 8 && ((tiles * splits * 2 <= room && g.chunks >= C::WK * 2 * splits) || scales(splits) > C::kMostScales)) splits *= 2;
+  *done = scales(splits) <= C::kMostScales;
+  if (!*done) return MVPA_OK;
+  g.per = (g.chunks + splits - 1) / splits;
+  g.splits = (g.chunks + g.per - 1) / g.per;
+  g.x = x;
+  g.ld_x = ld_x;
+  g.plane = plane;
+  const auto launch = [&](auto group) {
+    constexpr auto kernel = int4_few_kernel<T, decltype(group)::value, W, NT, PARTS>;
+    MVPA_CUDA_CHECK(grant_smem<kernel>(C::kBytes + C::kMostScales * 8));
+    MVPA_CUDA_CHECK(launch_dependent((unsigned)g.splits, kernel, dim3((unsigned)tiles, 1, g.splits), kFewWarps * 32, C::kBytes + scales(g.splits) * 8, s, g));
+    return MVPA_OK;
+  };
+  const int rc = g.group == 128  ? launch(std::integral_constant<int, 128>())
+                 : g.group == 64 ? launch(std::integral_constant<int, 64>())
+                                 : launch(std::integral_constant<int, 32>());
+  if (rc != MVPA_OK) return rc;
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
@@ -604,7 +756,6 @@ int run_few(const Int4Args& g, cudaStream_t s) {
 
 template <typename T, int W>
 int run_int4(Int4Args g, int32_t dtype, void* workspace, cudaStream_t s) {
-  if (g.M <= kFewTokens) return run_few<T, W>(g, s);
   const void* x = g.x;
   int64_t ld = g.ld_x, plane = g.ld_x * 8;  // (one part: the stride between parts is never used)
   if (!in_place(g.x, g.ld_x, dtype)) {
@@ -617,11 +768,18 @@ int run_int4(Int4Args g, int32_t dtype, void* workspace, cudaStream_t s) {
     MVPA_CUDA_CHECK(cudaGetLastError());
     x = workspace;
   }
-  if (g.M <= 16) return run_many<16, T, W>(x, ld, plane, g, s);
+  if (g.M <= kFewTokens) {
+    bool done = false;
+    const int rc = g.M <= 8 ? run_few<T, W, 1>(x, ld, plane, g, s, &done) : run_few<T, W, 2>(x, ld, plane, g, s, &done);
+    if (done || rc != MVPA_OK) return rc;
+  }
   if (g.M <= 32) return run_many<32, T, W>(x, ld, plane, g, s);
-  if constexpr (sizeof(T) == 2 && W == 1)
-    if (g.M > 64) return run_many<128, T, W>(x, ld, plane, g, s);
-  return run_many<64, T, W>(x, ld, plane, g, s);
+  if (g.M <= 64 || sizeof(T) == 4) return run_many<64, T, W>(x, ld, plane, g, s);
+  if constexpr (sizeof(T) == 2) {
+    if (g.M <= 128 || W == 2 || ((g.M + 255) / 256) * ((g.N + 127) / 128) < 74) return run_many<128, T, W>(x, ld, plane, g, s);
+    if constexpr (W == 1) return run_many<256, T, W>(x, ld, plane, g, s);
+  }
+  return MVPA_OK;
 }
 
 }  // namespace
@@ -630,7 +788,7 @@ int run_int4(Int4Args g, int32_t dtype, void* workspace, cudaStream_t s) {
 using namespace mvpa;
 
 extern "C" size_t mvpa_matmul_int4_workspace_bytes(const void* x, int64_t ld_x, int64_t M, int32_t K, int32_t dtype) {
-  if (M <= kFewTokens || K <= 0 || in_place(x, ld_x, dtype)) return 0;
+  if (M <= 0 || K <= 0 || in_place(x, ld_x, dtype)) return 0;
   return (size_t)M * (((size_t)K + 7) / 8 * 8) * 2 * (dtype == MVPA_F32 ? 3 : 1);
 }
 
@@ -685,7 +843,6 @@ extern "C" int mvpa_matmul_int4(const void* x, int64_t ld_x, const mvpa_int4* w,
   g.group = group;
   g.groups = (K + group - 1) / group;
   g.chunks = (K + kChunk - 1) / kChunk;
-  g.vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld_x * es % 16 == 0;
   g.status = status;
   if (dtype == MVPA_F32) return up != nullptr ? run_int4<float, 2>(g, dtype, workspace, s) : run_int4<float, 1>(g, dtype, workspace, s);
   return up != nullptr ? run_int4<__nv_bfloat16, 2>(g, dtype, workspace, s) : run_int4<__nv_bfloat16, 1>(g, dtype, workspace, s);

@@ -14,21 +14,48 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kLane = fp8::kLane;  // sixteen values a lane
 
-// Sixteen values are a lane's; a group's lanes are neighbours.  Lanes are numbered along the rows.
+// Sixteen values are a lane's; a group's lanes are neighbours.  Lanes are numbered along the rows; the row is the number by the lanes of a
+// row, for numbers below 2^31 a product with a multiplier that the host forms (n / d = (umulhi(n, m) + n) >> s with s = ceil log2 d and
+// m = floor(2^32 (2^s - d) / d) + 1), for more a division.
 struct Lanes {
   int64_t rows;
-  int per_row, width, groups, lanes;  // lanes of a row (whole groups) and of a group
-  Lanes(int64_t r, int w, int group) : rows(r), width(w), groups((w + group - 1) / group), lanes(group / kLane) { per_row = groups * lanes; }
+  int per_row, width, groups, each;  // lanes of a row (whole groups); log2 of the lanes of a group
+  uint32_t mul, shift;
+  bool small;
+  Lanes(int64_t r, int w, int group) : rows(r), width(w), groups((w + group - 1) / group), each(group == 32 ? 1 : group == 64 ? 2 : 3), shift(0) {
+    per_row = groups << each;
+    while (((uint64_t)1 << shift) < (uint64_t)per_row) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - per_row)) / per_row + 1);
+    small = rows * per_row + kThreads < ((int64_t)1 << 31);
+  }
   int64_t ctas() const { return (rows * per_row + kThreads - 1) / kThreads; }
 };
+struct Place {
+  int64_t row;
+  int lane, col, group;
+  __device__ __forceinline__ explicit Place(const Lanes& g) {
+    const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (g.small) {
+      const uint32_t r = (__umulhi((uint32_t)u, g.mul) + (uint32_t)u) >> g.shift;
+      row = r;
+      lane = (int)((uint32_t)u - r * (uint32_t)g.per_row);
+    } else {
+      row = u / g.per_row;
+      lane = (int)(u - row * g.per_row);
+    }
+    col = lane * kLane;
+    group = lane >> g.each;
+  }
+};
 
-// round(y / s) of the exact quotient, halves to even: the nearest whole number to y * (1 / s) may lie on the wrong side of a border, so
-// the border between it and the next one is looked at, y - (n + 1/2) s, of which the fused operation keeps the sign.
+// round(y / s) of the exact quotient, halves to even, for quotients of at most a few hundred, as kMagic + itself: added to 1.5 * 2^23 a
+// number is rounded to a whole one, which then stands in the low bits.  The nearest whole number to y * (1 / s) may lie on the wrong side
+// of a border, so the border between it and the next one is looked at, y - (n + 1/2) s, of which the fused operation keeps the sign.
+constexpr float kMagic = 12582912.f;
 __device__ __forceinline__ float nearest(float y, float s, float inverse) {
-  const float t = y * inverse, n = rintf(t), dir = copysignf(1.f, t - n);
+  const float t = y * inverse, m = t + kMagic, n = m - kMagic, dir = copysignf(1.f, t - n);
   const float d = fmaf(-(n + 0.5f * dir), s, y) * dir;
-  const bool odd = (static_cast<int>(n) & 1) != 0;
-  return d > 0.f || (d == 0.f && odd) ? n + dir : n;
+  return d > 0.f || (d == 0.f && (__float_as_uint(m) & 1u) != 0u) ? m + dir : m;
 }
 
 template <typename T, bool VEC, bool ZEROS>
@@ -37,9 +64,9 @@ __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __rest
                                                                  const Lanes g) {
   ptx::griddep_launch();
   ptx::griddep_wait();
-  const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = u / g.per_row;
-  const int lane = (int)(u - row * g.per_row), col = lane * kLane, group = lane / g.lanes;
+  const Place at(g);
+  const int64_t row = at.row;
+  const int col = at.col, group = at.group;
   const bool any = row < g.rows;
   float y[kLane];
   fp8::Raw<T> raw = {};
@@ -57,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __rest
       hi = fmaxf(hi, y[e]);
     }
   }
-  for (int m = 1; m < g.lanes; m *= 2) {
+  for (int m = 1; m < 1 << g.each; m *= 2) {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
     if constexpr (ZEROS) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
@@ -73,17 +100,20 @@ __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __rest
   const float up = s < 0x1p-60f ? 0x1p64f : 1.f;  // (away from the numbers below the smallest normal one)
   s *= up;
   const float inverse = some ? __frcp_rn(s) : 0.f;
-  const float zero = ZEROS && some ? fminf(fmaxf(nearest(-lo * up, s, inverse), 0.f), 15.f) : 0.f;
-  if (lane % g.lanes == 0) {
+  const float zero = ZEROS && some ? fminf(fmaxf(nearest(-lo * up, s, inverse) - kMagic, 0.f), 15.f) : 0.f;
+  if ((at.lane & ((1 << g.each) - 1)) == 0) {
     scales[row * ld_s + group] = finite ? rounded : from_f32<T>(__uint_as_float(0x7fffffffu));
     if constexpr (ZEROS) zeros[row * ld_z + group] = (uint8_t)zero;
   }
   uint32_t word[2] = {};
+  const float low = kMagic + (ZEROS ? 0.f : -8.f), shift = ZEROS ? zero : 0.f, none = kMagic;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) {
-    const float n = some ? nearest(y[e] * up, s, inverse) : 0.f;
-    const float v = ZEROS ? fminf(fmaxf(n + zero, 0.f), 15.f) : fminf(fmaxf(n, -8.f), 7.f) + 8.f;
-    word[e / 8] |= (col + e < g.width ? (uint32_t)v : 0u) << (4 * (e % 8));
+    float n = some ? nearest(y[e] * up, s, inverse) : none;
+    if constexpr (ZEROS) n += shift;  // (exact: whole numbers of 24 bits)
+    n = fminf(fmaxf(n, low), low + 15.f);
+    const uint32_t v = (__float_as_uint(n) + (ZEROS ? 0u : 8u)) & 15u;
+    word[e / 8] |= (col + e < g.width ? v : 0u) << (4 * (e % 8));
   }
   uint8_t* to = q + row * ld_q + col / 2;
   if (col + kLane <= g.width) {
@@ -99,9 +129,9 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) dequantize_int4_kernel(const Int4Weight w, T* __restrict__ out, int64_t ld_out, bool vec, const Lanes g) {
   ptx::griddep_launch();
   ptx::griddep_wait();
-  const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = u / g.per_row;
-  const int lane = (int)(u - row * g.per_row), col = lane * kLane, group = lane / g.lanes;
+  const Place at(g);
+  const int64_t row = at.row;
+  const int col = at.col, group = at.group;
   if (row >= g.rows || col >= g.width) return;
   const uint8_t* from = w.q + row * w.ld_q + col / 2;
   uint32_t word[2] = {};
@@ -114,10 +144,10 @@ __global__ void __launch_bounds__(kThreads) dequantize_int4_kernel(const Int4Wei
     for (int b = 0; b < 8; ++b)
       if (col + 2 * b < g.width) word[b / 4] |= (uint32_t)from[b] << (8 * (b % 4));
   }
-  const float s = w.scale(row, group), zero = (float)w.zero(row, group);
+  const float s = w.scale(row, group), zero = __uint_as_float(0x4b000000u | w.zero(row, group));  // (2^23 + zero)
   float y[kLane];
 #pragma unroll
-  for (int e = 0; e < kLane; ++e) y[e] = ((float)((word[e / 8] >> (4 * (e % 8))) & 15u) - zero) * s;
+  for (int e = 0; e < kLane; ++e) y[e] = (__uint_as_float(0x4b000000u | ((word[e / 8] >> (4 * (e % 8))) & 15u)) - zero) * s;
   T* to = out + row * ld_out;
   if (vec) {
     fp8::Raw<T> raw;

@@ -422,6 +422,21 @@ __device__ __forceinline__ void tma_load_2d_pair_w(uint32_t el, uint32_t smem_ds
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(el)
       : "memory");
 }
+// Loads into this CTA's shared memory, issued by the elected lane of a convergent warp.
+__device__ __forceinline__ void tma_load_2d_w(uint32_t el, uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred pe;\n\tsetp.ne.b32 pe, %5, 0;\n\t"
+      "@pe cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(el)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_w(uint32_t el, uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "{\n\t.reg .pred pe;\n\tsetp.ne.b32 pe, %6, 0;\n\t"
+      "@pe cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(el)
+      : "memory");
+}
 // The barrier of this place in each CTA of the cluster whose bit is set.
 __device__ __forceinline__ void mma_commit_pair_w(uint32_t el, uint16_t ctas, uint32_t bar) {
   asm volatile(
@@ -528,6 +543,23 @@ __device__ __forceinline__ void mma_ts_x4_w(uint32_t el, uint32_t d_tmem, uint32
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1 + 16], db, %5, p1;\n\t"
       "add.u32 lo, lo, %4;\n\t mov.b64 db, {lo, %3};\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1 + 24], db, %5, p1;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(b_step16), "r"(idesc), "r"(accumulate_first), "r"(el)
+      : "memory");
+}
+
+// Two steps of the same.
+__device__ __forceinline__ void mma_ts_x2_w(uint32_t el, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t b_step16,
+                                            uint32_t idesc, uint32_t accumulate_first) {
+  asm volatile(
+      "{\n\t.reg .pred p0, p1, pe;\n\t.reg .b64 db;\n\t.reg .b32 lo;\n\t"
+      "setp.ne.b32 p0, %6, 0;\n\t"
+      "setp.ne.b32 pe, %7, 0;\n\t"
+      "setp.eq.b32 p1, 0, 0;\n\t"
+      "mov.b32 lo, %2;\n\t"
+      "mov.b64 db, {lo, %3};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p0;\n\t"
+      "add.u32 lo, lo, %4;\n\t mov.b64 db, {lo, %3};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1 + 8], db, %5, p1;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(b_step16), "r"(idesc), "r"(accumulate_first), "r"(el)
       : "memory");
 }

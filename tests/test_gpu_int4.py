@@ -307,12 +307,13 @@ def test_offsets_past_32_bits(cuda):
     back = ops.dequantize_int4(q, s)
     assert torch.equal(back[-200:], ops.dequantize_int4(*last))
     del back, w
-    for M in (2, 20):
+    # (products against the definition: other sizes are summed in another order)
+    for M in (2, 20, 40):
         x = _randn(_gen(M), M, K, dtype=BF16)
-        assert torch.equal(ops.matmul_int4(x, q, s)[:, -200:], ops.matmul_int4(x, *last))
+        exact, bound, _ = ref.product(x, (*last, None), K, 128, 2.0 ** -8)
+        assert ((ops.matmul_int4(x, q, s)[:, -200:].double() - exact).abs() <= bound).all()
     x = torch.zeros(N, K, dtype=BF16, device="cuda")
     x[-300:] = _randn(_gen(7), 300, K, dtype=BF16)
     few = ops.quantize_int4(_randn(_gen(8), 2000, K, dtype=BF16))
-    # (against the definition: 300 rows alone are summed in another order, their columns being split over several CTAs)
     exact, bound, _ = ref.product(x[-300:], (*few, None), K, 128, 2.0 ** -8)
     assert ((ops.matmul_int4(x, *few)[-300:].double() - exact).abs() <= bound).all()

@@ -64,7 +64,7 @@ def test_entry_points_refuse():
     assert quant(N=0) == quant(K=0) == back(N=0) == back(K=0) == mul(M=0) == mul(N=0) == 0
     # a workspace where x has to be laid out again, and none where it has not
     need = lib.mvpa_matmul_int4_workspace_bytes
-    assert need(p, 64, 8, 64, 0) == 0 and need(p, 64, 9, 64, 1) == 0 and need(p, 64, 9, 60, 0) == 9 * 64 * 2 * 3 and need(p + 2, 64, 9, 60, 1) == 9 * 64 * 2
+    assert need(p, 64, 0, 64, 0) == 0 and need(p, 64, 9, 64, 1) == 0 and need(p, 64, 9, 60, 0) == 9 * 64 * 2 * 3 and need(p + 2, 64, 9, 60, 1) == 9 * 64 * 2
     assert need(p, 63, 9, 60, 1) == 9 * 64 * 2
     assert mul(M=9) == mul(M=9, ws=p, nbytes=9 * 64 * 6 - 1) == mul(M=9, ws=p + 8, nbytes=1 << 15) == -4
     assert "workspace" in nat.last_error()
