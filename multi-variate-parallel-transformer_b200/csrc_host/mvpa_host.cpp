@@ -259,8 +259,8 @@ PyObject* forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // backward(do, q, u, vt, z, k, r_time, r_chan, v, o, lse, sm_scale, window, status) -> the eight gradients or None
 PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 14)) return nullptr;
-  const bool status = a[13] == Py_True;
+  if (n != 14 && !arguments(n, 15)) return nullptr;
+  const bool status = a[13] == Py_True, gated = n > 14 && a[14] == Py_True;
   Ops x;
   double scale;
   int64_t window;
@@ -362,21 +362,31 @@ struct Body {
   explicit Body(const Tensor& t) : guard(t.device()) {}
 };
 
+// The kernels' status word, looked at after a call (which synchronises the stream) where calls are checked; else no tensor.
+Tensor status_word(bool status, const Tensor& like) {
+  return status ? at::zeros({64}, like.options().dtype(at::kInt).requires_grad(false)) : Tensor();
+}
+int32_t* word_of(const Tensor& word) { return word.defined() ? word.data_ptr<int32_t>() : nullptr; }
+void look_at(const Tensor& word, const Tensor& like, const char* what) {
+  if (word.defined()) check(api.fwd_status(word.data_ptr(), 256, stream_of(like)), what);
+}
+
 const char* part(const Tensor& t, int64_t elements) { return static_cast<const char*>(t.const_data_ptr()) + elements * t.element_size(); }
 
-// block_forward(x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, eps, window, H, Hkv, D, status)
-//   -> (h, xn, q, kv, g, up, rt, rc, o, lse, act): `block_grad.BlockFunction.forward`, or None
+// block_forward(x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, eps, window, H, Hkv, D, status, gated)
+//   -> (h, xn, q, kv, g, up, rt, rc, o, lse, act): `block_grad.BlockFunction.forward`, or None.  `gated` (bf16): the gate as one kernel,
+//   which keeps what the backward wants in one tensor of bytes, in g's place; up is None.
 PyObject* block_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 19)) return nullptr;
-  const bool status = a[18] == Py_True;
+  if (!arguments(n, 20)) return nullptr;
+  const bool status = a[18] == Py_True, gated = a[19] == Py_True;
   Tensor in[13];
   for (int i = 0; i < 13; ++i) {
     if (!THPVariable_CheckExact(a[i])) Py_RETURN_NONE;
     in[i] = THPVariable_Unpack(a[i]);
   }
   Dims d;
-  if (watched() || !block_dims(in, a + 15, d)) Py_RETURN_NONE;
+  if (watched() || !block_dims(in, a + 15, d) || (gated && (in[0].scalar_type() != at::kBFloat16 || d.E % 8 != 0 || d.I % 8 != 0))) Py_RETURN_NONE;
   const Tensor &x = in[0], &pos = in[1], &chan = in[2], &ln_w = in[3], &wq = in[4], &wkv = in[5], &wpos = in[6], &wchan = in[7],
                &bias = in[8], &wc = in[9], &wg = in[10], &wu = in[11], &wd = in[12];
   const double eps = PyFloat_AsDouble(a[13]);
@@ -392,8 +402,10 @@ PyObject* block_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       stream_of(x)), "mvpa_rmsnorm");
     q = at::mm(xn, wq.t());
     kv = at::mm(xn, wkv.t());
-    g = at::mm(xn, wg.t());
-    up = at::mm(xn, wu.t());
+    if (!gated) {
+      g = at::mm(xn, wg.t());
+      up = at::mm(xn, wu.t());
+    }
     const auto keys = [&](const Tensor& embeds, const Tensor& w) {  // (Hkv, rows, D)
       return at::mm(embeds.select(0, 0), w.t()).view({-1, d.Hkv, d.D}).transpose(0, 1).contiguous();
     };
@@ -404,9 +416,17 @@ PyObject* block_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     launch_fwd(d.problem(dt, 1.0 / std::sqrt((double)d.D), (int)window), columns(q, 0, d.N, d.D), columns(kv, 0, d.N, d.D),
                columns(kv, d.KV, d.N, d.D), part(bias, 0), part(bias, d.KV), part(bias, 2 * d.KV), rt, rc, columns(o, 0, d.N, d.D),
                lse.data_ptr<float>(), status);
-    act = at::empty_like(g);
-    check(api.silu_mul(g.const_data_ptr(), up.const_data_ptr(), g.stride(0), act.data_ptr(), act.stride(0), d.rows, (int32_t)g.size(1), dt,
-                       stream_of(x)), "mvpa_silu_mul");
+    act = at::empty({d.rows, d.I}, xn.options());
+    if (gated) {
+      g = scratch(api.gated_saved_bytes(d.rows, (int32_t)d.I), x);
+      const Tensor word = status_word(status, x);
+      check(api.gated_linear(xn.const_data_ptr(), d.E, wg.const_data_ptr(), wu.const_data_ptr(), act.data_ptr(), d.I, g.data_ptr(), d.rows,
+                             (int32_t)d.E, (int32_t)d.I, word_of(word), stream_of(x)), "mvpa_gated_linear");
+      look_at(word, x, "mvpa_gated_linear kernel");
+    } else {
+      check(api.silu_mul(g.const_data_ptr(), up.const_data_ptr(), g.stride(0), act.data_ptr(), act.stride(0), d.rows, (int32_t)g.size(1), dt,
+                         stream_of(x)), "mvpa_silu_mul");
+    }
     h = at::empty_like(x);  // (not a view of a matrix: the caller may change it in place)
     Tensor h2 = h.view({d.rows, d.E});
     at::addmm_out(h2, x2, act, wd.t());
@@ -417,13 +437,14 @@ PyObject* block_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // block_backward(dh, x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, xn, q, kv, g, up, rt, rc, o, lse, act, need, eps,
-//   window, H, Hkv, D, status) -> the thirteen gradients (None where the bit of `need` is clear), or None
+//   window, H, Hkv, D, status, gated) -> the thirteen gradients (None where the bit of `need` is clear), or None
 PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 31)) return nullptr;
-  const bool status = a[30] == Py_True;
+  if (!arguments(n, 32)) return nullptr;
+  const bool status = a[30] == Py_True, gated = a[31] == Py_True;
   Tensor in[24];
   for (int i = 0; i < 24; ++i) {
+    if (gated && i == 18) continue;  // (no `up`)
     if (!THPVariable_CheckExact(a[i])) Py_RETURN_NONE;
     in[i] = THPVariable_Unpack(a[i]);
   }
@@ -434,8 +455,12 @@ PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // (a saved-tensor hook may have brought anything back)
   const std::vector<int64_t> saved[10] = {{d.rows, d.E}, {d.rows, d.H * d.D}, {d.rows, 2 * d.KV}, {d.rows, d.I}, {d.rows, d.I},
                                           {d.Hkv, d.T, d.D}, {d.Hkv, d.C, d.D}, {d.rows, d.H * d.D}, {d.B * d.H, d.N}, {d.rows, d.I}};
-  for (int i = 0; i < 10; ++i)
+  for (int i = 0; i < 10; ++i) {
+    if (gated && (i == 3 || i == 4)) continue;
     if (!fits(in[14 + i], in[1], i == 8 ? at::kFloat : in[1].scalar_type(), saved[i])) Py_RETURN_NONE;
+  }
+  if (gated && (in[1].scalar_type() != at::kBFloat16 || !fits(in[17], in[1], at::kByte, {(int64_t)api.gated_saved_bytes(d.rows, (int32_t)d.I)})))
+    Py_RETURN_NONE;
   const Tensor &x = in[1], &pos = in[2], &chan = in[3], &ln_w = in[4], &wq = in[5], &wkv = in[6], &wpos = in[7], &wchan = in[8],
                &bias = in[9], &wc = in[10], &wg = in[11], &wu = in[12], &wd = in[13], &xn = in[14], &q = in[15], &kv = in[16],
                &g = in[17], &up = in[18], &rt = in[19], &rc = in[20], &o = in[21], &lse = in[22], &act = in[23];
@@ -454,9 +479,27 @@ PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     weight(9, dh2, o);
     weight(12, dh2, act);
     const Tensor dact = at::mm(dh2, wd);
-    const Tensor dg = at::empty({d.rows, g.size(1)}, g.options().requires_grad(false)), dup = at::empty_like(dg);
-    check(api.silu_mul_bwd(g.const_data_ptr(), up.const_data_ptr(), g.stride(0), dact.const_data_ptr(), dact.stride(0), dg.data_ptr(),
-                           dup.data_ptr(), g.size(1), d.rows, (int32_t)g.size(1), dt, stream_of(x)), "mvpa_silu_mul_bwd");
+    const Tensor dg = at::empty({d.rows, d.I}, xn.options().requires_grad(false)), dup = at::empty_like(dg);
+    Tensor dxn;  // of the normalised input
+    if (gated) {
+      if (needs(0) || needs(3)) dxn = at::empty_like(xn);
+      Tensor dwg, dwu;
+      if (needs(10) || needs(11)) {
+        dwg = at::empty_like(wg);
+        dwu = at::empty_like(wu);
+      }
+      const auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      const Tensor word = status_word(status, x);
+      check(api.gated_linear_bwd(dact.const_data_ptr(), d.I, g.const_data_ptr(), xn.const_data_ptr(), d.E, wg.const_data_ptr(), wu.const_data_ptr(),
+                                 dg.data_ptr(), dup.data_ptr(), ptr(dxn), ptr(dwg), ptr(dwu), d.rows, (int32_t)d.E, (int32_t)d.I, word_of(word),
+                                 stream_of(x)), "mvpa_gated_linear_bwd");
+      look_at(word, x, "mvpa_gated_linear_bwd kernel");
+      if (needs(10)) grad[10] = dwg;
+      if (needs(11)) grad[11] = dwu;
+    } else {
+      check(api.silu_mul_bwd(g.const_data_ptr(), up.const_data_ptr(), g.stride(0), dact.const_data_ptr(), dact.stride(0), dg.data_ptr(),
+                             dup.data_ptr(), g.size(1), d.rows, (int32_t)g.size(1), dt, stream_of(x)), "mvpa_silu_mul_bwd");
+    }
     const Tensor d_o = at::mm(dh2, wc), dq = at::empty_like(q), dkv = at::empty_like(kv);
     const auto q4 = [&](const Tensor& t) { return columns(t, 0, d.N, d.D); };
     const auto v4 = [&](const Tensor& t) { return columns(t, d.KV, d.N, d.D); };
@@ -472,13 +515,18 @@ PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     keys(3 * d.KV + d.T * d.KV, d.C, chan, 2, wchan, 7);
     weight(4, dq, xn);
     weight(5, dkv, xn);
-    weight(10, dg, xn);
-    weight(11, dup, xn);
+    if (!gated) {
+      weight(10, dg, xn);
+      weight(11, dup, xn);
+    }
     if (needs(0) || needs(3)) {
-      Tensor dxn = at::mm(dq, wq);
+      if (gated) dxn.addmm_(dq, wq);
+      else dxn = at::mm(dq, wq);
       dxn.addmm_(dkv, wkv);
-      dxn.addmm_(dg, wg);
-      dxn.addmm_(dup, wu);
+      if (!gated) {
+        dxn.addmm_(dg, wg);
+        dxn.addmm_(dup, wu);
+      }
       grad[0] = at::empty(x.sizes(), x.options().requires_grad(false));
       grad[3] = at::empty_like(ln_w);
       const size_t bytes = api.rmsnorm_bwd_bytes(d.rows, (int32_t)d.E);
@@ -491,12 +539,12 @@ PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// branches(x, w_in, w_out, bias, r_time, r_chan, window, B, T, C, H, Hkv, D, status): MLP(x) + Attn(x) of the fused inference block
-//   (`MVPFormerBlock.fused_branches`), or None
+// branches(x, w_in, w_out, bias, r_time, r_chan, window, B, T, C, H, Hkv, D, status[, gated]): MLP(x) + Attn(x) of the fused inference block
+//   (`MVPFormerBlock.fused_branches`), or None.  `gated` (bf16): the gate's projections and the gate as one kernel.
 PyObject* branches(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 14)) return nullptr;
-  const bool status = a[13] == Py_True;
+  if (n != 14 && !arguments(n, 15)) return nullptr;
+  const bool status = a[13] == Py_True, gated = n > 14 && a[14] == Py_True;
   Tensor in[6];
   for (int i = 0; i < 6; ++i) {
     if (!THPVariable_CheckExact(a[i])) Py_RETURN_NONE;
@@ -524,15 +572,23 @@ PyObject* branches(PyObject*, PyObject* const* a, Py_ssize_t n) {
     pybind11::gil_scoped_release nogil;
     c10::cuda::CUDAGuard guard(x.device());
     c10::NoGradGuard no_grad;
-    const Tensor big = at::linear(x, w_in);  // (rows, E + 2 KV + 2 I)
+    const int64_t g0 = d.E + 2 * d.KV;
+    const bool one = gated && dt == MVPA_BF16 && d.E % 8 == 0 && I % 8 == 0 && !at::autocast::is_autocast_enabled(at::kCUDA);
+    const Tensor big = at::linear(x, one ? w_in.narrow(0, 0, g0) : w_in);  // (rows, E + 2 KV (+ 2 I))
     if (big.scalar_type() == x.scalar_type()) {  // (autocast may have formed it in another type: Python's path follows that)
       const Tensor cat = at::empty({d.rows, d.E + I}, x.options().requires_grad(false));
       launch_fwd(d.problem(dt, 1.0 / std::sqrt((double)d.D), (int)v[0]), columns(big, 0, d.N, d.D), columns(big, d.E, d.N, d.D),
                  columns(big, d.E + d.KV, d.N, d.D), part(bias, 0), part(bias, d.KV), part(bias, 2 * d.KV), rt, rc,
                  columns(cat, 0, d.N, d.D), nullptr, status);
-      const int64_t g0 = d.E + 2 * d.KV;
-      check(api.silu_mul(part(big, g0), part(big, g0 + I), big.stride(0), const_cast<char*>(part(cat, d.E)), cat.stride(0), d.rows, (int32_t)I,
-                         dt, stream_of(x)), "mvpa_silu_mul");
+      if (one) {
+        const Tensor word = status_word(status, x);
+        check(api.gated_linear(x.const_data_ptr(), d.E, part(w_in, g0 * d.E), part(w_in, (g0 + I) * d.E), const_cast<char*>(part(cat, d.E)),
+                               cat.stride(0), nullptr, d.rows, (int32_t)d.E, (int32_t)I, word_of(word), stream_of(x)), "mvpa_gated_linear");
+        look_at(word, x, "mvpa_gated_linear kernel");
+      } else {
+        check(api.silu_mul(part(big, g0), part(big, g0 + I), big.stride(0), const_cast<char*>(part(cat, d.E)), cat.stride(0), d.rows, (int32_t)I,
+                           dt, stream_of(x)), "mvpa_silu_mul");
+      }
       out = at::linear(cat, w_out);
     }
   }
@@ -786,17 +842,13 @@ struct Gated {
     sizes.back() = width;
     return at::empty(sizes, x.options().requires_grad(false));
   }
-  Tensor word(bool status) const { return status ? at::zeros({64}, x.options().dtype(at::kInt).requires_grad(false)) : Tensor(); }
-  void look_at(const Tensor& w, const char* what) const {  // synchronises the stream
-    if (w.defined()) check(api.fwd_status(w.data_ptr(), 256, stream_of(x)), what);
-  }
   Tensor forward(Tensor* saved, bool status) const {
     Tensor h = like_x(I);
     if (saved) *saved = scratch(api.gated_saved_bytes(rows, (int32_t)I), x);
-    const Tensor w = word(status);
+    const Tensor w = status_word(status, x);
     check(api.gated_linear(x.const_data_ptr(), E, wg.const_data_ptr(), wu.const_data_ptr(), h.data_ptr(), I, saved ? saved->data_ptr() : nullptr,
-                           rows, (int32_t)E, (int32_t)I, w.defined() ? w.data_ptr<int32_t>() : nullptr, stream_of(x)), "mvpa_gated_linear");
-    look_at(w, "mvpa_gated_linear kernel");
+                           rows, (int32_t)E, (int32_t)I, word_of(w), stream_of(x)), "mvpa_gated_linear");
+    look_at(w, x, "mvpa_gated_linear kernel");
     return h;
   }
 };
@@ -851,7 +903,7 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     const Body body(g.x);
     const Tensor d = dh.is_contiguous() && aligned16(dh.const_data_ptr()) ? dh : dh.clone(at::MemoryFormat::Contiguous);
-    const Tensor dg = at::empty({2, g.rows, g.I}, g.x.options().requires_grad(false)), w = g.word(a[6] == Py_True);
+    const Tensor dg = at::empty({2, g.rows, g.I}, g.x.options().requires_grad(false)), w = status_word(a[6] == Py_True, g.x);
     if (need & 1) grad[0] = g.like_x(g.E);
     Tensor dwg, dwu;
     if (need & 6) {
@@ -861,9 +913,9 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
     check(api.gated_linear_bwd(d.const_data_ptr(), g.I, saved.const_data_ptr(), g.x.const_data_ptr(), g.E, g.wg.const_data_ptr(),
                                g.wu.const_data_ptr(), dg.data_ptr(), const_cast<char*>(part(dg, g.rows * g.I)), ptr(grad[0]), ptr(dwg), ptr(dwu),
-                               g.rows, (int32_t)g.E, (int32_t)g.I, w.defined() ? w.data_ptr<int32_t>() : nullptr, stream_of(g.x)),
+                               g.rows, (int32_t)g.E, (int32_t)g.I, word_of(w), stream_of(g.x)),
           "mvpa_gated_linear_bwd");
-    g.look_at(w, "mvpa_gated_linear_bwd kernel");
+    look_at(w, g.x, "mvpa_gated_linear_bwd kernel");
     if (need & 2) grad[1] = std::move(dwg);
     if (need & 4) grad[2] = std::move(dwu);
   }
@@ -1003,6 +1055,62 @@ PyObject* matmul_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// branches_int4(x, then (q, scales, zeros or None) of q k v, gate, up and the output, bias, r_time, r_chan, window, B, T, C, H, Hkv, D, group,
+//   status): the fused inference block with its weights in 4 bits (`MVPFormerBlock.fused_branches_int4`), or None
+PyObject* branches_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 25)) return nullptr;
+  const bool status = a[24] == Py_True;
+  Tensor x, bias, rt, rc;
+  Int4 w[4];  // q k v, gate, up, out
+  int64_t group, v[7];
+  if (a[0] == Py_None || a[13] == Py_None || a[14] == Py_None || a[15] == Py_None || !take(a[0], x) || !take(a[13], bias) || !take(a[14], rt) ||
+      !take(a[15], rc) || !group_of(a[23], &group))
+    Py_RETURN_NONE;
+  for (int i = 0; i < 4; ++i)
+    if (!w[i].take(a + 1 + 3 * i) || !fp8_inputs({&x, &w[i].q, &w[i].scales, &w[i].zeros})) Py_RETURN_NONE;
+  if (!fp8_inputs({&x, &bias, &rt, &rc}) || !bf16_or_fp32(x) || x.dim() != 2 || x.numel() == 0 || !x.is_contiguous()) Py_RETURN_NONE;
+  for (int i = 0; i < 7; ++i) v[i] = PyLong_AsLongLong(a[16 + i]);
+  if (PyErr_Occurred()) return nullptr;
+  Dims d;
+  d.B = v[1]; d.T = v[2]; d.C = v[3]; d.H = v[4]; d.Hkv = v[5]; d.D = v[6];
+  d.N = d.T * d.C; d.KV = d.Hkv * d.D; d.rows = d.B * d.N; d.E = d.H * d.D;
+  const int64_t I = w[1].q.dim() == 2 ? w[1].q.size(0) : 0, es = x.element_size(), K = d.E + I, Q = d.E + 2 * d.KV;
+  if (I <= 0 || d.KV <= 0 || d.rows <= 0 || x.size(0) != d.rows || x.size(1) != d.E || K > INT32_MAX - 1024 || !w[0].fits(Q, d.E, group) ||
+      !w[1].fits(I, d.E, group) || !w[2].fits(I, d.E, group) || !w[3].fits(d.E, K, group) || bias.numel() != 3 * d.KV || d.D * es % 16 != 0 ||
+      Q * es % 16 != 0 || rt.numel() != d.T * d.KV || rc.numel() != d.C * d.KV || rt.dim() < 2 || rc.dim() < 2 ||
+      rt.size(-2) != d.T || rc.size(-2) != d.C || w[2].scales.scalar_type() != w[1].scales.scalar_type())
+    Py_RETURN_NONE;
+  for (const Tensor* t : {&bias, &rt, &rc})
+    if (!t->is_contiguous() || t->scalar_type() != x.scalar_type() || !aligned16(t->const_data_ptr())) Py_RETURN_NONE;
+  Tensor out;
+  {
+    const Body body(x);
+    const int dt = dtype_code(x);
+    const Tensor word = status_word(status, x);
+    const auto product = [&](const Tensor& a, const Int4& w, const Int4* up, void* to, int64_t ld) {
+      const int64_t K = a.size(1);
+      const size_t bytes = api.int4_workspace_bytes(a.const_data_ptr(), a.stride(0), d.rows, (int32_t)K, dt);
+      const Tensor ws = bytes ? fresh({(int64_t)bytes}, {1}, at::kByte, x) : Tensor();
+      check(api.matmul_int4(a.const_data_ptr(), a.stride(0), &w.c, up ? &up->c : nullptr, dtype_code(w.scales), to, ld, d.rows,
+                            (int32_t)w.q.size(0), (int32_t)K, (int32_t)group, dt, bytes ? ws.data_ptr() : nullptr, bytes, word_of(word),
+                            stream_of(x)), "mvpa_matmul_int4");
+    };
+    const int64_t ld = (K + 7) / 8 * 8;  // (the attention writes 16-byte aligned rows)
+    const Tensor big = fresh({d.rows, Q}, {Q, 1}, x.scalar_type(), x), cat = fresh({d.rows, K}, {ld, 1}, x.scalar_type(), x);
+    product(x, w[0], nullptr, big.data_ptr(), Q);
+    launch_fwd(d.problem(dt, 1.0 / std::sqrt((double)d.D), (int)v[0]), columns(big, 0, d.N, d.D), columns(big, d.E, d.N, d.D),
+               columns(big, d.E + d.KV, d.N, d.D), part(bias, 0), part(bias, d.KV), part(bias, 2 * d.KV), rt, rc, columns(cat, 0, d.N, d.D),
+               nullptr, status);
+    product(x, w[1], &w[2], const_cast<char*>(part(cat, d.E)), ld);
+    out = fresh({d.rows, d.E}, {d.E, 1}, x.scalar_type(), x);
+    product(cat, w[3], nullptr, out.data_ptr(), d.E);
+    look_at(word, x, "mvpa_matmul_int4 kernel");
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // init(path of libmvpa_b200.so, which is already loaded; the class of the mode that a default device is)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 2)) return nullptr;
@@ -1038,7 +1146,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {FAST(init), FAST(attend), FAST(forward), FAST(backward), FAST(plain), FAST(block_forward),
                          FAST(block_backward), FAST(branches), FAST(quantize_fp8), FAST(rmsnorm_fp8), FAST(silu_mul_fp8),
                          FAST(matmul_fp8), FAST(branches_fp8), FAST(gated_linear), FAST(gated_forward), FAST(gated_backward),
-                         FAST(quantize_int4), FAST(dequantize_int4), FAST(matmul_int4), {nullptr, nullptr, 0, nullptr}};
+                         FAST(quantize_int4), FAST(dequantize_int4), FAST(matmul_int4), FAST(branches_int4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "mvpa_host_b200", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -22,7 +22,7 @@ from attentions import flashmvpa
 WINDOW = 10
 
 
-def expression(x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, eps, heads):
+def expression(x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, eps, heads, gated=False):
     """The block in differentiable operations (what a graph of the gradient is built from)."""
     H, Hkv, D = heads
     B, T, C, E = x.shape
@@ -34,7 +34,8 @@ def expression(x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, e
     rc = F.linear(chan, wchan).view(1, C, Hkv, D).permute(0, 2, 1, 3)
     u, vt, z = (b.view(1, Hkv, 1, D) for b in bias.clone().split(KV))    # (what a saved-tensor hook brought back may lie anywhere)
     o = flashmvpa(q, u, vt, z, k, rt, rc, v, causal=True, sm_scale=1.0 / (D ** 0.5), window_size=WINDOW)
-    mlp = F.linear(mvpa_ops.swiglu(F.linear(xn, wg), F.linear(xn, wu)), wd)
+    act = mvpa_ops.gated_linear(xn, wg, wu) if gated else mvpa_ops.swiglu(F.linear(xn, wg), F.linear(xn, wu))
+    mlp = F.linear(act, wd)
     return x + mlp + F.linear(o.permute(0, 2, 1, 3).reshape(B, T, C, H * D), wc)
 
 
@@ -53,13 +54,13 @@ class BlockFunction(torch.autograd.Function):
     """Forward and backward are one native call each (`csrc_host/mvpa_host.cpp`: block_forward, block_backward)."""
 
     @staticmethod
-    def forward(ctx, x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, eps, heads):
+    def forward(ctx, x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd, eps, heads, gated):
         given = (x, pos, chan, ln_w, wq, wkv, wpos, wchan, bias, wc, wg, wu, wd)
-        got = _host.module().block_forward(*given, eps, WINDOW, *heads, _attn._CHECK_STATUS)
+        got = _host.module().block_forward(*given, eps, WINDOW, *heads, _attn._CHECK_STATUS, gated)
         if got is None:
             raise RuntimeError("block: tensors that the kernels cannot take in place")   # (`applies` has looked at them)
-        ctx.save_for_backward(*given, *got[1:])      # ... xn, q, kv, g, up, rt, rc, o, lse, act
-        ctx.eps, ctx.heads = eps, heads
+        ctx.save_for_backward(*given, *got[1:])      # ... xn, q, kv, g, up, rt, rc, o, lse, act (gated: what its backward wants, None for g, up)
+        ctx.eps, ctx.heads, ctx.gated = eps, heads, gated
         return got[0]
 
     @staticmethod
@@ -68,13 +69,14 @@ class BlockFunction(torch.autograd.Function):
         need = ctx.needs_input_grad[:13]
         if not torch.is_grad_enabled() and _nat.untraced() and mvpa_ops._plain(dh.contiguous()):
             mask = sum(n << i for i, n in enumerate(need))
-            grads = _host.module().block_backward(dh, *saved, mask, ctx.eps, WINDOW, *ctx.heads, _attn._CHECK_STATUS)
+            grads = _host.module().block_backward(dh, *saved, mask, ctx.eps, WINDOW, *ctx.heads, _attn._CHECK_STATUS,
+                                                  ctx.gated)
             if grads is not None:
-                return (*grads, None, None)
+                return (*grads, None, None, None)
         # a graph of the gradient is wanted (or a transform is active): through the differentiable operations, in the forward's types
         with torch.autocast("cuda", enabled=False):
-            grads = through_expression(lambda *ins: expression(*ins, ctx.eps, ctx.heads), saved[:13], need, dh)
-        return (*grads, None, None)
+            grads = through_expression(lambda *ins: expression(*ins, ctx.eps, ctx.heads, ctx.gated), saved[:13], need, dh)
+        return (*grads, None, None, None)
 
 
 def shipped(cls):
@@ -133,4 +135,5 @@ def run(block, x, pos, chan):
     a, m = block.attn, block.mlp
     return BlockFunction.apply(x, pos, chan, block.ln_1.weight, a.q_attn.weight, a.c_attn.weight, a.position_net.weight,
                                a.channel_net.weight, a.attn_bias, a.c_proj.weight, m.gate_proj.weight, m.up_proj.weight,
-                               m.down_proj.weight, block.ln_1.eps, (a.num_heads, a.num_kv_heads, a.head_dim))
+                               m.down_proj.weight, block.ln_1.eps, (a.num_heads, a.num_kv_heads, a.head_dim),
+                               bool(m.fused_gate) and x.dtype == torch.bfloat16)

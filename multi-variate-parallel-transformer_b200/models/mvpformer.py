@@ -17,6 +17,9 @@ h = x + MLP(ln_1 x) + Attn(ln_1 x)) built for B200:
   * the relative keys of all layers (`position_net`, `channel_net` of the embeddings, which do not depend
     on the input) come from one GEMM each per forward.
 
+`MVPFormerModel.enable_fused_gate()` forms the gate and both its projections in one kernel (`mvpa_ops.gated_linear`), in training too;
+`enable_int4()` keeps the blocks' weights in 4 bits (`mvpa_ops.matmul_int4`, `gated_linear_int4`).
+
 `MVPFormerModel.enable_fp8()` runs both projections of every block in 8 bits (e4m3, a scale for each block of 128): the norm
 and the gate write their results in 8 bits, and `mvpa_ops.matmul_fp8` takes the place of the two GEMMs.
 
@@ -99,9 +102,17 @@ def _gate(gate, up):
     return F.silu(gate) * up
 
 
+def _plain_linear(m):
+    """A projection that nothing has replaced, hooked or wrapped: its weight is all there is to it."""
+    return block_grad._unhooked(m, block_grad._LINEAR) and m.bias is None
+
+
 class LlamaMLP(torch.nn.Module):
     """SwiGLU MLP with the parameter names of `transformers`' `LlamaMLP`, which the reference block uses
-    (`models/mvpformer.py:34, 114`): down_proj(silu(gate_proj(x)) * up_proj(x)), no biases."""
+    (`models/mvpformer.py:34, 114`): down_proj(silu(gate_proj(x)) * up_proj(x)), no biases.  `fused_gate`: what comes before the
+    down projection by `mvpa_ops.gated_linear`, with fewer roundings on the way (`MVPFormerModel.enable_fused_gate`)."""
+
+    fused_gate = False     # (of the class: modules pickled before have none of their own)
 
     def __init__(self, config):
         super().__init__()
@@ -110,6 +121,9 @@ class LlamaMLP(torch.nn.Module):
         self.down_proj = torch.nn.Linear(config.intermediate_size, config.hidden_size, bias=False)
 
     def forward(self, x):
+        if not torch.jit.is_scripting():
+            if self.fused_gate and _plain_linear(self.gate_proj) and _plain_linear(self.up_proj):
+                return self.down_proj(mvpa_ops.gated_linear(x, self.gate_proj.weight, self.up_proj.weight))
         gate, up = self.gate_proj(x), self.up_proj(x)
         if torch.jit.is_scripting():
             act = F.silu(gate) * up
@@ -122,7 +136,8 @@ _SHIPPED = tuple(block_grad.shipped(cls) for cls in (RMSNorm, MVPFormerGQAFlashA
 
 
 class MVPFormerBlock(Prepares, torch.nn.Module):
-    _prepared = ("_fused", "_fused_fp8")
+    _prepared = ("_fused", "_fused_fp8", "_fused_int4")
+    _fused_int4 = None     # (of the class: blocks pickled before have none of their own)
 
     def __init__(self, config, layer_idx=None):
         super().__init__()
@@ -130,7 +145,7 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         self.attn = MVPFormerGQAFlashAttention(config, layer_idx=layer_idx)
         self.ln_2 = RMSNorm(config.hidden_size, eps=config.layer_norm_epsilon)   # unused, as in the reference
         self.mlp = LlamaMLP(config)
-        self._fused = self._fused_fp8 = None
+        self._fused = self._fused_fp8 = self._fused_int4 = None
 
     def forward(self, hidden_states, positional_embedding, channel_embedding, layer_past=None, attention_mask=None,
                 head_mask=None, encoder_hidden_states=None, encoder_attention_mask=None, use_cache=False,
@@ -172,6 +187,45 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         made = prepared(self, "_fused_fp8", tag, in_8_bits)
         return made[:2], made[2:]
 
+    def fused_weights_int4(self, group, zeros):
+        """[q | k | v], gate, up and [c_proj | down_proj] in 4 bits, each (q, scales, zeros or None), quantised once per weight version."""
+        ws, tag = self._projections()
+
+        def in_4_bits():
+            w_in, w_out = self._concatenated(ws)
+            n = ws[0].shape[0] + ws[1].shape[0]
+            parts = (w_in[:n], w_in[n:n + ws[2].shape[0]], w_in[n + ws[2].shape[0]:], w_out)
+            return tuple(t for w in parts for t in mvpa_ops.quantize_int4(w, group, zeros))
+
+        made = prepared(self, "_fused_int4", (*tag, group, zeros), in_4_bits)
+        each = len(made) // 4
+        return [(*made[i:i + each], None)[:3] for i in range(0, len(made), each)]
+
+    @torch.no_grad()
+    def fused_branches_int4(self, x, r_time, r_chan, B, T, C, group, zeros):
+        """`fused_branches` with all weights in 4 bits: q, k and v from one product, the gate from another that forms both its projections
+        and writes beside the attention's output, where the output projection reads."""
+        a = self.attn
+        E, H, Hkv, D = a.embed_dim, a.num_heads, a.num_kv_heads, a.head_dim
+        N, KV, rows = T * C, Hkv * D, B * T * C
+        w_qkv, w_gate, w_up, w_out = self.fused_weights_int4(group, zeros)
+        r_time, r_chan = r_time.to(x.dtype), r_chan.to(x.dtype)
+        bias = a.attn_bias.detach().to(x.dtype)
+        if mvpa_host.usable(x):
+            out = mvpa_host.module().branches_int4(x, *w_qkv, *w_gate, *w_up, *w_out, bias, r_time, r_chan, 10, B, T, C, H, Hkv, D, group,
+                                                   attn_mod._CHECK_STATUS)
+            if out is not None:
+                return out
+        big = mvpa_ops.matmul_int4(x, *w_qkv, group=group)               # (rows, E + 2 KV)
+        head = lambda c, heads: big[:, c:c + heads * D].view(B, N, heads, D).permute(0, 2, 1, 3)
+        wide = E + w_gate[0].shape[0]
+        cat = torch.empty((rows, (wide + 7) // 8 * 8), dtype=x.dtype, device=x.device)[:, :wide]     # (the attention writes 16-byte aligned rows)
+        u, vt, z = (b.view(Hkv, D) for b in bias.split(KV))
+        flash_mvpa_into(cat[:, :E].view(B, N, H, D).permute(0, 2, 1, 3), head(0, H), u, vt, z, head(E, Hkv), r_time, r_chan, head(E + KV, Hkv),
+                        1.0 / (D ** 0.5), 10)
+        mvpa_ops.gated_linear_int4(x, w_gate, w_up, group=group, out=cat[:, E:])
+        return mvpa_ops.matmul_int4(cat, *w_out, group=group)
+
     @torch.no_grad()
     def fused_branches_fp8(self, pair, r_time, r_chan, B, T, C, dtype):
         """`fused_branches` on the block's normalised input in 8 bits (`mvpa_ops.rmsnorm_fp8`), with both projections in 8
@@ -211,10 +265,14 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         w_in, w_out = self.fused_weights()
         if mvpa_host.usable(x):
             out = mvpa_host.module().branches(x, w_in, w_out, a.attn_bias.detach().to(x.dtype), r_time, r_chan, 10, B, T, C, H, Hkv, D,
-                                              attn_mod._CHECK_STATUS)
+                                              attn_mod._CHECK_STATUS, bool(self.mlp.fused_gate))
             if out is not None:
                 return out
-        big = F.linear(x, w_in)                                          # (M, E + 2 KV + 2 I); under autocast in its type
+        g0 = E + 2 * KV
+        # (what cannot be one kernel, a type that autocast chooses among it, is as without the flag)
+        gated = (self.mlp.fused_gate and x.dtype == torch.bfloat16 and E % 8 == 0 and I % 8 == 0 and not torch.is_autocast_enabled("cuda")
+                 and x.is_contiguous() and x.data_ptr() % 16 == 0)
+        big = F.linear(x, w_in[:g0] if gated else w_in)                  # (M, E + 2 KV (+ 2 I)); under autocast in its type
         q4 = big[:, :E].view(B, N, H, D).permute(0, 2, 1, 3)
         k4 = big[:, E:E + KV].view(B, N, Hkv, D).permute(0, 2, 1, 3)
         v4 = big[:, E + KV:E + 2 * KV].view(B, N, Hkv, D).permute(0, 2, 1, 3)
@@ -222,8 +280,10 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         u, vt, z = (b.view(Hkv, D).to(big.dtype) for b in a.attn_bias.detach().split(KV))
         flash_mvpa_into(cat[:, :E].view(B, N, H, D).permute(0, 2, 1, 3), q4, u, vt, z, k4, r_time.to(big.dtype),
                         r_chan.to(big.dtype), v4, 1.0 / (D ** 0.5), 10)
-        g0 = E + 2 * KV
-        mvpa_ops.silu_mul(big[:, g0:g0 + I], big[:, g0 + I:g0 + 2 * I], cat[:, E:])
+        if gated:
+            mvpa_ops.gated_linear_into(cat[:, E:], x, w_in[g0:g0 + I], w_in[g0 + I:])
+        else:
+            mvpa_ops.silu_mul(big[:, g0:g0 + I], big[:, g0 + I:g0 + 2 * I], cat[:, E:])
         return F.linear(cat, w_out)
 
     @torch.no_grad()
@@ -265,6 +325,7 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
 class MVPFormerModel(Prepares, torch.nn.Module):
     _prepared = ("_rel",)
     _fp8 = False           # (of the class: modules pickled before there was an 8-bit path have none of their own)
+    _int4 = None           # (group, zeros) where the blocks' weights are in 4 bits
 
     def __init__(self, config, gradient_checkpointing=False):
         super().__init__()
@@ -338,6 +399,8 @@ class MVPFormerModel(Prepares, torch.nn.Module):
         the result is the graph's own buffer, overwritten by the next call."""
         if self._fp8:
             raise NotImplementedError("forward_time_sharded does not run in 8 bits: call enable_fp8(False) first")
+        if self._int4:
+            raise NotImplementedError("forward_time_sharded does not run in 4 bits: call enable_int4(False) first")
         if graph and transport == "p2p":
             key = ("sharded", tuple(embeds_local.shape), embeds_local.dtype, embeds_local.device.index, T, C, id(group))
             entry = self._graphs.get(key)
@@ -412,12 +475,39 @@ class MVPFormerModel(Prepares, torch.nn.Module):
         if flag and self.embed_dim % mvpa_ops.FP8_BLOCK:
             raise ValueError(f"enable_fp8: hidden_size must be a multiple of {mvpa_ops.FP8_BLOCK}, got {self.embed_dim}")
         self._fp8 = bool(flag)
+        if flag:
+            self._int4 = None
+        self._graphs = {}
+        return self
+
+    def enable_int4(self, flag: bool = True, group: int = 128, zeros: bool = False):
+        """Inference with the blocks' weights in 4 bits, with a scale (and, if asked for, a zero) for each group of 32, 64 or 128 neighbours
+        of a row (`mvpa_ops.quantize_int4`); activations, norms, attention and the residual stream as without.  A quarter of the weights'
+        memory, and of the bytes that a step of a few tokens is bound by.  No weight is rounded further in the products; the step to 4
+        bits itself is a relative rounding of up to a fourteenth of a group's largest weight.  Weights are quantised on first use, and
+        again after they change (as autograd counts changes: one made through `.data` goes unseen); those in 16 or 32 bits stay where they
+        are.  Concerns the fused forward alone (no gradients, eval mode) and not `forward_time_sharded`.  Autocast has no effect on these
+        products.  Takes the place of `enable_fp8`; captured graphs are dropped."""
+        if group not in mvpa_ops.INT4_GROUPS:
+            raise ValueError(f"enable_int4: group is 32, 64 or 128, got {group}")
+        self._int4 = (int(group), bool(zeros)) if flag else None
+        if flag:
+            self._fp8 = False
+        self._graphs = {}
+        return self
+
+    def enable_fused_gate(self, flag: bool = True):
+        """The blocks' gate and up projections, the activation and their product as one kernel (`mvpa_ops.gated_linear`), in training and in the
+        fused forward.  bf16; other types are not changed.  Results differ by roundings: the gate is formed in fp32 from the projections'
+        sums to its result and rounded once, where it is rounded four times without.  Captured graphs are dropped."""
+        for block in self.h:
+            block.mlp.fused_gate = bool(flag)
         self._graphs = {}
         return self
 
     def _kept(self):
         """The prepared weights as they are now."""
-        return [self._rel] + [(b._fused_fp8 if self._fp8 else b._fused) for b in self.h]
+        return [self._rel] + [(b._fused_fp8 if self._fp8 else b._fused_int4 if self._int4 else b._fused) for b in self.h]
 
     def reset_cuda_graphs(self):
         self._graphs = {}
@@ -473,7 +563,10 @@ class MVPFormerModel(Prepares, torch.nn.Module):
                 branches = block.fused_branches_fp8(pair, r_time[i], r_chan[i], B, T, C, h.dtype)
                 continue
             x = mvpa_ops.rmsnorm(h, w, block.ln_1.eps, add=branches, sum_out=sum_out)
-            branches = block.fused_branches(x, r_time[i], r_chan[i], B, T, C)
+            if self._int4:
+                branches = block.fused_branches_int4(x, r_time[i], r_chan[i], B, T, C, *self._int4)
+            else:
+                branches = block.fused_branches(x, r_time[i], r_chan[i], B, T, C)
         return mvpa_ops.rmsnorm(h, self.ln_f.weight.detach().to(h.dtype), self.ln_f.eps, add=branches, sum_out=h)
 
 

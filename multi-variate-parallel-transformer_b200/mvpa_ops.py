@@ -1,9 +1,11 @@
 """Torch-tensor front ends of the C-ABI kernels that surround the attention in an MVPFormer block,
 its encoder and its heads (``include/mvpa.h``: mvpa_rmsnorm, mvpa_silu_mul, mvpa_wave_encode,
-mvpa_channel_mean, mvpa_contrastive_logits, the backwards mvpa_rmsnorm_bwd, mvpa_silu_mul_bwd, and the
-block in 8 bits: mvpa_quantize_fp8, mvpa_rmsnorm_fp8, mvpa_silu_mul_fp8, mvpa_matmul_fp8).
-`rmsnorm_train` and `swiglu` are differentiable and take any tensor (torch expressions serve what the
-kernels do not); the others are forward only, CUDA tensors, bf16 or fp32 (and their pairs in 8 bits).
+mvpa_channel_mean, mvpa_contrastive_logits, the backwards mvpa_rmsnorm_bwd, mvpa_silu_mul_bwd, the gated
+projection mvpa_gated_linear(_bwd), the block in 8 bits: mvpa_quantize_fp8, mvpa_rmsnorm_fp8,
+mvpa_silu_mul_fp8, mvpa_matmul_fp8, and weights in 4 bits: mvpa_quantize_int4, mvpa_dequantize_int4,
+mvpa_matmul_int4).  `rmsnorm_train`, `swiglu` and `gated_linear` are differentiable and take any tensor
+(torch expressions serve what the kernels do not); the others are forward only, CUDA tensors, bf16 or
+fp32 (and their pairs in 8 or 4 bits).
 """
 from __future__ import annotations
 
@@ -277,6 +279,29 @@ def gated_linear(x, w_gate, w_up):
         if _plain(x, w_gate, w_up):
             return _GatedLinear.apply(x, w_gate, w_up)
     return swiglu(torch.nn.functional.linear(x, w_gate), torch.nn.functional.linear(x, w_up))
+
+
+def gated_linear_into(out, x, w_gate, w_up):
+    """Inference form of `gated_linear`: no autograd record, and the result goes into `out` (rows, I), which may be a column block of a
+    wider buffer.  x (rows, E) and weights (I, E) in bf16 with E and I multiples of 8, contiguous; rows on 16-byte boundaries."""
+    _fp8_inputs("gated_linear_into", x, w_gate, w_up, out)
+    if not (x.dtype == w_gate.dtype == w_up.dtype == out.dtype == torch.bfloat16):
+        raise RuntimeError(f"gated_linear_into: tensors are bfloat16, got {x.dtype}, {w_gate.dtype}, {w_up.dtype}, {out.dtype}")
+    if (x.dim() != 2 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[1] or out.shape != (x.shape[0], w_gate.shape[0])
+            or not (x.is_contiguous() and w_gate.is_contiguous() and w_up.is_contiguous())):
+        raise RuntimeError("gated_linear_into: shapes do not go together, or x or a weight is not contiguous: "
+                           + ", ".join(str(tuple(t.shape)) for t in (out, x, w_gate, w_up)))
+    (rows, E), I = x.shape, w_gate.shape[0]
+    ld = _fp8_rows("gated_linear_into", out, "out")
+    if rows == 0:
+        return out
+    with _nat.on_device(x.device):
+        status = _status_word(x.device)
+        st = _nat.lib().mvpa_gated_linear(x.data_ptr(), E, w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), ld, None, rows, E, I,
+                                          None if status is None else status.data_ptr(), _stream(x))
+        _nat.check(st, "mvpa_gated_linear")
+        _look_at(status, "mvpa_gated_linear", x)
+    return out
 
 
 @functools.lru_cache(maxsize=None)
