@@ -45,10 +45,13 @@ constexpr size_t kGatedSmem = 1024 + kGatedStages * kGatedStageBytes + kGatedOut
 
 enum : int { kGiveUpEmpty = 81, kGiveUpFull = 82, kGiveUpTmemEmpty = 83, kGiveUpTmemFull = 84, kGiveUpDrain = 85 };
 
-template <int MODE>
+// TN: columns of sums of a tile (256, 192 or 128; a gate's are half g, half u).
+template <int MODE, int TN>
 __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs g) {
   constexpr bool kGate = MODE <= kForwardSave, kRowsA = MODE == kWeights, kRowsB = MODE >= kInput;  // (rows along M / N: MN-major)
-  constexpr int kTileN = kGate ? 128 : 256;
+  constexpr int kTileN = kGate ? TN / 2 : TN, kHalfN = TN / 2;  // columns of the result; rows (or columns) of the right operand in each CTA
+  constexpr int kBoxes = (kHalfN + 63) / 64;                    // of 64 columns, of an operand whose rows lie along them (192: the last one half used)
+  constexpr int kLoadBytes = 128 * 128 + (kRowsB ? kBoxes * 64 : kHalfN) * 128;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[kGatedStages], s_empty[kGatedStages], s_tfull[2], s_tempty[2];
   __shared__ uint32_t s_tmem;
@@ -102,20 +105,20 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
     for (uint32_t t = pair; t < tiles && on; t += pairs) {
       const Tile at = tile_at<kTileN>(t, g.tiles_n, g.tiles_m);
       const uint32_t part = (uint32_t)at.m0 / 256 >= g.part ? 1 : 0;
-      const int row = left ? at.m0 - (int)(part * g.part * 256) + (int)half * 128 : kGate ? at.n0 : at.n0 + (int)half * 128;
+      const int row = left ? at.m0 - (int)(part * g.part * 256) + (int)half * 128 : kGate ? at.n0 : at.n0 + (int)half * kHalfN;
       for (int kb = 0; kb < blocks; ++kb, ++loads, st.step()) {
         if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
           on = false;
           break;
         }
-        if (left && half == 0 && el) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * kGatedStageBytes);
+        if (left && half == 0 && el) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * kLoadBytes);
         __syncwarp();
         const int seg = kb >= g.blocks ? 1 : 0, k = (kb - seg * g.blocks) * 64;
         const uint32_t to = stages + st.at * kGatedStageBytes + (left ? 0 : 128 * 128), bar = there + 8 * st.at;
         const CUtensorMap* map = left ? &maps.a[kRowsA ? part : seg] : &maps.b[kGate ? half : kRowsA ? 0 : seg];
         if (left ? kRowsA : kRowsB) {
           ptx::tma_load_2d_pair_w(el, to, map, bar, row, k);
-          ptx::tma_load_2d_pair_w(el, to + 64 * 128, map, bar, row + 64, k);
+          if (left || kBoxes == 2) ptx::tma_load_2d_pair_w(el, to + 64 * 128, map, bar, row + 64, k);
         } else {
           ptx::tma_load_2d_pair_w(el, to, map, bar, k, row);
         }
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
   } else if (warp == 1) {
     if (half == 0) {
       const uint32_t el = ptx::elect_one();
-      constexpr uint32_t idesc = ptx::make_idesc_bf16_ab(256, 256, kRowsA, kRowsB);
+      constexpr uint32_t idesc = ptx::make_idesc_bf16_ab(256, TN, kRowsA, kRowsB);
       constexpr uint32_t kStepA = kRowsA ? 128 : 2, kStepB = kRowsB ? 128 : 2;
       const ptx::DescHalves a0 = ptx::make_desc_halves_sw128(stages, kRowsA ? 64 * 128 : 16, 1024),
                             b0 = ptx::make_desc_halves_sw128(stages + 128 * 128, kRowsB ? 64 * 128 : 16, 1024);
@@ -206,6 +209,10 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
         }
       };
       if constexpr (kGate) {
+        if (group * 64 >= kTileN) {  // (no columns for these warps)
+          release();
+          continue;
+        }
         const int x = at.n0 + group * 64;
         const bool inside = y < g.rows && x < g.cols;  // (the same for the whole warp: a store does not begin past the matrix)
         if constexpr (MODE == kForwardSave) {
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
               uint32_t r[32];
-              ptx::tmem_ld32(from + sum * 128 + group * 64 + c, r);
+              ptx::tmem_ld32(from + sum * kHalfN + group * 64 + c, r);
               ptx::tmem_ld_wait();
               uint32_t b[8];
 #pragma unroll
@@ -247,7 +254,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
         for (int c = 0; c < 64; c += 32) {
           uint32_t rg[32], ru[32];
           ptx::tmem_ld32(from + group * 64 + c, rg);
-          ptx::tmem_ld32(from + 128 + group * 64 + c, ru);
+          ptx::tmem_ld32(from + kHalfN + group * 64 + c, ru);
           ptx::tmem_ld_wait();
           if (c == 32) release();
 #pragma unroll
@@ -261,14 +268,14 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
         else if (lane == 0) ptx::tma_store_commit();
       } else {
 #pragma unroll
-        for (int c = 0; c < 256; c += 128) {
-          const int x = at.n0 + c + group * 64;
+        for (int c = group * 64; c < TN; c += 128) {
+          const int x = at.n0 + c;
           const uint32_t to = place();
           uint32_t r0[32], r1[32];
-          ptx::tmem_ld32(from + c + group * 64, r0);
-          ptx::tmem_ld32(from + c + group * 64 + 32, r1);
+          ptx::tmem_ld32(from + c, r0);
+          ptx::tmem_ld32(from + c + 32, r1);
           ptx::tmem_ld_wait();
-          if (c == 128) release();
+          if (c + 128 >= TN) release();
           words(r0, to, 0);
           words(r1, to, 4);
           if (y < g.rows && x < g.cols) send(to, &maps.out[part], x, y);
@@ -347,14 +354,14 @@ int encode(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64
   return encode_bf16_sw128(map, base, 2, dims, strides, box);
 }
 
-template <int MODE>
-int run_gated(const GatedMaps& maps, GatedArgs g, cudaStream_t s) {
+template <int MODE, int TN>
+int launch_gated(const GatedMaps& maps, const GatedArgs& g, cudaStream_t s) {
   const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, pairs = device_sm_count() / 2;
   if (tiles * g.blocks * g.segments > 0x7fffffff) {
-    set_error("mvpa_gated_linear: more than 2^31 blocks of 256 x 256 x 64");
+    set_error("mvpa_gated_linear: more than 2^31 blocks of 256 x %d x 64", TN);
     return MVPA_ERR_UNSUPPORTED;
   }
-  constexpr auto kernel = gated_kernel<MODE>;
+  constexpr auto kernel = gated_kernel<MODE, TN>;
   MVPA_CUDA_CHECK(grant_smem<kernel>(kGatedSmem));
   MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kGatedThreads, kGatedSmem, s, maps, g));
   count_launch();
@@ -362,7 +369,35 @@ int run_gated(const GatedMaps& maps, GatedArgs g, cudaStream_t s) {
   return MVPA_OK;
 }
 
+// The width of the tiles: the one whose rounds over the pairs of multiprocessors take the least.  A block of 64 along the summed axis takes a
+// pair the longer of its products (256 columns 270 ns) and its loads (a multiprocessor takes some 150 bytes in a nanosecond): 270 ns at 256
+// columns, 218 at 192, 164 at 128.
+int tile_width(int64_t tiles_m, int64_t cols, bool gate) {
+  const int64_t pairs = device_sm_count() / 2;
+  constexpr int kWidths[3] = {256, 192, 128}, kTimes[3] = {270, 218, 164};
+  int best = 256;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < 3; ++i) {
+    if (gate && kWidths[i] == 192) continue;  // (96 features: not a whole number of the 64 that a warp takes)
+    const int64_t each = gate ? kWidths[i] / 2 : kWidths[i], tiles = tiles_m * ((cols + each - 1) / each);
+    const int64_t time = (tiles + pairs - 1) / pairs * kTimes[i];
+    if (time < least) {
+      least = time;
+      best = kWidths[i];
+    }
+  }
+  return best;
+}
+
 uint32_t tiles_of(int64_t n, int each) { return (uint32_t)((n + each - 1) / each); }
+
+// The gradients' products (tiles_n is filled in).
+template <int MODE>
+int run_gated(const GatedMaps& maps, GatedArgs g, cudaStream_t s) {
+  const int width = tile_width(g.tiles_m, g.cols, false);
+  g.tiles_n = tiles_of(g.cols, width);
+  return width == 256 ? launch_gated<MODE, 256>(maps, g, s) : width == 192 ? launch_gated<MODE, 192>(maps, g, s) : launch_gated<MODE, 128>(maps, g, s);
+}
 
 int check_sizes(const char* what, int64_t M, int32_t E, int32_t I) {
   constexpr int kMost = 0x7fffffff - 1024;  // (the first place past the last tile is a 32-bit coordinate)
@@ -393,10 +428,12 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
               "their widths");
     return MVPA_ERR_ALIGNMENT;
   }
+  const uint32_t tm = tiles_of(M, 256);
+  const int width = tile_width(tm, I, true);
   GatedMaps maps = {};
   int rc = encode(&maps.a[0], x, M, E, ld_x, 128);
-  if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, 128);
-  if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 128);
+  if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, width / 2);
+  if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, width / 2);
   if (rc == MVPA_OK) rc = encode(&maps.out[0], h, M, I, ld_h, 32);
   if (saved != nullptr) {
     const Saved kept(saved, M, I);
@@ -409,10 +446,10 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
     }
   }
   if (rc != MVPA_OK) return rc;
-  const uint32_t tm = tiles_of(M, 256);
-  const GatedArgs g = {tm, tiles_of(I, 128), tm, (int)tiles_of(E, 64), 1, (int)M, I, status};
+  const GatedArgs g = {tm, tiles_of(I, width / 2), tm, (int)tiles_of(E, 64), 1, (int)M, I, status};
   cudaStream_t s = (cudaStream_t)cuda_stream;
-  return saved != nullptr ? run_gated<kForwardSave>(maps, g, s) : run_gated<kForward>(maps, g, s);
+  if (width == 128) return saved != nullptr ? launch_gated<kForwardSave, 128>(maps, g, s) : launch_gated<kForward, 128>(maps, g, s);
+  return saved != nullptr ? launch_gated<kForwardSave, 256>(maps, g, s) : launch_gated<kForward, 256>(maps, g, s);
 }
 
 extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* saved, const void* x, int64_t ld_x, const void* w_gate,
@@ -443,7 +480,7 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
     if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 64);
     if (rc == MVPA_OK) rc = encode(&maps.out[0], dx, M, E, E, 32);
     const uint32_t tm = tiles_of(M, 256);
-    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, tiles_of(E, 256), tm, (int)tiles_of(I, 64), 2, (int)M, E, status}, s);
+    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, 0, tm, (int)tiles_of(I, 64), 2, (int)M, E, status}, s);
   }
   if (rc == MVPA_OK && dw_gate != nullptr) {
     GatedMaps maps = {};
@@ -453,7 +490,7 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
     if (rc == MVPA_OK) rc = encode(&maps.out[0], dw_gate, I, E, E, 32);
     if (rc == MVPA_OK) rc = encode(&maps.out[1], dw_up, I, E, E, 32);
     const uint32_t tm = tiles_of(I, 256);
-    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, tiles_of(E, 256), tm, (int)tiles_of(M, 64), 1, I, E, status}, s);
+    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, 0, tm, (int)tiles_of(M, 64), 1, I, E, status}, s);
   }
   return rc;
 }
