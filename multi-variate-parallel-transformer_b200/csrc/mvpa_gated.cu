@@ -39,9 +39,17 @@ struct GatedArgs {
 };
 
 constexpr int kGatedThreads = 384;
-constexpr int kGatedStages = 5, kGatedStageBytes = 2 * 128 * 128;
-constexpr int kGatedOutBytes = 8 * 2 * 4096;  // a warp's 32 rows x 64 columns on their way out, twice
-constexpr size_t kGatedSmem = 1024 + kGatedStages * kGatedStageBytes + kGatedOutBytes;
+// As many stages as there is room for: a block is some 2 us on its way from memory through the products and back to an empty stage, so that
+// with five of them a block took 0.4 us instead of 0.27.
+template <int MODE, int TN>
+struct Gated {
+  static constexpr int kHalfN = TN / 2;                // rows (or columns) of the right operand in each CTA
+  static constexpr int kBoxes = (kHalfN + 63) / 64;    // of 64 columns, of an operand whose rows lie along them (192: the last one half used)
+  static constexpr int kBytes = 128 * 128 + (MODE >= kInput ? kBoxes * 64 : kHalfN) * 128;
+  static constexpr int kOutBytes = 8 * 4096;           // a warp's 32 rows x 64 columns on their way out
+  static constexpr int kStages = (225 * 1024 - kOutBytes) / kBytes;
+  static constexpr size_t kSmem = 1024 + kStages * kBytes + kOutBytes;
+};
 
 enum : int { kGiveUpEmpty = 81, kGiveUpFull = 82, kGiveUpTmemEmpty = 83, kGiveUpTmemFull = 84, kGiveUpDrain = 85 };
 
@@ -49,11 +57,10 @@ enum : int { kGiveUpEmpty = 81, kGiveUpFull = 82, kGiveUpTmemEmpty = 83, kGiveUp
 template <int MODE, int TN>
 __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs g) {
   constexpr bool kGate = MODE <= kForwardSave, kRowsA = MODE == kWeights, kRowsB = MODE >= kInput;  // (rows along M / N: MN-major)
-  constexpr int kTileN = kGate ? TN / 2 : TN, kHalfN = TN / 2;  // columns of the result; rows (or columns) of the right operand in each CTA
-  constexpr int kBoxes = (kHalfN + 63) / 64;                    // of 64 columns, of an operand whose rows lie along them (192: the last one half used)
-  constexpr int kLoadBytes = 128 * 128 + (kRowsB ? kBoxes * 64 : kHalfN) * 128;
+  using C = Gated<MODE, TN>;
+  constexpr int kTileN = kGate ? TN / 2 : TN, kHalfN = C::kHalfN;  // (columns of the result)
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_full[kGatedStages], s_empty[kGatedStages], s_tfull[2], s_tempty[2];
+  __shared__ __align__(8) uint64_t s_full[C::kStages], s_empty[C::kStages], s_tfull[2], s_tempty[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;  // a wait ran out: nothing waits any more, and the results are NaN
   const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
@@ -65,7 +72,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
     ptx::prefetch_tensormap(&maps.b[0]);
   } else if (warp == 1) {
     if (lane == 0) {
-      for (int i = 0; i < kGatedStages; ++i) {
+      for (int i = 0; i < C::kStages; ++i) {
         ptx::mbar_init(&s_full[i], 1);
         ptx::mbar_init(&s_empty[i], 1);
       }
@@ -99,7 +106,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
   if (warp == 0 || warp == 2) {  // left operand, right operand: a warp of each CTA loads its CTA's 128 rows (or columns) a block
     const bool left = warp == 0;
     const uint32_t el = ptx::elect_one(), there = ptx::cluster_map(ptx::smem_u32(s_full), 0);
-    Ring<kGatedStages> st;
+    Ring<C::kStages> st;
     uint32_t loads = 0;
     bool on = true;
     for (uint32_t t = pair; t < tiles && on; t += pairs) {
@@ -111,23 +118,23 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
           on = false;
           break;
         }
-        if (left && half == 0 && el) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * kLoadBytes);
+        if (left && half == 0 && el) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * C::kBytes);
         __syncwarp();
         const int seg = kb >= g.blocks ? 1 : 0, k = (kb - seg * g.blocks) * 64;
-        const uint32_t to = stages + st.at * kGatedStageBytes + (left ? 0 : 128 * 128), bar = there + 8 * st.at;
+        const uint32_t to = stages + st.at * C::kBytes + (left ? 0 : 128 * 128), bar = there + 8 * st.at;
         const CUtensorMap* map = left ? &maps.a[kRowsA ? part : seg] : &maps.b[kGate ? half : kRowsA ? 0 : seg];
         if (left ? kRowsA : kRowsB) {
           ptx::tma_load_2d_pair_w(el, to, map, bar, row, k);
-          if (left || kBoxes == 2) ptx::tma_load_2d_pair_w(el, to + 64 * 128, map, bar, row + 64, k);
+          if (left || C::kBoxes == 2) ptx::tma_load_2d_pair_w(el, to + 64 * 128, map, bar, row + 64, k);
         } else {
           ptx::tma_load_2d_pair_w(el, to, map, bar, k, row);
         }
       }
     }
     if (left && half == 0) {  // no copy is in flight when the CTAs end (the other one waits for this one at the end)
-      const uint32_t n = min(loads, (uint32_t)kGatedStages);
+      const uint32_t n = min(loads, (uint32_t)C::kStages);
       for (uint32_t k = loads - n; k != loads; ++k)
-        if (!ptx::mbar_wait(&s_full[k % kGatedStages], (k / kGatedStages) & 1, g.status, kGiveUpDrain)) break;
+        if (!ptx::mbar_wait(&s_full[k % C::kStages], (k / C::kStages) & 1, g.status, kGiveUpDrain)) break;
     }
   } else if (warp == 1) {
     if (half == 0) {
@@ -136,25 +143,32 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
       constexpr uint32_t kStepA = kRowsA ? 128 : 2, kStepB = kRowsB ? 128 : 2;
       const ptx::DescHalves a0 = ptx::make_desc_halves_sw128(stages, kRowsA ? 64 * 128 : 16, 1024),
                             b0 = ptx::make_desc_halves_sw128(stages + 128 * 128, kRowsB ? 64 * 128 : 16, 1024);
-      Ring<kGatedStages> st;
+      // (The loop has to be shorter than a block's products: its barriers by address, and the next block's looked at while the products of
+      // this one are on their way.)
+      const uint32_t full = ptx::smem_u32(s_full), empty = ptx::smem_u32(s_empty);
+      Ring<C::kStages> st;
       Ring<2> buf;
       uint32_t last = 0, last_parity = 0;
-      bool on = true, any = false;
+      bool on = true, any = false, there = false;
       for (uint32_t t = pair; t < tiles && on; t += pairs, buf.step()) {
         if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
         ptx::tc_fence_after();
-        for (int kb = 0; kb < blocks; ++kb, st.step()) {
-          if (!wait(s_full[st.at], st.parity, kGiveUpFull)) {
+        const uint32_t d = tmem + buf.at * 256;
+#pragma unroll 4
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!there && !wait(s_full[st.at], st.parity, kGiveUpFull)) {
             on = false;
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t off = st.at * (kGatedStageBytes >> 4);
-          ptx::mma_f16_ss_x4_pair_w(el, tmem + buf.at * 256, {a0.lo + off, a0.hi}, {b0.lo + off, b0.hi}, kStepA, kStepB, idesc, kb > 0);
-          ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_empty[st.at]));
+          const uint32_t off = st.at * (C::kBytes >> 4);
+          ptx::mma_f16_ss_x4_pair_w(el, d, {a0.lo + off, a0.hi}, {b0.lo + off, b0.hi}, kStepA, kStepB, idesc, kb > 0);
+          ptx::mma_commit_pair_w(el, 3, empty + 8 * st.at);
           last = st.at;
           last_parity = st.parity;
           any = true;
+          st.step();
+          there = ptx::mbar_test_wait_a(full + 8 * st.at, st.parity);
         }
         if (on) ptx::mma_commit_pair_w(el, 3, ptx::smem_u32(&s_tfull[buf.at]));
       }
@@ -164,13 +178,11 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
     // Eight warps take the sums home: a thread one row, every other 64 columns.  A warp puts 32 rows x 64 columns into shared memory in
     // the 128-byte swizzle and leaves them to the TMA, which skips what lies past the matrix.
     const int quad = warp & 3, group = (warp - 4) >> 2;
-    const uint32_t outs = stages + kGatedStages * kGatedStageBytes + (warp - 4) * 8192, at_tmem = tmem + ((uint32_t)quad << 21);
-    uint32_t which = 0;
-    const auto place = [&]() {
-      if (lane == 0) ptx::tma_store_wait_read<1>();
+    const uint32_t out = stages + C::kStages * C::kBytes + (warp - 4) * 4096, at_tmem = tmem + ((uint32_t)quad << 21);
+    const auto place = [&]() {  // (once the store before has been read)
+      if (lane == 0) ptx::tma_store_wait_read<0>();
       __syncwarp();
-      which ^= 1;
-      return outs + which * 4096;
+      return out;
     };
     const auto put = [&](uint32_t to, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + lane * 128 + ((piece ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d)
@@ -218,35 +230,34 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
         if constexpr (MODE == kForwardSave) {
 #pragma unroll 1
           for (int sum = 0; sum < 2; ++sum) {  // g, then u: the numbers' upper halves, and the byte after
-            if (lane == 0) ptx::tma_store_wait_read<0>();  // (both places at once)
-            __syncwarp();
-            const uint32_t upper = outs + (which ^ 1) * 4096, lower = outs + which * 4096;
+            uint32_t lower[2][8];
+            place();
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
               uint32_t r[32];
               ptx::tmem_ld32(from + sum * kHalfN + group * 64 + c, r);
               ptx::tmem_ld_wait();
-              uint32_t b[8];
 #pragma unroll
               for (int j = 0; j < 32; ++j) r[j] |= poison;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const auto two = [&](int i) { return __byte_perm(r[k * 8 + 2 * i], r[k * 8 + 2 * i + 1], 0x7632); };
-                put(upper, c / 8 + k, two(0), two(1), two(2), two(3));
+                put(out, c / 8 + k, two(0), two(1), two(2), two(3));
               }
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                b[k] = __byte_perm(__byte_perm(r[4 * k], r[4 * k + 1], 0x0051), __byte_perm(r[4 * k + 2], r[4 * k + 3], 0x0051), 0x5410);
-#pragma unroll
-              for (int k = 0; k < 2; ++k)  // (rows of 64 bytes, in the 64-byte swizzle)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(lower + lane * 64 + (((c / 16 + k) ^ ((lane >> 1) & 3)) << 4)),
-                             "r"(b[4 * k]), "r"(b[4 * k + 1]), "r"(b[4 * k + 2]), "r"(b[4 * k + 3])
-                             : "memory");
+                lower[c / 32][k] = __byte_perm(__byte_perm(r[4 * k], r[4 * k + 1], 0x0051), __byte_perm(r[4 * k + 2], r[4 * k + 3], 0x0051), 0x5410);
             }
-            if (inside) {
-              send(upper, &maps.out[1 + sum], x, y);
-              send(lower, &maps.out[3 + sum], x, y);
-            }  // (the next use of a place is of the upper one, whose group is not the newest)
+            if (inside) send(out, &maps.out[1 + sum], x, y);
+            place();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // (rows of 64 bytes, in the 64-byte swizzle)
+              const uint32_t* b = lower[k / 2] + (k % 2) * 4;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)), "r"(b[0]), "r"(b[1]),
+                           "r"(b[2]), "r"(b[3])
+                           : "memory");
+            }
+            if (inside) send(out, &maps.out[3 + sum], x, y);
           }
         }
         const uint32_t to = place();
@@ -265,7 +276,6 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
           words(rg, to, c / 8);
         }
         if (inside) send(to, &maps.out[0], x, y);
-        else if (lane == 0) ptx::tma_store_commit();
       } else {
 #pragma unroll
         for (int c = group * 64; c < TN; c += 128) {
@@ -279,7 +289,6 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
           words(r0, to, 0);
           words(r1, to, 4);
           if (y < g.rows && x < g.cols) send(to, &maps.out[part], x, y);
-          else if (lane == 0) ptx::tma_store_commit();
         }
       }
     }
@@ -362,8 +371,8 @@ int launch_gated(const GatedMaps& maps, const GatedArgs& g, cudaStream_t s) {
     return MVPA_ERR_UNSUPPORTED;
   }
   constexpr auto kernel = gated_kernel<MODE, TN>;
-  MVPA_CUDA_CHECK(grant_smem<kernel>(kGatedSmem));
-  MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kGatedThreads, kGatedSmem, s, maps, g));
+  MVPA_CUDA_CHECK(grant_smem<kernel>(Gated<MODE, TN>::kSmem));
+  MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kGatedThreads, Gated<MODE, TN>::kSmem, s, maps, g));
   count_launch();
   MVPA_CUDA_CHECK(cudaGetLastError());
   return MVPA_OK;
