@@ -39,8 +39,8 @@ struct GatedArgs {
 };
 
 constexpr int kGatedThreads = 384;
-// As many stages as there is room for: a block is some 2 us on its way from memory through the products and back to an empty stage, so that
-// with five of them a block took 0.4 us instead of 0.27.
+// As many stages as there is room for: a block is some 2 us on its way from memory through the products and back to an empty stage
+// (16384 x 2048 x 5632: 493 us with five, 476 with six; where the power does not bound it a block still takes 0.4 us, its products 0.27).
 template <int MODE, int TN>
 struct Gated {
   static constexpr int kHalfN = TN / 2;                // rows (or columns) of the right operand in each CTA

@@ -327,11 +327,14 @@ __global__ void __launch_bounds__(kFewWarps * 32) int4_few_kernel(const Int4Args
 // ---- many rows --------------------------------------------------------------------------------------------------------------------------
 // 128 weight rows x NT tokens a CTA.  Warps: 0 loads a chunk of 128 columns of both operands (TMA), 1 issues a group's products, whose left
 // operand is weights unpacked into TMEM, for 128 tokens at a time, 4 to 11 unpack, a row a thread, four warps every other chunk, and 12 to 19
-// fetch a group's sums, scale them and add them up in registers.  A chunk takes four unpacking warps some 1500 cycles from its arrival to
-// the product, half of them instructions, and the products of 256 tokens 1024: two sets of unpackers and four places in TMEM for what they
-// unpack keep up with that (with one set of eight warps, half a row each, and two places: 2200 x 15360 x 2048 185 us).    The CTAs are resident and take their tiles one
-// after the other; few tiles: the chunks are split over the CTAs of a cluster, whose sums meet through distributed shared memory in a
-// fixed order.
+// fetch a group's sums, scale them and add them up in registers.  The CTAs are resident and
+// take their tiles one after the other; few tiles: the chunks are split over the CTAs of a cluster, whose sums meet through distributed
+// shared memory in a fixed order.
+//
+// 2200 x 15360 x 2048 takes 175 us, the tensor pipe active 40 % of it.  A chunk of 128 columns and 256 tokens takes some 2400 cycles, 1024
+// of them products: the warp that issues looks at four barriers a chunk, 150 cycles and more each, and shares its scheduler with four
+// others.  Without the unpacking, or without most of the additions, it takes as long.  (One set of eight unpacking warps, half a row each,
+// with two places in TMEM: 185 us; all adding warps on both products in turn: 189; barriers looked at ahead: 180 to 215.)
 template <int NT, int W, int PARTS>
 struct Many {
   static constexpr int kWBytes = 128 * 64, kXBytes = NT * 256;  // of a chunk: 128 rows x 64 bytes; two halves of NT rows x 128 bytes
@@ -768,6 +771,8 @@ int run_int4(Int4Args g, int32_t dtype, void* workspace, cudaStream_t s) {
     MVPA_CUDA_CHECK(cudaGetLastError());
     x = workspace;
   }
+  // (us, few / many at 16 tokens and 17: 15360 x 2048 11.9 / 14.5, 2048 x 7680 8.3 / 13.6, 768 x 2496 5.6 / 6.4; with 32 tokens in four groups the
+  // former took 22, 22 and 7.6, the latter 14.7, 15.1 and 6.4.)
   if (g.M <= kFewTokens) {
     bool done = false;
     const int rc = g.M <= 8 ? run_few<T, W, 1>(x, ld, plane, g, s, &done) : run_few<T, W, 2>(x, ld, plane, g, s, &done);
@@ -776,7 +781,10 @@ int run_int4(Int4Args g, int32_t dtype, void* workspace, cudaStream_t s) {
   if (g.M <= 32) return run_many<32, T, W>(x, ld, plane, g, s);
   if (g.M <= 64 || sizeof(T) == 4) return run_many<64, T, W>(x, ld, plane, g, s);
   if constexpr (sizeof(T) == 2) {
-    if (g.M <= 128 || W == 2 || ((g.M + 255) / 256) * ((g.N + 127) / 128) < 74) return run_many<128, T, W>(x, ld, plane, g, s);
+    // 256 tokens a tile where that leaves half of the multiprocessors one (us, 128 / 256: 550 x 768 x 2496 10.9 / 20.6, 256 x 5632 x 2048 17.9 /
+    // 20.8).  A gate's two weights take a thread's registers for 128.
+    const int64_t wide = ((g.M + 255) / 256) * ((g.N + 127) / 128);
+    if (g.M <= 128 || W == 2 || 2 * wide < device_sm_count()) return run_many<128, T, W>(x, ld, plane, g, s);
     if constexpr (W == 1) return run_many<256, T, W>(x, ld, plane, g, s);
   }
   return MVPA_OK;

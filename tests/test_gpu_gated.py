@@ -108,6 +108,43 @@ def test_unaligned_rows_by_torch(cuda):
     torch.testing.assert_close(ops.gated_linear(moved, wg, wu), ops.gated_linear(x, wg, wu), rtol=2 ** -6, atol=2 ** -6)
 
 
+def test_python_path_is_the_same(cuda, monkeypatch):
+    """Without the extension: the same kernels and results, forward and backward."""
+    ins = _inputs(300, 264, 200)
+    native = _all(*ins)
+    monkeypatch.setattr(ops._host, "usable", lambda t: False)
+    assert all(torch.equal(a, b) for a, b in zip(native, _all(*ins)))
+
+
+def test_into_a_column_block(cuda):
+    x, wg, wu, _ = _inputs(150, 64, 72)
+    with torch.no_grad():
+        want = ops.gated_linear(x, wg, wu)
+    wide = torch.full((152, 200), 3.0, dtype=BF16, device="cuda")
+    got = ops.gated_linear_into(wide[1:151, 64:136], x, wg, wu)
+    assert torch.equal(got, want)
+    wide[1:151, 64:136] = 3
+    assert bool((wide == 3).all())
+    out = torch.empty_like(want)
+    wrong = [lambda: ops.gated_linear_into(out, x.float(), wg, wu), lambda: ops.gated_linear_into(out[:, :64], x, wg, wu),
+             lambda: ops.gated_linear_into(out, x, wg, wu[:64]), lambda: ops.gated_linear_into(out, x.t().contiguous().t(), wg, wu),
+             lambda: ops.gated_linear_into(out.cpu(), x, wg, wu), lambda: ops.gated_linear_into(out, x.clone().requires_grad_(), wg, wu),
+             lambda: ops.gated_linear_into(wide[1:151, 63:135], x, wg, wu), lambda: ops.gated_linear_into(out, x[:, :60].contiguous(), wg[:, :60].contiguous(), wu[:, :60].contiguous())]
+    for i, call in enumerate(wrong):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+def test_saved_tensors_may_move(cuda):
+    """What the forward keeps goes to the host and back (a saved-tensor hook) without changing a bit."""
+    ins = _inputs(130, 64, 72)
+    want = _all(*ins)
+    with torch.autograd.graph.save_on_cpu():
+        got = _all(*ins)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def _gates(values, ups, dhs):
     """Gates and ups that are exactly these numbers: x holds them beside ones and zeros."""
     n = len(values)

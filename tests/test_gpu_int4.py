@@ -128,6 +128,20 @@ def test_models_sizes(cuda, M, N, K):
         assert torch.equal(y, ops.matmul_int4(x, *w))
 
 
+@pytest.mark.parametrize("M,N,K,group", [(5000, 3000, 2176, 128), (3000, 4000, 900, 64), (2600, 20000, 384, 32)])
+@pytest.mark.parametrize("gate", [False, True])
+def test_many_tiles_a_cta(cuda, M, N, K, group, gate):
+    """Resident CTAs with several tiles each, odd numbers of chunks among them: rings that do not come out even with a tile's chunks."""
+    g = _gen(M, N, K)
+    w, up, x = _weight(g, N, K, group, True, BF16), _weight(g, N, K, group, True, BF16), _randn(g, M, K, dtype=BF16)
+    run = lambda: ops.gated_linear_int4(x, w, up, group=group) if gate else ops.matmul_int4(x, *w, group=group)
+    y = run()
+    exact, bound = ref.gated(x, w, up, K, group, 2.0 ** -8) if gate else ref.product(x, w, K, group, 2.0 ** -8)[:2]
+    assert ((y.double() - exact).abs() <= bound).all()
+    for _ in range(5):
+        assert torch.equal(y, run())
+
+
 @pytest.mark.parametrize("M", [1, 8, 20, 60, 200])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_strides_and_places(cuda, M, dtype):
