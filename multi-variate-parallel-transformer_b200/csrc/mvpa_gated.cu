@@ -35,6 +35,7 @@ struct GatedArgs {
   int blocks;        // blocks along the summed axis in a segment (kInput: dg Wg, then du Wu)
   int segments;
   int rows, cols;    // of the results
+  int few;           // rows of the left operand where there are up to 128 (a multiple of 8), else 0
   int* status;
 };
 
@@ -118,8 +119,12 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
           on = false;
           break;
         }
-        if (left && half == 0 && el) ptx::mbar_arrive_expect_tx(&s_full[st.at], 2 * C::kBytes);
+        // (Up to 128 rows are the first CTA's alone, in boxes of that many: rows past the matrix take the TMA as long as others, some 1.6
+        // cycles of 128 bytes.  Whatever else lies in the stage is other rows' sums, which are not stored.)
+        if (left && half == 0 && el)
+          ptx::mbar_arrive_expect_tx(&s_full[st.at], g.few > 0 ? 2 * (C::kBytes - 128 * 128) + g.few * 128 : 2 * C::kBytes);
         __syncwarp();
+        if (left && half == 1 && g.few > 0) continue;
         const int seg = kb >= g.blocks ? 1 : 0, k = (kb - seg * g.blocks) * 64;
         const uint32_t to = stages + st.at * C::kBytes + (left ? 0 : 128 * 128), bar = there + 8 * st.at;
         const CUtensorMap* map = left ? &maps.a[kRowsA ? part : seg] : &maps.b[kGate ? half : kRowsA ? 0 : seg];
@@ -400,6 +405,8 @@ int tile_width(int64_t tiles_m, int64_t cols, bool gate) {
 
 uint32_t tiles_of(int64_t n, int each) { return (uint32_t)((n + each - 1) / each); }
 
+int few_rows(int64_t rows) { return rows <= 128 ? ((int)rows + 7) / 8 * 8 : 0; }
+
 // The gradients' products (tiles_n is filled in).
 template <int MODE>
 int run_gated(const GatedMaps& maps, GatedArgs g, cudaStream_t s) {
@@ -440,7 +447,8 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
   const uint32_t tm = tiles_of(M, 256);
   const int width = tile_width(tm, I, true);
   GatedMaps maps = {};
-  int rc = encode(&maps.a[0], x, M, E, ld_x, 128);
+  const int few = few_rows(M);
+  int rc = encode(&maps.a[0], x, M, E, ld_x, few > 0 ? few : 128);
   if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, width / 2);
   if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, width / 2);
   if (rc == MVPA_OK) rc = encode(&maps.out[0], h, M, I, ld_h, 32);
@@ -455,7 +463,7 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
     }
   }
   if (rc != MVPA_OK) return rc;
-  const GatedArgs g = {tm, tiles_of(I, width / 2), tm, (int)tiles_of(E, 64), 1, (int)M, I, status};
+  const GatedArgs g = {tm, tiles_of(I, width / 2), tm, (int)tiles_of(E, 64), 1, (int)M, I, few, status};
   cudaStream_t s = (cudaStream_t)cuda_stream;
   if (width == 128) return saved != nullptr ? launch_gated<kForwardSave, 128>(maps, g, s) : launch_gated<kForward, 128>(maps, g, s);
   return saved != nullptr ? launch_gated<kForwardSave, 256>(maps, g, s) : launch_gated<kForward, 256>(maps, g, s);
@@ -483,13 +491,14 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
   int rc = MVPA_OK;
   if (dx != nullptr) {
     GatedMaps maps = {};
-    rc = encode(&maps.a[0], dgate, M, I, I, 128);
-    if (rc == MVPA_OK) rc = encode(&maps.a[1], dup, M, I, I, 128);
+    const int few = few_rows(M), box = few > 0 ? few : 128;
+    rc = encode(&maps.a[0], dgate, M, I, I, box);
+    if (rc == MVPA_OK) rc = encode(&maps.a[1], dup, M, I, I, box);
     if (rc == MVPA_OK) rc = encode(&maps.b[0], w_gate, I, E, E, 64);
     if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 64);
     if (rc == MVPA_OK) rc = encode(&maps.out[0], dx, M, E, E, 32);
     const uint32_t tm = tiles_of(M, 256);
-    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, 0, tm, (int)tiles_of(I, 64), 2, (int)M, E, status}, s);
+    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, 0, tm, (int)tiles_of(I, 64), 2, (int)M, E, few, status}, s);
   }
   if (rc == MVPA_OK && dw_gate != nullptr) {
     GatedMaps maps = {};
@@ -499,7 +508,7 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
     if (rc == MVPA_OK) rc = encode(&maps.out[0], dw_gate, I, E, E, 32);
     if (rc == MVPA_OK) rc = encode(&maps.out[1], dw_up, I, E, E, 32);
     const uint32_t tm = tiles_of(I, 256);
-    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, 0, tm, (int)tiles_of(M, 64), 1, I, E, status}, s);
+    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, 0, tm, (int)tiles_of(M, 64), 1, I, E, 0, status}, s);
   }
   return rc;
 }
