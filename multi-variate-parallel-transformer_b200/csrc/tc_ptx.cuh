@@ -422,21 +422,6 @@ __device__ __forceinline__ void tma_load_2d_pair_w(uint32_t el, uint32_t smem_ds
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(el)
       : "memory");
 }
-// Loads into this CTA's shared memory, issued by the elected lane of a convergent warp.
-__device__ __forceinline__ void tma_load_2d_w(uint32_t el, uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
-  asm volatile(
-      "{\n\t.reg .pred pe;\n\tsetp.ne.b32 pe, %5, 0;\n\t"
-      "@pe cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(smem_dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(el)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_3d_w(uint32_t el, uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
-  asm volatile(
-      "{\n\t.reg .pred pe;\n\tsetp.ne.b32 pe, %6, 0;\n\t"
-      "@pe cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(smem_dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(el)
-      : "memory");
-}
 // The barrier of this place in each CTA of the cluster whose bit is set.
 __device__ __forceinline__ void mma_commit_pair_w(uint32_t el, uint16_t ctas, uint32_t bar) {
   asm volatile(
