@@ -189,6 +189,17 @@ def test_not_finite(cuda, bad):
     assert not bool(h[131].isfinite().all()) and not bool(dwg[:, 5].isfinite().all())
 
 
+@pytest.mark.parametrize("M", [1, 7, 8, 9, 31, 33, 120, 121, 127, 128, 129])
+def test_few_rows(cuda, M):
+    """Up to 128 rows are loaded alone: what larger calls left in shared memory, here NaN, reaches no result."""
+    ins = _inputs(M, 264, 1368)
+    big = [torch.full_like(t, float("nan")) for t in _inputs(40000, 264, 1368)]
+    _all(*big)
+    got = _all(*ins)
+    _check(got, *ins)
+    assert all(bool(t.isfinite().all()) for t in got)
+
+
 def test_second_derivative(cuda):
     x, wg, wu, dh = _inputs(6, 16, 24)
     leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
