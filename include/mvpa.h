@@ -291,11 +291,14 @@ int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate, const voi
 /*
  * Its gradients from dh (M, I; leading dimension ld_dh) and what the forward saved: dx = dg Wg + du Wu (M, E) unless dx is NULL,
  * dw_gate = dg^T x and dw_up = du^T x (I, E) unless they are NULL; all contiguous, sums in fp32, in an order that depends on the sizes
- * alone, rounded once.  `dgate` and `dup` ((M, I), contiguous) receive dg and du in bf16, the operands of those products.
+ * and the device alone, rounded once.  `dgate` and `dup` ((M, I), contiguous) receive dg and du in bf16, the operands of those products.
+ * `workspace` (16-byte aligned, of mvpa_gated_linear_bwd_workspace_bytes bytes, which may be 0) holds the sums of pieces where a long
+ * axis is split over the device; with NULL none is.
  */
+size_t mvpa_gated_linear_bwd_workspace_bytes(int64_t M, int32_t E, int32_t I);
 int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* saved, const void* x, int64_t ld_x, const void* w_gate,
                           const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up, int64_t M, int32_t E, int32_t I,
-                          int32_t* status, void* cuda_stream);
+                          void* workspace, size_t workspace_bytes, int32_t* status, void* cuda_stream);
 
 /* ---- the block in 8 bits ----------------------------------------------------------------------
  * A row in 8 bits is a pair: q in e4m3, and one scale for each block of 128 neighbours (the row's last

@@ -17,6 +17,8 @@
 // dg and du are rounded to bf16 between the kernels: the products take 16-bit operands, and each of their sums is over hundreds of
 // terms, whose roundings (2^-9 each) leave the sum as exact as its own rounding to bf16 does.
 #include "block_rows.cuh"
+#include <algorithm>
+
 #include "silu.cuh"
 #include "tc_pairs.cuh"
 #include "tc_tma_host.cuh"
@@ -37,6 +39,8 @@ struct GatedArgs {
   int rows, cols;    // of the results
   int few;           // rows of the left operand where there are up to 128 (a multiple of 8), else 0
   int* status;
+  int splits, per;   // the summed axis in `splits` pieces of up to `per` blocks, each a tile of its own, whose sums go to `sums` in fp32
+  float* sums;       // [splits][parts][rows][cols]
 };
 
 constexpr int kGatedThreads = 384;
@@ -55,7 +59,7 @@ struct Gated {
 enum : int { kGiveUpEmpty = 81, kGiveUpFull = 82, kGiveUpTmemEmpty = 83, kGiveUpTmemFull = 84, kGiveUpDrain = 85 };
 
 // TN: columns of sums of a tile (256, 192 or 128; a gate's are half g, half u).
-template <int MODE, int TN>
+template <int MODE, int TN, bool SPLIT>
 __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs g) {
   constexpr bool kGate = MODE <= kForwardSave, kRowsA = MODE == kWeights, kRowsB = MODE >= kInput;  // (rows along M / N: MN-major)
   using C = Gated<MODE, TN>;
@@ -66,8 +70,10 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
   __shared__ int s_dead;  // a wait ran out: nothing waits any more, and the results are NaN
   const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t half = ptx::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = g.tiles_m * g.tiles_n;
-  const int blocks = g.blocks * g.segments;
+  const uint32_t half = ptx::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, each = g.tiles_m * g.tiles_n, tiles = SPLIT ? each * g.splits : each;
+  const int all = g.blocks * g.segments;
+  const auto piece_of = [&](uint32_t t) { return SPLIT ? t / each : 0u; };
+  const auto blocks_of = [&](uint32_t piece) { return SPLIT ? min(g.per, all - (int)piece * g.per) : all; };
   if (warp == 0) {
     ptx::prefetch_tensormap(&maps.a[0]);
     ptx::prefetch_tensormap(&maps.b[0]);
@@ -111,10 +117,12 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
     uint32_t loads = 0;
     bool on = true;
     for (uint32_t t = pair; t < tiles && on; t += pairs) {
-      const Tile at = tile_at<kTileN>(t, g.tiles_n, g.tiles_m);
+      const uint32_t piece = piece_of(t);
+      const Tile at = tile_at<kTileN>(t - piece * each, g.tiles_n, g.tiles_m);
       const uint32_t part = (uint32_t)at.m0 / 256 >= g.part ? 1 : 0;
       const int row = left ? at.m0 - (int)(part * g.part * 256) + (int)half * 128 : kGate ? at.n0 : at.n0 + (int)half * kHalfN;
-      for (int kb = 0; kb < blocks; ++kb, ++loads, st.step()) {
+      const int first = (int)piece * g.per, end = first + blocks_of(piece);
+      for (int kb = first; kb < end; ++kb, ++loads, st.step()) {
         if (!wait(s_empty[st.at], st.parity ^ 1, kGiveUpEmpty)) {
           on = false;
           break;
@@ -159,6 +167,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
         if (!wait(s_tempty[buf.at], buf.parity ^ 1, kGiveUpTmemEmpty)) break;
         ptx::tc_fence_after();
         const uint32_t d = tmem + buf.at * 256;
+        const int blocks = blocks_of(piece_of(t));
 #pragma unroll 4
         for (int kb = 0; kb < blocks; ++kb) {
           if (!there && !wait(s_full[st.at], st.parity, kGiveUpFull)) {
@@ -203,7 +212,8 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
     };
     Ring<2> buf;
     for (uint32_t t = pair; t < tiles; t += pairs, buf.step()) {
-      const Tile at = tile_at<kTileN>(t, g.tiles_n, g.tiles_m);
+      const uint32_t piece = piece_of(t);
+      const Tile at = tile_at<kTileN>(t - piece * each, g.tiles_n, g.tiles_m);
       const uint32_t part = (uint32_t)at.m0 / 256 >= g.part ? 1 : 0;
       const int y = at.m0 - (int)(part * g.part * 256) + (int)half * 128 + quad * 32;
       wait(s_tfull[buf.at], buf.parity, kGiveUpTmemFull);
@@ -285,12 +295,27 @@ __global__ void __launch_bounds__(kGatedThreads, 1) gated_kernel(const __grid_co
 #pragma unroll
         for (int c = group * 64; c < TN; c += 128) {
           const int x = at.n0 + c;
-          const uint32_t to = place();
+          const uint32_t to = SPLIT ? 0 : place();
           uint32_t r0[32], r1[32];
           ptx::tmem_ld32(from + c, r0);
           ptx::tmem_ld32(from + c + 32, r1);
           ptx::tmem_ld_wait();
           if (c + 128 >= TN) release();
+          if constexpr (SPLIT) {
+            if (y + lane < g.rows) {
+              float* row = g.sums + (((int64_t)piece * (kRowsA ? 2 : 1) + part) * g.rows + y + lane) * g.cols + x;
+              const auto store = [&](const uint32_t (&r)[32], int to) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                  if (x + to + j < g.cols)
+                    *reinterpret_cast<uint4*>(row + to + j) = make_uint4(r[j] | poison, r[j + 1] | poison, r[j + 2] | poison, r[j + 3] | poison);
+              };
+              store(r0, 0);
+              store(r1, 32);
+            }
+            __syncwarp();
+            continue;
+          }
           words(r0, to, 0);
           words(r1, to, 4);
           if (y < g.rows && x < g.cols) send(to, &maps.out[part], x, y);
@@ -368,14 +393,14 @@ int encode(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64
   return encode_bf16_sw128(map, base, 2, dims, strides, box);
 }
 
-template <int MODE, int TN>
+template <int MODE, int TN, bool SPLIT = false>
 int launch_gated(const GatedMaps& maps, const GatedArgs& g, cudaStream_t s) {
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, pairs = device_sm_count() / 2;
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n * (SPLIT ? g.splits : 1), pairs = device_sm_count() / 2;
   if (tiles * g.blocks * g.segments > 0x7fffffff) {
     set_error("mvpa_gated_linear: more than 2^31 blocks of 256 x %d x 64", TN);
     return MVPA_ERR_UNSUPPORTED;
   }
-  constexpr auto kernel = gated_kernel<MODE, TN>;
+  constexpr auto kernel = gated_kernel<MODE, TN, SPLIT>;
   MVPA_CUDA_CHECK(grant_smem<kernel>(Gated<MODE, TN>::kSmem));
   MVPA_CUDA_CHECK(launch_dependent(dim3(2), kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), kGatedThreads, Gated<MODE, TN>::kSmem, s, maps, g));
   count_launch();
@@ -383,36 +408,93 @@ int launch_gated(const GatedMaps& maps, const GatedArgs& g, cudaStream_t s) {
   return MVPA_OK;
 }
 
-// The width of the tiles: the one whose rounds over the pairs of multiprocessors take the least.  A block of 64 along the summed axis takes a
-// pair the longer of its products (256 columns 270 ns) and its loads (a multiprocessor takes some 150 bytes in a nanosecond): 270 ns at 256
-// columns, 218 at 192, 164 at 128.
-int tile_width(int64_t tiles_m, int64_t cols, bool gate) {
+// The width of the gate's tiles: the one whose rounds over the pairs of multiprocessors take the least.  A block of 64 along the summed axis
+// takes a pair the longer of its products (256 columns 270 ns) and its loads (a multiprocessor takes some 150 bytes in a nanosecond): 270 ns
+// at 256 columns, 218 at 192, 164 at 128.
+int tile_width(int64_t tiles_m, int64_t cols) {
   const int64_t pairs = device_sm_count() / 2;
-  constexpr int kWidths[3] = {256, 192, 128}, kTimes[3] = {270, 218, 164};
-  int best = 256;
-  int64_t least = INT64_MAX;
-  for (int i = 0; i < 3; ++i) {
-    if (gate && kWidths[i] == 192) continue;  // (96 features: not a whole number of the 64 that a warp takes)
-    const int64_t each = gate ? kWidths[i] / 2 : kWidths[i], tiles = tiles_m * ((cols + each - 1) / each);
-    const int64_t time = (tiles + pairs - 1) / pairs * kTimes[i];
-    if (time < least) {
-      least = time;
-      best = kWidths[i];
-    }
-  }
-  return best;
+  const auto time = [&](int width, int each) { return (tiles_m * ((cols + width / 2 - 1) / (width / 2)) + pairs - 1) / pairs * each; };
+  return time(128, 164) < time(256, 270) ? 128 : 256;  // (192: 96 features are not a whole number of the 64 that a warp takes)
 }
 
 uint32_t tiles_of(int64_t n, int each) { return (uint32_t)((n + each - 1) / each); }
 
 int few_rows(int64_t rows) { return rows <= 128 ? ((int)rows + 7) / 8 * 8 : 0; }
 
-// The gradients' products (tiles_n is filled in).
+// The gradients' products: how wide their tiles are, and in how many pieces the summed axis, by the longest pair's blocks.  Pieces are for
+// few tiles along a long axis, up to one a pair and eight blocks a piece at least; they cost a launch more and their sums' way to memory
+// and back.
+struct Plan {
+  int width, splits, per;
+  size_t bytes;
+};
+Plan plan_of(int64_t tiles_m, int64_t cols, int64_t blocks, int64_t rows, bool may_split) {
+  const int64_t pairs = device_sm_count() / 2;
+  constexpr int kWidths[3] = {256, 192, 128}, kTimes[3] = {270, 218, 164};
+  constexpr int kJoin = 5000, kSumBytes = 3000;  // ns, bytes a ns
+  Plan best = {256, 1, 0, 0};
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t tiles = tiles_m * ((cols + kWidths[i] - 1) / kWidths[i]);
+    for (int n = 1; n == 1 || (may_split && tiles * n <= pairs && blocks >= 8 * n); ++n) {
+      const int64_t per = (blocks + n - 1) / n;
+      if ((blocks + per - 1) / per != n) continue;
+      const int64_t time = (tiles * n + pairs - 1) / pairs * per * kTimes[i] + (n > 1 ? kJoin + n * rows * cols * 8 / kSumBytes : 0);
+      if (time < least) {
+        least = time;
+        best = {kWidths[i], n, (int)per, n > 1 ? (size_t)n * rows * cols * 4 : 0};
+      }
+    }
+  }
+  return best;
+}
+Plan plan_dx(int64_t M, int32_t E, int32_t I, bool may_split) { return plan_of(tiles_of(M, 256), E, 2 * (int64_t)tiles_of(I, 64), M, may_split); }
+Plan plan_dw(int64_t M, int32_t E, int32_t I, bool may_split) {
+  return plan_of(2 * (int64_t)tiles_of(I, 256), E, tiles_of(M, 64), 2 * (int64_t)I, may_split);
+}
+
+// The pieces' sums of one result or two, `each` numbers (a multiple of 8), added in their order and rounded once.
+__global__ void __launch_bounds__(256) gated_join_kernel(const float* __restrict__ sums, int splits, int64_t each, int results,
+                                                         __nv_bfloat16* __restrict__ out0, __nv_bfloat16* __restrict__ out1) {
+  ptx::griddep_launch();
+  ptx::griddep_wait();
+  const int64_t all = each * results;
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < all; i += (int64_t)gridDim.x * blockDim.x * 4) {
+    float4 v = *reinterpret_cast<const float4*>(sums + i);
+#pragma unroll 8
+    for (int z = 1; z < splits; ++z) {
+      const float4 a = *reinterpret_cast<const float4*>(sums + z * all + i);
+      v.x += a.x;
+      v.y += a.y;
+      v.z += a.z;
+      v.w += a.w;
+    }
+    *reinterpret_cast<uint2*>(i < each ? out0 + i : out1 + (i - each)) = make_uint2(ptx::pack_bf16(v.x, v.y), ptx::pack_bf16(v.z, v.w));
+  }
+}
+
+// (tiles_n is filled in.)
 template <int MODE>
-int run_gated(const GatedMaps& maps, GatedArgs g, cudaStream_t s) {
-  const int width = tile_width(g.tiles_m, g.cols, false);
-  g.tiles_n = tiles_of(g.cols, width);
-  return width == 256 ? launch_gated<MODE, 256>(maps, g, s) : width == 192 ? launch_gated<MODE, 192>(maps, g, s) : launch_gated<MODE, 128>(maps, g, s);
+int run_gated(const GatedMaps& maps, GatedArgs g, const Plan& plan, float* sums, void* out0, void* out1, cudaStream_t s) {
+  g.tiles_n = tiles_of(g.cols, plan.width);
+  if (plan.splits == 1)
+    return plan.width == 256   ? launch_gated<MODE, 256>(maps, g, s)
+           : plan.width == 192 ? launch_gated<MODE, 192>(maps, g, s)
+                               : launch_gated<MODE, 128>(maps, g, s);
+  g.splits = plan.splits;
+  g.per = plan.per;
+  g.sums = sums;
+  const int rc = plan.width == 256   ? launch_gated<MODE, 256, true>(maps, g, s)
+                 : plan.width == 192 ? launch_gated<MODE, 192, true>(maps, g, s)
+                                     : launch_gated<MODE, 128, true>(maps, g, s);
+  if (rc != MVPA_OK) return rc;
+  const int results = MODE == kWeights ? 2 : 1;
+  const int64_t each = (int64_t)g.rows * g.cols, ctas = (each * results / 4 + 255) / 256, most = (int64_t)device_sm_count() * 8;
+  MVPA_CUDA_CHECK(launch_dependent(1, gated_join_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, s, (const float*)sums, plan.splits, each,
+                                   results, (__nv_bfloat16*)out0, (__nv_bfloat16*)out1));
+  count_launch();
+  MVPA_CUDA_CHECK(cudaGetLastError());
+  return MVPA_OK;
 }
 
 int check_sizes(const char* what, int64_t M, int32_t E, int32_t I) {
@@ -445,7 +527,7 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
     return MVPA_ERR_ALIGNMENT;
   }
   const uint32_t tm = tiles_of(M, 256);
-  const int width = tile_width(tm, I, true);
+  const int width = tile_width(tm, I);
   GatedMaps maps = {};
   const int few = few_rows(M);
   int rc = encode(&maps.a[0], x, M, E, ld_x, few > 0 ? few : 128);
@@ -463,15 +545,20 @@ extern "C" int mvpa_gated_linear(const void* x, int64_t ld_x, const void* w_gate
     }
   }
   if (rc != MVPA_OK) return rc;
-  const GatedArgs g = {tm, tiles_of(I, width / 2), tm, (int)tiles_of(E, 64), 1, (int)M, I, few, status};
+  const GatedArgs g = {tm, tiles_of(I, width / 2), tm, (int)tiles_of(E, 64), 1, (int)M, I, few, status, 1, 0, nullptr};
   cudaStream_t s = (cudaStream_t)cuda_stream;
   if (width == 128) return saved != nullptr ? launch_gated<kForwardSave, 128>(maps, g, s) : launch_gated<kForward, 128>(maps, g, s);
   return saved != nullptr ? launch_gated<kForwardSave, 256>(maps, g, s) : launch_gated<kForward, 256>(maps, g, s);
 }
 
+extern "C" size_t mvpa_gated_linear_bwd_workspace_bytes(int64_t M, int32_t E, int32_t I) {
+  if (M < 1 || E < 1 || I < 1) return 0;
+  return std::max(plan_dx(M, E, I, true).bytes, plan_dw(M, E, I, true).bytes);
+}
+
 extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* saved, const void* x, int64_t ld_x, const void* w_gate,
                                      const void* w_up, void* dgate, void* dup, void* dx, void* dw_gate, void* dw_up, int64_t M, int32_t E,
-                                     int32_t I, int32_t* status, void* cuda_stream) {
+                                     int32_t I, void* workspace, size_t workspace_bytes, int32_t* status, void* cuda_stream) {
   const int rc0 = check_sizes("mvpa_gated_linear_bwd", M, E, I);
   if (rc0 != MVPA_OK) return rc0;
   if (!rows_fit(dh, ld_dh, I) || saved == nullptr || (reinterpret_cast<uintptr_t>(saved) & 15) != 0 || !rows_fit(dgate, I, I) ||
@@ -481,6 +568,12 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
     set_error("mvpa_gated_linear_bwd: every matrix must be 16-byte aligned with rows of a multiple of 16 bytes, not shorter than its width; "
               "dw_gate and dw_up are wanted both or neither");
     return MVPA_ERR_ALIGNMENT;
+  }
+  const Plan to_x = plan_dx(M, E, I, workspace != nullptr), to_w = plan_dw(M, E, I, workspace != nullptr);
+  const size_t need = std::max(dx != nullptr ? to_x.bytes : 0, dw_gate != nullptr ? to_w.bytes : 0);
+  if (workspace != nullptr && ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need)) {
+    set_error("mvpa_gated_linear_bwd: the workspace needs %zu bytes on a 16-byte boundary (got %zu)", need, workspace_bytes);
+    return MVPA_ERR_WORKSPACE;
   }
   cudaStream_t s = (cudaStream_t)cuda_stream;
   const int64_t ctas = (M * (I / 8) + 255) / 256, most = (int64_t)device_sm_count() * 16;
@@ -498,7 +591,7 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
     if (rc == MVPA_OK) rc = encode(&maps.b[1], w_up, I, E, E, 64);
     if (rc == MVPA_OK) rc = encode(&maps.out[0], dx, M, E, E, 32);
     const uint32_t tm = tiles_of(M, 256);
-    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, 0, tm, (int)tiles_of(I, 64), 2, (int)M, E, few, status}, s);
+    if (rc == MVPA_OK) rc = run_gated<kInput>(maps, {tm, 0, tm, (int)tiles_of(I, 64), 2, (int)M, E, few, status, 1, 0, nullptr}, to_x, (float*)workspace, dx, nullptr, s);
   }
   if (rc == MVPA_OK && dw_gate != nullptr) {
     GatedMaps maps = {};
@@ -508,7 +601,7 @@ extern "C" int mvpa_gated_linear_bwd(const void* dh, int64_t ld_dh, const void* 
     if (rc == MVPA_OK) rc = encode(&maps.out[0], dw_gate, I, E, E, 32);
     if (rc == MVPA_OK) rc = encode(&maps.out[1], dw_up, I, E, E, 32);
     const uint32_t tm = tiles_of(I, 256);
-    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, 0, tm, (int)tiles_of(M, 64), 1, I, E, 0, status}, s);
+    if (rc == MVPA_OK) rc = run_gated<kWeights>(maps, {2 * tm, 0, tm, (int)tiles_of(M, 64), 1, I, E, 0, status, 1, 0, nullptr}, to_w, (float*)workspace, dw_gate, dw_up, s);
   }
   return rc;
 }

@@ -52,6 +52,7 @@ struct Api {
   decltype(&mvpa_gated_linear) gated_linear;
   decltype(&mvpa_gated_linear_bwd) gated_linear_bwd;
   decltype(&mvpa_gated_linear_saved_bytes) gated_saved_bytes;
+  decltype(&mvpa_gated_linear_bwd_workspace_bytes) gated_bwd_bytes;
   decltype(&mvpa_quantize_int4) quantize_int4;
   decltype(&mvpa_dequantize_int4) dequantize_int4;
   decltype(&mvpa_matmul_int4) matmul_int4;
@@ -490,9 +491,11 @@ PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       const auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
       const Tensor word = status_word(status, x);
+      const size_t bytes = api.gated_bwd_bytes(d.rows, (int32_t)d.E, (int32_t)d.I);
+      const Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
       check(api.gated_linear_bwd(dact.const_data_ptr(), d.I, g.const_data_ptr(), xn.const_data_ptr(), d.E, wg.const_data_ptr(), wu.const_data_ptr(),
-                                 dg.data_ptr(), dup.data_ptr(), ptr(dxn), ptr(dwg), ptr(dwu), d.rows, (int32_t)d.E, (int32_t)d.I, word_of(word),
-                                 stream_of(x)), "mvpa_gated_linear_bwd");
+                                 dg.data_ptr(), dup.data_ptr(), ptr(dxn), ptr(dwg), ptr(dwu), d.rows, (int32_t)d.E, (int32_t)d.I, ptr(ws),
+                                 bytes, word_of(word), stream_of(x)), "mvpa_gated_linear_bwd");
       look_at(word, x, "mvpa_gated_linear_bwd kernel");
       if (needs(10)) grad[10] = dwg;
       if (needs(11)) grad[11] = dwu;
@@ -911,9 +914,11 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       dwu = at::empty_like(g.wu);
     }
     const auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const size_t bytes = api.gated_bwd_bytes(g.rows, (int32_t)g.E, (int32_t)g.I);
+    const Tensor ws = bytes ? at::empty({(int64_t)bytes}, g.x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
     check(api.gated_linear_bwd(d.const_data_ptr(), g.I, saved.const_data_ptr(), g.x.const_data_ptr(), g.E, g.wg.const_data_ptr(),
                                g.wu.const_data_ptr(), dg.data_ptr(), const_cast<char*>(part(dg, g.rows * g.I)), ptr(grad[0]), ptr(dwg), ptr(dwu),
-                               g.rows, (int32_t)g.E, (int32_t)g.I, word_of(w), stream_of(g.x)),
+                               g.rows, (int32_t)g.E, (int32_t)g.I, ptr(ws), bytes, word_of(w), stream_of(g.x)),
           "mvpa_gated_linear_bwd");
     look_at(w, g.x, "mvpa_gated_linear_bwd kernel");
     if (need & 2) grad[1] = std::move(dwg);
@@ -1135,7 +1140,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(api.quantize_fp8, "mvpa_quantize_fp8"); get(api.rmsnorm_fp8, "mvpa_rmsnorm_fp8");
   get(api.silu_mul_fp8, "mvpa_silu_mul_fp8"); get(api.matmul_fp8, "mvpa_matmul_fp8");
   get(api.gated_linear, "mvpa_gated_linear"); get(api.gated_linear_bwd, "mvpa_gated_linear_bwd");
-  get(api.gated_saved_bytes, "mvpa_gated_linear_saved_bytes");
+  get(api.gated_saved_bytes, "mvpa_gated_linear_saved_bytes"); get(api.gated_bwd_bytes, "mvpa_gated_linear_bwd_workspace_bytes");
   get(api.quantize_int4, "mvpa_quantize_int4"); get(api.dequantize_int4, "mvpa_dequantize_int4");
   get(api.matmul_int4, "mvpa_matmul_int4"); get(api.int4_workspace_bytes, "mvpa_matmul_int4_workspace_bytes");
   if (missing) { PyErr_Format(PyExc_ImportError, "%s has no %s", p, missing); return nullptr; }

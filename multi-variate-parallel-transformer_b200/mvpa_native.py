@@ -152,6 +152,7 @@ EXPORTS = ("mvpa_fwd", "mvpa_bwd", "mvpa_fwd_workspace_bytes", "mvpa_bwd_workspa
            "mvpa_wave_encode", "mvpa_channel_mean", "mvpa_contrastive_logits", "mvpa_peer_gather", "mvpa_peer_signal",
            "mvpa_peer_wait", "mvpa_rmsnorm_bwd", "mvpa_rmsnorm_bwd_workspace_bytes", "mvpa_silu_mul_bwd", "mvpa_quantize_fp8",
            "mvpa_rmsnorm_fp8", "mvpa_silu_mul_fp8", "mvpa_matmul_fp8", "mvpa_gated_linear", "mvpa_gated_linear_bwd", "mvpa_gated_linear_saved_bytes",
+           "mvpa_gated_linear_bwd_workspace_bytes",
            "mvpa_quantize_int4", "mvpa_dequantize_int4", "mvpa_matmul_int4_workspace_bytes", "mvpa_matmul_int4")
 ABI_VERSION = 3   # mvpa_abi_version() of the header this shim was written against
 
@@ -222,7 +223,9 @@ def lib() -> ctypes.CDLL:
         L.mvpa_gated_linear_saved_bytes.restype = ctypes.c_size_t
         L.mvpa_gated_linear_saved_bytes.argtypes = [i64, i32]
         L.mvpa_gated_linear_bwd.restype = ctypes.c_int
-        L.mvpa_gated_linear_bwd.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, vp]
+        L.mvpa_gated_linear_bwd.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, ctypes.c_size_t, vp, vp]
+        L.mvpa_gated_linear_bwd_workspace_bytes.restype = ctypes.c_size_t
+        L.mvpa_gated_linear_bwd_workspace_bytes.argtypes = [i64, i32, i32]
         I4 = ctypes.POINTER(Int4)
         L.mvpa_quantize_int4.restype = ctypes.c_int
         L.mvpa_quantize_int4.argtypes = [vp, i64, I4, i64, i32, i32, i32, vp]

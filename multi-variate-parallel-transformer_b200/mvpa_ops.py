@@ -224,9 +224,11 @@ def _gated_kernel_bwd(dh, x, w_gate, w_up, saved, need_x, need_w):
     ptr = lambda t: None if t is None else t.data_ptr()
     with _nat.on_device(x.device):
         status = _status_word(x.device)
+        nbytes = _nat.lib().mvpa_gated_linear_bwd_workspace_bytes(rows, E, I)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         st = _nat.lib().mvpa_gated_linear_bwd(dh.data_ptr(), I, saved.data_ptr(), x.data_ptr(), E, w_gate.data_ptr(), w_up.data_ptr(),
-                                              dgate.data_ptr(), dup.data_ptr(), ptr(dx), ptr(dw_gate), ptr(dw_up), rows, E, I, ptr(status),
-                                              _stream(x))
+                                              dgate.data_ptr(), dup.data_ptr(), ptr(dx), ptr(dw_gate), ptr(dw_up), rows, E, I, ptr(ws), nbytes,
+                                              ptr(status), _stream(x))
         _nat.check(st, "mvpa_gated_linear_bwd")
         _look_at(status, "mvpa_gated_linear_bwd", x)
     return dx, dw_gate, dw_up

@@ -42,7 +42,7 @@ def test_entry_points_refuse():
     fwd = lambda x=p, ld_x=64, wg=p, wu=p, h=p, ld_h=64, saved=None, M=4, E=64, I=64: lib.mvpa_gated_linear(
         x, ld_x, wg, wu, h, ld_h, saved, M, E, I, None, None)
     bwd = lambda dh=p, ld=64, saved=p, x=p, dg=p, du=p, dx=p, dwg=p, dwu=p, M=4, E=64, I=64: lib.mvpa_gated_linear_bwd(
-        dh, ld, saved, x, 64, p, p, dg, du, dx, dwg, dwu, M, E, I, None, None)
+        dh, ld, saved, x, 64, p, p, dg, du, dx, dwg, dwu, M, E, I, None, 0, None, None)
     assert lib.mvpa_gated_linear_saved_bytes(5, 24) == 5 * (2 * 48 + 2 * 32) and lib.mvpa_gated_linear_saved_bytes(0, 24) == 0
     shape = (dict(M=0), dict(E=0), dict(I=0), dict(E=60), dict(I=4), dict(M=-1), dict(M=2 ** 31))
     for bad in shape:
