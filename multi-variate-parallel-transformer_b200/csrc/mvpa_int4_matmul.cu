@@ -380,7 +380,7 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
         ptx::mbar_init(&s_full[i], 1);
-        ptx::mbar_init(&s_empty[i], 1 + 4);  // the products that read x, and the four warps that read the weights
+        ptx::mbar_init(&s_empty[i], 1 + 8);  // the products that read x, and the unpacking warps: four read the weights, and all look at s_full
       }
       for (int i = 0; i < C::kA; ++i) {
         ptx::mbar_init(&s_afull[i], 4);
@@ -519,8 +519,12 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
       uint32_t next[W];
       zeros_of(c0 + ((turn ^ set) & 1), next);
       for (int c = c0; c < c0 + nc; ++c, ++turn, st.step()) {
-        wait(s_full[st.at], st.parity, kGiveUpFull);  // (each one's: a pass over the ring that is not waited for would make the next look done)
+        // Each stage's, the other set's too: a pass over the ring that is not waited for would make the next look done.  And it is not filled
+        // again before this set has looked: of two passes, a look at the first would find the second, and wait for good.
+        wait(s_full[st.at], st.parity, kGiveUpFull);
         if (((turn ^ set) & 1) != 0) {  // the other set's
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&s_empty[st.at]);
 #pragma unroll
           for (int w = 0; w < W; ++w) a.step();
           continue;

@@ -142,6 +142,24 @@ def test_many_tiles_a_cta(cuda, M, N, K, group, gate):
         assert torch.equal(y, run())
 
 
+@pytest.mark.parametrize("M,dtype", [(17, BF16), (32, BF16), (32, F32), (50, BF16)])
+@pytest.mark.parametrize("K", [100, 128, 300, 640])
+@pytest.mark.parametrize("gate", [False, True])
+def test_many_small_tiles_a_cta(cuda, M, dtype, K, gate):
+    """The smallest tiles, several a resident CTA, of one, three and five chunks in groups of 32 with zeros: at each tile's border one set of
+    unpacking warps is at the new row's zeros while the other has its next chunk, and the stages go round under both."""
+    N, group = 128 * 400 + 40, 32
+    g = _gen(M, K, gate)
+    w, up = (_weight(g, N, K, group, True, dtype) for _ in range(2))
+    x = _randn(g, M, K, dtype=dtype)
+    run = lambda: ops.gated_linear_int4(x, w, up, group=group) if gate else ops.matmul_int4(x, *w, group=group)
+    y, half = run(), torch.finfo(dtype).eps / 2
+    exact, bound = ref.gated(x, w, up, K, group, half) if gate else ref.product(x, w, K, group, half)[:2]
+    assert ((y.double() - exact).abs() <= bound).all()
+    for _ in range(5):
+        assert torch.equal(y, run())
+
+
 @pytest.mark.parametrize("M", [1, 8, 20, 60, 200])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_strides_and_places(cuda, M, dtype):
