@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(256) gate_bwd_kernel(const __nv_bfloat16* __re
 #pragma unroll
     for (int e = 0; e < V::N; ++e) {
       const Sigmoid s(x[e]);
-      const float dg = s.times(d[e], u[e]) * fmaf(x[e], s.other, 1.f);
+      const float dg = s.times_slope(d[e], u[e], x[e]);
       u[e] = s.times(d[e], x[e]);
       x[e] = dg;
     }

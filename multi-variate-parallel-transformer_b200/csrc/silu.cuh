@@ -18,8 +18,12 @@ struct Sigmoid {
     part = g < 0.f ? a : 1.f;
     other = g < 0.f ? r : e * r;
   }
-  // a b s
-  __device__ __forceinline__ float times(float a, float b) const { return (a * part * part) * (b * part * part) * r; }
+  // a b s: each product on the way is at most the larger of |a| and |b| or the result, so none overflows before it.
+  __device__ __forceinline__ float times(float a, float b) const { return (a * part * part * r) * (b * part * part); }
+  // a b s (1 + g (1 - s)).  The last two factors are one number between -0.1 and 1.1, which goes into `a` before `b` does, as half of it.
+  __device__ __forceinline__ float times_slope(float a, float b, float g) const {
+    return (a * part * part * (r * fmaf(g, 0.5f * other, 0.5f))) * (b * part * part) * 2.f;
+  }
 };
 
 // silu(g) u, for results in 32 bits: the library's exponential, and the same parts where e^-|g| would leave the normal numbers.

@@ -176,6 +176,39 @@ def test_gates_of_any_size(cuda):
         assert bool((off <= 2.1 * (ref.HALF + ref.GATE) * du.abs() + 16 * small).all()), up
 
 
+def test_products_next_to_the_largest_number(cuda):
+    """Results that fp32 can hold beside products of some of their factors that it cannot: gate times up, dh times up, dh times gate, dh
+    times the derivative, which is 1.1 at most and passes through zero near -1.28."""
+    cases = [(1.203125, 3e38, 1e-3), (0.5, -3.3e38, 2.0), (2.0, 3.3e38, 1e-20), (1.203125, 1.0, 3e38), (0.01, 1.0, -3.3e38), (-1.25, 3e38, 8.0),
+             (-1.28125, -3e38, 30.0), (2.40625, 0.5, 3.3e38), (2.40625, -1e-30, 3.3e38), (-0.5, 3.3e38, 3.0), (3e38, 1.1, 0.5), (3e38, 1.0, 1.1),
+             (20.0, 3e38, 1.0), (-20.0, 3e38, 1e6)]
+    g, u, d = (torch.tensor(c, dtype=torch.float64) for c in zip(*cases))
+    x, wg, wu, dh = (torch.zeros(s, dtype=BF16, device="cuda") for s in ((len(cases), 8), (8, 8), (8, 8), (len(cases), 8)))
+    x[:, 0], x[:, 1], dh[:, 0], wg[0, 0], wu[0, 1] = g.to(BF16), u.to(BF16), d.to(BF16), 1, 1       # one feature
+    h, dx, _, _ = _all(x, wg, wu, dh)
+    g, u, d = x[:, 0].double(), x[:, 1].double(), dh[:, 0].double()
+    s = torch.sigmoid(g)
+    f = 1 + g * (1 - s)
+    lose = 1 + (1 + g.abs() * (1 - s)) / f.abs()         # what the derivative's difference makes of its terms' errors
+    most = 3.39e38
+    off = lambda got, want, err: (got.double() - want).abs() - err * want.abs() - 2.0 ** -133
+    want = g * s * u
+    assert bool((off(h[:, 0], want, ref.HALF + ref.GATE)[want.abs() <= most] <= 0).all())
+    assert bool(h[:, 0][want.abs() > most].isinf().all()) and int((want.abs() > most).sum()) == 2
+    dg, du = d * u * s * f, d * g * s
+    fits = (dg.abs() <= most) & (du.abs() <= most)        # (where one is infinite, the other's column of dx is infinity times zero beside it)
+    assert int(fits.sum()) == 11 and not bool(dx[~fits].isfinite().all(1).any())
+    assert bool((off(dx[:, 0], dg, ref.HALF + ref.GATE * lose)[fits] <= 0).all())
+    assert bool((off(dx[:, 1], du, ref.HALF + ref.GATE)[fits] <= 0).all())
+    # dg where du alone is infinite: by the gate's weights
+    x, dh = torch.zeros(1, 8, dtype=BF16, device="cuda"), torch.zeros(1, 8, dtype=BF16, device="cuda")
+    x[0, 0], x[0, 1], x[0, 3], dh[0, 0] = 2.40625, 0.5, 2.0 ** -10, 3.3e38
+    got = _all(x, wg, wu, dh)[2][0, 3].double()
+    s = 1 / (1 + torch.exp(torch.tensor(-2.40625, dtype=torch.float64)))
+    want = dh[0, 0].double() * 0.5 * s * (1 + 2.40625 * (1 - s)) * 2.0 ** -10
+    assert abs(got - want) <= (2 * ref.HALF + 3 * ref.GATE + 2.0 ** -16) * want
+
+
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
 def test_not_finite(cuda, bad):
     """A row that holds an infinity or a NaN concerns itself alone in h and dx, and every weight's gradient that it touches."""

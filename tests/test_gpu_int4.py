@@ -222,6 +222,21 @@ def test_values_at_their_ends(cuda, M, dtype):
     assert ((odd.double() - exact).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("M", [1, 12, 40, 100])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gate_next_to_the_largest_number(cuda, M, dtype):
+    """gate times up past fp32's largest number, silu(gate) times up not."""
+    gate, up = (torch.full((1, 16), 0x88, dtype=torch.uint8, device="cuda") for _ in range(2))
+    gate[0, 0], up[0, 0] = 0x89, 0x98                   # columns 0 and 1
+    s = torch.ones(1, 1, dtype=dtype, device="cuda")
+    x = torch.zeros(M, 32, dtype=dtype, device="cuda")
+    x[:, 0] = torch.linspace(0.25, 1.25, M).to(dtype)
+    x[:, 1] = 3e38
+    got = ops.gated_linear_int4(x, (gate, s), (up, s), group=32)[:, 0].double()
+    want = x[:, 0].double() * torch.sigmoid(x[:, 0].double()) * x[:, 1].double()
+    assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -18 if dtype == BF16 else 2.0 ** -20) * want.abs()).all())
+
+
 def test_last_row_ends_with_its_bytes(cuda):
     """A packed matrix whose last row ends with the memory it lies in."""
     N, K = 20, 70
