@@ -20,15 +20,18 @@ struct Int4Weight {
   __device__ __forceinline__ uint32_t zero(int64_t row, int group) const { return zeros != nullptr ? zeros[row * ld_z + group] : 8u; }
 };
 
-// Eight values of a word as pairs of bf16, (0, 4), (1, 5), (2, 6), (3, 7): a nibble in the low bits of 128's mantissa is 128 + q, from
-// which 128 + zero (`minus`, twice) is taken.  Whole numbers from -15 to 15: exact.
-__device__ __forceinline__ uint32_t int4_minus(uint32_t zero) { return 0x43004300u | zero | zero << 16; }
+// Eight values of a word as pairs of bf16, (0, 4), (1, 5), (2, 6), (3, 7), each 2^-11 of q - zero: a nibble in the low bits of the mantissa
+// of 128 / 2^11 is (128 + q) / 2^11, from which (128 + zero) / 2^11 (`minus`, twice) is taken.  Whole numbers from -15 to 15 beside a power
+// of two: exact.  The power keeps a group's sum, 128 terms of up to 15 |x|, below the largest |x|: only what the scales make of the sums
+// can leave fp32, and that where the result does (kInt4Unit takes the power back last).
+constexpr float kInt4Unit = 2048.f;
+__device__ __forceinline__ uint32_t int4_minus(uint32_t zero) { return 0x3d803d80u | zero | zero << 16; }
 __device__ __forceinline__ void int4_pairs(uint32_t w, uint32_t minus, uint32_t (&p)[4]) {
   const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&minus);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t v;  // (w >> 4 i) & 0x000f000f | 0x43004300 in one operation: both constants in registers, or the compiler makes it two
-    asm("{\n\t.reg .b32 mask, one;\n\tmov.b32 mask, 0x000f000f;\n\tmov.b32 one, 0x43004300;\n\tlop3.b32 %0, %1, mask, one, 0xea;\n\t}" : "=r"(v) : "r"(w >> (4 * i)));
+    uint32_t v;  // (w >> 4 i) & 0x000f000f | 0x3d803d80 in one operation: both constants in registers, or the compiler makes it two
+    asm("{\n\t.reg .b32 mask, one;\n\tmov.b32 mask, 0x000f000f;\n\tmov.b32 one, 0x3d803d80;\n\tlop3.b32 %0, %1, mask, one, 0xea;\n\t}" : "=r"(v) : "r"(w >> (4 * i)));
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), m);
     p[i] = *reinterpret_cast<const uint32_t*>(&d);
   }

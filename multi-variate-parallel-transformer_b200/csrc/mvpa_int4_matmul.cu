@@ -3,7 +3,7 @@
 //   x W^T [m, n] = sum over groups k of scale[n, k] * sum_{j in k} x[m, j] (q[n, j] - zero[n, k])
 //
 // The whole numbers q - zero are exact in bf16, so the inner sums are products of bf16 on the tensor cores with fp32 sums, and a group's
-// sum is scaled in fp32: no weight is rounded.  An fp32 x goes in as the three bf16 that it is the sum of.  Two kernels:
+// sum is scaled in fp32: no weight is rounded.  (2^-11 of them, that is, up to the last step: see int4_pairs.)  An fp32 x goes in as the three bf16 that it is the sum of.  Two kernels:
 //   few     up to 16 tokens: a warp forms 2 x 16 weight rows x 8 or 16 tokens from registers
 //   many    128 weight rows x up to 256 tokens a CTA: the weights are the product's M side, unpacked into TMEM on their way
 #include <algorithm>
@@ -35,10 +35,13 @@ struct Int4Args {
 
 constexpr int kChunk = 128;
 
-template <typename T>
-__device__ __forceinline__ float gate_of(float g, float u) {
-  if constexpr (sizeof(T) == 4) return silu_mul_f32(g, u);
-  else return Sigmoid(g).times(g, u);
+// A result of its sums (a gate's two), 2^-11 of them up to here.
+template <typename T, int W>
+__device__ __forceinline__ T result_of(const float (&v)[W]) {
+  const float g = v[0] * kInt4Unit;
+  if constexpr (W == 1) return from_f32<T>(g);
+  else if constexpr (sizeof(T) == 4) return from_f32<T>(silu_mul_f32(g, v[1] * kInt4Unit));
+  else return from_f32<T>(Sigmoid(g).times(g, v[1] * kInt4Unit));
 }
 
 __device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) int4_few_kernel(const Int4Args
 #pragma unroll
         for (int w = 0; w < W; ++w) v[w] += s_sum[k * C::kSums + w * kHalf + i];
     }
-    static_cast<T*>(g.out)[m * g.ld_out + n] = from_f32<T>(W == 2 ? gate_of<T>(v[0], v[W - 1]) : v[0]);
+    static_cast<T*>(g.out)[m * g.ld_out + n] = result_of<T>(v);
   }
   if (g.splits > 1) {
     __syncwarp();
@@ -628,7 +631,12 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
         T* out = static_cast<T*>(g.out) + (int64_t)(m0 + first) * g.ld_out + n0 + row;
 #pragma unroll
         for (int j = 0; j < C::kColumns; ++j)
-          if (m0 + first + j < g.M) out[j * g.ld_out] = from_f32<T>(W == 2 ? gate_of<T>(at(0, j), at(W - 1, j)) : at(0, j));
+          if (m0 + first + j < g.M) {
+            float v[W];
+#pragma unroll
+            for (int w = 0; w < W; ++w) v[w] = at(w, j);
+            out[j * g.ld_out] = result_of<T>(v);
+          }
       }
     }
   }
@@ -648,7 +656,7 @@ int4_many_kernel(const __grid_constant__ Int4Maps maps, const Int4Args g) {
       for (int z = 0; z < 8; ++z)
 #pragma unroll
         for (int w = 0; w < W; ++w) v[w] += part[w][z];
-      static_cast<T*>(g.out)[(int64_t)(m0 + j) * g.ld_out + n0 + row] = from_f32<T>(W == 2 ? gate_of<T>(v[0], v[W - 1]) : v[0]);
+      static_cast<T*>(g.out)[(int64_t)(m0 + j) * g.ld_out + n0 + row] = result_of<T>(v);
     }
     __syncwarp();
     ptx::cluster_sync();  // nobody's memory goes while it is read

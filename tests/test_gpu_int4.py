@@ -237,6 +237,24 @@ def test_gate_next_to_the_largest_number(cuda, M, dtype):
     assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -18 if dtype == BF16 else 2.0 ** -20) * want.abs()).all())
 
 
+@pytest.mark.parametrize("M", [1, 9, 40, 100, 300])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("K", [32, 128, 2048])
+def test_groups_next_to_the_largest_number(cuda, M, dtype, K):
+    """Sums of x (q - zero) past fp32's largest number, whose scale takes them back; scales and results of any size; and small ones, which
+    lose no more than fp32's own sums do: an x whose last bits lie above 2^-133, results above 2^-110."""
+    N, group = 150, min(K, 128)
+    g = _gen(M, K, 3)
+    q, zeros = ops.quantize_int4(_randn(g, N, K, dtype=dtype), group, True)[::2]
+    for x_size, scale in ((2e37, 1e-3), (3e35, 0.01), (1e36, 1e-30), (1e-30, 1e35), (1e-9, 4e36), (1e-31, 2e-2), (1.0, 1e-32)):
+        s = (torch.full((N, -(-K // group)), scale) * torch.exp(0.1 * torch.randn(N, -(-K // group), generator=g))).to(dtype).cuda()
+        x = (torch.randn(M, K, generator=g).sign() * (1 + torch.rand(M, K, generator=g)) * x_size).to(dtype).cuda()
+        w = (q, s, zeros)
+        exact, bound, _ = ref.product(x, w, K, group, torch.finfo(dtype).eps / 2)
+        assert exact.abs().max() < 3e38
+        assert ((ops.matmul_int4(x, *w, group=group).double() - exact).abs() <= bound).all(), (x_size, scale)
+
+
 def test_last_row_ends_with_its_bytes(cuda):
     """A packed matrix whose last row ends with the memory it lies in."""
     N, K = 20, 70
