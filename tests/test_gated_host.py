@@ -1,9 +1,11 @@
 """CPU: the gated projection's definition against differences, and what the C entry points refuse before they touch a GPU."""
 import ctypes
 
+import pytest
 import torch
 
 import gated_oracle as ref
+import mvpa_host
 import mvpa_native as nat
 
 
@@ -51,3 +53,12 @@ def test_entry_points_refuse():
         assert fwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad
     for bad in (dict(dh=None), dict(ld=60), dict(saved=None), dict(du=p + 4), dict(dwg=None), dict(dx=p + 2), dict(x=None)):
         assert bwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad
+
+
+@pytest.mark.parametrize("name,count", [("backward", 14), ("branches", 15), ("block_forward", 20), ("block_backward", 32)])
+def test_native_calls_count_their_arguments(name, count):
+    call = getattr(mvpa_host.module(), name)
+    assert call(*[None] * count) is None          # (no tensors: Python's path answers)
+    for other in (count - 1, count + 1):
+        with pytest.raises(TypeError, match="number of arguments"):
+            call(*[None] * other)
