@@ -255,6 +255,11 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         mvpa_ops.silu_mul_fp8(big[:, g0:g0 + I], big[:, g0 + I:], out=(q[:, E:], scales[:, blocks:]))
         return mvpa_ops.matmul_fp8(q, scales, *w_out, dtype=dtype)
 
+    def _gate_is_one_kernel(self, x):
+        """(What cannot be one kernel, a type that autocast chooses among it, is as without the flag.)"""
+        return (self.mlp.fused_gate and x.dtype == torch.bfloat16 and x.shape[1] % 8 == 0 and self.mlp.gate_proj.out_features % 8 == 0
+                and not torch.is_autocast_enabled("cuda") and x.is_contiguous() and x.data_ptr() % 16 == 0)
+
     @torch.no_grad()
     def fused_branches(self, x, r_time, r_chan, B, T, C):
         """x (B*T*C, E): the block's normalised input.  Returns MLP(x) + Attn(x), (B*T*C, E)."""
@@ -268,10 +273,7 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
                                               attn_mod._CHECK_STATUS, bool(self.mlp.fused_gate))
             if out is not None:
                 return out
-        g0 = E + 2 * KV
-        # (what cannot be one kernel, a type that autocast chooses among it, is as without the flag)
-        gated = (self.mlp.fused_gate and x.dtype == torch.bfloat16 and E % 8 == 0 and I % 8 == 0 and not torch.is_autocast_enabled("cuda")
-                 and x.is_contiguous() and x.data_ptr() % 16 == 0)
+        g0, gated = E + 2 * KV, self._gate_is_one_kernel(x)
         big = F.linear(x, w_in[:g0] if gated else w_in)                  # (M, E + 2 KV (+ 2 I)); under autocast in its type
         q4 = big[:, :E].view(B, N, H, D).permute(0, 2, 1, 3)
         k4 = big[:, E:E + KV].view(B, N, Hkv, D).permute(0, 2, 1, 3)
@@ -299,7 +301,8 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         I = self.mlp.gate_proj.out_features
         KV = Hkv * D
         w_in, w_out = self.fused_weights()
-        big = F.linear(x, w_in)                                          # (rows of this rank, E + 2 KV + 2 I)
+        g0, gated = E + 2 * KV, self._gate_is_one_kernel(x)
+        big = F.linear(x, w_in[:g0] if gated else w_in)                  # (rows of this rank, E + 2 KV (+ 2 I))
         cat = torch.empty((x.shape[0], E + I), dtype=big.dtype, device=x.device)
         u, vt, z = (b.view(Hkv, D).to(big.dtype) for b in a.attn_bias.detach().split(KV))
         r_time, r_chan = r_time.to(big.dtype), r_chan.to(big.dtype)
@@ -314,10 +317,14 @@ class MVPFormerBlock(Prepares, torch.nn.Module):
         def op(q, u_, vt_, z_, k, rt, rc, v, causal, sm_scale, window_size, q_time_range):
             return flash_mvpa_into(next(outs), q, u_, vt_, z_, k, rt, rc, v, sm_scale, window_size, q_time_range)
 
-        g0 = E + 2 * KV
+        def gate():
+            if gated:
+                mvpa_ops.gated_linear_into(cat[:, E:], x, w_in[g0:g0 + I], w_in[g0 + I:])
+            else:
+                mvpa_ops.silu_mul(big[:, g0:g0 + I], big[:, g0 + I:g0 + 2 * I], cat[:, E:])
+
         mvpa_shard.time_sharded_attention(
-            op, q_loc, u, vt, z, kv_loc, r_time, r_chan, None, T, C, 1.0 / (D ** 0.5), 10, group=group,
-            overlap=lambda: mvpa_ops.silu_mul(big[:, g0:g0 + I], big[:, g0 + I:g0 + 2 * I], cat[:, E:]),
+            op, q_loc, u, vt, z, kv_loc, r_time, r_chan, None, T, C, 1.0 / (D ** 0.5), 10, group=group, overlap=gate,
             transport=transport)
         return F.linear(cat, w_out)
 

@@ -227,6 +227,31 @@ def test_fused_gate_other_types_and_autocast(cuda):
         assert torch.equal(auto, m.enable_fused_gate(False)(inputs_embeds=x).last_hidden_state)
 
 
+def _sharded_worker(rank, port, path):
+    import os
+    import torch.distributed as dist
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("nccl", rank=0, world_size=1, device_id=torch.device("cuda:0"))
+    try:
+        m, x = _model(BF16), _embeds(BF16, B=1)
+        same = []
+        for flag in (True, False):
+            m.enable_fused_gate(flag)
+            same.append(torch.equal(m.forward_time_sharded(x.view(-1, 256), 7, 9, transport="nccl"), _run(m, x).view(-1, 256)))
+        torch.save(same, path)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_time_sharded_forward_with_the_fused_gate(cuda, tmp_path):
+    """One rank that holds the whole sample: the same kernels on the same rows, hence the plain forward's bits, with the flag and without."""
+    import os
+    import torch.multiprocessing as mp
+    path = str(tmp_path / "same")
+    mp.spawn(_sharded_worker, args=(29500 + os.getpid() % 2000, path), nprocs=1, join=True)
+    assert torch.load(path) == [True, True]
+
+
 def test_training_step_in_a_graph(cuda, monkeypatch):
     """Forward, loss and gradients of a fused-gate model captured once and replayed on another batch."""
     monkeypatch.setattr(models.mvpformer.attn_mod, "_CHECK_STATUS", False)

@@ -1,6 +1,7 @@
 """CPU: host-side logic of the model-level package: state-dict layout against the fixture written from the
 reference's `MVPFormerModel`, configuration aliases, encoder sizes, and the synthetic iEEG generator."""
 import numpy as np
+import pytest
 import torch
 
 import models
@@ -267,3 +268,34 @@ def test_a_graph_is_kept_with_the_weights_that_it_reads(monkeypatch):
         assert not {id(r()) for r in first} & {id(r()) for r in read}
         m.reset_cuda_graphs()
         assert all(r() is None for r in first)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("rows", [(4, 2), (6, 0)])
+def test_the_time_sharded_forward_follows_the_fused_gate(monkeypatch, fused, rows):
+    """On a rank's tokens: q, k and v alone are formed before the gather where the gate is one kernel, which then runs while it does."""
+    import mvpa_shard
+    mv, E, I, C = models.mvpformer, 32, 48, 2
+    torch.manual_seed(0)
+    cfg = models.MVPFormerConfig(n_positions=8, n_channels=8, n_embd=E, n_layer=1, n_head=2, n_head_kv=1, n_inner=I)
+    m = models.MVPFormerModel(cfg).to(torch.bfloat16).eval().enable_fused_gate(fused)
+    block, calls = m.h[0], []
+
+    def attention(op, q_loc, u, vt, z, kv_loc, *rest, overlap, **kw):
+        overlap()
+        calls.append([None if t is None else tuple(t.shape) for t in (*q_loc, *kv_loc)])
+        return []
+
+    monkeypatch.setattr(mvpa_shard, "time_sharded_attention", attention)
+    monkeypatch.setattr(mv.mvpa_ops, "gated_linear_into", lambda out, x, wg, wu: calls.append("gated") or out.copy_(
+        torch.nn.functional.silu(x.float() @ wg.float().t()) * (x.float() @ wu.float().t())))
+    monkeypatch.setattr(mv.mvpa_ops, "silu_mul", lambda g, u, out: calls.append("apart") or out.copy_(torch.nn.functional.silu(g.float()) * u.float()))
+    x = torch.randn(sum(rows), E).to(torch.bfloat16)
+    empty = torch.empty
+    monkeypatch.setattr(mv.torch, "empty", lambda *a, **k: empty(*a, **k).zero_())      # (the attention's columns, which nothing writes here)
+    got = block.fused_branches_time_sharded(x, torch.zeros(1, 4, 16), torch.zeros(1, C, 16), 4, C, rows, None, "nccl")
+    heads = lambda n, h: (1, n, h, 16) if n else None
+    assert calls == ["gated" if fused else "apart", [heads(rows[0], 2), heads(rows[1], 2), heads(rows[0], 2), heads(rows[1], 2)]]
+    mlp = block.mlp
+    want = mlp.down_proj.float()((torch.nn.functional.silu(mlp.gate_proj.float()(x.float())) * mlp.up_proj.float()(x.float())))
+    assert (got.float() - want).abs().max() <= 2.0 ** -5 * want.abs().max()
