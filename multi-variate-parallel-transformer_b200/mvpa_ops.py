@@ -257,12 +257,14 @@ class _GatedLinear(torch.autograd.Function):
             if _plain(d, x, w_gate, w_up) and saved.device == x.device and saved.is_contiguous() and saved.data_ptr() % 16 == 0:
                 dx, dw_gate, dw_up = _gated_kernel_bwd(d.view(-1, I), x.view(-1, E), w_gate, w_up, saved, need[0], need[1] or need[2])
                 return dx.view(x.shape) if need[0] else None, dw_gate if need[1] else None, dw_up if need[2] else None
-        # a graph of the gradient is wanted (or a transform is active): the same formula in torch operations
-        x2, d = x.reshape(-1, E), dh.reshape(-1, I).float()
-        g, u = torch.nn.functional.linear(x2, w_gate).float(), torch.nn.functional.linear(x2, w_up).float()
-        s = torch.sigmoid(g)
-        dg, du = (d * u * (s * (1 + g * (1 - s)))).to(x.dtype), (d * (g * s)).to(x.dtype)
-        return (dg @ w_gate + du @ w_up).view(x.shape), dg.t() @ x2, du.t() @ x2
+        # a graph of the gradient is wanted (or a transform is active): the same formula in torch operations, in fp32 as the kernels' sums
+        # are and rounded once, whatever region the backward runs in
+        with torch.autocast("cuda", enabled=False):
+            x2, d, wg, wu = x.reshape(-1, E).float(), dh.reshape(-1, I).float(), w_gate.float(), w_up.float()
+            g, u = torch.nn.functional.linear(x2, wg), torch.nn.functional.linear(x2, wu)
+            s = torch.sigmoid(g)
+            dg, du = d * (s * (1 + g * (1 - s))) * u, d * (g * s)
+            return (dg @ wg + du @ wu).to(x.dtype).view(x.shape), (dg.t() @ x2).to(x.dtype), (du.t() @ x2).to(x.dtype)
 
 
 def gated_linear(x, w_gate, w_up):

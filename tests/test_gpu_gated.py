@@ -275,6 +275,26 @@ def test_second_derivative(cuda):
         assert (a.double() - b).abs().max() <= 16 * ref.HALF * b.abs().max()
 
 
+@pytest.mark.parametrize("M,E,I", [(6, 16, 24), (300, 264, 200)])
+@pytest.mark.parametrize("autocast", [None, BF16, torch.float16])
+def test_gradients_that_have_a_graph(cuda, M, E, I, autocast):
+    """As near to 64 bits as those without (fp32 throughout, one rounding at the end: within the bounds of the kernels' sums alone), also where
+    the backward runs inside an autocast region that the forward was outside of."""
+    x, wg, wu, dh = _inputs(M, E, I, spread=3.0)
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    h = ops.gated_linear(*leaves)
+    with torch.autocast("cuda", dtype=autocast or BF16, enabled=autocast is not None):
+        got = torch.autograd.grad(h, leaves, dh * 64, create_graph=True)
+    assert all(t.dtype == BF16 and t.requires_grad for t in got)
+    ins = [t.double() for t in (x, wg, wu, dh * 64)]
+    small = [t.abs() for t in ins]                 # the sums of magnitudes: fp32 additions and some twenty roundings of 2^-24 on the way
+    g, u = small[0] @ small[1].t(), small[0] @ small[2].t()
+    s = small[3] * 1.5 * (1 + u) * (1 + g)
+    sums = (s @ small[1] + s @ small[2], s.t() @ small[0], s.t() @ small[0])
+    for a, b, size in zip(got, ref.gradients(*ins), sums):
+        assert bool(((a.double() - b).abs() <= ref.HALF * b.abs() + (M + E + 2 * I + 20) * ref.CUT * size).all())
+
+
 def test_graph_capture_of_a_step(cuda):
     """Forward and backward in one captured graph, replayed on new inputs."""
     x, wg, wu, dh = _inputs(500, 264, 136)
