@@ -104,7 +104,7 @@ def _gate(gate, up):
 
 def _plain_linear(m):
     """A projection that nothing has replaced, hooked or wrapped: its weight is all there is to it."""
-    return block_grad._unhooked(m, block_grad._LINEAR) and m.bias is None
+    return block_grad._unhooked(m, block_grad._LINEAR) and m.bias is None and not torch.nn.modules.module._has_any_global_hook()
 
 
 class LlamaMLP(torch.nn.Module):

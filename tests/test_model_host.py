@@ -299,3 +299,29 @@ def test_the_time_sharded_forward_follows_the_fused_gate(monkeypatch, fused, row
     mlp = block.mlp
     want = mlp.down_proj.float()((torch.nn.functional.silu(mlp.gate_proj.float()(x.float())) * mlp.up_proj.float()(x.float())))
     assert (got.float() - want).abs().max() <= 2.0 ** -5 * want.abs().max()
+
+
+def test_the_fused_gate_leaves_no_hook_out():
+    """A hook on a projection, on every module (torch's global hooks) or on the gradients: the projections are called, as without the flag."""
+    mlp = models.mvpformer.LlamaMLP(models.MVPFormerConfig(n_embd=8, n_inner=16))
+    mlp.fused_gate = True
+    x, seen = torch.randn(3, 8), []
+    note = lambda m, *_: seen.append(m) and None
+    every = torch.nn.modules.module
+    for register in (mlp.gate_proj.register_forward_hook, mlp.gate_proj.register_forward_pre_hook, mlp.gate_proj.register_full_backward_hook,
+                     every.register_module_forward_hook, every.register_module_forward_pre_hook, every.register_module_full_backward_hook):
+        handle = register(note)
+        try:
+            mlp(x.clone().requires_grad_()).sum().backward()
+        finally:
+            handle.remove()
+        assert any(m is mlp.gate_proj for m in seen), register
+        seen.clear()
+    called = []
+    original, mlp_ops = models.mvpformer.mvpa_ops.gated_linear, models.mvpformer.mvpa_ops
+    try:
+        mlp_ops.gated_linear = lambda *a: called.append(1) or original(*a)
+        mlp(x)
+    finally:
+        mlp_ops.gated_linear = original
+    assert called
