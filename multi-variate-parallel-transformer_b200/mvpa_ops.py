@@ -276,7 +276,9 @@ def gated_linear(x, w_gate, w_up):
         h = _host.module().gated_linear(x, w_gate, w_up, _attn._CHECK_STATUS)     # (an ordinary call that no gradient flows through)
         if h is not None:
             return h
-    if (not torch.is_autocast_enabled("cuda") and x.dtype == torch.bfloat16 and x.dim() > 1 and w_gate.dim() == 2 and w_gate.shape == w_up.shape
+    # (types first: a symbolic value answers no question about itself)
+    if (all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in (x, w_gate, w_up)) and not torch.is_autocast_enabled("cuda")
+            and x.dtype == torch.bfloat16 and x.dim() > 1 and w_gate.dim() == 2 and w_gate.shape == w_up.shape
             and x.shape[-1] == w_gate.shape[1] and x.shape[-1] % 8 == 0 and w_gate.shape[0] % 8 == 0):
         if not x.is_contiguous():
             x = x.contiguous()

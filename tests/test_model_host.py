@@ -325,3 +325,14 @@ def test_the_fused_gate_leaves_no_hook_out():
     finally:
         mlp_ops.gated_linear = original
     assert called
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_mlp_with_the_fused_gate_can_be_traced_scripted_and_compiled(dtype):
+    m = models.mvpformer.LlamaMLP(models.MVPFormerConfig(n_embd=8, n_inner=16)).to(dtype)
+    m.fused_gate = True
+    x = torch.randn(3, 8).to(dtype)
+    want = m.down_proj(torch.nn.functional.silu(m.gate_proj(x)) * m.up_proj(x))
+    for form in (m, torch.fx.symbolic_trace(m), torch.jit.script(m), torch.jit.trace(m, x),
+                 torch.compile(m, backend="eager", fullgraph=True), torch.export.export(m, (x,)).module(), torch.vmap(m)):
+        torch.testing.assert_close(form(x), want)
