@@ -110,7 +110,8 @@ def _plain_linear(m):
 class LlamaMLP(torch.nn.Module):
     """SwiGLU MLP with the parameter names of `transformers`' `LlamaMLP`, which the reference block uses
     (`models/mvpformer.py:34, 114`): down_proj(silu(gate_proj(x)) * up_proj(x)), no biases.  `fused_gate`: what comes before the
-    down projection by `mvpa_ops.gated_linear`, with fewer roundings on the way (`MVPFormerModel.enable_fused_gate`)."""
+    down projection by the kernel of `mvpa_ops.gated_linear` where there is one for it, with fewer roundings on the way
+    (`MVPFormerModel.enable_fused_gate`)."""
 
     fused_gate = False     # (of the class: modules pickled before have none of their own)
 
@@ -123,7 +124,9 @@ class LlamaMLP(torch.nn.Module):
     def forward(self, x):
         if not torch.jit.is_scripting():
             if self.fused_gate and _plain_linear(self.gate_proj) and _plain_linear(self.up_proj):
-                return self.down_proj(mvpa_ops.gated_linear(x, self.gate_proj.weight, self.up_proj.weight))
+                act = mvpa_ops.gated_linear_kernel(x, self.gate_proj.weight, self.up_proj.weight)
+                if act is not None:
+                    return self.down_proj(act)
         gate, up = self.gate_proj(x), self.up_proj(x)
         if torch.jit.is_scripting():
             act = F.silu(gate) * up

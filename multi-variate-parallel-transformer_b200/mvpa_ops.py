@@ -267,11 +267,8 @@ class _GatedLinear(torch.autograd.Function):
             return (dg @ wg + du @ wu).to(x.dtype).view(x.shape), (dg.t() @ x2).to(x.dtype), (du.t() @ x2).to(x.dtype)
 
 
-def gated_linear(x, w_gate, w_up):
-    """Differentiable silu(x w_gate^T) * (x w_up^T) for x (..., E) and weights (I, E): the MLP up to its down projection.  bf16 with E
-    and I multiples of 8: one kernel forward, with both products and the activation in fp32, rounded once; the backward is one for the
-    gate and one for each matrix product (the gradient of x, that of both weights), from the two products, of which the forward keeps
-    24 bits each where a gradient is wanted.  Everything else, and calls under autocast, by torch operations."""
+def gated_linear_kernel(x, w_gate, w_up):
+    """`gated_linear` where it is one kernel, else None."""
     if _host.usable(x):
         h = _host.module().gated_linear(x, w_gate, w_up, _attn._CHECK_STATUS)     # (an ordinary call that no gradient flows through)
         if h is not None:
@@ -284,7 +281,16 @@ def gated_linear(x, w_gate, w_up):
             x = x.contiguous()
         if _plain(x, w_gate, w_up):
             return _GatedLinear.apply(x, w_gate, w_up)
-    return swiglu(torch.nn.functional.linear(x, w_gate), torch.nn.functional.linear(x, w_up))
+    return None
+
+
+def gated_linear(x, w_gate, w_up):
+    """Differentiable silu(x w_gate^T) * (x w_up^T) for x (..., E) and weights (I, E): the MLP up to its down projection.  bf16 with E
+    and I multiples of 8: one kernel forward, with both products and the activation in fp32, rounded once; the backward is one for the
+    gate and one for each matrix product (the gradient of x, that of both weights), from the two products, of which the forward keeps
+    24 bits each where a gradient is wanted.  Everything else, and calls under autocast, by torch operations."""
+    h = gated_linear_kernel(x, w_gate, w_up)
+    return swiglu(torch.nn.functional.linear(x, w_gate), torch.nn.functional.linear(x, w_up)) if h is None else h
 
 
 def gated_linear_into(out, x, w_gate, w_up):

@@ -227,6 +227,23 @@ def test_fused_gate_other_types_and_autocast(cuda):
         assert torch.equal(auto, m.enable_fused_gate(False)(inputs_embeds=x).last_hidden_state)
 
 
+@pytest.mark.parametrize("dtype,inner,autocast", [(F32, 352, False), (F32, 352, True), (torch.float16, 352, False), (BF16, 204, False)])
+def test_fused_gate_changes_nothing_else(cuda, dtype, inner, autocast):
+    """Other types, autocast and widths that the kernel does not take, through the modules: the bits and the launches of a model without the flag."""
+    m = _model(dtype, inner=inner).train()
+    m.h[0].ln_1.register_forward_hook(lambda *_: None)
+    mlp, x = m.h[0].mlp, _embeds(dtype).requires_grad_()
+    got = []
+    for flag in (False, True):
+        m.enable_fused_gate(flag)
+        launched = nat.lib().mvpa_launch_count()
+        with torch.autocast("cuda", dtype=BF16, enabled=autocast):
+            y = mlp(x)
+        grads = torch.autograd.grad(y.float().square().sum(), [x, *mlp.parameters()])
+        got.append((nat.lib().mvpa_launch_count() - launched, y, *grads))
+    assert got[0][0] == got[1][0] and all(torch.equal(a, b) for a, b in zip(got[0][1:], got[1][1:]))
+
+
 def _sharded_worker(rank, port, path):
     import os
     import torch.distributed as dist
