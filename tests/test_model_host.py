@@ -328,3 +328,26 @@ def test_mlp_with_the_fused_gate_can_be_traced_scripted_and_compiled(dtype):
     for form in (m, torch.fx.symbolic_trace(m), torch.jit.script(m), torch.jit.trace(m, x),
                  torch.compile(m, backend="eager", fullgraph=True), torch.export.export(m, (x,)).module(), torch.vmap(m)):
         torch.testing.assert_close(form(x), want)
+
+
+def test_weights_that_are_no_longer_read_are_released():
+    """`enable_int4` takes the place of the weights in 16 and 8 bits, and leaves none in 4 bits behind when it goes."""
+    m = models.MVPFormerModel(models.MVPFormerConfig(n_positions=4, n_channels=4, n_embd=128, n_layer=2, n_head=2, n_head_kv=1, n_inner=16))
+    kept = lambda: [(b._fused is not None, b._fused_fp8 is not None, b._fused_int4 is not None) for b in m.h]
+
+    def fill():
+        for b in m.h:
+            b._fused = b._fused_fp8 = b._fused_int4 = ("tag", (torch.zeros(1),), set())
+
+    fill()
+    m.enable_int4()
+    assert kept() == [(False, False, True)] * 2
+    fill()
+    m.enable_int4(False)
+    assert kept() == [(True, True, False)] * 2
+    fill()
+    m.enable_fp8()
+    assert kept() == [(True, True, False)] * 2
+    fill()
+    m.enable_fp8(False)
+    assert kept() == [(True, True, True)] * 2
