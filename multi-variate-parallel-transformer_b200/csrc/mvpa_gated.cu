@@ -15,7 +15,8 @@
 //                  (MN-major), the right one: the sum of both products is formed in TMEM.
 //   weights        both operands have the summed axis, the tokens, outermost (MN-major).
 // dg and du are rounded to bf16 between the kernels: the products take 16-bit operands, and each of their sums is over hundreds of
-// terms, whose roundings (2^-9 each) leave the sum as exact as its own rounding to bf16 does.
+// terms, whose roundings (up to 2^-8 each, of either sign) leave the sum nearly as exact as its own rounding to bf16 does: the gradients are
+// 0.0023 of their size from 64 bits, with dg and du in fp32 they would be 0.0017.
 #include "block_rows.cuh"
 #include <algorithm>
 

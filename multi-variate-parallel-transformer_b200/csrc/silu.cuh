@@ -8,7 +8,8 @@ namespace {
 
 // For results in 16 bits.  With a = e^(-|g| / 4) (which leaves the normal numbers below |g| = 349, where the product with any
 // factor rounds to zero) the factor s = 1 / (1 + e^-g) of a negative g is a^4 / (1 + a^4), taken into a product in four parts, so that
-// nothing underflows that the result does not.  Errors: an ulp or two of a, four times over, 2^-19 against the 2^-9 of the result's rounding.
+// nothing underflows that the result does not.  Relative errors of a^4: |g| 2^-23.7 from the rounding of a's argument (2^-18 near 50, 2^-15.3
+// at the end), and an ulp or two of a, four times over, 2^-20; the result's own rounding to bf16 is one of up to 2^-8.
 struct Sigmoid {
   float part, r;  // e^(-|g| / 4) where g < 0, else 1;  1 / (1 + e^-|g|)
   float other;    // 1 - s

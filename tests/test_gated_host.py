@@ -37,6 +37,17 @@ def test_gradients_against_autograd():
         torch.testing.assert_close(a, b, rtol=1e-12, atol=1e-13)
 
 
+def test_bound_of_the_gates_factor():
+    """e^-|g| as the fourth power of 2^(|g| c) in fp32, with an exact power of two: what the argument's rounding alone makes of it, over the gates
+    in bf16.  From |g| of some 50 on that is more than 2^-18."""
+    g = torch.arange(0x3f80, 0x43ad, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).double()     # 1 to 345
+    c = torch.tensor(0.25 * 1.4426950408889634, dtype=torch.float32)
+    t = (g.float() * c).double()
+    off = (torch.exp2(-4 * t) / torch.exp(-g) - 1).abs()
+    assert bool((off <= ref.gate(-g) - ref.GATE).all())
+    assert float(off.max()) > 2.0 ** -17 > ref.GATE and bool((off[g < 20] < ref.GATE).all())
+
+
 def test_entry_points_refuse():
     lib = nat.lib()
     buf = ctypes.create_string_buffer(1 << 16)
