@@ -234,6 +234,10 @@ int check_int4(const char* what, int64_t N, int32_t K, int32_t group, int32_t sc
     return MVPA_ERR_DTYPE;
   }
   if (N == 0 || K == 0) return MVPA_OK;
+  if (w == nullptr) {
+    set_error("%s: a weight is NULL", what);
+    return MVPA_ERR_ALIGNMENT;
+  }
   const int groups = (K + group - 1) / group;
   if (w->q == nullptr || (reinterpret_cast<uintptr_t>(w->q) & 15) != 0 || w->ld_q % 16 != 0 || w->ld_q < (K + 1) / 2 || w->scales == nullptr ||
       (reinterpret_cast<uintptr_t>(w->scales) & (scale_dtype == MVPA_F32 ? 3 : 1)) != 0 || w->ld_s < groups ||

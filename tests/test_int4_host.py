@@ -68,3 +68,14 @@ def test_entry_points_refuse():
     assert need(p, 63, 9, 60, 1) == 9 * 64 * 2
     assert mul(M=9) == mul(M=9, ws=p, nbytes=9 * 64 * 6 - 1) == mul(M=9, ws=p + 8, nbytes=1 << 15) == -4
     assert "workspace" in nat.last_error()
+
+
+def test_entry_points_refuse_no_weight():
+    """NULL in the place of a weight is an error like the others, not a crash; where nothing is to be done it is not looked at."""
+    lib = nat.lib()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    assert lib.mvpa_quantize_int4(p, 64, None, 4, 64, 64, 0, None) == -3 and "NULL" in nat.last_error()
+    assert lib.mvpa_dequantize_int4(None, 0, p, 64, 4, 64, 64, 0, None) == -3 and "NULL" in nat.last_error()
+    assert lib.mvpa_matmul_int4(p, 64, None, None, 0, p, 64, 2, 4, 64, 64, 0, None, 0, None, None) == -3 and "NULL" in nat.last_error()
+    assert lib.mvpa_quantize_int4(p, 64, None, 0, 64, 64, 0, None) == 0 and lib.mvpa_dequantize_int4(None, 0, p, 64, 4, 0, 64, 0, None) == 0
