@@ -837,7 +837,8 @@ struct Gated {
     E = x.size(-1);
     I = wg.size(0);
     rows = x.numel() / E;
-    return E % 8 == 0 && I % 8 == 0 && I > 0 && E <= INT32_MAX && I <= INT32_MAX && fits(x, x, at::kBFloat16, x.sizes()) &&
+    constexpr int64_t kMost = INT32_MAX - 1024;
+    return E % 8 == 0 && I % 8 == 0 && I > 0 && E <= kMost && I <= kMost && rows <= kMost && fits(x, x, at::kBFloat16, x.sizes()) &&
            fits(wg, x, at::kBFloat16, {I, E}) && fits(wu, x, at::kBFloat16, {I, E});
   }
   Tensor like_x(int64_t width) const {  // (..., width)

@@ -267,6 +267,9 @@ class _GatedLinear(torch.autograd.Function):
             return (dg @ wg + du @ wu).to(x.dtype).view(x.shape), (dg.t() @ x2).to(x.dtype), (du.t() @ x2).to(x.dtype)
 
 
+_MOST = 2 ** 31 - 1025     # rows, columns and features that the gated projection's kernels count (include/mvpa.h)
+
+
 def gated_linear_kernel(x, w_gate, w_up):
     """`gated_linear` where it is one kernel, else None."""
     if _host.usable(x):
@@ -279,7 +282,7 @@ def gated_linear_kernel(x, w_gate, w_up):
             and x.shape[-1] == w_gate.shape[1] and x.shape[-1] % 8 == 0 and w_gate.shape[0] % 8 == 0):
         if not x.is_contiguous():
             x = x.contiguous()
-        if _plain(x, w_gate, w_up):
+        if _plain(x, w_gate, w_up) and max(x.numel() // x.shape[-1], *w_gate.shape) <= _MOST:
             return _GatedLinear.apply(x, w_gate, w_up)
     return None
 

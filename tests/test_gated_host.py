@@ -7,6 +7,7 @@ import torch
 import gated_oracle as ref
 import mvpa_host
 import mvpa_native as nat
+import mvpa_ops as ops
 
 
 def _inputs(M, E, I, seed=0):
@@ -73,3 +74,17 @@ def test_native_calls_count_their_arguments(name, count):
     for other in (count - 1, count + 1):
         with pytest.raises(TypeError, match="number of arguments"):
             call(*[None] * other)
+
+
+def test_more_rows_than_the_kernels_count(monkeypatch):
+    """2^31 - 1024 rows and more are served by torch's operations, like everything that the kernels do not take."""
+    lib = nat.lib()
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    assert lib.mvpa_gated_linear(p, 8, p, p, p, 8, None, ops._MOST + 1, 8, 8, None, None) == -1 and str(ops._MOST) in nat.last_error()
+    monkeypatch.setattr(ops, "_plain", lambda *ts: True)
+    monkeypatch.setattr(ops._GatedLinear, "apply", lambda *a: pytest.fail("the kernel was asked for"))
+    monkeypatch.setattr(ops, "_MOST", 8)
+    monkeypatch.setattr(ops, "swiglu", lambda g, u: torch.nn.functional.silu(g) * u)
+    x, w = torch.ones(9, 8, dtype=torch.bfloat16), torch.ones(8, 8, dtype=torch.bfloat16)
+    assert ops.gated_linear(x, w, w).shape == (9, 8)
