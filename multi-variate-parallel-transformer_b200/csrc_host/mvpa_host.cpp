@@ -542,12 +542,12 @@ PyObject* block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// branches(x, w_in, w_out, bias, r_time, r_chan, window, B, T, C, H, Hkv, D, status, gated): MLP(x) + Attn(x) of the fused inference block
+// branches(x, w_in, w_out, bias, r_time, r_chan, window, B, T, C, H, Hkv, D, status[, gated]): MLP(x) + Attn(x) of the fused inference block
 //   (`MVPFormerBlock.fused_branches`), or None.  `gated` (bf16): the gate's projections and the gate as one kernel.
 PyObject* branches(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 15)) return nullptr;
-  const bool status = a[13] == Py_True, gated = a[14] == Py_True;
+  if (n != 14 && !arguments(n, 15)) return nullptr;
+  const bool status = a[13] == Py_True, gated = n > 14 && a[14] == Py_True;
   Tensor in[6];
   for (int i = 0; i < 6; ++i) {
     if (!THPVariable_CheckExact(a[i])) Py_RETURN_NONE;

@@ -67,11 +67,12 @@ def test_entry_points_refuse():
         assert bwd(**bad) not in (0, -1) and "16-byte" in nat.last_error(), bad
 
 
-@pytest.mark.parametrize("name,count", [("backward", 14), ("branches", 15), ("block_forward", 20), ("block_backward", 32)])
-def test_native_calls_count_their_arguments(name, count):
+@pytest.mark.parametrize("name,counts", [("backward", (14,)), ("branches", (14, 15)), ("block_forward", (20,)), ("block_backward", (32,))])
+def test_native_calls_count_their_arguments(name, counts):
     call = getattr(mvpa_host.module(), name)
-    assert call(*[None] * count) is None          # (no tensors: Python's path answers)
-    for other in (count - 1, count + 1):
+    for count in counts:
+        assert call(*[None] * count) is None      # (no tensors: Python's path answers)
+    for other in (counts[0] - 1, counts[-1] + 1):
         with pytest.raises(TypeError, match="number of arguments"):
             call(*[None] * other)
 
