@@ -333,7 +333,7 @@ int mvpa_silu_mul_fp8(const void* gate, const void* up, int64_t ld_in, void* q, 
  * out = A B^T:  out[m, n] = sum_kb a_scales[m, kb] b_scales[n / 128, kb] sum_{k in kb} a[m, k] b[n, k].
  * a (M, K) and b (N, K) in e4m3, bases and rows (ld_a, ld_b) on 16-byte boundaries; scales MVPA_E8M0 or
  * MVPA_F32 (both the same), any strides in elements; out (M, N) MVPA_BF16 or MVPA_F32, leading dimension
- * ld_out.  All sums are in fp32, in an order that depends on the sizes alone, and rounded once.  A block's
+ * ld_out.  All sums are in fp32, in an order that depends on the sizes and the device alone, and rounded once.  A block's
  * products are scaled by the two scales' product, which for a few rows (up to 32) and for fp32 scales is
  * formed in fp32: it must not overflow there, and counts as zero below 2^-150.  K = 0 gives zeros.  `status` (may be
  * NULL): 64 ints, zeroed by the caller, of which the first is non-zero afterwards if one of the kernel's
@@ -376,7 +376,7 @@ int mvpa_dequantize_int4(const mvpa_int4* w, int32_t scale_dtype, void* out, int
  * out = x W^T, or with `up` (may be NULL) out = silu(x W^T) * (x Up^T); x (M, K) and out (M, N) MVPA_F32 or MVPA_BF16, both `dtype`,
  * any alignment to their elements (16-byte aligned rows of x are read faster).  Whole numbers q - zero and x are multiplied exactly (an
  * fp32 x in three parts) and added in fp32 over a group; the groups' sums are scaled and added in fp32, in an order that depends on the
- * sizes alone, and rounded once.  K = 0 gives zeros.  `workspace`: 16-byte aligned, of at least
+ * sizes and the device alone, and rounded once.  None of these sums leaves fp32 where the scaled ones do not.  K = 0 gives zeros.  `workspace`: 16-byte aligned, of at least
  * mvpa_matmul_int4_workspace_bytes(...) bytes, which may be 0.  `status` (may be NULL): as for mvpa_matmul_fp8.
  */
 size_t mvpa_matmul_int4_workspace_bytes(const void* x, int64_t ld_x, int64_t M, int32_t K, int32_t dtype);

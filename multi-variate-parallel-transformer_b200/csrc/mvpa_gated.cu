@@ -10,7 +10,7 @@
 //                  sums finds g and u of one feature 128 columns apart: h leaves from fp32 in one rounding, and g and u go to memory
 //                  only where a backward pass will want them: 24 bits of each, the upper half of the fp32 number and the byte after it,
 //                  in matrices of their own.  (In bf16 their roundings are half of the gradients' error: 0.0031 of the gradients' size
-//                  against 0.0024, of which 0.0017 is the results' own rounding.)
+//                  against 0.0023, of which 0.0017 is the results' own rounding.)
 //   input          dg and du are the left operand one after the other, Wg and Wu, whose rows lie along the columns of the result
 //                  (MN-major), the right one: the sum of both products is formed in TMEM.
 //   weights        both operands have the summed axis, the tokens, outermost (MN-major).
@@ -424,7 +424,7 @@ int few_rows(int64_t rows) { return rows <= 128 ? ((int)rows + 7) / 8 * 8 : 0; }
 
 // The gradients' products: how wide their tiles are, and in how many pieces the summed axis, by the longest pair's blocks.  Pieces are for
 // few tiles along a long axis, up to one a pair and eight blocks a piece at least; they cost a launch more and their sums' way to memory
-// and back.  In pieces and whole: weights' gradient of 65536 x 64 x 64 15 and 176 us, of 9973 x 64 x 72 10 and 39; dx of 22 x 2048 x 5632 13
+// and back.  In pieces and whole, operands in L2: weights' gradient of 65536 x 64 x 64 15 and 176 us, of 9973 x 64 x 72 10 and 39; dx of 22 x 2048 x 5632 13
 // and 36, of 22 x 768 x 1728 8 and 13.
 struct Plan {
   int width, splits, per;

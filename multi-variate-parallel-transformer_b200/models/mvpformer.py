@@ -526,8 +526,13 @@ class MVPFormerModel(Prepares, torch.nn.Module):
 
     def enable_fused_gate(self, flag: bool = True):
         """The blocks' gate and up projections, the activation and their product as one kernel (`mvpa_ops.gated_linear`), in training and in the
-        fused forward.  bf16; other types are not changed.  Results differ by roundings: the gate is formed in fp32 from the projections'
-        sums to its result and rounded once, where it is rounded four times without.  Captured graphs are dropped."""
+        fused forward, the time-sharded one too.  bf16; other types are not changed.  Results differ by roundings: the gate is formed in
+        fp32 from the projections' sums to its result and rounded once, where it is rounded four times without.  Captured graphs are
+        dropped.
+
+        In training each block keeps 6 bytes a token and feature of the gate for the backward (24 bits of both projections) where it keeps
+        4 without.  Faster for batches of some thousand tokens; few tokens in a graph are slower: 25 x 22 through MVPFormer-S 0.53 ms for
+        0.46, 22 0.42 for 0.34."""
         for block in self.h:
             block.mlp.fused_gate = bool(flag)
         self._graphs = {}
